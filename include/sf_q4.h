@@ -41,12 +41,15 @@ typedef enum {
   SF_ERR_UNSUPPORTED = 6, /* valid request this build does not implement       */
   SF_ERR_TIMEOUT = 7,     /* a device-side bounded wait expired                */
   SF_ERR_COMM = 8,        /* tensor-parallel peer exchange failed              */
-  SF_ERR_CAPTURE = 9      /* library scratch must grow while the stream is being
+  SF_ERR_CAPTURE = 9,     /* library scratch must grow while the stream is being
                              captured: run the same shape once on that stream
                              before capturing                                  */
+  SF_ERR_INDEX = 10       /* a kernel met a page, position or length outside its
+                             tensor; the access was skipped                    */
 } sf_status;
 
-typedef enum { SF_F32 = 0, SF_F16 = 1, SF_BF16 = 2 } sf_dtype;
+typedef enum { SF_F32 = 0, SF_F16 = 1, SF_BF16 = 2,
+               SF_E4M3 = 3 /* 8-bit float, 3 significand bits; only where a comment names it */ } sf_dtype;
 
 /* Human-readable text of a status code, and the detailed message of the last
    failing call on this host thread (mirrors bindings.cpp:27-39 wording). */
@@ -271,6 +274,101 @@ int sf_kv_attention_decode(const void* q, int q_dtype, const int8_t* k_codes, co
                            int B, int H, int Hkv, int T, int D, int n_split, void* workspace,
                            size_t workspace_bytes, void* stream);
 
+/* ==== 8-bit decoder operators ===============================================
+ * Norm, linear, rotary, cache and attention of a decoder whose activations and
+ * cache are held in e4m3.  No counterpart in the reference, whose activations
+ * stay fp32 and whose cache is int8 per vector.  Strides are in elements; the
+ * last dimension of every tensor is contiguous.  A call with no rows (T = 0)
+ * launches nothing and returns SF_OK.
+ *
+ * ---- RMS norm with the residual's addition ---------------------------------
+ *   h = x + residual (x when residual is NULL), in fp32
+ *   y = h / sqrt(mean(h^2) + eps) * weight      (weight NULL: ones)
+ * x, residual and h_out [T, K] of x_dtype (row strides ldx, ldr, K); weight
+ * [K] of w_dtype; h_out may be x's or residual's own memory, and is NULL exactly
+ * when residual is.  y of y_dtype [T, K], row stride ldy; for SF_E4M3, y holds
+ * codes and scales [T, ceil(K/128)] receives, for each row and 128 columns,
+ * max|y| / 448 (1 where that is 0, at least 2^-126), codes the e4m3 values
+ * nearest to y / scale.  A group that holds an infinity or NaN decodes to NaN.
+ * sf_quantize_e4m3: the same codes and scales of x itself. */
+int sf_rms_norm(const void* x, int x_dtype, long long ldx, const void* residual, long long ldr, void* h_out,
+                const void* weight, int w_dtype, float eps, void* y, int y_dtype, long long ldy, float* scales,
+                int T, int K, void* stream);
+int sf_quantize_e4m3(const void* x, int x_dtype, long long ldx, uint8_t* codes, long long ldy, float* scales,
+                     int T, int K, void* stream);
+
+/* ---- linear over e4m3 rows and e4m3 weights ---------------------------------
+ *   Y[t,n] = sum_kb xs[t,kb] * ws[n/128,kb] * sum_{k in block kb} X[t,k] * W[n,k] (+ bias[n])
+ * X [T, K] codes (row stride ldx), xs [T, ceil(K/128)] fp32 as written by
+ * sf_rms_norm / sf_quantize_e4m3; W [N, K] codes (row stride ldw), ws
+ * [ceil(N/128), ceil(K/128)] fp32; bias [N] fp32 or NULL; Y [T, N] of y_dtype
+ * (SF_F32 / SF_F16 / SF_BF16), contiguous.  fp32 accumulation.  X and W start
+ * at multiples of 16 bytes, ldx and ldw are multiples of 16. */
+int sf_fp8_linear(const uint8_t* X, long long ldx, const float* xs, const uint8_t* W, long long ldw, const float* ws,
+                  const float* bias, void* Y, int y_dtype, int T, int N, int K, void* stream);
+
+/* ---- rotary positions ---------------------------------------------------------
+ * out[t,h,:] = x[t,h,:] with its first `rot` elements turned, pair by pair, by
+ * the angle whose cosine and sine table[pos][j] and table[pos][rot/2 + j] hold:
+ * pair j is elements (j, rot/2 + j), or (2j, 2j + 1) when interleaved != 0.
+ * x [T, H, D] of dtype with token and head strides xts, xhs; out likewise (it may
+ * be x itself); positions [T] int32 (pos64 = 0) or int64; table fp32
+ * [max_pos, rot].  rot even, rot <= D.  A position outside [0, max_pos) gives
+ * NaN in the turned elements and SF_ERR_INDEX at the next error check. */
+int sf_rotary(const void* x, int dtype, long long xts, long long xhs, void* out, long long ots, long long ohs,
+              const void* positions, int pos64, const float* table, int max_pos, int rot, int interleaved, int T,
+              int H, int D, void* stream);
+
+/* ---- a paged cache in e4m3 ------------------------------------------------------
+ * k_codes, v_codes [num_pages, n_kv_heads, page_size, head_dim] e4m3, k_scales,
+ * v_scales [num_pages, n_kv_heads] fp32: value = code * scale of its page and
+ * head.  Token j of sequence b is slot j % page_size of page
+ * block_table[b][j / page_size].  seq_lens [batch] counts the tokens INCLUDING
+ * the call's new ones; the call's token rows are packed, sequence b's being
+ * rows starts[b] .. starts[b+1]-1 (starts NULL: T / batch rows each), and are
+ * the sequence's last tokens.  A sequence with fewer tokens than rows has padding
+ * rows in front: nothing of them is written, their query is turned as at
+ * position 0, and they see no key.  page_size 16, 32, 64, 128 or 256; head_dim 64, 96,
+ * 128 or 256; batch <= 4096.  block_table, seq_lens and starts are int32 device
+ * arrays; a page, length or position outside its tensor is skipped and reported
+ * as SF_ERR_INDEX by sf_q4_check_device_error. */
+typedef struct {
+  uint8_t* k_codes;
+  float* k_scales;
+  uint8_t* v_codes;
+  float* v_scales;
+  const int* block_table; /* [batch, pages_per_seq] */
+  const int* seq_lens;    /* [batch] */
+  const int* starts;      /* [batch + 1] or NULL */
+  int num_pages, n_kv_heads, page_size, head_dim, batch, pages_per_seq;
+} sf_paged_cache;
+
+/* Writes k and v [T, n_kv_heads, D] of dtype (token and head strides) as the last
+ * tokens of their sequences, k turned by its position first when table is not
+ * NULL; with q != NULL, also q_out [T, H, D] (contiguous) = q turned likewise.
+ * A page and head keeps one scale, 2^e with the least e >= -64 for which its
+ * largest finite value is <= 448 * 2^e.  When rows are added to a page that holds
+ * tokens and they need a larger e, its older codes are rewritten for it (exact
+ * but where they become subnormal).  Infinities are stored as +-448 * 2^e, NaN as
+ * NaN, and neither counts for the scale.  Two sequences of one call must not
+ * write to the same page. */
+int sf_paged_append(const sf_paged_cache* cache, const void* k, long long kts, long long khs, const void* v,
+                    long long vts, long long vhs, const void* q, long long qts, long long qhs, void* q_out, int dtype,
+                    int H, int T, const float* table, int max_pos, int rot, int interleaved, void* stream);
+
+/* Attention of q [T, H, D] over these pages: row i of sequence b's n rows has
+ * position p = seq_lens[b] - n + i and sees keys max(0, p - window + 1) .. p
+ * (window <= 0: 0 .. p);
+ *   out[t,h,:] = sum_j softmax_j(scale * q . k_j) v_j,  lse[t,h] = log sum_j e^(scale * q . k_j).
+ * H % n_kv_heads == 0 (any group size).  A row that sees no key gives 0, and lse
+ * -inf.  out [T, H, D] of out_dtype, contiguous; lse [T, H] fp32 or NULL.  The
+ * workspace belongs to the caller and needs
+ * sf_paged_attention_workspace_bytes(head_dim) bytes, 16-byte aligned. */
+size_t sf_paged_attention_workspace_bytes(int head_dim);
+int sf_paged_attention(const sf_paged_cache* cache, const void* q, int q_dtype, long long qts, long long qhs, void* out,
+                       int out_dtype, float* lse, int H, int T, float scale, int window, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
 /* Device dequant to fp32/fp16/bf16 [N, K].  fp32 output is bit-exact with
    dequantize_sym / dequantize_asym (siliconfer/quant/primitives.py:54-75,
    117-140); fp16/bf16 are that value rounded to nearest even. */
@@ -285,9 +383,11 @@ int sf_q4_quantize_pack(const float* W, uint8_t* packed, float* scales, float* z
                         int N, int K, int group_size, void* stream);
 
 /* Sticky device-side error word (set when a bounded wait inside a kernel
-   expires, or when a tensor-parallel kernel met a poisoned communicator).
-   Synchronous: reads and clears it.  Returns SF_OK, SF_ERR_TIMEOUT, or
-   SF_ERR_COMM (poisoned communicator; takes precedence). */
+   expires, when a tensor-parallel kernel met a poisoned communicator, or when a
+   paged-cache or rotary kernel met an index outside its tensor).
+   Synchronous: reads and clears it.  Returns SF_OK, SF_ERR_TIMEOUT,
+   SF_ERR_INDEX, or SF_ERR_COMM (poisoned communicator; takes precedence, then
+   an expired wait). */
 int sf_q4_check_device_error(void);
 
 /* Number of kernels this library has launched since load (host counter). */

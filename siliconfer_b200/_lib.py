@@ -13,13 +13,13 @@ import pathlib
 _PKG = pathlib.Path(__file__).resolve().parent
 LIB_PATH = _PKG / "libsf_q4.so"
 
-SF_F32, SF_F16, SF_BF16 = 0, 1, 2
+SF_F32, SF_F16, SF_BF16, SF_E4M3 = 0, 1, 2, 3
 SF_FLAG_PDL = 1
 SF_EPI_SWIGLU = 1
 SF_OK = 0
 
 _P, _I, _LL = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
-_SZ = ctypes.c_size_t
+_SZ, _F = ctypes.c_size_t, ctypes.c_float
 
 
 class Q4Task(ctypes.Structure):
@@ -27,6 +27,14 @@ class Q4Task(ctypes.Structure):
     _fields_ = [("W", _P), ("scales", _P), ("zeros", _P), ("bias", _P), ("X", _P), ("Y", _P),
                 ("N", _I), ("K", _I), ("T", _I), ("group_size", _I), ("x_dtype", _I),
                 ("y_dtype", _I), ("wait_before", _I), ("epilogue", _I), ("bits", _I)]
+
+
+class PagedCache(ctypes.Structure):
+    """Mirror of sf_paged_cache (include/sf_q4.h)."""
+    _fields_ = [("k_codes", _P), ("k_scales", _P), ("v_codes", _P), ("v_scales", _P), ("block_table", _P),
+                ("seq_lens", _P), ("starts", _P), ("num_pages", _I), ("n_kv_heads", _I), ("page_size", _I),
+                ("head_dim", _I), ("batch", _I), ("pages_per_seq", _I)]
+
 
 # name -> argtypes (restype is int unless listed in _RESTYPES)
 SIGNATURES = {
@@ -61,11 +69,19 @@ SIGNATURES = {
     "sf_kv_attention_workspace_bytes": [_I, _I, _I, _I],
     "sf_kv_attention_splits": [_I, _I, _I],
     "sf_kv_attention_decode": [_P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _SZ, _P],
+    "sf_rms_norm": [_P, _I, _LL, _P, _LL, _P, _P, _I, _F, _P, _I, _LL, _P, _I, _I, _P],
+    "sf_quantize_e4m3": [_P, _I, _LL, _P, _LL, _P, _I, _I, _P],
+    "sf_fp8_linear": [_P, _LL, _P, _P, _LL, _P, _P, _P, _I, _I, _I, _I, _P],
+    "sf_rotary": [_P, _I, _LL, _LL, _P, _LL, _LL, _P, _I, _P, _I, _I, _I, _I, _I, _I, _P],
+    "sf_paged_append": [ctypes.POINTER(PagedCache), _P, _LL, _LL, _P, _LL, _LL, _P, _LL, _LL, _P, _I, _I, _I, _P, _I,
+                        _I, _I, _P],
+    "sf_paged_attention_workspace_bytes": [_I],
+    "sf_paged_attention": [ctypes.POINTER(PagedCache), _P, _I, _LL, _LL, _P, _I, _P, _I, _I, _F, _I, _P, _SZ, _P],
 }
 _RESTYPES = {"sf_status_string": ctypes.c_char_p, "sf_last_error": ctypes.c_char_p,
              "sf_q4_launch_count": _LL, "sf_q4_step_workspace_bytes": _SZ,
              "sf_q4_step_destroy": None, "sf_tp_handle_bytes": _SZ, "sf_tp_comm_destroy": None,
-             "sf_kv_attention_workspace_bytes": _SZ}
+             "sf_kv_attention_workspace_bytes": _SZ, "sf_paged_attention_workspace_bytes": _SZ}
 
 _lib = None
 

@@ -295,6 +295,7 @@ const char* sf_status_string(int status) {
     case SF_ERR_TIMEOUT: return "device wait timed out";
     case SF_ERR_COMM: return "peer exchange failed";
     case SF_ERR_CAPTURE: return "scratch must grow during stream capture";
+    case SF_ERR_INDEX: return "index outside its tensor";
     default: return "unknown status";
   }
 }
@@ -381,14 +382,19 @@ int sf_q4_quantize_pack(const float* W, uint8_t* packed, float* scales, float* z
 
 int sf_q4_check_device_error(void) {
   const unsigned int a = take_dev_error_gemv(), b = take_dev_error_tc(),
-                     c = take_dev_error_tile() | take_dev_error_tp();
-  if (a == 0xffffffffu || b == 0xffffffffu || c == 0xffffffffu)
+                     c = take_dev_error_tile() | take_dev_error_tp(), d = take_dev_error_fp8(),
+                     e = take_dev_error_rotary(), f = take_dev_error_paged();
+  if (a == 0xffffffffu || b == 0xffffffffu || c == 0xffffffffu || d == 0xffffffffu || e == 0xffffffffu ||
+      f == 0xffffffffu)
     return fail(SF_ERR_CUDA, "reading the device error word failed");
   if ((a | b | c) & kErrPoisoned)
     return fail(SF_ERR_COMM,
                 "a tensor-parallel exchange met a poisoned communicator (a rank's bounded wait expired in an "
                 "earlier call; create the communicator again) (code %u)", a | b | c);
-  if (a | b | c) return fail(SF_ERR_TIMEOUT, "a device-side wait expired (code %u)", a | b | c);
+  const unsigned int waits = (a | b | c | d | e | f) & ~kErrIndex;
+  if (waits) return fail(SF_ERR_TIMEOUT, "a device-side wait expired (code %u)", waits);
+  if (d | e | f)
+    return fail(SF_ERR_INDEX, "a kernel met a page, position or length outside its tensor and skipped the access");
   return SF_OK;
 }
 

@@ -53,6 +53,9 @@ static __device__ unsigned int g_dev_error = 0;
 // Error-word bit of a kernel that met a poisoned tensor-parallel communicator
 // (sf_q4_check_device_error reports SF_ERR_COMM); other bits are expired waits.
 constexpr unsigned int kErrPoisoned = 1u << 20;
+// Error-word bit of a kernel that skipped an access outside a tensor
+// (sf_q4_check_device_error reports SF_ERR_INDEX).
+constexpr unsigned int kErrIndex = 1u << 21;
 // Flag value that a rank whose exchange wait expired stores into its peers'
 // flag words: a peer that arrives late sees it and fails instead of reading
 // a slot that no longer belongs to its call.
@@ -61,6 +64,9 @@ unsigned int take_dev_error_gemv();
 unsigned int take_dev_error_tc();
 unsigned int take_dev_error_tile();
 unsigned int take_dev_error_tp();
+unsigned int take_dev_error_fp8();
+unsigned int take_dev_error_rotary();
+unsigned int take_dev_error_paged();
 
 // Carves one exchange region for a pushed task from a tensor-parallel
 // communicator's arena (same order on every rank, so the same offsets):

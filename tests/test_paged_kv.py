@@ -1,0 +1,483 @@
+"""The paged e4m3 cache and attention over it, against plain 64-bit arithmetic over the pages.
+
+Bounds.
+  * append: a page's scale is the least power of two, 2^-64 at least, that keeps its largest value within 448 (the
+    rows' own and, on a page that held tokens, its former scale), so scales are compared bit for bit, and so are the
+    codes of values, which divide exactly; a turned key may fall on the other side of a tie: half a code step
+    (2^-4 of the value, 2^-10 of the scale when subnormal) instead of equality.
+  * attention, fp32: a score of magnitude up to about 40 is off by 2^-21 of itself and the products' rounding, so a
+    weight by some 2e-5 of itself, and the output by that share of max|v|: 3e-5 max|v|.  16-bit queries: weights enter
+    the second product in fp16 (2^-11 each), the output is rounded to its type: 2^-10 max|v| + 2^-8 |out| (2^-11 in fp16).
+    The log-sum keeps fp32: 4e-5.
+"""
+import math
+import random
+
+import pytest
+import torch
+
+E4M3_MAX = 448.0
+
+
+class Batch:
+    """Sequences of the given lengths, of which the last `news` tokens are the call's, over pages in random order."""
+
+    def __init__(self, lens, news, H, Hkv, D, page, dtype, seed=0, ragged=True, spare=3, fill=None):
+        self.lens, self.news, self.H, self.Hkv, self.D, self.page = lens, news, H, Hkv, D, page
+        g = torch.Generator(device="cuda").manual_seed(seed + sum(lens) + D)
+        self.g, self.dtype = g, dtype
+        B, per = len(lens), max(1, max(-(-l // page) for l in lens))
+        self.P = B * per + spare
+        self.table = torch.randperm(self.P, generator=g, device="cuda")[:B * per].view(B, per).to(torch.int32)
+        self.seq_lens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        self.starts = torch.tensor([sum(news[:b]) for b in range(B + 1)], dtype=torch.int32, device="cuda") if ragged else None
+        self.T = sum(news)
+        shape = (self.P, Hkv, page, D)
+        mk = lambda: (torch.randn(shape, generator=g, device="cuda") * 80).clamp(-448, 448).to(torch.float8_e4m3fn)
+        sc = lambda: torch.exp2(torch.randint(-8, -4, shape[:2], generator=g, device="cuda").float())
+        self.k, self.v, self.ks, self.vs = mk(), mk(), sc(), sc()
+        if fill is not None:   # what lies beyond a sequence's end
+            for b, l in enumerate(lens):
+                for j in range(per):
+                    for t in (self.k, self.v):
+                        t.view(torch.uint8)[self.table[b, j], :, max(0, min(page, l - j * page)):] = fill
+        self.q = (1.5 * torch.randn(self.T, H, D, generator=g, device="cuda")).to(dtype)
+
+    def args(self):
+        return self.k, self.ks, self.v, self.vs, self.table, self.seq_lens
+
+    def rows(self):
+        at = 0
+        for b, (l, n) in enumerate(zip(self.lens, self.news)):
+            yield b, l, n, at
+            at += n
+
+    def values(self, codes, scales, b, l):
+        p = self.table[b, :-(-l // self.page)].long()
+        x = codes[p].double() * scales[p].double()[:, :, None, None]
+        return x.permute(1, 0, 2, 3).reshape(self.Hkv, -1, self.D)[:, :l]
+
+    def ref(self, scale=None, window=0):
+        out = torch.zeros(self.T, self.H, self.D, dtype=torch.float64, device="cuda")
+        lse = torch.full((self.T, self.H), -math.inf, dtype=torch.float64, device="cuda")
+        vmax = 0.0
+        G = self.H // self.Hkv
+        for b, l, n, at in self.rows():
+            if not n or not l:
+                continue
+            k, v = self.values(self.k, self.ks, b, l), self.values(self.v, self.vs, b, l)
+            vmax = max(vmax, float(v.abs().max()))
+            q = self.q[at:at + n].double().view(n, self.Hkv, G, self.D)
+            s = torch.einsum("nhgd,hjd->nhgj", q, k) * (self.D ** -0.5 if scale is None else scale)
+            far = torch.arange(l - n, l, device="cuda")[:, None] - torch.arange(l, device="cuda")
+            hidden = (far < 0) | ((far >= window) if window else False)
+            s = s.masked_fill(hidden[:, None, None], -math.inf)
+            out[at:at + n] = torch.einsum("nhgj,hjd->nhgd", s.softmax(-1), v).reshape(n, self.H, self.D)
+            lse[at:at + n] = s.logsumexp(-1).reshape(n, self.H)
+        return out, lse, vmax
+
+
+def check_attention(batch, out_dtype=None, **kw):
+    from siliconfer_b200 import _lib
+    from siliconfer_b200.paged_kv import paged_attention
+    out, lse = paged_attention(batch.q, *batch.args(), starts=batch.starts, out_dtype=out_dtype, return_lse=True, **kw)
+    ref, lref, vmax = batch.ref(**kw)
+    dtype = out_dtype or batch.dtype
+    assert out.dtype == dtype and out.shape == ref.shape and lse.dtype == torch.float32
+    bound = 3e-5 * vmax if batch.dtype == torch.float32 else 2.0 ** -10 * vmax
+    bound = bound + {torch.float32: 0.0, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[dtype] * ref.abs()
+    assert ((out.double() - ref).abs() <= bound).all()
+    empty = lref == -math.inf
+    assert torch.equal(empty, lse == -math.inf)
+    assert ((lse.double() - lref)[~empty].abs() <= 4e-5 + 2e-6 * lref[~empty].abs()).all()
+    assert _lib.load().sf_q4_check_device_error() == 0
+    return out
+
+
+HEADS = [(1, 1), (8, 8), (14, 2), (8, 1), (12, 4), (64, 8), (16, 1), (40, 2), (9, 3)]
+LENS = [1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 127, 128, 129, 255, 500, 1000, 2049]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+@pytest.mark.parametrize("H,Hkv", HEADS)
+def test_single_tokens(cuda, H, Hkv, D, dtype):
+    """One new token each, a batch of every length, each page size."""
+    for i, page in enumerate((16, 32, 64, 128, 256)):
+        lens = LENS[i::2] if Hkv == 8 else LENS[i::3]
+        check_attention(Batch(lens, [1] * len(lens), H, Hkv, D, page, dtype, seed=page, ragged=False))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("H,Hkv,D", [(14, 2, 64), (8, 8, 128), (64, 8, 128), (8, 1, 256), (20, 4, 96)])
+def test_several_tokens(cuda, H, Hkv, D, dtype):
+    """Ragged counts of new tokens from none to whole prompts, with empty sequences between."""
+    check_attention(Batch([70, 5, 0, 300, 129, 64], [7, 5, 0, 1, 40, 64], H, Hkv, D, 32, dtype))
+    check_attention(Batch([33, 257], [33, 200], H, Hkv, D, 64, dtype))
+    check_attention(Batch([100, 100, 100], [4, 4, 4], H, Hkv, D, 16, dtype, ragged=False))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("window", [1, 7, 16, 33, 100, 5000])
+def test_window(cuda, window, dtype):
+    check_attention(Batch([1, 40, 500, 130], [1, 9, 3, 130], 8, 2, 64, 32, dtype), window=window)
+    check_attention(Batch([700] * 3, [1] * 3, 16, 2, 128, 64, dtype, ragged=False), window=window, scale=0.3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_long_sequences_and_uneven_batches(cuda, dtype):
+    check_attention(Batch([40000], [1], 8, 1, 128, 64, dtype, ragged=False))
+    check_attention(Batch([9000, 1, 0, 17, 3001], [1, 1, 0, 1, 1], 64, 8, 128, 64, dtype))
+    rng = random.Random(4)
+    lens = [rng.randint(1, 400) for _ in range(200)]
+    check_attention(Batch(lens, [1] * 200, 4, 2, 64, 16, dtype, ragged=False))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_all_rows_empty_and_no_rows(cuda, dtype):
+    from siliconfer_b200.paged_kv import paged_attention
+    b = Batch([5, 6], [1, 1], 8, 2, 64, 16, dtype, ragged=False)
+    b.seq_lens.zero_()
+    # a length below its number of new rows: the rows before the sequence see nothing, and nothing is out of range
+    out, lse = paged_attention(b.q, *b.args(), return_lse=True)
+    assert (out == 0).all() and (lse == -math.inf).all()
+    out = paged_attention(b.q[:0], *b.args(), starts=torch.zeros(3, dtype=torch.int32, device="cuda"))
+    assert out.shape == (0, 8, 64)
+    b = Batch([3, 40], [5, 2], 8, 2, 64, 16, dtype)     # two of the five rows lie before their sequence
+    out, lse = paged_attention(b.q, *b.args(), starts=b.starts, return_lse=True)
+    assert (out[:2] == 0).all() and (lse[:2] == -math.inf).all() and torch.isfinite(lse[2:]).all()
+    c = Batch([3, 40], [3, 2], 8, 2, 64, 16, dtype)
+    c.q, c.k, c.v, c.ks, c.vs, c.table = b.q[2:], b.k, b.v, b.ks, b.vs, b.table
+    ref, lref, vmax = c.ref()
+    assert ((out[2:].double() - ref).abs() <= 2.0 ** -10 * vmax + 2.0 ** -8 * ref.abs()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fill", [0x7f, 0xff, 0x7e])
+def test_contents_beyond_the_end_do_not_matter(cuda, fill):
+    """NaN and the largest codes in every slot past a sequence's end, and in pages of no sequence."""
+    for dtype in (torch.float32, torch.bfloat16):
+        check_attention(Batch([1, 20, 100, 130], [1, 1, 1, 1], 14, 2, 64, 64, dtype, ragged=False, fill=fill))
+        check_attention(Batch([9, 33, 65], [9, 2, 33], 8, 8, 128, 16, dtype, fill=fill))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_large_and_small_values(cuda, dtype):
+    """Scores that would overflow e^s, scales far apart between pages, zero scales, queries near their type's limits."""
+    b = Batch([200, 300], [1, 1], 8, 2, 64, 16, dtype, ragged=False)
+    check_attention(b, scale=3.0 / 8)
+    b.vs = torch.exp2(torch.randint(-40, 12, b.vs.shape, generator=b.g, device="cuda").float())
+    check_attention(b)
+    b.vs[::2] = 0
+    check_attention(b)
+    b.q = (b.q.float() * (2.0 ** -12)).to(dtype)
+    check_attention(b, scale=512.0)
+    if dtype != torch.float16:
+        b.q = (b.q.float() * 2.0 ** 60).to(dtype)
+        check_attention(b, scale=2.0 ** -54)
+    b.q.zero_()
+    check_attention(b)
+
+
+@pytest.mark.gpu
+def test_non_finite_values_stay_in_their_rows(cuda):
+    from siliconfer_b200.paged_kv import paged_attention
+    b = Batch([50, 60], [2, 2], 8, 2, 64, 16, torch.bfloat16, ragged=False)
+    b.q[0, 3, 5] = float("nan")
+    b.v.view(torch.uint8)[b.table[1, 0], 1, 3, 7] = 0x7f      # sequence 1, kv head 1, column 7
+    out = paged_attention(b.q, *b.args())
+    bad = torch.zeros_like(out, dtype=torch.bool)
+    bad[0, 3] = True
+    bad[2:, 4:, 7] = True
+    assert torch.equal(out.isnan(), bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,Hkv", [(8, 2), (32, 4)])
+def test_strided_queries_types_and_repeats(cuda, H, Hkv):
+    b = Batch([300, 1000, 90], [1, 4, 2], H, Hkv, 128, 64, torch.bfloat16)
+    first = check_attention(b, out_dtype=torch.float32)
+    wide = torch.zeros(b.T, (H + 3) * 128 + 1, device="cuda", dtype=torch.bfloat16)
+    q = b.q
+    for off in (0, 1, 130):
+        wide[:, off:off + H * 128] = q.reshape(b.T, -1)
+        b.q = wide[:, off:off + H * 128].view(b.T, H, 128)
+        assert torch.equal(check_attention(b, out_dtype=torch.float32), first)
+    b.q = q.transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(check_attention(b, out_dtype=torch.float32), first)
+    check_attention(b, out_dtype=torch.float16)
+
+
+@pytest.mark.gpu
+def test_streams_and_capture(cuda):
+    from siliconfer_b200.paged_kv import paged_attention
+    a = Batch([3000, 10], [1, 1], 32, 4, 128, 64, torch.bfloat16, ragged=False)
+    b = Batch([100, 2000, 77], [1, 1, 1], 32, 4, 128, 64, torch.bfloat16, ragged=False, seed=9)
+    ra, rb = paged_attention(a.q, *a.args()), paged_attention(b.q, *b.args())
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(20):
+        for s, x in zip(streams, (a, b)):
+            with torch.cuda.stream(s):
+                got.append(paged_attention(x.q, *x.args()))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, r) for y, r in zip(got, [ra, rb] * 20))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = paged_attention(a.q, *a.args())
+    for lens in ([3000, 10], [17, 2]):       # lengths are read when the graph runs
+        a.lens = lens
+        a.seq_lens.copy_(torch.tensor(lens))
+        graph.replay()
+        torch.cuda.synchronize()
+        ref, _, vmax = a.ref()
+        assert ((y.double() - ref).abs() <= 2.0 ** -10 * vmax + 2.0 ** -8 * ref.abs()).all()
+
+
+@pytest.mark.gpu
+def test_pages_past_31_bits(cuda):
+    """A pool of more than 2^31 codes: the pages at its end are read and written like the first ones."""
+    from siliconfer_b200.paged_kv import paged_append
+    b = Batch([40, 90], [1, 1], 8, 2, 128, 64, torch.bfloat16, ragged=False)
+    P = 2 ** 31 // (2 * 64 * 128) + 40
+    big = [torch.zeros(P, 2, 64, 128, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for _ in range(2)]
+    far = P - b.P
+    for dst, src in zip(big, (b.k, b.v)):
+        dst.view(torch.uint8)[far:] = src.view(torch.uint8)
+    ref, _, vmax = b.ref()
+    pad = lambda s: torch.cat([torch.ones(far, 2, device="cuda"), s])
+    b.k, b.v, b.ks, b.vs, b.table = big[0], big[1], pad(b.ks), pad(b.vs), b.table + far
+    out = check_attention(b)
+    assert ((out.double() - ref).abs() <= 2.0 ** -10 * vmax + 2.0 ** -8 * ref.abs()).all()
+    v = torch.full((2, 2, 128), 3.0, device="cuda", dtype=torch.bfloat16)
+    paged_append(v, v, *b.args())
+    p = int(b.table[1, 1])
+    assert (b.v[p, :, 89 - 64].float() * b.vs[p][:, None] - 3).abs().max() <= 3 * 2.0 ** -4
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# append
+# ---------------------------------------------------------------------------------------------------------------------
+def e4m3(x):
+    return x.clamp(-E4M3_MAX, E4M3_MAX).float().to(torch.float8_e4m3fn).double()
+
+
+def append_ref(codes, scales, batch, rows):
+    """rows [T, Hkv, D] in 64 bits into (codes, scales), a page at a time; returns both as 64-bit tensors."""
+    c, s = codes.double(), scales.double()
+    for b, l, n, at in batch.rows():
+        for j in range((l - n) // batch.page, -(-l // batch.page)) if n else ():
+            lo, hi = max(l - n, j * batch.page), min(l, (j + 1) * batch.page)
+            p, base = int(batch.table[b, j]), j * batch.page
+            new = rows[at + lo - (l - n):at + hi - (l - n)].transpose(0, 1)
+            for h in range(batch.Hkv):
+                fin = new[h][torch.isfinite(new[h])].abs()
+                amax = float(fin.max()) if fin.numel() else 0.0
+                e = -64
+                if amax > 0:
+                    e = math.floor(math.log2(amax)) - 9
+                    while amax > E4M3_MAX * 2.0 ** e:
+                        e += 1
+                scale = 2.0 ** max(e, -64)
+                if lo > base:
+                    old = float(s[p, h])
+                    scale = max(scale, old)
+                    c[p, h, :lo - base] = e4m3(c[p, h, :lo - base] * (old / scale))
+                c[p, h, lo - base:hi - base] = e4m3(new[h] / scale)
+                s[p, h] = scale
+    return c, s
+
+
+def same(a, b):
+    return torch.equal(torch.nan_to_num(a, nan=1e9), torch.nan_to_num(b, nan=1e9))
+
+
+def check_append(batch, dtype, rot=None, interleaved=False, turn=True, values=None, strided=False):
+    from siliconfer_b200 import _lib
+    from siliconfer_b200.paged_kv import paged_append
+    from siliconfer_b200.rotary import rotary_table
+    from test_rotary import check as check_rotary, turned
+    T, Hkv, H, D = batch.T, batch.Hkv, batch.H, batch.D
+    qkv = torch.randn(T, (H + 2 * Hkv) * D + 1, generator=batch.g, device="cuda").to(dtype)
+    off = 1 if strided else 0
+    part = lambda a, h: qkv[:, off + a * D:off + (a + h) * D].view(T, h, D)
+    q, k, v = part(0, H), part(H, Hkv), part(H + Hkv, Hkv)
+    if values is not None:
+        values(k, v)
+    pos = torch.cat([torch.arange(l - n, l, device="cuda") for _, l, n, _ in batch.rows()] or [torch.zeros(0)]).long()
+    table = rotary_table(max(batch.lens) + 1, rot or D) if turn else None
+    kr = (turned(k, pos, table, interleaved)[0] if turn else k.double())
+    kc, kscale = append_ref(batch.k, batch.ks, batch, kr)
+    vc, vscale = append_ref(batch.v, batch.vs, batch, v.double())
+    got = paged_append(k, v, *batch.args(), starts=batch.starts, q=q if turn else None, table=table,
+                       interleaved=interleaved)
+    assert _lib.load().sf_q4_check_device_error() == 0
+    assert torch.equal(batch.ks.double(), kscale) and torch.equal(batch.vs.double(), vscale)
+    assert same(batch.v.double(), vc)
+    diff = batch.k.double() - kc
+    if turn:
+        assert (diff.nan_to_num().abs() <= 0.1251 * kc.nan_to_num().abs() + 2.0 ** -9).all()   # one step at most
+        assert ((diff != 0) & ~diff.isnan()).float().mean() <= 1e-4
+        check_rotary(got, *turned(q, pos, table, interleaved), dtype)
+    else:
+        assert same(batch.k.double(), kc) and got is None
+    assert torch.equal(batch.k.double().isnan(), kc.isnan())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("H,Hkv,D", [(14, 2, 64), (8, 8, 128), (6, 3, 96), (4, 1, 256)])
+@pytest.mark.parametrize("page", [16, 64, 256])
+def test_append(cuda, page, H, Hkv, D, dtype):
+    lens = [1, page, page + 1, 2 * page - 1, 3 * page + 5, 1000]
+    check_append(Batch(lens, [1] * 6, H, Hkv, D, page, dtype, ragged=False), dtype)
+    check_append(Batch(lens, [1, 3, page, 0, 2 * page + 7, 1000], H, Hkv, D, page, dtype), dtype, turn=False)
+    check_append(Batch(lens, [1, page, page + 1, 5, 2 * page, 900], H, Hkv, D, page, dtype), dtype, interleaved=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rot", [32, 48, 20, 2])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_append_partial_rotary_and_strides(cuda, rot, interleaved):
+    for dtype in (torch.bfloat16, torch.float32):
+        b = lambda: Batch([70, 9, 0, 130], [6, 9, 0, 1], 5, 2, 64, 32, dtype, seed=rot)
+        check_append(b(), dtype, rot=rot, interleaved=interleaved)
+        check_append(b(), dtype, rot=rot, interleaved=interleaved, strided=True)
+
+
+@pytest.mark.gpu
+def test_append_scales_grow_and_special_values(cuda):
+    """Pages whose old scale is smaller, larger and equal; zero rows; infinities and NaN among the new values."""
+    def values(k, v):
+        v[0] = 0
+        v[1] *= 1000
+        v[2, 0, 3], v[2, 0, 4], v[2, 0, 5] = float("inf"), float("-inf"), float("nan")
+        v[3] = 448.0
+        v[4] = 449.0
+        v[5] = float("nan")
+        v[6] = 1e-30
+        k[1] *= 1e-6
+        k[2, 1, 0] = float("nan")
+    for dtype in (torch.float32, torch.bfloat16):
+        check_append(Batch([20, 20, 20, 20, 20, 33, 33], [1] * 7, 4, 2, 64, 32, dtype, ragged=False), dtype, turn=False,
+                     values=values)
+    # a page filled a token at a time ends like the page's largest scale
+    from siliconfer_b200.paged_kv import PagedKVCache
+    cache = PagedKVCache(2, 1, 64, page_size=16)
+    x = torch.randn(16, 1, 64, device="cuda") * torch.linspace(0.01, 5, 16, device="cuda")[:, None, None]
+    table = torch.tensor([[1]], dtype=torch.int32, device="cuda")
+    for i in range(16):
+        cache.append(x[i:i + 1], x[i:i + 1], table, torch.tensor([i + 1], dtype=torch.int32, device="cuda"))
+    got = cache.v_codes[1, 0].double() * cache.v_scales[1, 0].double()
+    step = 2.0 ** -4 * x[:, 0].double().abs() + 2.0 ** -10 * cache.v_scales[1, 0].double()
+    # rounded once, and once more (half a subnormal step) for each of the scale's growths
+    assert ((got - x[:, 0].double()).abs() <= step + 16 * 2.0 ** -10 * cache.v_scales[1, 0].double()).all()
+    out = cache.attend(x[15:16], table, torch.tensor([16], dtype=torch.int32, device="cuda"))
+    assert torch.isfinite(out).all()
+
+
+@pytest.mark.gpu
+def test_indices_outside_their_tensors_are_skipped_and_reported(cuda):
+    from siliconfer_b200 import _lib
+    from siliconfer_b200.paged_kv import paged_append, paged_attention
+    from siliconfer_b200.rotary import rotary_table
+    lib = _lib.load()
+    mk = lambda: Batch([40, 50], [1, 1], 8, 2, 64, 16, torch.bfloat16, ragged=False)
+    kv = torch.randn(2, 2, 64, device="cuda", dtype=torch.bfloat16)
+    # a page outside the pool: its keys are left out of the sums
+    b = mk()
+    b.table[0, 1], b.table[1, 3] = 10 ** 6, -5
+    before = b.k.clone().view(torch.uint8)
+    out = paged_attention(b.q, *b.args())
+    assert lib.sf_q4_check_device_error() == 10 and torch.isfinite(out).all()
+    paged_append(kv, kv, *b.args())
+    assert lib.sf_q4_check_device_error() == 10
+    changed = (b.k.view(torch.uint8) != before).any(-1).any(-1).any(-1).nonzero().flatten().tolist()
+    assert changed == [int(b.table[0, 2])]
+    # lengths beyond the block table, negative ones, more new rows than tokens
+    for lens in ([10 ** 9, 50], [-3, 50]):
+        b = mk()
+        b.seq_lens.copy_(torch.tensor(lens))
+        before = b.k.clone().view(torch.uint8)
+        out = paged_attention(b.q, *b.args())
+        assert lib.sf_q4_check_device_error() == 10 and torch.isfinite(out).all()
+        paged_append(kv, kv, *b.args())
+        assert lib.sf_q4_check_device_error() == 10
+        changed = (b.k.view(torch.uint8) != before).any(-1).any(-1).any(-1).nonzero().flatten().tolist()
+        assert changed == [int(b.table[1, 3])]
+    # starts that leave the rows
+    b = mk()
+    starts = torch.tensor([0, 5000, 2], dtype=torch.int32, device="cuda")
+    out = paged_attention(b.q, *b.args(), starts=starts)
+    paged_append(kv, kv, *b.args(), starts=starts)
+    assert lib.sf_q4_check_device_error() == 10
+    # a rotary table that ends before the position
+    b = mk()
+    paged_append(kv, kv, *b.args(), q=b.q, table=rotary_table(45, 64))
+    assert lib.sf_q4_check_device_error() == 10
+    assert (b.k[b.table[1, 3].long(), :, 1].float()).isnan().all()
+    assert lib.sf_q4_check_device_error() == 0
+
+
+@pytest.mark.gpu
+def test_refusals(cuda):
+    from siliconfer_b200.paged_kv import paged_append, paged_attention
+    b = Batch([40, 50], [1, 1], 8, 2, 64, 16, torch.bfloat16, ragged=False)
+    k, ks, v, vs, table, lens = b.args()
+    x = torch.randn(2, 2, 64, device="cuda", dtype=torch.bfloat16)
+    t = torch.zeros(100, 64, device="cuda")
+    att = lambda q=b.q, k=k, ks=ks, v=v, vs=vs, table=table, lens=lens, **kw: paged_attention(q, k, ks, v, vs, table, lens, **kw)
+    app = lambda a=x, c=x, k=k, ks=ks, table=table, lens=lens, **kw: paged_append(a, c, k, ks, v, vs, table, lens, **kw)
+    for bad in (lambda: att(q=b.q.cpu()), lambda: att(q=b.q.double()), lambda: att(q=b.q[:, :7]), lambda: att(q=b.q[:, :, :32]),
+                lambda: att(q=b.q[:1]), lambda: att(q=b.q[0]), lambda: att(k=k.float()), lambda: att(k=k[:, :1]),
+                lambda: att(k=k.transpose(1, 2)), lambda: att(ks=ks[:1]), lambda: att(ks=ks.half()), lambda: att(vs=vs.cpu()),
+                lambda: att(table=table.long()), lambda: att(table=table[0]), lambda: att(lens=lens.long()),
+                lambda: att(lens=lens[:1]), lambda: att(starts=lens), lambda: att(starts=torch.zeros(3, device="cuda")),
+                lambda: att(out_dtype=torch.int32), lambda: att(k=k[:, :, :8].contiguous(), v=v[:, :, :8].contiguous()),
+                lambda: att(table=table[:, :0]), lambda: app(a=x.cpu()), lambda: app(a=x[:1]), lambda: app(c=x.float()),
+                lambda: app(a=x[:, :1], c=x[:, :1]), lambda: app(q=b.q), lambda: app(q=b.q[:1], table=t),
+                lambda: app(q=b.q.float(), table=t), lambda: app(table=t.half()), lambda: app(table=t[:, :63]),
+                lambda: app(a=x.double(), c=x.double()), lambda: app(lens=lens.float())):
+        with pytest.raises(RuntimeError):
+            bad()
+    odd = torch.zeros(4, 2, 24, 64, dtype=torch.uint8, device="cuda")
+    with pytest.raises(RuntimeError, match="page_size"):
+        att(k=odd, v=odd, ks=torch.ones(4, 2, device="cuda"), vs=torch.ones(4, 2, device="cuda"))
+
+
+def test_validation_without_gpu():
+    import ctypes
+
+    from siliconfer_b200 import _lib
+    lib, F = _lib.load(), 0x1000
+
+    def cache(**k):
+        return ctypes.byref(_lib.PagedCache(**{**dict(k_codes=F, k_scales=F, v_codes=F, v_scales=F, block_table=F, seq_lens=F,
+                                                      starts=None, num_pages=4, n_kv_heads=2, page_size=16, head_dim=64,
+                                                      batch=1, pages_per_seq=4), **k}))
+
+    big = 1 << 30
+    att = lambda c=None, **k: lib.sf_paged_attention(c or cache(), *{**dict(q=F, qd=0, ts=512, hs=64, o=F, od=0, lse=None, H=8,
+                                                                          T=1, s=1.0, w=0, ws=F, wb=big, st=None), **k}.values())
+    app = lambda c=None, **k: lib.sf_paged_append(c or cache(), *{**dict(k=F, a=128, b=64, v=F, c=128, d=64, q=None, e=0, f=0,
+                                                                       qo=None, dt=0, H=0, T=1, t=None, mp=0, rot=0, il=0,
+                                                                       st=None), **k}.values())
+    for call in (att, app):
+        assert call(cache(page_size=24)) == 6 and call(cache(head_dim=80)) == 6 and call(cache(batch=5000)) == 6
+        assert call(cache(batch=0)) == 2 and call(cache(num_pages=0)) == 2 and call(cache(batch=2)) == 2 and call(T=-1) == 2
+        assert call(cache(pages_per_seq=1 << 28)) == 2
+        assert call(cache(k_codes=None)) == 1 and call(cache(seq_lens=None)) == 1 and call(cache(v_codes=0x1008)) == 4
+        assert call(T=0) == 0
+    assert att(H=7) == 2 and att(H=0) == 2 and att(qd=3) == 3 and att(od=9) == 3 and att(q=None) == 1 and att(ws=None) == 1
+    assert att(wb=0) == 2 and b"workspace" in lib.sf_last_error()
+    assert app(dt=5) == 3 and app(k=None) == 1 and app(q=F) == 1 and app(q=F, qo=F) == 2
+    assert app(t=F, mp=8, rot=65) == 2 and app(t=F, mp=0, rot=64) == 2
+    assert lib.sf_paged_attention(None, F, 0, 512, 64, F, 0, None, 8, 1, 1.0, 0, F, big, None) == 1
+    assert lib.sf_paged_attention_workspace_bytes(128) > 0

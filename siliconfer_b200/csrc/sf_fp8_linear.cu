@@ -1,7 +1,26 @@
 // sf_fp8_linear.cu -- Y = X W^T over e4m3 rows (one scale per row and 128 columns) and e4m3 weights (one scale per
-// 128 x 128 block), accumulated in fp32.
+// 128 x 128 block) on the sm_100a tcgen05 tensor cores.
+//
+//   Y[t,n] = sum_kb xs[t,kb] * ws[n/128,kb] * sum_{k in block kb} X[t,k] * W[n,k]  (+ bias[n])
+//
+// Tokens are the rows of the MMA (M = 128: one TMEM lane each), weight rows its columns, so that a k-block's scale
+// is one number per thread: xs of its lane's token times ws of its 128 columns.  Each k-block of 128 is one set of
+// four tcgen05.mma.kind::f8f6f4 into a fresh TMEM buffer; eight warps read it back and add it, scaled, to sums that
+// stay in registers in fp32 for the whole of K, while the next k-block's MMAs fill the other buffer.
+//
+// Two shapes of the same pipeline (TMA -> shared memory -> MMA -> TMEM -> registers):
+//  * split: one 128 x 128 tile per CTA, K cut between the S CTAs of a cluster.  Their sums meet in shared memory over
+//    the cluster (each CTA adds the S parts of its share of the columns, in rank order), so that few tokens still
+//    spread the weight read over the SMs, in one launch and with the same result every time.  With few tokens only
+//    the rows that exist are loaded; what the MMA reads above them ends in TMEM lanes that nothing looks at.
+//  * persistent: 128 x 256 tiles in turn on one CTA per SM, stored through shared memory by TMA.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include <atomic>
 #include <cstdint>
+#include <cstring>
+#include <mutex>
 
 #include "sf_e4m3.h"
 #include "sf_q4_internal.h"
@@ -12,50 +31,476 @@ extern std::atomic<long long> g_launches;
 
 namespace {
 
-struct Fp8Args {
-  const uint8_t* X;
-  const uint8_t* W;
+constexpr int kBK = 128;                // k per stage: one 128-byte swizzle row, and one block of scales
+constexpr int kSumWarps = 8, kProdWarp = 8, kMmaWarp = 9, kThreads = 320;
+constexpr int kSmemLimit = 232448;      // 227 KB opt-in per block
+constexpr unsigned kErrProd = 1u << 13, kErrMma = 1u << 14, kErrSum = 1u << 15, kErrDrain = 1u << 16;
+
+struct Fp8Params {
   const float* xs;
   const float* ws;
   const float* bias;
   void* Y;
-  long long ldx, ldw;
-  int T, N, K, y_dtype;
+  int T, N, KB, y_dtype;
+  int mtiles, ntiles;
+  int rows;        // rows of X that a stage holds (16, 32, 64 or 128)
+  int stages;
+  int split;       // CTAs of a cluster along K
+  int tma_store;
 };
 
-// 64 tokens x 64 rows per block, 4 x 4 outputs per thread; tiles of 32 k are decoded into shared memory.
-__global__ void __launch_bounds__(256) fp8_linear_kernel(const Fp8Args a) {
-  __shared__ float xt[32][65], wt[32][65];
-  const int t0 = blockIdx.y * 64, n0 = blockIdx.x * 64, KB = (a.K + 127) / 128;
-  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < a.K; k0 += 32) {
-    for (int i = threadIdx.x; i < 64 * 32; i += 256) {
-      const int r = i / 32, k = k0 + i % 32, t = t0 + r, n = n0 + r;
-      xt[i % 32][r] = t < a.T && k < a.K ? from_e4m3(a.X[t * a.ldx + k]) * a.xs[(size_t)t * KB + k / 128] : 0.f;
-      wt[i % 32][r] = n < a.N && k < a.K ? from_e4m3(a.W[n * a.ldw + k]) * a.ws[(size_t)(n / 128) * KB + k / 128] : 0.f;
+// ---------------------------------------------------------------------------
+// PTX wrappers
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity), "r"(20000u)
+      : "memory");
+  return ok != 0;
+}
+// Bounded wait that also gives up when another role raised the abort flag.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, unsigned code, volatile int* abort_flag) {
+  if (bar_try(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!bar_try(bar, parity)) {
+    if (*abort_flag) return false;
+    if (clock64() - t0 > kWaitCycles) {
+      atomicOr(&g_dev_error, code);
+      *abort_flag = 1;
+      return false;
     }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 32; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(xt[k][ty + 16 * i], wt[k][tx + 16 * j], acc[i][j]);
-    __syncthreads();
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int t = t0 + ty + 16 * i, n = n0 + tx + 16 * j;
-      if (t >= a.T || n >= a.N) continue;
-      const float y = acc[i][j] + (a.bias ? a.bias[n] : 0.f);
-      const size_t o = (size_t)t * a.N + n;
-      if (a.y_dtype == SF_F32) static_cast<float*>(a.Y)[o] = y;
-      else if (a.y_dtype == SF_F16) static_cast<__half*>(a.Y)[o] = __float2half_rn(y);
-      else static_cast<__nv_bfloat16*>(a.Y)[o] = __float2bfloat16_rn(y);
+  return true;
+}
+// Bounded wait for something that is under way whatever the others do.
+__device__ __forceinline__ void bar_drain(uint32_t bar, uint32_t parity) {
+  if (bar_try(bar, parity)) return;
+  const long long t0 = clock64();
+  while (!bar_try(bar, parity))
+    if (clock64() - t0 > kWaitCycles) {
+      atomicOr(&g_dev_error, kErrDrain);
+      return;
     }
+}
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void bar_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, int x, int y, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y),
+               "r"(src)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+
+// Shared-memory matrix descriptor of a K-major tile with 128-byte rows in the 128-byte swizzle (8-row atoms of 1024
+// bytes).  32 k (32 bytes) further inside the atom adds 2 to the start-address field.
+__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// Instruction descriptor of kind::f8f6f4: D fp32 (bits 4-5 = 1), A and B e4m3 (0), both K-major, N >> 3 in bits
+// 17-22, M >> 4 in bits 24-28.
+__host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N) {
+  return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+__device__ __forceinline__ void mma_e4m3(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+
+// 32 fp32 columns of this warp's 32 TMEM lanes; the registers hold them after tmem_wait on the same array.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+        "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+        "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+
+// Two fp32 lanes per instruction.
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_cluster(uint32_t saddr, uint32_t rank) {
+  uint32_t a;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(saddr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ void store_y(void* Y, size_t o, float v, int dt) {
+  if (dt == SF_F32) static_cast<float*>(Y)[o] = v;
+  else if (dt == SF_F16) static_cast<__half*>(Y)[o] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16*>(Y)[o] = __float2bfloat16_rn(v);
+}
+__device__ __forceinline__ uint32_t pack16(float lo, float hi, int dt) {
+  uint32_t d;
+  if (dt == SF_BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+
+// Shared memory: `stages` x (X rows, then W tile), then for the persistent kernel one 4 KB store buffer per warp,
+// then the barriers.  An MMA reads 128 rows wherever X starts: with fewer loaded, the rest are bytes of the same
+// stage's W tile.  The split kernel reuses the stages for the sums that the cluster exchanges.
+template <bool SPLIT>
+struct Plan {
+  static constexpr int BN = SPLIT ? 128 : 256;
+  static constexpr int NBUF = 2;
+  static constexpr uint32_t TMEM_COLS = NBUF * BN;
+  static constexpr int CW = BN / 2;                      // columns of a summing warp
+  static constexpr uint32_t W = BN * kBK;
+  static constexpr uint32_t CTL = 512;
+  static constexpr uint32_t TAIL = SPLIT ? 0 : kSumWarps * 4096;
+  static constexpr int MAX_STAGES = 12;
+  static constexpr uint32_t stage(int rows) { return W + (uint32_t)rows * kBK; }
+  static constexpr size_t bytes(int rows, int stages) { return 1024 + (size_t)stages * stage(rows) + TAIL + CTL; }
+};
+
+template <bool SPLIT>
+__global__ void __launch_bounds__(kThreads, SPLIT ? 2 : 1)
+    fp8_linear_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__ CUtensorMap mapW,
+                      const __grid_constant__ CUtensorMap mapY, const Fp8Params p) {
+  using L = Plan<SPLIT>;
+  constexpr int BN = L::BN, NBUF = L::NBUF;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  const uint32_t xbytes = (uint32_t)p.rows * kBK, stage_bytes = L::W + xbytes;
+  const uint32_t tail = base + (uint32_t)p.stages * stage_bytes;
+  const uint32_t ctl = tail + L::TAIL;
+  const uint32_t full0 = ctl, empty0 = ctl + 8 * L::MAX_STAGES, accf0 = ctl + 16 * L::MAX_STAGES, acce0 = accf0 + 16,
+                 drain = acce0 + 16;
+  uint8_t* ctl_gen = smem_raw + (ctl - raw);
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(ctl_gen + 400);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(ctl_gen + 408);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int S = p.stages;
+  // lane quarters that hold tokens: their two warps each release an accumulator buffer
+  const int quarters = SPLIT ? (p.rows + 31) / 32 : 4;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      bar_init(full0 + 8 * s, 1);
+      bar_init(empty0 + 8 * s, 1);
+    }
+    for (int b = 0; b < NBUF; ++b) {
+      bar_init(accf0 + 8 * b, 1);
+      bar_init(acce0 + 8 * b, 2 * quarters);
+    }
+    bar_init(drain, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kProdWarp && lane == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mapX) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mapW) : "memory");
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32((const void*)tmem_slot)),
+                 "r"(L::TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  const int ntiles = p.mtiles * p.ntiles;
+  const int rank = SPLIT ? (int)(blockIdx.x % p.split) : 0;
+  const int kb0 = SPLIT ? (int)((long long)p.KB * rank / p.split) : 0;
+  const int kb1 = SPLIT ? (int)((long long)p.KB * (rank + 1) / p.split) : p.KB;
+  const int tile0 = SPLIT ? (int)(blockIdx.x / p.split) : (int)blockIdx.x;
+  const int tile_step = SPLIT ? ntiles : (int)gridDim.x;   // the split kernel has one tile
+
+  if (warp == kProdWarp) {
+    // ---------------- TMA producer ----------------
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int tile = tile0; tile < ntiles && ok; tile += tile_step) {
+        const int m0 = (tile % p.mtiles) * 128, n0 = (tile / p.mtiles) * BN;
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const uint32_t s = it % S, ph = (it / S) & 1;
+          if (!bar_wait(empty0 + 8 * s, ph ^ 1, kErrProd, abort_flag)) { ok = false; break; }
+          const uint32_t st = base + s * stage_bytes;
+          bar_expect_tx(full0 + 8 * s, stage_bytes);
+          tma_load(st, &mapX, kb * kBK, m0, full0 + 8 * s);
+          tma_load(st + xbytes, &mapW, kb * kBK, n0, full0 + 8 * s);
+        }
+      }
+      // every issued copy has landed before the block goes on
+      const uint32_t pending = it < (uint32_t)S ? it : (uint32_t)S;
+      for (uint32_t j = it - pending; j < it; ++j) bar_drain(full0 + 8 * (j % S), (j / S) & 1);
+    }
+  } else if (warp == kMmaWarp) {
+    // ---------------- MMA issuer ----------------
+    if (lane == 0) {
+      const uint32_t idesc = idesc_e4m3(128, BN);
+      uint32_t it = 0;
+      bool ok = true;
+      for (int tile = tile0; tile < ntiles && ok; tile += tile_step) {
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const uint32_t s = it % S, ph = (it / S) & 1, b = it % NBUF, use = it / NBUF;
+          if (!bar_wait(acce0 + 8 * b, (use & 1) ^ 1, kErrMma, abort_flag) ||
+              !bar_wait(full0 + 8 * s, ph, kErrMma, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t st = base + s * stage_bytes;
+#pragma unroll
+          for (int kk = 0; kk < kBK / 32; ++kk)
+            mma_e4m3(tmem + b * BN, sw128_desc(st + kk * 32), sw128_desc(st + xbytes + kk * 32), idesc, kk != 0);
+          mma_commit(empty0 + 8 * s);
+          mma_commit(accf0 + 8 * b);
+        }
+      }
+      // every issued MMA has completed before TMEM is freed
+      mma_commit(drain);
+      bar_drain(drain, 0);
+    }
+  } else {
+    // ---------------- scaled sums ----------------
+    // Warp w: tokens 32 (w % 4) .. of the tile, columns CW (w / 4) .. (inside one 128-column block of ws).
+    const int q = warp & 3, c0 = (warp >> 2) * L::CW;
+    const uint32_t lane_base = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)c0;
+    uint32_t it = 0;
+    if (q < quarters) {
+      for (int tile = tile0; tile < ntiles; tile += tile_step) {
+        const int m0 = (tile % p.mtiles) * 128, n0 = (tile / p.mtiles) * BN;
+        const int t = m0 + 32 * q + lane, nb = (n0 + c0) / 128;
+        const bool in = t < p.T && nb * 128 < p.N;
+        const float* xrow = p.xs + (size_t)(in ? t : 0) * p.KB;
+        const float* wrow = p.ws + (size_t)(in ? nb : 0) * p.KB;
+        uint64_t acc[L::CW / 2];
+#pragma unroll
+        for (int i = 0; i < L::CW / 2; ++i) acc[i] = 0;
+        float sx = __ldg(xrow + kb0), sw = __ldg(wrow + kb0);
+        bool ok = true;
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const uint32_t b = it % NBUF, use = it / NBUF;
+          const float s = sx * sw;
+          const uint64_t s2 = pack2(s, s);
+          if (kb + 1 < kb1) {
+            sx = __ldg(xrow + kb + 1);
+            sw = __ldg(wrow + kb + 1);
+          }
+          if (!bar_wait(accf0 + 8 * b, use & 1, kErrSum, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          uint32_t r[2][32];
+          tmem_ld32(lane_base + b * BN, r[0]);
+#pragma unroll
+          for (int c = 0; c < L::CW / 32; ++c) {
+            tmem_wait(r[c & 1]);
+            if (c + 1 < L::CW / 32) {
+              tmem_ld32(lane_base + b * BN + 32 * (c + 1), r[(c + 1) & 1]);
+            } else {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) bar_arrive(acce0 + 8 * b);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              acc[16 * c + i] = fma2(pack2(__uint_as_float(r[c & 1][2 * i]), __uint_as_float(r[c & 1][2 * i + 1])), s2,
+                                     acc[16 * c + i]);
+          }
+        }
+        if (!ok) break;
+        if constexpr (SPLIT) {
+          // the sums as [column][token], one column further than the tokens apart: neither the lanes of this store
+          // (tokens) nor those of the reduction (columns) meet in a bank.  The stages are free: every MMA that read
+          // them has been waited for.
+          const uint32_t pitch = 4u * (32 * quarters + 1);
+          const uint32_t at = base + (uint32_t)(32 * q + lane) * 4;
+#pragma unroll
+          for (int i = 0; i < L::CW / 2; ++i) {
+            const float2 f = unpack2(acc[i]);
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + (c0 + 2 * i) * pitch), "f"(f.x) : "memory");
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + (c0 + 2 * i + 1) * pitch), "f"(f.y) : "memory");
+          }
+        } else if (p.tma_store) {
+          // 128 bytes of each of the warp's 32 tokens at a time, in the 128-byte swizzle, stored by TMA, which
+          // leaves out rows past T and columns past N
+          const uint32_t buf = tail + (uint32_t)warp * 4096;
+          const int per = p.y_dtype == SF_F32 ? 32 : 64;
+#pragma unroll
+          for (int g = 0; g < L::CW / 32; ++g) {
+            if (per == 64 && (g & 1)) continue;
+            if (n0 + c0 + 32 * g >= p.N) break;
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              uint32_t w[4];
+              if (per == 32) {
+                const float2 f0 = unpack2(acc[16 * g + 2 * j]), f1 = unpack2(acc[16 * g + 2 * j + 1]);
+                float v[4] = {f0.x, f0.y, f1.x, f1.y};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const int n = n0 + c0 + 32 * g + 4 * j + e;
+                  if (p.bias && n < p.N) v[e] += __ldg(p.bias + n);
+                  w[e] = __float_as_uint(v[e]);
+                }
+              } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  float2 f = unpack2(acc[(16 * g + 4 * j + e) % (L::CW / 2)]);
+                  const int n = n0 + c0 + 32 * g + 8 * j + 2 * e;
+                  if (p.bias && n < p.N) f.x += __ldg(p.bias + n);
+                  if (p.bias && n + 1 < p.N) f.y += __ldg(p.bias + n + 1);
+                  w[e] = pack16(f.x, f.y, p.y_dtype);
+                }
+              }
+              asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(buf + lane * 128 + ((j ^ (lane & 7)) << 4)),
+                           "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                           : "memory");
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0 && m0 + 32 * q < p.T) tma_store(&mapY, n0 + c0 + 32 * g, m0 + 32 * q, buf);
+          }
+        } else if (t < p.T) {
+#pragma unroll
+          for (int i = 0; i < L::CW / 2; ++i) {
+            const float2 f = unpack2(acc[i]);
+            const int n = n0 + c0 + 2 * i;
+            if (n < p.N) store_y(p.Y, (size_t)t * p.N + n, f.x + (p.bias ? __ldg(p.bias + n) : 0.f), p.y_dtype);
+            if (n + 1 < p.N) store_y(p.Y, (size_t)t * p.N + n + 1, f.y + (p.bias ? __ldg(p.bias + n + 1) : 0.f), p.y_dtype);
+          }
+        }
+      }
+      if (!SPLIT && p.tma_store && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::TMEM_COLS) : "memory");
+  }
+  if constexpr (SPLIT) {
+    // ---------------- the cluster's sums ----------------
+    cluster_sync();
+    const int m0 = (tile0 % p.mtiles) * 128, n0 = (tile0 / p.mtiles) * BN;
+    const int cols = BN / p.split, rows = min(p.rows, p.T - m0);
+    const uint32_t pitch = 4u * (32 * quarters + 1);
+    for (int i = threadIdx.x; i < cols * rows; i += kThreads) {
+      const int c = rank * cols + i % cols, t = i / cols, n = n0 + c;
+      if (n >= p.N) continue;
+      const uint32_t at = base + (uint32_t)c * pitch + 4u * t;
+      float v = 0.f;
+#pragma unroll 8
+      for (int r = 0; r < p.split; ++r) v += ld_cluster(at, r);
+      store_y(p.Y, (size_t)(m0 + t) * p.N + n, v + (p.bias ? __ldg(p.bias + n) : 0.f), p.y_dtype);
+    }
+    cluster_sync();   // no CTA leaves while another reads its sums
+  }
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  });
+  return fn;
+}
+bool make_map(CUtensorMap* m, CUtensorMapDataType dt, const void* base, uint64_t inner, uint64_t rows, uint64_t pitch,
+              uint32_t box_inner, uint32_t box_rows) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {inner, rows};
+  const cuuint64_t strides[1] = {pitch};
+  const cuuint32_t box[2] = {box_inner, box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  return fn(m, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool SPLIT>
+cudaError_t launch(const CUtensorMap& mx, const CUtensorMap& mw, const CUtensorMap& my, const Fp8Params& p, int grid,
+                   cudaStream_t st) {
+  auto* fn = fp8_linear_kernel<SPLIT>;
+  const size_t smem = Plan<SPLIT>::bytes(p.rows, p.stages);
+  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)p.split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.split > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, fn, mx, mw, my, p);
 }
 
 }  // namespace
@@ -73,10 +518,46 @@ extern "C" int sf_fp8_linear(const uint8_t* X, long long ldx, const float* xs, c
   if (ldx < K || ldw < K) return fail(SF_ERR_SHAPE, "a row stride is below K");
   if (((reinterpret_cast<uintptr_t>(X) | reinterpret_cast<uintptr_t>(W)) & 15) || ldx % 16 || ldw % 16)
     return fail(SF_ERR_ALIGN, "X and W must start at multiples of 16 bytes and have row strides that are multiples of 16");
-  const Fp8Args a{X, W, xs, ws, bias, Y, ldx, ldw, T, N, K, y_dtype};
-  const dim3 grid((unsigned)((N + 63) / 64), (unsigned)((T + 63) / 64));
-  fp8_linear_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(a);
-  const cudaError_t e = cudaGetLastError();
+  DeviceInfo& di = device_info();
+  Fp8Params p{};
+  p.xs = xs; p.ws = ws; p.bias = bias; p.Y = Y;
+  p.T = T; p.N = N; p.KB = (K + kBK - 1) / kBK; p.y_dtype = y_dtype;
+  p.mtiles = (T + 127) / 128;
+  p.rows = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
+  // 128 x 256 tiles on every SM when there are enough of them, else 128 x 128 tiles with K cut until the SMs are busy
+  const bool split = (long long)p.mtiles * ((N + 255) / 256) < di.sms;
+  const int BN = split ? 128 : 256;
+  p.ntiles = (N + BN - 1) / BN;
+  if ((long long)p.mtiles * p.ntiles > (1 << 28)) return fail(SF_ERR_UNSUPPORTED, "too many tiles");
+  const int tiles = p.mtiles * p.ntiles;
+  p.split = 1;
+  if (split)
+    while (p.split < 8 && tiles * p.split * 2 <= 2 * di.sms && p.KB >= 2 * 2 * p.split) p.split *= 2;
+  CUtensorMap mx, mw, my;
+  memset(&my, 0, sizeof(my));
+  if (!make_map(&mx, CU_TENSOR_MAP_DATA_TYPE_UINT8, X, (uint64_t)K, (uint64_t)T, (uint64_t)ldx, kBK, (uint32_t)p.rows) ||
+      !make_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, W, (uint64_t)K, (uint64_t)N, (uint64_t)ldw, kBK, (uint32_t)BN))
+    return fail(SF_ERR_CUDA, "cuTensorMapEncodeTiled failed (T=%d N=%d K=%d)", T, N, K);
+  cudaError_t e;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (split) {
+    using L = Plan<true>;
+    // two CTAs fit an SM; the cluster's sums (128 columns of up to 129 floats) fit the stages
+    const int most = (int)((kSmemLimit / 2 - 1024 - 1024 - L::CTL) / L::stage(p.rows));
+    p.stages = most > L::MAX_STAGES ? L::MAX_STAGES : most;
+    e = launch<true>(mx, mw, my, p, tiles * p.split, st);
+  } else {
+    using L = Plan<false>;
+    p.stages = 4;
+    const int es = y_dtype == SF_F32 ? 4 : 2;
+    p.tma_store = reinterpret_cast<uintptr_t>(Y) % 16 == 0 && (size_t)N * es % 16 == 0 &&
+                  make_map(&my, y_dtype == SF_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                : y_dtype == SF_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                     : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                           Y, (uint64_t)N, (uint64_t)T, (uint64_t)N * es, 128 / es, 32);
+    static_assert(L::bytes(128, 4) <= (size_t)kSmemLimit, "shared memory plan");
+    e = launch<false>(mx, mw, my, p, tiles < di.sms ? tiles : di.sms, st);
+  }
   if (e != cudaSuccess) return cuda_fail(e, "fp8_linear_kernel launch");
   g_launches.fetch_add(1, std::memory_order_relaxed);
   return SF_OK;

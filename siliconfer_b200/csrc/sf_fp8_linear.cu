@@ -32,7 +32,7 @@ extern std::atomic<long long> g_launches;
 namespace {
 
 constexpr int kBK = 128;                // k per stage: one 128-byte swizzle row, and one block of scales
-constexpr int kSumWarps = 8, kProdWarp = 8, kMmaWarp = 9, kThreads = 320;
+constexpr int kSumWarps = 8, kProdWarp = 8, kMmaWarp = 9;
 constexpr int kSmemLimit = 232448;      // 227 KB opt-in per block
 constexpr unsigned kErrProd = 1u << 13, kErrMma = 1u << 14, kErrSum = 1u << 15, kErrDrain = 1u << 16;
 
@@ -135,8 +135,17 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 
-// 32 fp32 columns of this warp's 32 TMEM lanes; the registers hold them after tmem_wait on the same array.
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+// C fp32 columns of this warp's 32 TMEM lanes; the registers hold them after tmem_wait on the same array.
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+        "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
       "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
@@ -147,6 +156,13 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
         "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
         "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
 }
 __device__ __forceinline__ void tmem_wait(uint32_t (&r)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
@@ -179,12 +195,10 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float ld_cluster(uint32_t saddr, uint32_t rank) {
+__device__ __forceinline__ void st_cluster(uint32_t saddr, uint32_t rank, float v) {
   uint32_t a;
-  float v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(saddr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-  return v;
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
 }
 
 __device__ __forceinline__ void store_y(void* Y, size_t o, float v, int dt) {
@@ -208,6 +222,12 @@ struct Plan {
   static constexpr int NBUF = 2;
   static constexpr uint32_t TMEM_COLS = NBUF * BN;
   static constexpr int CW = BN / 2;                      // columns of a summing warp
+  static constexpr int CH = SPLIT ? 16 : 32;             // columns it reads at a time
+  static constexpr int NR = SPLIT ? 1 : 2;               // reads in flight
+  static constexpr int LA = SPLIT ? 2 : 4;               // k-blocks whose scales are loaded ahead
+  // The persistent kernel has a third warpgroup so that setmaxnreg can move registers from it to the summing warps,
+  // which keep 128 sums each: launched with 384 x 168 = 64512, then 256 x 232 + 128 x 40 = 64512.
+  static constexpr int THREADS = SPLIT ? 320 : 384;
   static constexpr uint32_t W = BN * kBK;
   static constexpr uint32_t CTL = 512;
   static constexpr uint32_t TAIL = SPLIT ? 0 : kSumWarps * 4096;
@@ -217,11 +237,11 @@ struct Plan {
 };
 
 template <bool SPLIT>
-__global__ void __launch_bounds__(kThreads, SPLIT ? 2 : 1)
+__global__ void __launch_bounds__(Plan<SPLIT>::THREADS, SPLIT ? 2 : 1)
     fp8_linear_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__ CUtensorMap mapW,
                       const __grid_constant__ CUtensorMap mapY, const Fp8Params p) {
   using L = Plan<SPLIT>;
-  constexpr int BN = L::BN, NBUF = L::NBUF;
+  constexpr int BN = L::BN, NBUF = L::NBUF, CW = L::CW, CH = L::CH;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -236,6 +256,7 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 2 : 1)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int S = p.stages;
+  griddep_launch_dependents();
   // lane quarters that hold tokens: their two warps each release an accumulator buffer
   const int quarters = SPLIT ? (p.rows + 31) / 32 : 4;
   if (threadIdx.x == 0) {
@@ -266,6 +287,7 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 2 : 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  griddep_wait();   // the set-up above runs beside the end of the kernel before; memory is touched from here on
 
   const int ntiles = p.mtiles * p.ntiles;
   const int rank = SPLIT ? (int)(blockIdx.x % p.split) : 0;
@@ -274,56 +296,77 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 2 : 1)
   const int tile0 = SPLIT ? (int)(blockIdx.x / p.split) : (int)blockIdx.x;
   const int tile_step = SPLIT ? ntiles : (int)gridDim.x;   // the split kernel has one tile
 
-  if (warp == kProdWarp) {
-    // ---------------- TMA producer ----------------
-    if (lane == 0) {
-      uint32_t it = 0;
-      bool ok = true;
-      for (int tile = tile0; tile < ntiles && ok; tile += tile_step) {
-        const int m0 = (tile % p.mtiles) * 128, n0 = (tile / p.mtiles) * BN;
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const uint32_t s = it % S, ph = (it / S) & 1;
-          if (!bar_wait(empty0 + 8 * s, ph ^ 1, kErrProd, abort_flag)) { ok = false; break; }
-          const uint32_t st = base + s * stage_bytes;
-          bar_expect_tx(full0 + 8 * s, stage_bytes);
-          tma_load(st, &mapX, kb * kBK, m0, full0 + 8 * s);
-          tma_load(st + xbytes, &mapW, kb * kBK, n0, full0 + 8 * s);
+  // Ends a role: all MMAs and copies of the block are done (of the cluster, before its sums are exchanged).
+  const auto meet = [&] {
+    tc_fence_before();
+    __syncthreads();
+    if (SPLIT && p.split > 1) cluster_sync();
+  };
+  const uint32_t pitch = 4u * (32 * quarters + 1);   // of the exchanged sums, below
+  const int cols = SPLIT ? BN / p.split : BN, lg_cols = 31 - __clz(cols);
+
+  if (warp >= kProdWarp) {
+    // one instruction for the warpgroup
+    if (!SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == kProdWarp) {
+      // ---------------- TMA producer ----------------
+      if (lane == 0) {
+        uint32_t it = 0;
+        bool ok = true;
+        for (int tile = tile0; tile < ntiles && ok; tile += tile_step) {
+          const int m0 = (tile % p.mtiles) * 128, n0 = (tile / p.mtiles) * BN;
+          for (int kb = kb0; kb < kb1; ++kb, ++it) {
+            const uint32_t s = it % S, ph = (it / S) & 1;
+            if (!bar_wait(empty0 + 8 * s, ph ^ 1, kErrProd, abort_flag)) { ok = false; break; }
+            const uint32_t st = base + s * stage_bytes;
+            bar_expect_tx(full0 + 8 * s, stage_bytes);
+            tma_load(st, &mapX, kb * kBK, m0, full0 + 8 * s);
+            tma_load(st + xbytes, &mapW, kb * kBK, n0, full0 + 8 * s);
+          }
         }
+        // every issued copy has landed before the block goes on
+        const uint32_t pending = it < (uint32_t)S ? it : (uint32_t)S;
+        for (uint32_t j = it - pending; j < it; ++j) bar_drain(full0 + 8 * (j % S), (j / S) & 1);
       }
-      // every issued copy has landed before the block goes on
-      const uint32_t pending = it < (uint32_t)S ? it : (uint32_t)S;
-      for (uint32_t j = it - pending; j < it; ++j) bar_drain(full0 + 8 * (j % S), (j / S) & 1);
-    }
-  } else if (warp == kMmaWarp) {
-    // ---------------- MMA issuer ----------------
-    if (lane == 0) {
-      const uint32_t idesc = idesc_e4m3(128, BN);
-      uint32_t it = 0;
-      bool ok = true;
-      for (int tile = tile0; tile < ntiles && ok; tile += tile_step) {
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const uint32_t s = it % S, ph = (it / S) & 1, b = it % NBUF, use = it / NBUF;
-          if (!bar_wait(acce0 + 8 * b, (use & 1) ^ 1, kErrMma, abort_flag) ||
-              !bar_wait(full0 + 8 * s, ph, kErrMma, abort_flag)) { ok = false; break; }
-          tc_fence_after();
-          const uint32_t st = base + s * stage_bytes;
-#pragma unroll
-          for (int kk = 0; kk < kBK / 32; ++kk)
-            mma_e4m3(tmem + b * BN, sw128_desc(st + kk * 32), sw128_desc(st + xbytes + kk * 32), idesc, kk != 0);
-          mma_commit(empty0 + 8 * s);
-          mma_commit(accf0 + 8 * b);
+      __syncwarp();
+      meet();
+    } else if (warp == kMmaWarp) {
+      // ---------------- MMA issuer ----------------
+      if (lane == 0) {
+        const uint32_t idesc = idesc_e4m3(128, BN);
+        uint32_t it = 0;
+        bool ok = true;
+        for (int tile = tile0; tile < ntiles && ok; tile += tile_step) {
+          for (int kb = kb0; kb < kb1; ++kb, ++it) {
+            const uint32_t s = it % S, ph = (it / S) & 1, b = it % NBUF, use = it / NBUF;
+            if (!bar_wait(acce0 + 8 * b, (use & 1) ^ 1, kErrMma, abort_flag) ||
+                !bar_wait(full0 + 8 * s, ph, kErrMma, abort_flag)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t st = base + s * stage_bytes;
+  #pragma unroll
+            for (int kk = 0; kk < kBK / 32; ++kk)
+              mma_e4m3(tmem + b * BN, sw128_desc(st + kk * 32), sw128_desc(st + xbytes + kk * 32), idesc, kk != 0);
+            mma_commit(empty0 + 8 * s);
+            mma_commit(accf0 + 8 * b);
+          }
         }
+        // every issued MMA has completed before TMEM is freed
+        mma_commit(drain);
+        bar_drain(drain, 0);
       }
-      // every issued MMA has completed before TMEM is freed
-      mma_commit(drain);
-      bar_drain(drain, 0);
+      __syncwarp();
+      meet();
+    } else {
+      meet();
     }
   } else {
     // ---------------- scaled sums ----------------
     // Warp w: tokens 32 (w % 4) .. of the tile, columns CW (w / 4) .. (inside one 128-column block of ws).
-    const int q = warp & 3, c0 = (warp >> 2) * L::CW;
+    if (!SPLIT) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    const int q = warp & 3, c0 = (warp >> 2) * CW;
     const uint32_t lane_base = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)c0;
     uint32_t it = 0;
+    uint64_t acc[CW / 2];
     if (q < quarters) {
       for (int tile = tile0; tile < ntiles; tile += tile_step) {
         const int m0 = (tile % p.mtiles) * 128, n0 = (tile / p.mtiles) * BN;
@@ -331,52 +374,56 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 2 : 1)
         const bool in = t < p.T && nb * 128 < p.N;
         const float* xrow = p.xs + (size_t)(in ? t : 0) * p.KB;
         const float* wrow = p.ws + (size_t)(in ? nb : 0) * p.KB;
-        uint64_t acc[L::CW / 2];
 #pragma unroll
-        for (int i = 0; i < L::CW / 2; ++i) acc[i] = 0;
-        float sx = __ldg(xrow + kb0), sw = __ldg(wrow + kb0);
-        bool ok = true;
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const uint32_t b = it % NBUF, use = it / NBUF;
-          const float s = sx * sw;
-          const uint64_t s2 = pack2(s, s);
-          if (kb + 1 < kb1) {
-            sx = __ldg(xrow + kb + 1);
-            sw = __ldg(wrow + kb + 1);
+        for (int i = 0; i < CW / 2; ++i) acc[i] = 0;
+        // the scales of the next LA k-blocks are loaded while these are used: the rows of a full tile are too many
+        // for what shared memory leaves of L1
+        constexpr int LA = L::LA;
+        float s4[LA], x4[LA], w4[LA];
+        const auto fetch = [&](int kb) {
+#pragma unroll
+          for (int i = 0; i < LA; ++i) {
+            const int k = min(kb + i, kb1 - 1);
+            x4[i] = __ldg(xrow + k);
+            w4[i] = __ldg(wrow + k);
           }
-          if (!bar_wait(accf0 + 8 * b, use & 1, kErrSum, abort_flag)) { ok = false; break; }
-          tc_fence_after();
-          uint32_t r[2][32];
-          tmem_ld32(lane_base + b * BN, r[0]);
+        };
+        fetch(kb0);
+        bool ok = true;
+        for (int kb = kb0; kb < kb1 && ok; kb += LA) {
 #pragma unroll
-          for (int c = 0; c < L::CW / 32; ++c) {
-            tmem_wait(r[c & 1]);
-            if (c + 1 < L::CW / 32) {
-              tmem_ld32(lane_base + b * BN + 32 * (c + 1), r[(c + 1) & 1]);
-            } else {
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) bar_arrive(acce0 + 8 * b);
+          for (int i = 0; i < LA; ++i) s4[i] = x4[i] * w4[i];
+          fetch(kb + LA);
+#pragma unroll
+          for (int i = 0; i < LA; ++i) {
+            if (kb + i >= kb1) break;
+            const uint32_t b = it % NBUF, use = it / NBUF;
+            ++it;
+            const uint64_t s2 = pack2(s4[i], s4[i]);
+            if (!bar_wait(accf0 + 8 * b, use & 1, kErrSum, abort_flag)) { ok = false; break; }
+            tc_fence_after();
+            uint32_t r[L::NR][CH];
+            tmem_ld(lane_base + b * BN, r[0]);
+#pragma unroll
+            for (int c = 0; c < CW / CH; ++c) {
+              tmem_wait(r[c % L::NR]);
+              if (L::NR == 2 && c + 1 < CW / CH) tmem_ld(lane_base + b * BN + CH * (c + 1), r[(c + 1) % L::NR]);
+              if (c + 1 == CW / CH) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(acce0 + 8 * b);
+              }
+#pragma unroll
+              for (int e = 0; e < CH / 2; ++e)
+                acc[CH / 2 * c + e] = fma2(pack2(__uint_as_float(r[c % L::NR][2 * e]),
+                                                 __uint_as_float(r[c % L::NR][2 * e + 1])), s2, acc[CH / 2 * c + e]);
+              if (L::NR == 1 && c + 1 < CW / CH) tmem_ld(lane_base + b * BN + CH * (c + 1), r[0]);
             }
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              acc[16 * c + i] = fma2(pack2(__uint_as_float(r[c & 1][2 * i]), __uint_as_float(r[c & 1][2 * i + 1])), s2,
-                                     acc[16 * c + i]);
           }
         }
         if (!ok) break;
         if constexpr (SPLIT) {
-          // the sums as [column][token], one column further than the tokens apart: neither the lanes of this store
-          // (tokens) nor those of the reduction (columns) meet in a bank.  The stages are free: every MMA that read
-          // them has been waited for.
-          const uint32_t pitch = 4u * (32 * quarters + 1);
-          const uint32_t at = base + (uint32_t)(32 * q + lane) * 4;
-#pragma unroll
-          for (int i = 0; i < L::CW / 2; ++i) {
-            const float2 f = unpack2(acc[i]);
-            asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + (c0 + 2 * i) * pitch), "f"(f.x) : "memory");
-            asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + (c0 + 2 * i + 1) * pitch), "f"(f.y) : "memory");
-          }
+          // stored below, when the cluster's stages are free
         } else if (p.tma_store) {
           // 128 bytes of each of the warp's 32 tokens at a time, in the 128-byte swizzle, stored by TMA, which
           // leaves out rows past T and columns past N
@@ -430,30 +477,46 @@ __global__ void __launch_bounds__(kThreads, SPLIT ? 2 : 1)
       }
       if (!SPLIT && p.tma_store && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
+    __syncwarp();
+    meet();
+    if (SPLIT && q < quarters && 32 * q + lane < p.rows) {
+      // To the CTA of the cluster that adds this column: [rank][column][token], one float further than the tokens
+      // apart, so that neither the lanes here (tokens) nor those of the addition (columns) meet in a bank.
+      const uint32_t at = base + (uint32_t)(32 * q + lane) * 4;
+#pragma unroll
+      for (int i = 0; i < CW; ++i) {
+        const int c = c0 + i;
+        const float2 f = unpack2(acc[i / 2]);
+        const uint32_t o = at + (uint32_t)(rank * cols + (c & (cols - 1))) * pitch;
+        if (p.split > 1) st_cluster(o, (uint32_t)(c >> lg_cols), i & 1 ? f.y : f.x);
+        else asm volatile("st.shared.f32 [%0], %1;" ::"r"(o), "f"(i & 1 ? f.y : f.x) : "memory");
+      }
+    }
   }
 
-  tc_fence_before();
-  __syncthreads();
   if (warp == kMmaWarp) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::TMEM_COLS) : "memory");
   }
   if constexpr (SPLIT) {
-    // ---------------- the cluster's sums ----------------
-    cluster_sync();
-    const int m0 = (tile0 % p.mtiles) * 128, n0 = (tile0 / p.mtiles) * BN;
-    const int cols = BN / p.split, rows = min(p.rows, p.T - m0);
-    const uint32_t pitch = 4u * (32 * quarters + 1);
-    for (int i = threadIdx.x; i < cols * rows; i += kThreads) {
-      const int c = rank * cols + i % cols, t = i / cols, n = n0 + c;
+    // ---------------- the cluster's sums, in rank order ----------------
+    __syncwarp();
+    if (p.split > 1) cluster_sync();
+    else __syncthreads();
+    const int m0 = (tile0 % p.mtiles) * 128, n0 = (tile0 / p.mtiles) * BN + rank * cols;
+    const int rows = min(p.rows, p.T - m0);
+    const float* sums = reinterpret_cast<const float*>(smem_raw + (base - raw));
+    const int step = cols * (int)(pitch / 4);
+    for (int i = threadIdx.x; i < cols * rows; i += L::THREADS) {
+      const int c = i & (cols - 1), t = i >> lg_cols, n = n0 + c;
       if (n >= p.N) continue;
-      const uint32_t at = base + (uint32_t)c * pitch + 4u * t;
+      const float* at = sums + c * (int)(pitch / 4) + t;
       float v = 0.f;
-#pragma unroll 8
-      for (int r = 0; r < p.split; ++r) v += ld_cluster(at, r);
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < p.split) v += at[r * step];
       store_y(p.Y, (size_t)(m0 + t) * p.N + n, v + (p.bias ? __ldg(p.bias + n) : 0.f), p.y_dtype);
     }
-    cluster_sync();   // no CTA leaves while another reads its sums
   }
 }
 
@@ -491,15 +554,17 @@ cudaError_t launch(const CUtensorMap& mx, const CUtensorMap& mw, const CUtensorM
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(Plan<SPLIT>::THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)p.split;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)p.split;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = p.split > 1 ? 1 : 0;
+  cfg.numAttrs = p.split > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, fn, mx, mw, my, p);
 }
 

@@ -199,6 +199,32 @@ def test_non_finite_values_stay_in_their_rows(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_values_that_a_row_does_not_see_cannot_reach_it(cuda, D, dtype):
+    """NaN keys and values of later tokens of the same call, and of tokens before a row's window."""
+    from siliconfer_b200.paged_kv import paged_attention
+    b = Batch([90], [60], 8, 2, D, 16, dtype)
+    ref, _, vmax = b.ref(window=10)
+    k, v = b.k.view(torch.uint8), b.v.view(torch.uint8)
+    for at in (40, 47, 70):
+        k[b.table[0, at // 16], 1, at % 16] = 0x7f
+        v[b.table[0, at // 16], 1, at % 16, 3] = 0xff
+        v[b.table[0, at // 16], 0, at % 16, D - 1] = 0x7f
+    out = paged_attention(b.q, *b.args(), starts=b.starts, window=10)
+    pos = torch.arange(30, 90, device="cuda")
+    sees = torch.zeros(60, dtype=torch.bool, device="cuda")
+    for at in (40, 47, 70):
+        sees |= (pos >= at) & (pos < at + 10)
+    bad = torch.zeros_like(out, dtype=torch.bool)
+    bad[sees, 4:] = True
+    bad[sees, :4, D - 1] = True
+    assert torch.equal(out.isnan(), bad)
+    assert (~sees).sum() > 5
+    assert ((out.double() - ref).abs()[~bad] <= 2.0 ** -10 * vmax + 2.0 ** -8 * ref.abs()[~bad]).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("H,Hkv", [(8, 2), (32, 4)])
 def test_strided_queries_types_and_repeats(cuda, H, Hkv):
     b = Batch([300, 1000, 90], [1, 4, 2], H, Hkv, 128, 64, torch.bfloat16)

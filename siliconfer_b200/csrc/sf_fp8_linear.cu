@@ -14,16 +14,13 @@
 //    spread the weight read over the SMs, in one launch and with the same result every time.  With few tokens only
 //    the rows that exist are loaded; what the MMA reads above them ends in TMEM lanes that nothing looks at.
 //  * persistent: 128 x 256 tiles in turn on one CTA per SM, stored through shared memory by TMA.
-#include <cuda.h>
-#include <cudaTypedefs.h>
-
 #include <atomic>
 #include <cstdint>
 #include <cstring>
-#include <mutex>
 
 #include "sf_e4m3.h"
 #include "sf_q4_internal.h"
+#include "sf_tcgen05.h"
 
 namespace sf {
 SF_DEFINE_ERROR_READER(take_dev_error_fp8)
@@ -49,130 +46,9 @@ struct Fp8Params {
   int tma_store;
 };
 
-// ---------------------------------------------------------------------------
-// PTX wrappers
-// ---------------------------------------------------------------------------
-__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity), "r"(20000u)
-      : "memory");
-  return ok != 0;
-}
-// Bounded wait that also gives up when another role raised the abort flag.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, unsigned code, volatile int* abort_flag) {
-  if (bar_try(bar, parity)) return true;
-  const long long t0 = clock64();
-  while (!bar_try(bar, parity)) {
-    if (*abort_flag) return false;
-    if (clock64() - t0 > kWaitCycles) {
-      atomicOr(&g_dev_error, code);
-      *abort_flag = 1;
-      return false;
-    }
-  }
-  return true;
-}
-// Bounded wait for something that is under way whatever the others do.
-__device__ __forceinline__ void bar_drain(uint32_t bar, uint32_t parity) {
-  if (bar_try(bar, parity)) return;
-  const long long t0 = clock64();
-  while (!bar_try(bar, parity))
-    if (clock64() - t0 > kWaitCycles) {
-      atomicOr(&g_dev_error, kErrDrain);
-      return;
-    }
-}
-__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-__device__ __forceinline__ void bar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void bar_expect_tx(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-      "l"(map), "r"(x), "r"(y), "r"(bar)
-      : "memory");
-}
-__device__ __forceinline__ void tma_store(const CUtensorMap* map, int x, int y, uint32_t src) {
-  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y),
-               "r"(src)
-               : "memory");
-  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-}
-
-// Shared-memory matrix descriptor of a K-major tile with 128-byte rows in the 128-byte swizzle (8-row atoms of 1024
-// bytes).  32 k (32 bytes) further inside the atom adds 2 to the start-address field.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
-  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-// Instruction descriptor of kind::f8f6f4: D fp32 (bits 4-5 = 1), A and B e4m3 (0), both K-major, N >> 3 in bits
-// 17-22, M >> 4 in bits 24-28.
-__host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N) {
-  return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
-}
-__device__ __forceinline__ void mma_e4m3(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void mma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-
-// C fp32 columns of this warp's 32 TMEM lanes; the registers hold them after tmem_wait on the same array.
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
-        "=r"(r[15])
-      : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
-        "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
-        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
-        "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-               :
-               : "memory");
-}
-__device__ __forceinline__ void tmem_wait(uint32_t (&r)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
-                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
-                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
-               :
-               : "memory");
-}
+// K-major tile of 128-byte rows in the 128-byte swizzle (8-row atoms of 1024 bytes); 32 k further inside the atom are
+// 32 bytes of the start address.
+__device__ __forceinline__ uint64_t rows128_desc(uint32_t saddr) { return smem_desc(saddr, 16, 1024, kSw128); }
 
 // Two fp32 lanes per instruction.
 __device__ __forceinline__ uint64_t pack2(float lo, float hi) {
@@ -273,15 +149,11 @@ __global__ void __launch_bounds__(Plan<SPLIT>::THREADS, SPLIT ? 2 : 1)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kProdWarp && lane == 0) {
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&mapX) : "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&mapW) : "memory");
+    prefetch_map(&mapX);
+    prefetch_map(&mapW);
   }
   if (warp == kMmaWarp) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                     smem_u32((const void*)tmem_slot)),
-                 "r"(L::TMEM_COLS)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    tmem_alloc(smem_u32((const void*)tmem_slot), L::TMEM_COLS);
   }
   tc_fence_before();
   __syncthreads();
@@ -326,7 +198,7 @@ __global__ void __launch_bounds__(Plan<SPLIT>::THREADS, SPLIT ? 2 : 1)
         }
         // every issued copy has landed before the block goes on
         const uint32_t pending = it < (uint32_t)S ? it : (uint32_t)S;
-        for (uint32_t j = it - pending; j < it; ++j) bar_drain(full0 + 8 * (j % S), (j / S) & 1);
+        for (uint32_t j = it - pending; j < it; ++j) bar_drain(full0 + 8 * (j % S), (j / S) & 1, kErrDrain);
       }
       __syncwarp();
       meet();
@@ -345,14 +217,14 @@ __global__ void __launch_bounds__(Plan<SPLIT>::THREADS, SPLIT ? 2 : 1)
             const uint32_t st = base + s * stage_bytes;
   #pragma unroll
             for (int kk = 0; kk < kBK / 32; ++kk)
-              mma_e4m3(tmem + b * BN, sw128_desc(st + kk * 32), sw128_desc(st + xbytes + kk * 32), idesc, kk != 0);
+              mma_f8(tmem + b * BN, rows128_desc(st + kk * 32), rows128_desc(st + xbytes + kk * 32), idesc, kk != 0);
             mma_commit(empty0 + 8 * s);
             mma_commit(accf0 + 8 * b);
           }
         }
         // every issued MMA has completed before TMEM is freed
         mma_commit(drain);
-        bar_drain(drain, 0);
+        bar_drain(drain, 0, kErrDrain);
       }
       __syncwarp();
       meet();
@@ -461,7 +333,7 @@ __global__ void __launch_bounds__(Plan<SPLIT>::THREADS, SPLIT ? 2 : 1)
                            "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
                            : "memory");
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            fence_async_smem();
             __syncwarp();
             if (lane == 0 && m0 + 32 * q < p.T) tma_store(&mapY, n0 + c0 + 32 * g, m0 + 32 * q, buf);
           }
@@ -496,7 +368,7 @@ __global__ void __launch_bounds__(Plan<SPLIT>::THREADS, SPLIT ? 2 : 1)
 
   if (warp == kMmaWarp) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::TMEM_COLS) : "memory");
+    tmem_free(tmem, L::TMEM_COLS);
   }
   if constexpr (SPLIT) {
     // ---------------- the cluster's sums, in rank order ----------------
@@ -520,29 +392,9 @@ __global__ void __launch_bounds__(Plan<SPLIT>::THREADS, SPLIT ? 2 : 1)
   }
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
-  });
-  return fn;
-}
 bool make_map(CUtensorMap* m, CUtensorMapDataType dt, const void* base, uint64_t inner, uint64_t rows, uint64_t pitch,
               uint32_t box_inner, uint32_t box_rows) {
-  auto fn = encode_fn();
-  if (!fn) return false;
-  const cuuint64_t dims[2] = {inner, rows};
-  const cuuint64_t strides[1] = {pitch};
-  const cuuint32_t box[2] = {box_inner, box_rows};
-  const cuuint32_t estr[2] = {1, 1};
-  return fn(m, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return make_tensor_map(m, dt, base, inner, rows, pitch, box_inner, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <bool SPLIT>

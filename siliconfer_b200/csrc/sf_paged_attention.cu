@@ -1,26 +1,29 @@
-// sf_paged_attention.cu -- attention over the pages of an e4m3 cache.
+// sf_paged_attention.cu -- attention over the pages of an e4m3 cache on the sm_100a tcgen05 tensor cores.
 //
 //   p_j = softmax_j(scale * q . k_j),  out = sum_j p_j v_j,  k_j = code * scale of its page and head
 //
-// The softmax keeps a running maximum m and sum l: keys in order, out and l are multiplied by e^(m - m') when the
-// maximum grows to m'.  Parts of a row's keys merge by the same rule.
+// The softmax keeps a running reference m and sum l: keys in order, out and l are multiplied by e^(m - m') when the
+// reference grows to m'.  Parts of a row's keys merge by the same rule.  m is the largest score plus the logarithm of
+// its page's V scale, so that a weight times that scale is at most 1.
 //
-// A call's work is a list of units of 4 * WB keys, for each (sequence, kv head, tile of query rows) in turn; a row is
+// A call's work is a list of units of 128 keys, for each (sequence, kv head, tile of RT query rows) in turn; a row is
 // one (new token, query head of the kv head's group), so that a group reads its keys once.  Every CTA takes an equal,
 // contiguous share of that list, whatever the sequences' lengths: it finds its place from a prefix sum over the
 // batch.  A CTA that holds all of a tile's units writes the result; the others leave their parts in the workspace,
 // which a second kernel merges.
 //
-// Per warp, WB keys at a time, on mma.sync m16n8k16 (fp16 in, fp32 sums):
-//  * S = Q K^T, rows of the tile by keys.  K's codes become fp16 exactly; its fragments are 32-bit words of a key's
-//    row, for which the 16 columns of an MMA are taken in the order 4t .. 4t+3 per lane t, in Q and in K alike.
-//  * O += P V with P's accumulators as the next MMA's operand.  A lane's words of four keys, byte-transposed, are its
-//    fragments for four 8-column tiles: column g of tile j is column 4g + j of each 32.
-//  * Tiles of at most 8 rows put a row's high part in MMA row g and its low part in row g + 8: queries and weights
-//    keep 22 bits for the price of the padding that 16 rows would be.  Tiles of 16 rows (16-bit queries, which fp16
-//    holds exactly after a power-of-two scaling of each row) round weights to 11 bits.
-//  * V's scales fold into P relative to the largest one met (exact: powers of two), times 2^10 to keep small weights
-//    clear of fp16's subnormals.
+// Both products run on the codes as they lie in the cache (kind::f8f6f4), and no code is ever converted:
+//  * S^T[key, column] = K Q^T: 128 keys are the MMA's rows.  A query row is scaled by a power of two to at most 256 and
+//    cut into e4m3 parts of 4 bits each, 2^4 apart; each part is a column, so its sums are exact on their own and are
+//    added, scaled, in fp32.  2 parts hold a bf16 row, 3 an fp16 row, 6 an fp32 row (24 bits; elements far below the
+//    row's largest lose what lies under 2^-17, 2^-21 or 2^-33 of it).
+//  * out^T[d, column] = V^T P^T: the head's columns are the MMA's rows, V is its transposed operand.  Weights are cut
+//    into as many parts as queries: 8, 12 or 24 bits, and no coarser than 2^-22 of the largest for bf16.
+// Both scores and partial sums go to fresh TMEM buffers, two each; a thread is one key for the scores and one column d
+// for the sums, which it keeps in registers in fp32.
+//
+// Warps 0-3: softmax and sums.  Warp 4: TMA copies of pages.  Warp 5: MMAs.  Every wait is bounded: on expiry the
+// kernel records it in the device error word and raises a flag on which the other roles stop waiting.
 #include <atomic>
 #include <cmath>
 #include <cstdint>
@@ -28,6 +31,7 @@
 #include "sf_e4m3.h"
 #include "sf_q4_internal.h"
 #include "sf_paged.h"
+#include "sf_tcgen05.h"
 
 namespace sf {
 SF_DEFINE_ERROR_READER(take_dev_error_paged)
@@ -35,10 +39,13 @@ extern std::atomic<long long> g_launches;
 
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kMaxCtasPerSm = 3;
-constexpr float kPScale = 1024.f;
+constexpr int UNIT = 128;            // keys of a tile
+constexpr int RT = 8;                // query rows of a tile
+constexpr int kSoftWarps = 4, kProdWarp = 4, kMmaWarp = 5, kThreads = 192;
+constexpr int kMaxCtasPerSm = 4;
+constexpr float kPScale = 256.f;     // of the largest weight: within e4m3
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr unsigned kErrProd = 1u << 17, kErrMma = 1u << 18, kErrSoft = 1u << 19, kErrDrain = 1u << 22;
 
 struct AttnArgs {
   sf_paged_cache c;
@@ -46,7 +53,7 @@ struct AttnArgs {
   long long qts, qhs;
   void* out;
   float* lse;
-  float* part;          // [CTA][2][16][D + 2]: unnormalised sums, then m and l
+  float* part;          // [CTA][2][RT x D unnormalised sums, then RT x (m, l)]
   int* desc;            // [CTA][8]: the tile that this CTA began and others ended
   int H, T, G, q_dtype, out_dtype, window, lg_page;
   float scale;
@@ -72,77 +79,135 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-// four e4m3 codes -> two fp16 pairs, exactly
-__device__ __forceinline__ void e4m3x4_to_h2x2(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
-      : "=r"(lo), "=r"(hi)
-      : "r"(w));
-}
-__device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-__device__ __forceinline__ void split_h2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(x0, x1);
-  const float2 f = __half22float2(h);
-  hi = h2u(h);
-  lo = h2u(__floats2half2_rn(x0 - f.x, x1 - f.y));
-}
-__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
-  uint32_t d;
-  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(sel));
-  return d;
-}
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+// four values of at most 448, to e4m3 codes, leaving what they lack, times 16
+__device__ __forceinline__ uint32_t take_e4m3(float (&v)[4]) {
+  const uint32_t c0 = to_e4m3x2(v[0], v[1]), c1 = to_e4m3x2(v[2], v[3]);
+  const __half2_raw h0 = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)c0, __NV_E4M3),
+                    h1 = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)c1, __NV_E4M3);
+  const float2 a = __half22float2(__half2(h0)), b = __half22float2(__half2(h1));
+  v[0] = (v[0] - a.x) * 16.f;
+  v[1] = (v[1] - a.y) * 16.f;
+  v[2] = (v[2] - b.x) * 16.f;
+  v[3] = (v[3] - b.y) * 16.f;
+  return c0 | (c1 << 16);
 }
 
-// Shared memory: per warp STAGES x (WB key rows, then WB value rows), a row D + 16 bytes apart so that the fragment
-// reads of 8 key rows, and of 4 value rows by 32 bytes, fall into different banks; then the batch's SeqInfo.  The
-// stages hold the warps' sums when a CTA's part of a tile ends.
-template <int D>
+// A tile's rows lie in shared memory as TMA brings them: sub-tiles of INNER bytes a row in the swizzle of that width.
+//  K (rows = keys) is a K-major operand: a step of 32 columns is 32 bytes further in the sub-tile, or, where INNER is
+//  32, the next sub-tile.  V (rows = keys) is an MN-major operand: a step of 32 keys is 32 rows further, the MMA's
+//  128 rows are 128 / INNER sub-tiles, and those beyond the head's columns are whatever lies there, in TMEM lanes
+//  that nothing looks at.
+//  Q^T: [column][d] in cores of 8 columns x 16 bytes, without swizzle.  P^T: [key][16 columns], likewise.
+template <int D, int PARTS>
 struct Lay {
-  static constexpr int WB = D <= 128 ? 32 : 16;
-  static constexpr int STAGES = 2;
-  static constexpr int RP = D + 16;
-  static constexpr int KV = WB * RP;
-  static constexpr int WARP = STAGES * 2 * KV;
-  static constexpr int UNIT = kWarps * WB;
-  static constexpr size_t smem(int batch) { return (size_t)kWarps * WARP + (size_t)batch * sizeof(SeqInfo); }
+  static constexpr int INNER = D % 128 == 0 ? 128 : D == 64 ? 64 : 32;
+  static constexpr int SUBS = D / INNER;                  // sub-tiles of a tile
+  static constexpr uint32_t SUB = UNIT * INNER;
+  static constexpr uint32_t TILE = UNIT * D;              // bytes of a K or V tile
+  static constexpr int STAGES = D == 64 ? 3 : 2;
+  static constexpr int MT = (D + 127) / 128;              // MMAs over d
+  static constexpr int N = (RT * PARTS + 15) / 16 * 16;   // columns
+  static constexpr uint32_t TMEM_USED = 2 * N + 2 * MT * N;
+  static constexpr uint32_t TMEM_COLS = TMEM_USED <= 64 ? 64 : TMEM_USED <= 128 ? 128 : TMEM_USED <= 256 ? 256 : 512;
+  static constexpr uint32_t K0 = 0, V0 = STAGES * TILE, Q0 = 2 * STAGES * TILE, P0 = Q0 + N * D;
+  static constexpr uint32_t P = N * UNIT;                 // bytes of a P buffer
+  // V's operand may reach 128 rows of SUB bytes beyond the last tile's start: inside the block's memory
+  static constexpr uint32_t REACH = V0 + (STAGES - 1) * TILE + (128 / INNER > SUBS ? 128 / INNER : SUBS) * SUB;
+  static constexpr uint32_t CTL = P0 + 2 * P > REACH ? P0 + 2 * P : REACH;
+  static constexpr uint32_t INFO = CTL + 2048;
+  static constexpr uint64_t SWZ = INNER == 128 ? kSw128 : INNER == 64 ? kSw64 : kSw32;
+  static constexpr size_t smem(int batch) { return 1024 + INFO + (size_t)batch * sizeof(SeqInfo); }
+  static_assert(TMEM_USED <= 512, "TMEM plan");
 };
 
-// Keys that the sequence's units cover: from lo (a multiple of 16) to len.
+// First key that the sequence's units cover, a multiple of UNIT.
 __device__ __forceinline__ int keys_from(const AttnArgs& a, int len, int n) {
-  return a.window > 0 ? max(0, len - n + 1 - a.window) & ~15 : 0;
+  return a.window > 0 ? max(0, len - n + 1 - a.window) & ~(UNIT - 1) : 0;
 }
 
-template <int D, bool HL>
-__global__ void __launch_bounds__(32 * kWarps, D <= 128 ? kMaxCtasPerSm : 2) paged_attention_kernel(const AttnArgs a) {
-  using L = Lay<D>;
-  constexpr int WB = L::WB, RT = HL ? 8 : 16, RPL = HL ? 1 : 2;   // rows of a tile, rows of a lane
-  constexpr int KS = D / 16, NT = WB / 8, DB = D / 32, CH = D / 16;
-  constexpr int GPB = WB / 16, NB = 32 / GPB;                      // 16-key granules of a block, blocks of 32 granules
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float wm[kWarps][16], wl[kWarps][16], wv[kWarps];
-  __shared__ long long wsum[kWarps];
-  SeqInfo* info = reinterpret_cast<SeqInfo*>(smem + kWarps * L::WARP);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+// The part of a tile of query rows that begins at unit u and is this CTA's.
+struct Part {
+  int b, kvh, row0, last_row, r_first, pos0;
+  int ta, tb;                 // keys [ta, tb), ta a multiple of UNIT
+  int tile_lo, all_lo, all_hi;   // first key that some row sees; keys that every row sees
+  long long u1, seg0, seg1;   // end of the part; units of the whole tile
+};
+__device__ __forceinline__ Part part_at(const AttnArgs& a, const SeqInfo* info, long long u, long long u_end, int& b) {
+  while (b + 1 < a.c.batch && info[b + 1].first <= u) ++b;
+  const SeqInfo s = info[b];
+  Part p;
+  p.b = b;
+  const int tiles = (int)(((long long)s.n * a.G + RT - 1) / RT);
+  const int from = keys_from(a, s.len, s.n), per = max(1, (s.len - from + UNIT - 1) / UNIT);
+  const long long rel = u - s.first, seg = rel / per;
+  const int j0 = (int)(rel - seg * per);
+  p.kvh = (int)(seg / tiles);
+  p.row0 = (int)(seg % tiles) * RT;
+  p.seg0 = s.first + seg * per;
+  p.seg1 = p.seg0 + per;
+  p.u1 = p.seg1 < u_end ? p.seg1 : u_end;
+  p.r_first = first_row(a.c, a.T, b);
+  p.pos0 = s.len - s.n;
+  p.last_row = min(p.row0 + RT, s.n * a.G) - 1;
+  const int tile_hi = p.pos0 + p.last_row / a.G + 1;
+  p.all_hi = p.pos0 + p.row0 / a.G + 1;
+  p.tile_lo = a.window > 0 ? max(0, p.all_hi - a.window) : 0;
+  p.all_lo = a.window > 0 ? max(0, tile_hi - a.window) : 0;
+  // tiles of keys without one that some row sees are left out
+  p.ta = max(from + j0 * UNIT, p.tile_lo & ~(UNIT - 1));
+  p.tb = (int)min((long long)tile_hi, from + (long long)(j0 + (p.u1 - u)) * UNIT);
+  return p;
+}
+
+template <int D, int PARTS>
+__global__ void __launch_bounds__(kThreads, D == 64 ? 4 : D <= 128 ? 3 : 1)
+    paged_attention_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
+                           const AttnArgs a) {
+  using L = Lay<D, PARTS>;
+  constexpr int N = L::N, MT = L::MT, ST = L::STAGES;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ __align__(16) float red[2][RT][4];           // one number per row and softmax warp, two buffers
+  __shared__ float row_f[RT];
+  __shared__ long long wsum[kThreads / 32];
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  uint8_t* mem = smem_raw + (base - raw);
+  SeqInfo* info = reinterpret_cast<SeqInfo*>(mem + L::INFO);
+  const uint32_t ctl = base + L::CTL;
+  const uint32_t kfull = ctl, kempty = ctl + 32, vfull = ctl + 64, vempty = ctl + 96, sfull = ctl + 128, pfull = ctl + 144,
+                 ofull = ctl + 160, qfull = ctl + 176, drain = ctl + 184;
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(mem + L::CTL + 256);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(mem + L::CTL + 264);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   griddep_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; ++s) {
+      bar_init(kfull + 8 * s, 1);
+      bar_init(kempty + 8 * s, 1);
+      bar_init(vfull + 8 * s, 1);
+      bar_init(vempty + 8 * s, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      bar_init(sfull + 8 * i, 1);
+      bar_init(pfull + 8 * i, kSoftWarps);
+      bar_init(ofull + 8 * i, 1);
+    }
+    bar_init(qfull, kSoftWarps);
+    bar_init(drain, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kProdWarp && lane == 0) {
+    prefetch_map(&mapK);
+    prefetch_map(&mapV);
+  }
+  if (warp == kMmaWarp) tmem_alloc(smem_u32((const void*)tmem_slot), L::TMEM_COLS);
+  griddep_wait();   // the set-up above runs beside the end of the kernel before; memory is touched from here on
 
   // ---- the batch's units, and this CTA's share ----
   const int B = a.c.batch, Hkv = a.c.n_kv_heads, page_size = a.c.page_size;
   long long total = 0;
-  for (int base = 0; base < B; base += 32 * kWarps) {
-    const int b = base + threadIdx.x;
+  for (int at = 0; at < B; at += kThreads) {
+    const int b = at + threadIdx.x;
     long long u = 0;
     int len = 0, n = 0;
     if (b < B) {
@@ -158,7 +223,7 @@ __global__ void __launch_bounds__(32 * kWarps, D <= 128 ? kMaxCtasPerSm : 2) pag
         atomicOr(&g_dev_error, kErrIndex);
       }
       const int tiles = (int)(((long long)n * a.G + RT - 1) / RT);
-      u = (long long)tiles * Hkv * max(1, (len - keys_from(a, len, n) + L::UNIT - 1) / L::UNIT);
+      u = (long long)tiles * Hkv * max(1, (len - keys_from(a, len, n) + UNIT - 1) / UNIT);
     }
     long long incl = u;
 #pragma unroll
@@ -170,7 +235,7 @@ __global__ void __launch_bounds__(32 * kWarps, D <= 128 ? kMaxCtasPerSm : 2) pag
     __syncthreads();
     long long before = total;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < kThreads / 32; ++w) {
       if (w < warp) before += wsum[w];
       total += wsum[w];
     }
@@ -179,364 +244,433 @@ __global__ void __launch_bounds__(32 * kWarps, D <= 128 ? kMaxCtasPerSm : 2) pag
   }
   const long long C = min((long long)gridDim.x, total), cta = blockIdx.x;   // CTAs with a share: at least a unit each
   if (threadIdx.x == 0) a.desc[8 * cta] = 0;
-  if (cta >= C) return;
-  long long u = total * cta / C;
-  const long long u_end = total * (cta + 1) / C;
+  long long u = 0, u_end = 0;
   int b = 0;
-  for (int lo = 0, hi = B; hi - lo > 1;) {
-    const int mid = (lo + hi) >> 1;
-    if (info[mid].first <= u) lo = mid;
-    else hi = mid;
-    b = lo;
+  if (cta < C) {
+    u = total * cta / C;
+    u_end = total * (cta + 1) / C;
+    for (int lo = 0, hi = B; hi - lo > 1;) {
+      const int mid = (lo + hi) >> 1;
+      if (info[mid].first <= u) lo = mid;
+      else hi = mid;
+      b = lo;
+    }
   }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot, tmem_s = tmem, tmem_o = tmem + 2 * N;
 
-  const uint32_t wbase = smem_u32(smem + warp * L::WARP);
-  for (; u < u_end;) {
-    // ---- the tile that holds unit u, and the part [u, u1) of its units that is this CTA's ----
-    while (b + 1 < B && info[b + 1].first <= u) ++b;
-    const SeqInfo s = info[b];
-    const int tiles = (int)(((long long)s.n * a.G + RT - 1) / RT);
-    const int from = keys_from(a, s.len, s.n);
-    const int per = max(1, (s.len - from + L::UNIT - 1) / L::UNIT);
-    const long long rel = u - s.first, seg = rel / per;
-    const int j0 = (int)(rel % per), kvh = (int)(seg / tiles), row0 = (int)(seg % tiles) * RT;
-    const long long seg0 = s.first + seg * per, seg1 = seg0 + per;
-    const long long u1 = seg1 < u_end ? seg1 : u_end;
-    const int r_first = first_row(a.c, a.T, b);
-    const int pos0 = s.len - s.n;                                // position of the sequence's first new row
-    const int last_row = min(row0 + RT, s.n * a.G) - 1;
-    const int tile_hi = pos0 + last_row / a.G + 1;               // keys that some row sees: [tile_lo, tile_hi)
-    const int tile_lo = a.window > 0 ? max(0, pos0 + row0 / a.G + 1 - a.window) : 0;
-    const int all_hi = pos0 + row0 / a.G + 1;                    // keys that every row sees: [all_lo, all_hi)
-    const int all_lo = a.window > 0 ? max(0, tile_hi - a.window) : 0;
-    // the unit grid starts at `from`; blocks without a key that some row sees are left out
-    int ta = from + j0 * L::UNIT;
-    const int tb = (int)min((long long)tile_hi, from + (long long)(j0 + (u1 - u)) * L::UNIT);
-    if (ta < (tile_lo & ~15)) ta = tile_lo & ~15;
-
-    // ---- query fragments ----
-    uint32_t qf[KS][4];
-    float f[RPL];
-    int rhi[RPL], rlo[RPL];
+  if (warp == kProdWarp) {
+    // ---------------- page copies ----------------
+    const int box = min(page_size, UNIT), boxes = UNIT / box;
+    uint32_t it = 0;
+    bool ok = true;
+    while (u < u_end && ok) {
+      const Part p = part_at(a, info, u, u_end, b);
+      const int* pages = a.c.block_table + (size_t)p.b * a.c.pages_per_seq;
+      const auto page_of = [&](int key) {
+        return lane < boxes && key < p.tb ? __ldg(pages + (key >> a.lg_page)) : -1;
+      };
+      int key = p.ta + lane * box, next = page_of(key);
+      for (int k0 = p.ta; k0 < p.tb; k0 += UNIT, ++it, key += UNIT) {
+        const int page = next;
+        next = page_of(key + UNIT);
+        const bool load = page >= 0 && page < a.c.num_pages;
+        const int y = load ? (page * Hkv + p.kvh) * page_size + (key & (page_size - 1)) : 0;
+        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, load)) * (uint32_t)(box * D);
+        const uint32_t s = it % ST, ph = (it / ST) & 1;
 #pragma unroll
-    for (int i = 0; i < RPL; ++i) {
-      const int row = row0 + g + 8 * i;
-      const bool in = row <= last_row;
-      const int tok = row / a.G, pos = pos0 + tok;
-      rhi[i] = in ? pos + 1 : 0;
-      rlo[i] = in && a.window > 0 ? max(0, pos + 1 - a.window) : 0;
-      const long long qo = (long long)(r_first + tok) * a.qts + (long long)(kvh * a.G + row % a.G) * a.qhs;
-      uint32_t top = 0;
-      for (int k = 0; k < KS && in; ++k)
+        for (int v = 0; v < 2; ++v) {
+          const uint32_t full = (v ? vfull : kfull) + 8 * s, empty = (v ? vempty : kempty) + 8 * s;
+          ok = ok && bar_wait(empty, ph ^ 1, kErrProd, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (lane == 0) bar_expect_tx(full, bytes);
+          __syncwarp();
+          const uint32_t dst = base + (v ? L::V0 : L::K0) + s * L::TILE + (uint32_t)(lane * box * L::INNER);
+          if (load) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(load_q(a, qo + 16 * k + 4 * t + e)) & 0x7fffffffu);
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // the row over 2^ex, which puts its largest value in [1, 2); zero, subnormal and non-finite rows as they are
-      int ex = (int)(top >> 23) - 127;
-      if (ex == -127 || ex == 128) ex = 0;
-      if (ex > 126) ex = 126;                                    // 2^-ex has to be a normal number
-      const float down = __int_as_float((127 - ex) << 23);
-      f[i] = __int_as_float((127 + ex) << 23) * (a.scale * kLog2e);
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
-        if (in) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = load_q(a, qo + 16 * k + 4 * t + e) * down;
-        }
-        if constexpr (HL) {
-          split_h2(v[0], v[1], qf[k][0], qf[k][1]);
-          split_h2(v[2], v[3], qf[k][2], qf[k][3]);
-        } else {
-          qf[k][i] = h2u(__floats2half2_rn(v[0], v[1]));
-          qf[k][2 + i] = h2u(__floats2half2_rn(v[2], v[3]));
-        }
-      }
-    }
-
-    // ---- this warp's blocks: keys ta + WB (warp + 4 i) .. ----
-    // Lane l of a set holds page and scales of the set's granule l: block l / GPB, its keys 16 (l % GPB) ..
-    struct Set {
-      int page;
-      float ks, vs;
-    };
-    const auto load_set = [&](int set) {
-      Set x{-1, 0.f, 0.f};
-      const long long tok = ta + (long long)WB * (warp + kWarps * (NB * set + lane / GPB)) + 16 * (lane % GPB);
-      if (tok < tb) {
-        const int page = a.c.block_table[(size_t)b * a.c.pages_per_seq + (tok >> a.lg_page)];
-        if (page >= 0 && page < a.c.num_pages) {
-          x.page = page;
-          x.ks = a.c.k_scales[(size_t)page * Hkv + kvh];
-          x.vs = a.c.v_scales[(size_t)page * Hkv + kvh];
-        } else {
-          atomicOr(&g_dev_error, kErrIndex);
-        }
-      }
-      return x;
-    };
-    Set cur = load_set(0), nxt = load_set(1);
-    const auto issue = [&](int i, const Set& x) {
-      const int base = ta + WB * (warp + kWarps * i);
-      int pg[GPB];
-#pragma unroll
-      for (int e = 0; e < GPB; ++e) pg[e] = __shfl_sync(0xffffffffu, x.page, (i % NB) * GPB + e);
-      if (base < tb) {
-        const uint32_t st = wbase + (uint32_t)(i % L::STAGES) * (2 * L::KV);
-#pragma unroll
-        for (int k = 0; k < WB * CH / 32; ++k) {
-          const int c = lane + 32 * k, r = c / CH, dp = (c % CH) * 16, key = base + r;
-          const int page = GPB == 1 ? pg[0] : (r < 16 ? pg[0] : pg[GPB - 1]);
-          // rows of no key are zeros: what lies past a sequence's end may be NaN, and 0 * NaN is not 0
-          const bool v = key < tb && key >= tile_lo && page >= 0;
-          const size_t at = (((size_t)(v ? page : 0) * Hkv + kvh) * page_size + (v ? key & (page_size - 1) : 0)) * D + dp;
-          cp_async16(st + r * L::RP + dp, a.c.k_codes + at, v);
-          cp_async16(st + L::KV + r * L::RP + dp, a.c.v_codes + at, v);
-        }
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-
-    float m[RPL], l[RPL], o[4 * DB][4], vref = 0x1p-100f;
-#pragma unroll
-    for (int i = 0; i < RPL; ++i) {
-      m[i] = -INFINITY;
-      l[i] = 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < 4 * DB; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-
-    issue(0, cur);
-    for (int i = 0;; ++i) {
-      const int base = ta + WB * (warp + kWarps * i);
-      if (base >= tb) break;
-      issue(i + 1, (i + 1) % NB ? cur : nxt);
-      asm volatile("cp.async.wait_group 1;" ::: "memory");
-      __syncwarp();
-      const uint32_t st = wbase + (uint32_t)(i % L::STAGES) * (2 * L::KV);
-      float ks[GPB], vs[GPB];
-      bool whole = base + WB <= tb && base >= all_lo && base + WB <= all_hi;
-#pragma unroll
-      for (int e = 0; e < GPB; ++e) {
-        const int src = (i % NB) * GPB + e;
-        ks[e] = __shfl_sync(0xffffffffu, cur.ks, src);
-        vs[e] = __shfl_sync(0xffffffffu, cur.vs, src);
-        if (__shfl_sync(0xffffffffu, cur.page, src) < 0) whole = false;
-      }
-      // ---- scores ----
-      float x[NT][2 * RPL];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        const uint32_t kr = st + (8 * j + g) * L::RP + 4 * t;
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          uint32_t b0, b1;
-          e4m3x4_to_h2x2(lds32(kr + 16 * k), b0, b1);
-          mma16816(acc, qf[k], b0, b1);
-        }
-        const float sk = ks[j / 2];
-        if constexpr (HL) {
-          x[j][0] = (acc[0] + acc[2]) * (f[0] * sk);
-          x[j][1] = (acc[1] + acc[3]) * (f[0] * sk);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[j][e] = acc[e] * (f[e / 2] * sk);
-        }
-      }
-      if (!whole) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const bool there = __shfl_sync(0xffffffffu, cur.page, (i % NB) * GPB + j / 2) >= 0;
-#pragma unroll
-          for (int e = 0; e < 2 * RPL; ++e) {
-            const int key = base + 8 * j + 2 * t + (e & 1), r = e / 2;
-            if (!there || key < rlo[r] || key >= rhi[r] || key >= tb) x[j][e] = -INFINITY;
+            for (int i = 0; i < L::SUBS; ++i) tma_load(dst + i * L::SUB, v ? &mapV : &mapK, i * L::INNER, y, full);
           }
         }
+        if (!ok) break;
       }
-      // ---- running softmax ----
-      float ref[RPL], corr[RPL];
-      float vmax = vs[0];
-#pragma unroll
-      for (int e = 1; e < GPB; ++e) vmax = fmaxf(vmax, vs[e]);
-      const float vnew = fmaxf(vref, vmax), vinv = 1.f / vnew, vdown = vref * vinv;
-      vref = vnew;
-#pragma unroll
-      for (int r = 0; r < RPL; ++r) {
-        float bm = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < NT; ++j) bm = fmaxf(bm, fmaxf(x[j][2 * r], x[j][2 * r + 1]));
-        bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 1));
-        bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 2));
-        const float mn = fmaxf(m[r], bm);
-        ref[r] = mn == -INFINITY ? 0.f : mn;
-        corr[r] = ex2(m[r] - ref[r]);
-        m[r] = mn;
-        l[r] *= corr[r];
-        corr[r] *= vdown;
+      u = p.u1;
+    }
+    // every issued copy has landed before the block ends
+    const uint32_t pending = it < (uint32_t)ST ? it : (uint32_t)ST;
+    if (lane == 0 && ok)
+      for (uint32_t j = it - pending; j < it; ++j) {
+        bar_drain(kfull + 8 * (j % ST), (j / ST) & 1, kErrDrain);
+        bar_drain(vfull + 8 * (j % ST), (j / ST) & 1, kErrDrain);
       }
-      bool same = corr[0] == 1.f;
-      if (RPL == 2) same = same && corr[RPL - 1] == 1.f;
-      if (!__all_sync(0xffffffffu, same)) {
+    // after an expired wait the copies under way are not counted any more: give them time
+    if (!ok) {
+      const long long t0 = clock64();
+      while (clock64() - t0 < kWaitCycles / 64) {
+      }
+    }
+    __syncwarp();
+  } else if (warp == kMmaWarp) {
+    // ---------------- MMAs ----------------
+    if (lane == 0) {
+      constexpr uint32_t idesc_s = idesc_e4m3(128, N), idesc_o = idesc_e4m3(128, N, true, true);
+      uint32_t it = 0, seg = 0;
+      bool ok = true;
+      const auto scores = [&](uint32_t j) {
+        const uint32_t s = j % ST, st = base + L::K0 + s * L::TILE;
+        if (!bar_wait(kfull + 8 * s, (j / ST) & 1, kErrMma, abort_flag)) return false;
+        tc_fence_after();
 #pragma unroll
-        for (int i2 = 0; i2 < 4 * DB; ++i2) {
-          o[i2][0] *= corr[0];
-          o[i2][1] *= corr[0];
-          o[i2][2] *= corr[RPL - 1];
-          o[i2][3] *= corr[RPL - 1];
+        for (int k = 0; k < D / 32; ++k) {
+          const uint32_t at = L::INNER == 32 ? k * L::SUB : k / (L::INNER / 32) * L::SUB + k % (L::INNER / 32) * 32;
+          mma_f8(tmem_s + (j & 1) * N, smem_desc(st + at, 16, 8 * L::INNER, L::SWZ),
+                 smem_desc(base + L::Q0 + k * 256, 128, D / 16 * 128, kSwNone), idesc_s, k != 0);
+        }
+        mma_commit(kempty + 8 * s);
+        mma_commit(sfull + 8 * (j & 1));
+        return true;
+      };
+      const auto sums = [&](uint32_t j) {
+        const uint32_t s = j % ST, st = base + L::V0 + s * L::TILE, pb = base + L::P0 + (j & 1) * L::P;
+        if (!bar_wait(vfull + 8 * s, (j / ST) & 1, kErrMma, abort_flag) ||
+            !bar_wait(pfull + 8 * (j & 1), (j >> 1) & 1, kErrMma, abort_flag))
+          return false;
+        tc_fence_after();
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int k = 0; k < UNIT / 32; ++k)
+            mma_f8(tmem_o + ((j & 1) * MT + m) * N,
+                   smem_desc(st + m * L::SUB + k * 32 * L::INNER, L::SUB, 8 * L::INNER, L::SWZ),
+                   smem_desc(pb + k * 512, 128, UNIT * 16, kSwNone), idesc_o, k != 0);
+        mma_commit(vempty + 8 * s);
+        mma_commit(ofull + 8 * (j & 1));
+        return true;
+      };
+      while (u < u_end && ok) {
+        const Part p = part_at(a, info, u, u_end, b);
+        const int tiles = p.tb > p.ta ? (p.tb - p.ta + UNIT - 1) / UNIT : 0;
+        if (tiles > 0) {
+          ok = bar_wait(qfull, seg & 1, kErrMma, abort_flag);
+          ++seg;
+          if (ok) {
+            tc_fence_after();
+            ok = scores(it);
+          }
+          for (int i = 0; i < tiles && ok; ++i) {
+            if (i + 1 < tiles) ok = scores(it + i + 1);
+            if (ok) ok = sums(it + i);
+          }
+          it += tiles;
+        }
+        u = p.u1;
+      }
+      // every issued MMA has completed before TMEM is freed
+      mma_commit(drain);
+      bar_drain(drain, 0, kErrDrain);
+    }
+    __syncwarp();
+  } else {
+    // ---------------- softmax and sums: a thread is key tid of a tile, and column tid of the head ----------------
+    // After an expired wait these warps go on through their loops (every wait then returns at once), so that none of
+    // them waits for another in the block's barrier.
+    const int tid = threadIdx.x;
+    const uint32_t my_lanes = (uint32_t)(32 * warp) << 16;
+    uint32_t it = 0, seg = 0;
+    float part_scale[PARTS];
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) part_scale[i] = __int_as_float((127 - 4 * i) << 23);
+    // one number per row over the 128 threads: a row's lanes hold its 4 warps' results after the barrier
+    const auto over_keys = [&](float (&v)[RT], int buf, auto&& op) {
+#pragma unroll
+      for (int n = RT / 2, o = 16; n >= 1; n >>= 1, o >>= 1) {
+        const bool up = lane & o;
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+          const float mine = up ? v[i + n] : v[i], other = up ? v[i] : v[i + n];
+          v[i] = op(mine, __shfl_xor_sync(0xffffffffu, other, o));
         }
       }
-      uint32_t pf[NT / 2][4];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const float fold = vs[j / 2] * (kPScale * vinv);
-        float p[2 * RPL];
+      for (int o = 16 / RT; o >= 1; o >>= 1) v[0] = op(v[0], __shfl_xor_sync(0xffffffffu, v[0], o));
+      if (lane % (32 / RT) == 0) red[buf][lane / (32 / RT)][warp] = v[0];
+      named_barrier_sync(1, 32 * kSoftWarps);
 #pragma unroll
-        for (int e = 0; e < 2 * RPL; ++e) {
-          p[e] = ex2(x[j][e] - ref[e / 2]);
-          l[e / 2] += p[e];
-          p[e] *= fold;
-        }
-        if constexpr (HL) {
-          split_h2(p[0], p[1], pf[j / 2][2 * (j & 1)], pf[j / 2][2 * (j & 1) + 1]);
-        } else {
-          pf[j / 2][2 * (j & 1)] = h2u(__floats2half2_rn(p[0], p[1]));
-          pf[j / 2][2 * (j & 1) + 1] = h2u(__floats2half2_rn(p[2 * RPL - 2], p[2 * RPL - 1]));
-        }
+      for (int r = 0; r < RT; ++r) {
+        const float4 w = *reinterpret_cast<const float4*>(red[buf][r]);
+        v[r] = op(op(w.x, w.y), op(w.z, w.w));
       }
-      // ---- values ----
-      // Where rows see different keys, a NaN among the values must reach only the rows that see its key, and 0 * NaN
-      // is not 0: such a block's NaN codes are put into those rows' sums by hand, and become zeros.
-      if (!(base >= all_lo && min(base + WB, tb) <= all_hi)) {
-        const uint32_t sv = st + L::KV;
-        uint32_t found = 0;
-        for (int c = lane; c < WB * D / 4; c += 32) {
-          const uint32_t w = lds32(sv + (c / (D / 4)) * L::RP + (c % (D / 4)) * 4);
-          found |= ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-        }
-        if (__any_sync(0xffffffffu, found != 0)) {
-          for (int r = 0; r < WB; ++r) {
+    };
+    int buf = 0;
+    while (u < u_end) {
+      const Part p = part_at(a, info, u, u_end, b);
+      const int tiles = p.tb > p.ta ? (p.tb - p.ta + UNIT - 1) / UNIT : 0;
+      float m[RT], l[RT], o[MT][RT], corr[RT];
 #pragma unroll
-            for (int e = 0; e < RPL; ++e) {
-              const int key = base + r;
-              if (key < rlo[e] || key >= rhi[e] || key >= tb) continue;
+      for (int r = 0; r < RT; ++r) {
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+        corr[r] = 0.f;
 #pragma unroll
-              for (int db = 0; db < DB; ++db)
+        for (int mt = 0; mt < MT; ++mt) o[mt][r] = 0.f;
+      }
+      if (tiles > 0) {
+        // ---- query parts: 16 threads a row, D / 16 columns each ----
+        {
+          constexpr int E = D / 16;
+          const int r = tid >> 4, row = p.row0 + r, d0 = (tid & 15) * E;
+          float v[E];
+          uint32_t top = 0;
+          const long long qo = (long long)(p.r_first + row / a.G) * a.qts + (long long)(p.kvh * a.G + row % a.G) * a.qhs + d0;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                  const uint32_t w = lds32(sv + r * L::RP + 32 * db + 8 * t + 4 * h);
+          for (int e = 0; e < E; ++e) {
+            v[e] = row <= p.last_row ? load_q(a, qo + e) : 0.f;
+            top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+          }
 #pragma unroll
-                  for (int j = 0; j < 4; ++j)
-                    if (((w >> (8 * j)) & 0x7fu) == 0x7fu) o[4 * db + j][2 * e + h] = __int_as_float(0x7fffffff);
-                }
+          for (int o2 = 8; o2; o2 >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o2));
+          // the row's largest value to [128, 256) by a power of two
+          const int ex = min(max((int)(top >> 23) - 134, -126), 126);
+          const float down = __int_as_float((127 - ex) << 23);
+          if ((tid & 15) == 0) {
+            // an infinity would saturate: its row is NaN
+            row_f[r] = top >= 0x7f800000u ? __int_as_float(0x7fffffff)
+                                          : __int_as_float((127 + ex) << 23) * (a.scale * kLog2e);
+          }
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const int d = d0 + e;
+            float x = v[e] * down;
+#pragma unroll
+            for (int i = 0; i < PARTS; ++i) {
+              const uint8_t c = to_e4m3(x);
+              x = (x - from_e4m3(c)) * 16.f;
+              const int col = i * RT + r;
+              mem[L::Q0 + (col / 8) * (D * 8) + (d / 16) * 128 + (col % 8) * 16 + d % 16] = c;
             }
           }
-          __syncwarp();
-          for (int c = lane; c < WB * D / 4; c += 32) {
-            const uint32_t at = sv + (c / (D / 4)) * L::RP + (c % (D / 4)) * 4;
-            uint32_t w = lds32(at);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (((w >> (8 * j)) & 0x7fu) == 0x7fu) w &= ~(0xffu << (8 * j));
-            asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(w) : "memory");
-          }
-          __syncwarp();
+          fence_async_smem();
+          named_barrier_sync(1, 32 * kSoftWarps);   // row_f, too
+          if (lane == 0) bar_arrive(qfull);
         }
-      }
-      const uint32_t vr = st + L::KV + 2 * t * L::RP + 4 * g;
+        float f[RT];
 #pragma unroll
-      for (int kk = 0; kk < NT / 2; ++kk) {
-#pragma unroll
-        for (int db = 0; db < DB; ++db) {
-          const uint32_t at = vr + 16 * kk * L::RP + 32 * db;
-          const uint32_t w0 = lds32(at), w1 = lds32(at + L::RP), w2 = lds32(at + 8 * L::RP), w3 = lds32(at + 9 * L::RP);
-          uint32_t b0[4], b1[4];
-          e4m3x4_to_h2x2(prmt(w0, w1, 0x5140), b0[0], b0[1]);
-          e4m3x4_to_h2x2(prmt(w0, w1, 0x7362), b0[2], b0[3]);
-          e4m3x4_to_h2x2(prmt(w2, w3, 0x5140), b1[0], b1[1]);
-          e4m3x4_to_h2x2(prmt(w2, w3, 0x7362), b1[2], b1[3]);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) mma16816(o[4 * db + j], pf[kk], b0[j], b1[j]);
-        }
-      }
-      __syncwarp();   // the stage may be filled again
-      if ((i + 1) % NB == 0) {
-        cur = nxt;
-        nxt = load_set((i + 1) / NB + 1);
-      }
-    }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+        for (int r = 0; r < RT; ++r) f[r] = row_f[r];
 
-    // ---- the four warps' parts ----
+        // page and scales of this thread's key, one and two tiles ahead
+        const int* pages = a.c.block_table + (size_t)p.b * a.c.pages_per_seq;
+        const auto page_of = [&](int key) {
+          if (key >= p.tb || key < p.tile_lo) return -1;
+          const int page = __ldg(pages + (key >> a.lg_page));
+          if (page >= 0 && page < a.c.num_pages) return page;
+          atomicOr(&g_dev_error, kErrIndex);
+          return -1;
+        };
+        const auto scales_of = [&](int page, float& ks, float& vs) {
+          const size_t at = (size_t)max(page, 0) * Hkv + p.kvh;
+          ks = page >= 0 ? __ldg(a.c.k_scales + at) : 0.f;
+          vs = page >= 0 ? __ldg(a.c.v_scales + at) : 0.f;
+        };
+        int page = page_of(p.ta + tid), page1 = page_of(p.ta + UNIT + tid);
+        float ks, vs;
+        scales_of(page, ks, vs);
+
+        // adds the sums of tile j, which are relative to the reference after it
+        const auto add_sums = [&](uint32_t j, const float (&c)[RT]) {
+          bar_wait(ofull + 8 * (j & 1), (j >> 1) & 1, kErrSoft, abort_flag);
+          tc_fence_after();
 #pragma unroll
-    for (int r = 0; r < RPL; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    }
-    __syncthreads();   // every warp is done with its stages
-    float* sums = reinterpret_cast<float*>(smem);   // [warp][row][D]
-    const float unit = vref * (1.f / kPScale);
+          for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
-    for (int r = 0; r < RPL; ++r) {
-      if (t == 0) {
-        wm[warp][g + 8 * r] = m[r];
-        wl[warp][g + 8 * r] = l[r];
-      }
+            for (int r = 0; r < RT; ++r) o[mt][r] *= c[r];
 #pragma unroll
-      for (int db = 0; db < DB; ++db)
+            for (int n = 0; n < N; n += 16) {
+              uint32_t w[16];
+              tmem_ld(tmem_o + my_lanes + ((j & 1) * MT + mt) * N + n, w);
+              tmem_wait(w);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float4 v;
-          float* p = &v.x;
+              for (int e = 0; e < 16; ++e)
+                if (n + e < RT * PARTS)
+                  o[mt][(n + e) % RT] = fmaf(__uint_as_float(w[e]), part_scale[(n + e) / RT], o[mt][(n + e) % RT]);
+            }
+          }
+        };
+
+        for (int i = 0; i < tiles; ++i) {
+          const uint32_t j = it + i;
+          const int k0 = p.ta + UNIT * i, key = k0 + tid;
+          const bool there = page >= 0;
+          const float ks_i = ks, vs_i = vs;
+          page = page1;
+          scales_of(page, ks, vs);
+          page1 = page_of(key + 2 * UNIT);
+          // ---- scores ----
+          float x[RT];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) p[j] = HL ? o[4 * db + j][h] + o[4 * db + j][2 + h] : o[4 * db + j][2 * r + h];
-          *reinterpret_cast<float4*>(sums + ((size_t)warp * RT + g + 8 * r) * D + 32 * db + 8 * t + 4 * h) = v;
+          for (int r = 0; r < RT; ++r) x[r] = 0.f;
+          bar_wait(sfull + 8 * (j & 1), (j >> 1) & 1, kErrSoft, abort_flag);
+          tc_fence_after();
+#pragma unroll
+          for (int n = 0; n < N; n += 16) {
+            uint32_t w[16];
+            tmem_ld(tmem_s + my_lanes + (j & 1) * N + n, w);
+            tmem_wait(w);
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (n + e < RT * PARTS)
+                x[(n + e) % RT] = fmaf(__uint_as_float(w[e]), part_scale[(n + e) / RT], x[(n + e) % RT]);
+          }
+          const bool alike = k0 >= p.all_lo && min(k0 + UNIT, p.tb) <= p.all_hi;   // rows see the same of these keys
+#pragma unroll
+          for (int r = 0; r < RT; ++r) x[r] = there ? x[r] * (f[r] * ks_i) : -INFINITY;
+          if (!alike) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+              const int pos = p.pos0 + (p.row0 + r) / a.G;
+              if (key > pos || (a.window > 0 && key <= pos - a.window)) x[r] = -INFINITY;
+            }
+          }
+          // ---- reference ----
+          const float lv = fmaxf(__log2f(vs_i), -60.f);
+          float top[RT];
+#pragma unroll
+          for (int r = 0; r < RT; ++r) top[r] = x[r] + lv;
+          over_keys(top, buf, [](float s, float t) { return fmaxf(s, t); });
+          buf ^= 1;
+          float c[RT], pw[RT];
+          const float fold = vs_i * kPScale;
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            const float mn = fmaxf(m[r], top[r]), ref = mn == -INFINITY ? 0.f : mn;
+            c[r] = ex2(m[r] - ref);
+            m[r] = mn;
+            const float w = ex2(x[r] - ref);
+            l[r] = fmaf(l[r], c[r], w);
+            pw[r] = w * fold;
+          }
+          // ---- weights to shared memory ----
+          uint32_t w[N / 8][2];
+#pragma unroll
+          for (int r = 0; r < RT; r += 4) {
+            float v[4] = {pw[r], pw[r + 1], pw[r + 2], pw[r + 3]};
+#pragma unroll
+            for (int q = 0; q < N / RT; ++q) {
+              if (q < PARTS - 1) w[q][r / 4] = take_e4m3(v);
+              else if (q < PARTS) w[q][r / 4] = to_e4m3x2(v[0], v[1]) | (to_e4m3x2(v[2], v[3]) << 16);
+              else w[q][r / 4] = 0;
+            }
+          }
+          uint8_t* pb = mem + L::P0 + (j & 1) * L::P;
+#pragma unroll
+          for (int n = 0; n < N / 16; ++n)
+            *reinterpret_cast<uint4*>(pb + n * UNIT * 16 + tid * 16) =
+                make_uint4(w[2 * n][0], w[2 * n][1], w[2 * n + 1][0], w[2 * n + 1][1]);
+          // ---- values that must not reach a sum, where 0 * NaN is not 0 ----
+          uint8_t* vt = mem + L::V0 + (j % ST) * L::TILE;
+          if (!__all_sync(0xffffffffu, there)) {
+            // rows of no key of the sequence: whatever their page holds becomes 0
+            bar_wait(vfull + 8 * (j % ST), (j / ST) & 1, kErrSoft, abort_flag);
+            if (!there) {
+#pragma unroll
+              for (int s = 0; s < L::SUBS; ++s)
+#pragma unroll
+                for (int e = 0; e < L::INNER; e += 16)
+                  *reinterpret_cast<uint4*>(vt + s * L::SUB + tid * L::INNER + e) = make_uint4(0, 0, 0, 0);
+            }
+          }
+          if (!alike) {
+            // a NaN code reaches only the rows that see its key: it is put into their sums by hand, and becomes 0
+            bar_wait(vfull + 8 * (j % ST), (j / ST) & 1, kErrSoft, abort_flag);
+            named_barrier_sync(1, 32 * kSoftWarps);   // the zeros above
+            uint32_t found = 0;
+            for (uint32_t at = tid * 4; at < L::TILE; at += 512) {
+              const uint32_t y = *reinterpret_cast<const uint32_t*>(vt + at);
+              found |= ((y & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+            }
+            int any;
+            asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, %2, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
+                         : "=r"(any) : "r"(found), "r"(32 * kSoftWarps) : "memory");
+            if (any) {
+              for (int kk = 0; kk < UNIT && k0 + kk < p.tb; ++kk)
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                  const int d = 128 * mt + tid;
+                  if (d >= D) continue;
+                  const uint32_t at = d / L::INNER * L::SUB + kk * L::INNER + d % L::INNER;
+                  // TMA's swizzle: 16-byte pieces of a row exchanged by the row's place in 8 rows (16 or 32 bits apart)
+                  const uint32_t sw = at ^ (L::INNER == 128 ? (at >> 3) & 0x70 : L::INNER == 64 ? (at >> 3) & 0x30 : (at >> 3) & 0x10);
+                  if ((vt[sw] & 0x7fu) != 0x7fu) continue;
+#pragma unroll
+                  for (int r = 0; r < RT; ++r) {
+                    const int pos = p.pos0 + (p.row0 + r) / a.G;
+                    if (k0 + kk <= pos && (a.window <= 0 || k0 + kk > pos - a.window)) o[mt][r] = __int_as_float(0x7fffffff);
+                  }
+                }
+              named_barrier_sync(1, 32 * kSoftWarps);
+              for (uint32_t at = tid; at < L::TILE; at += 128)
+                if ((vt[at] & 0x7fu) == 0x7fu) vt[at] = 0;
+            }
+          }
+          fence_async_smem();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) bar_arrive(pfull + 8 * (j & 1));
+          // ---- the tile before ----
+          if (i > 0) add_sums(j - 1, corr);
+#pragma unroll
+          for (int r = 0; r < RT; ++r) corr[r] = c[r];
         }
-    }
-    if (lane == 0) wv[warp] = unit;
-    __syncthreads();
-    const bool begins = u == seg0, ends = u1 == seg1;
-    float* part = a.part + ((size_t)cta * 2 + (begins ? 1 : 0)) * 16 * (D + 2);
-    for (int i = threadIdx.x; i < RT * D; i += 32 * kWarps) {
-      const int row = i / D, d = i % D;
-      if (row0 + row > last_row) break;
-      float M = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) M = fmaxf(M, wm[w][row]);
-      float A = 0.f, Ls = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float c = M == -INFINITY ? 0.f : ex2(wm[w][row] - M);
-        A += sums[(w * RT + row) * D + d] * (c * wv[w]);
-        Ls += wl[w][row] * c;
+        add_sums(it + tiles - 1, corr);
+        it += tiles;
+        ++seg;
       }
-      if (begins && ends) {
-        const int q_row = row0 + row, head = kvh * a.G + q_row % a.G;
-        const size_t th = (size_t)(r_first + q_row / a.G) * a.H + head;
-        store_out(a, th * D + d, Ls == 0.f ? 0.f : A / Ls);
-        if (d == 0 && a.lse) a.lse[th] = Ls == 0.f ? -INFINITY : M * kLn2 + logf(Ls);
-      } else {
-        part[row * D + d] = A;
-        if (d == 0) {
-          part[16 * D + 2 * row] = M;
-          part[16 * D + 2 * row + 1] = Ls;
+      // ---- the part's result ----
+      over_keys(l, buf, [](float s, float t) { return s + t; });
+      buf ^= 1;
+      const bool begins = u == p.seg0, ends = p.u1 == p.seg1;
+      float* part = a.part + ((size_t)cta * 2 + (begins ? 1 : 0)) * RT * (D + 2);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        const int row = p.row0 + r;
+        if (row > p.last_row) break;
+        const size_t th = (size_t)(p.r_first + row / a.G) * a.H + p.kvh * a.G + row % a.G;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          const int d = 128 * mt + tid;
+          const float A = o[mt][r] * (1.f / kPScale);
+          if (d < D) {
+            if (begins && ends) store_out(a, th * D + d, l[r] == 0.f ? 0.f : A / l[r]);
+            else part[r * D + d] = A;
+          }
+        }
+        if (tid == 0) {
+          if (!(begins && ends)) {
+            part[RT * D + 2 * r] = m[r];
+            part[RT * D + 2 * r + 1] = l[r];
+          } else if (a.lse) {
+            a.lse[th] = l[r] == 0.f ? -INFINITY : m[r] * kLn2 + logf(l[r]);
+          }
         }
       }
+      if (begins && !ends && tid == 0) {
+        // CTAs of the tile's parts: this one to the one that holds its last unit
+        int* dsc = a.desc + 8 * cta;
+        dsc[0] = (int)((p.seg1 * C - 1) / total - cta + 1);
+        dsc[1] = p.r_first;
+        dsc[2] = p.kvh;
+        dsc[3] = p.row0;
+        dsc[4] = p.last_row;
+      }
+      u = p.u1;
     }
-    if (begins && !ends && threadIdx.x == 0) {
-      // CTAs of the tile's parts: this one to the one that holds its last unit
-      const long long last = (seg1 * C - 1) / total;
-      int* dsc = a.desc + 8 * cta;
-      dsc[0] = (int)(last - cta + 1);
-      dsc[1] = r_first;
-      dsc[2] = kvh;
-      dsc[3] = row0;
-      dsc[4] = last_row;
-    }
-    __syncthreads();   // sums is stages again
-    u = u1;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_free(tmem, L::TMEM_COLS);
   }
 }
 
@@ -549,44 +683,58 @@ __global__ void __launch_bounds__(D) paged_attention_merge_kernel(const AttnArgs
   const int parts = dsc[0], row = blockIdx.y, q_row = dsc[3] + row;
   if (parts == 0 || q_row > dsc[4]) return;
   const auto part = [&](int i) {
-    return a.part + ((size_t)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * 16 * (D + 2);
+    return a.part + ((size_t)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * RT * (D + 2);
   };
   float M = -INFINITY;
-  for (int i = 0; i < parts; ++i) M = fmaxf(M, part(i)[16 * D + 2 * row]);
+  for (int i = 0; i < parts; ++i) M = fmaxf(M, part(i)[RT * D + 2 * row]);
   float A = 0.f, Ls = 0.f;
 #pragma unroll 4
   for (int i = 0; i < parts; ++i) {
     const float* p = part(i);
-    const float c = M == -INFINITY ? 0.f : ex2(p[16 * D + 2 * row] - M);
+    const float c = M == -INFINITY ? 0.f : ex2(p[RT * D + 2 * row] - M);
     A += p[row * D + threadIdx.x] * c;
-    Ls += p[16 * D + 2 * row + 1] * c;
+    Ls += p[RT * D + 2 * row + 1] * c;
   }
   const size_t th = (size_t)(dsc[1] + q_row / a.G) * a.H + dsc[2] * a.G + q_row % a.G;
   store_out(a, th * D + threadIdx.x, Ls == 0.f ? 0.f : A / Ls);
   if (threadIdx.x == 0 && a.lse) a.lse[th] = Ls == 0.f ? -INFINITY : M * kLn2 + logf(Ls);
 }
 
-template <int D, bool HL>
-cudaError_t launch(const AttnArgs& a, cudaStream_t st) {
-  using L = Lay<D>;
-  static_assert(kWarps * L::WARP >= kWarps * 16 * D * 4 || HL, "the sums must fit the stages");
-  auto* fn = paged_attention_kernel<D, HL>;
-  const size_t smem = L::smem(a.c.batch);
+template <int D, int PARTS>
+int launch(const AttnArgs& a, cudaStream_t st) {
+  using L = Lay<D, PARTS>;
+  const sf_paged_cache& c = a.c;
+  const uint64_t rows = (uint64_t)c.num_pages * c.n_kv_heads * c.page_size;
+  if (rows > 0x7fffffffull) return fail(SF_ERR_UNSUPPORTED, "the cache has more than 2^31 - 1 rows");
+  const CUtensorMapSwizzle swz = L::INNER == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                                 : L::INNER == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                  : CU_TENSOR_MAP_SWIZZLE_32B;
+  const uint32_t box = c.page_size < UNIT ? c.page_size : UNIT;
+  CUtensorMap mk, mv;
+  if (!make_tensor_map(&mk, CU_TENSOR_MAP_DATA_TYPE_UINT8, c.k_codes, D, rows, D, L::INNER, box, swz) ||
+      !make_tensor_map(&mv, CU_TENSOR_MAP_DATA_TYPE_UINT8, c.v_codes, D, rows, D, L::INNER, box, swz))
+    return fail(SF_ERR_CUDA, "cuTensorMapEncodeTiled failed for the cache");
+  auto* fn = paged_attention_kernel<D, PARTS>;
+  const size_t smem = L::smem(c.batch);
+  if (smem > (size_t)device_info().smem_optin && device_info().smem_optin > 0)
+    return fail(SF_ERR_UNSUPPORTED, "batch %d is too large for head_dim %d", c.batch, D);
   cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return e;
+  if (e != cudaSuccess) return cuda_fail(e, "paged_attention_kernel shared memory");
+  // what shared memory, TMEM and registers let an SM hold
   int per_sm = (int)(228 * 1024 / (smem + 2048));
-  const int most = D <= 128 ? kMaxCtasPerSm : 2;
-  per_sm = per_sm > most ? most : per_sm < 1 ? 1 : per_sm;
+  const int most = D == 64 ? 4 : D <= 128 ? 3 : 1;
+  if (per_sm > most) per_sm = most;
+  if (per_sm > 512 / (int)L::TMEM_COLS) per_sm = 512 / (int)L::TMEM_COLS;
+  if (per_sm < 1) per_sm = 1;
   // no more CTAs than units there may be
-  const long long cap = ((long long)a.c.pages_per_seq * a.c.page_size + L::UNIT - 1) / L::UNIT;
-  const long long tiles = (long long)a.T * a.G / (HL ? 8 : 16) + a.c.batch;
-  const double units = (double)cap * (double)tiles * a.c.n_kv_heads;
+  const double cap = ((double)c.pages_per_seq * c.page_size + UNIT - 1) / UNIT;
+  const double units = cap * ((double)a.T * a.G / RT + c.batch) * c.n_kv_heads;
   int grid = device_info().sms * per_sm;
   if (units < grid) grid = (int)units;
-  e = launch_kernel(fn, grid, 32 * kWarps, smem, st, false, a);
-  if (e != cudaSuccess) return e;
+  e = launch_kernel(fn, grid, kThreads, smem, st, true, mk, mv, a);
+  if (e != cudaSuccess) return cuda_fail(e, "paged_attention_kernel launch");
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid, HL ? 8 : 16);
+  cfg.gridDim = dim3((unsigned)grid, RT);
   cfg.blockDim = dim3(D);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -594,7 +742,10 @@ cudaError_t launch(const AttnArgs& a, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_attention_merge_kernel<D>, a);
+  e = cudaLaunchKernelEx(&cfg, paged_attention_merge_kernel<D>, a);
+  if (e != cudaSuccess) return cuda_fail(e, "paged_attention_merge_kernel launch");
+  g_launches.fetch_add(2, std::memory_order_relaxed);
+  return SF_OK;
 }
 
 }  // namespace
@@ -607,7 +758,7 @@ extern "C" {
 size_t sf_paged_attention_workspace_bytes(int head_dim) {
   if (head_dim <= 0) return 0;
   const size_t ctas = (size_t)device_info().sms * kMaxCtasPerSm;
-  return ctas * (2 * 16 * ((size_t)head_dim + 2) * 4 + 32);
+  return ctas * (2 * RT * ((size_t)head_dim + 2) * 4 + 32);
 }
 
 int sf_paged_attention(const sf_paged_cache* cache, const void* q, int q_dtype, long long qts, long long qhs, void* out,
@@ -631,19 +782,14 @@ int sf_paged_attention(const sf_paged_cache* cache, const void* q, int q_dtype, 
   a.scale = scale;
   if ((long long)T * a.G > 0x7fffffffll) return fail(SF_ERR_UNSUPPORTED, "too many query rows");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // 8 rows in two parts when a sequence has no more rows, or for fp32 queries, which one fp16 part cannot hold
-  const bool hl = q_dtype == SF_F32 || (!cache->starts && (long long)(T / cache->batch) * a.G <= 8) || (T == 1 && a.G <= 8);
   const auto go = [&](auto d) {
     constexpr int DD = decltype(d)::value;
-    return hl ? launch<DD, true>(a, st) : launch<DD, false>(a, st);
+    return q_dtype == SF_BF16 ? launch<DD, 2>(a, st) : q_dtype == SF_F16 ? launch<DD, 3>(a, st) : launch<DD, 6>(a, st);
   };
-  const cudaError_t e = D == 64    ? go(std::integral_constant<int, 64>())
-                        : D == 96  ? go(std::integral_constant<int, 96>())
-                        : D == 128 ? go(std::integral_constant<int, 128>())
-                                   : go(std::integral_constant<int, 256>());
-  if (e != cudaSuccess) return cuda_fail(e, "paged_attention_kernel launch");
-  g_launches.fetch_add(2, std::memory_order_relaxed);
-  return SF_OK;
+  return D == 64    ? go(std::integral_constant<int, 64>())
+         : D == 96  ? go(std::integral_constant<int, 96>())
+         : D == 128 ? go(std::integral_constant<int, 128>())
+                    : go(std::integral_constant<int, 256>());
 }
 
 }  // extern "C"

@@ -2,9 +2,10 @@
 //
 //   p_j = softmax_j(scale * q . k_j),  out = sum_j p_j v_j,  k_j = code * scale of its page and head
 //
-// The softmax keeps a running reference m and sum l: keys in order, out and l are multiplied by e^(m - m') when the
-// reference grows to m'.  Parts of a row's keys merge by the same rule.  m is the largest score plus the logarithm of
-// its page's V scale, so that a weight times that scale is at most 1.
+// The softmax keeps a running reference m and sum l of e^(score - m): keys in order, out and l are multiplied by
+// e^(m - m') when the reference moves to m'.  Parts of a row's keys merge by the same rule.  m is a largest score plus
+// the logarithm of its page's V scale; it moves only when a key would exceed it by a factor of 2, so that a weight
+// times its scale is at most 2 and most tiles of keys need no reduction over the threads.
 //
 // A call's work is a list of units of 128 keys, for each (sequence, kv head, tile of RT query rows) in turn; a row is
 // one (new token, query head of the kv head's group), so that a group reads its keys once.  Every CTA takes an equal,
@@ -18,7 +19,7 @@
 //    added, scaled, in fp32.  2 parts hold a bf16 row, 3 an fp16 row, 6 an fp32 row (24 bits; elements far below the
 //    row's largest lose what lies under 2^-17, 2^-21 or 2^-33 of it).
 //  * out^T[d, column] = V^T P^T: the head's columns are the MMA's rows, V is its transposed operand.  Weights are cut
-//    into as many parts as queries: 8, 12 or 24 bits, and no coarser than 2^-22 of the largest for bf16.
+//    into as many parts as queries: 8, 12 or 24 bits, and no coarser than 2^-21 of the reference for bf16.
 // Both scores and partial sums go to fresh TMEM buffers, two each; a thread is one key for the scores and one column d
 // for the sums, which it keeps in registers in fp32.
 //
@@ -40,10 +41,11 @@ extern std::atomic<long long> g_launches;
 namespace {
 
 constexpr int UNIT = 128;            // keys of a tile
-constexpr int RT = 8;                // query rows of a tile
+constexpr int kMaxRows = 8;          // query rows of a tile: 8, or 1 where no sequence has more
 constexpr int kSoftWarps = 4, kProdWarp = 4, kMmaWarp = 5, kThreads = 192;
 constexpr int kMaxCtasPerSm = 4;
-constexpr float kPScale = 256.f;     // of the largest weight: within e4m3
+constexpr float kPScale = 128.f;     // of a weight: at most 256, within e4m3
+constexpr float kNone = -1e30f;      // the reference of a part without a key
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr unsigned kErrProd = 1u << 17, kErrMma = 1u << 18, kErrSoft = 1u << 19, kErrDrain = 1u << 22;
 
@@ -53,7 +55,7 @@ struct AttnArgs {
   long long qts, qhs;
   void* out;
   float* lse;
-  float* part;          // [CTA][2][RT x D unnormalised sums, then RT x (m, l)]
+  float* part;          // [CTA][2][rows x D unnormalised sums, then rows x (m, l)], up to kMaxRows
   int* desc;            // [CTA][8]: the tile that this CTA began and others ended
   int H, T, G, q_dtype, out_dtype, window, lg_page;
   float scale;
@@ -76,8 +78,79 @@ __device__ __forceinline__ void store_out(const AttnArgs& a, size_t o, float v) 
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float warp_max(float x) {
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Arrives at barrier 1 of the softmax warps, and says whether any thread's p is true.
+__device__ __forceinline__ bool any_of(bool p) {
+  int any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbar.red.or.pred q, 1, %2, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"((int)p), "r"(32 * 4)
+      : "memory");
+  return any;
+}
+// d = a * b + c and d = a + b over rows, two to an instruction
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+template <int R, typename A, typename B, typename C>
+__device__ __forceinline__ void fma_rows(float (&d)[R], A&& a, B&& b, C&& c) {
+  if constexpr (R % 2 == 0) {
+#pragma unroll
+    for (int r = 0; r < R; r += 2) {
+      uint64_t v;
+      asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(pack2(a(r), a(r + 1))), "l"(pack2(b(r), b(r + 1))), "l"(pack2(c(r), c(r + 1))));
+      unpack2(v, d[r], d[r + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < R; ++r) d[r] = fmaf(a(r), b(r), c(r));
+  }
+}
+template <int R, typename A, typename B>
+__device__ __forceinline__ void mul_rows(float (&d)[R], A&& a, B&& b) {
+  if constexpr (R % 2 == 0) {
+#pragma unroll
+    for (int r = 0; r < R; r += 2) {
+      uint64_t v;
+      asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(pack2(a(r), a(r + 1))), "l"(pack2(b(r), b(r + 1))));
+      unpack2(v, d[r], d[r + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < R; ++r) d[r] = a(r) * b(r);
+  }
+}
+template <int R, typename A, typename B>
+__device__ __forceinline__ void add_rows(float (&d)[R], A&& a, B&& b) {
+  if constexpr (R % 2 == 0) {
+#pragma unroll
+    for (int r = 0; r < R; r += 2) {
+      uint64_t v;
+      asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(pack2(a(r), a(r + 1))), "l"(pack2(b(r), b(r + 1))));
+      unpack2(v, d[r], d[r + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < R; ++r) d[r] = a(r) + b(r);
+  }
 }
 // four values of at most 448, to e4m3 codes, leaving what they lack, times 16
 __device__ __forceinline__ uint32_t take_e4m3(float (&v)[4]) {
@@ -98,7 +171,7 @@ __device__ __forceinline__ uint32_t take_e4m3(float (&v)[4]) {
 //  128 rows are 128 / INNER sub-tiles, and those beyond the head's columns are whatever lies there, in TMEM lanes
 //  that nothing looks at.
 //  Q^T: [column][d] in cores of 8 columns x 16 bytes, without swizzle.  P^T: [key][16 columns], likewise.
-template <int D, int PARTS>
+template <int D, int PARTS, int RT>
 struct Lay {
   static constexpr int INNER = D % 128 == 0 ? 128 : D == 64 ? 64 : 32;
   static constexpr int SUBS = D / INNER;                  // sub-tiles of a tile
@@ -132,6 +205,7 @@ struct Part {
   int tile_lo, all_lo, all_hi;   // first key that some row sees; keys that every row sees
   long long u1, seg0, seg1;   // end of the part; units of the whole tile
 };
+template <int RT>
 __device__ __forceinline__ Part part_at(const AttnArgs& a, const SeqInfo* info, long long u, long long u_end, int& b) {
   while (b + 1 < a.c.batch && info[b + 1].first <= u) ++b;
   const SeqInfo s = info[b];
@@ -159,14 +233,14 @@ __device__ __forceinline__ Part part_at(const AttnArgs& a, const SeqInfo* info, 
   return p;
 }
 
-template <int D, int PARTS>
+template <int D, int PARTS, int RT>
 __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : D <= 128 ? 3 : 1)
     paged_attention_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
                            const AttnArgs a) {
-  using L = Lay<D, PARTS>;
+  using L = Lay<D, PARTS, RT>;
   constexpr int N = L::N, MT = L::MT, ST = L::STAGES;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ __align__(16) float red[2][RT][4];           // one number per row and softmax warp, two buffers
+  __shared__ __align__(16) float red[RT][4];              // one number per row and softmax warp
   __shared__ float row_f[RT];
   __shared__ long long wsum[kThreads / 32];
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
@@ -267,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : D <= 128 ? 3 : 1)
     uint32_t it = 0;
     bool ok = true;
     while (u < u_end && ok) {
-      const Part p = part_at(a, info, u, u_end, b);
+      const Part p = part_at<RT>(a, info, u, u_end, b);
       const int* pages = a.c.block_table + (size_t)p.b * a.c.pages_per_seq;
       const auto page_of = [&](int key) {
         return lane < boxes && key < p.tb ? __ldg(pages + (key >> a.lg_page)) : -1;
@@ -350,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : D <= 128 ? 3 : 1)
         return true;
       };
       while (u < u_end && ok) {
-        const Part p = part_at(a, info, u, u_end, b);
+        const Part p = part_at<RT>(a, info, u, u_end, b);
         const int tiles = p.tb > p.ta ? (p.tb - p.ta + UNIT - 1) / UNIT : 0;
         if (tiles > 0) {
           ok = bar_wait(qfull, seg & 1, kErrMma, abort_flag);
@@ -379,40 +453,16 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : D <= 128 ? 3 : 1)
     const int tid = threadIdx.x;
     const uint32_t my_lanes = (uint32_t)(32 * warp) << 16;
     uint32_t it = 0, seg = 0;
-    float part_scale[PARTS];
-#pragma unroll
-    for (int i = 0; i < PARTS; ++i) part_scale[i] = __int_as_float((127 - 4 * i) << 23);
-    // one number per row over the 128 threads: a row's lanes hold its 4 warps' results after the barrier
-    const auto over_keys = [&](float (&v)[RT], int buf, auto&& op) {
-#pragma unroll
-      for (int n = RT / 2, o = 16; n >= 1; n >>= 1, o >>= 1) {
-        const bool up = lane & o;
-#pragma unroll
-        for (int i = 0; i < n; ++i) {
-          const float mine = up ? v[i + n] : v[i], other = up ? v[i] : v[i + n];
-          v[i] = op(mine, __shfl_xor_sync(0xffffffffu, other, o));
-        }
-      }
-#pragma unroll
-      for (int o = 16 / RT; o >= 1; o >>= 1) v[0] = op(v[0], __shfl_xor_sync(0xffffffffu, v[0], o));
-      if (lane % (32 / RT) == 0) red[buf][lane / (32 / RT)][warp] = v[0];
-      named_barrier_sync(1, 32 * kSoftWarps);
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        const float4 w = *reinterpret_cast<const float4*>(red[buf][r]);
-        v[r] = op(op(w.x, w.y), op(w.z, w.w));
-      }
-    };
-    int buf = 0;
+    const auto part_scale = [](int part) { return __int_as_float((127 - 4 * part) << 23); };   // 2^(-4 part)
     while (u < u_end) {
-      const Part p = part_at(a, info, u, u_end, b);
+      const Part p = part_at<RT>(a, info, u, u_end, b);
       const int tiles = p.tb > p.ta ? (p.tb - p.ta + UNIT - 1) / UNIT : 0;
-      float m[RT], l[RT], o[MT][RT], corr[RT];
+      float nm[RT], l[RT], o[MT][RT];   // minus the reference; this thread's share of l; the sums of column tid
+      uint32_t fresh = (1u << RT) - 1;  // rows that have no reference yet; the same in every thread
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
-        m[r] = -INFINITY;
+        nm[r] = 0.f;
         l[r] = 0.f;
-        corr[r] = 0.f;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) o[mt][r] = 0.f;
       }
@@ -426,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : D <= 128 ? 3 : 1)
           const long long qo = (long long)(p.r_first + row / a.G) * a.qts + (long long)(p.kvh * a.G + row % a.G) * a.qhs + d0;
 #pragma unroll
           for (int e = 0; e < E; ++e) {
-            v[e] = row <= p.last_row ? load_q(a, qo + e) : 0.f;
+            v[e] = r < RT && row <= p.last_row ? load_q(a, qo + e) : 0.f;
             top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
           }
 #pragma unroll
@@ -434,21 +484,23 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : D <= 128 ? 3 : 1)
           // the row's largest value to [128, 256) by a power of two
           const int ex = min(max((int)(top >> 23) - 134, -126), 126);
           const float down = __int_as_float((127 - ex) << 23);
-          if ((tid & 15) == 0) {
+          if (r < RT && (tid & 15) == 0) {
             // an infinity would saturate: its row is NaN
             row_f[r] = top >= 0x7f800000u ? __int_as_float(0x7fffffff)
                                           : __int_as_float((127 + ex) << 23) * (a.scale * kLog2e);
           }
+          if (r < RT) {
 #pragma unroll
-          for (int e = 0; e < E; ++e) {
-            const int d = d0 + e;
-            float x = v[e] * down;
+            for (int e = 0; e < E; ++e) {
+              const int d = d0 + e;
+              float x = v[e] * down;
 #pragma unroll
-            for (int i = 0; i < PARTS; ++i) {
-              const uint8_t c = to_e4m3(x);
-              x = (x - from_e4m3(c)) * 16.f;
-              const int col = i * RT + r;
-              mem[L::Q0 + (col / 8) * (D * 8) + (d / 16) * 128 + (col % 8) * 16 + d % 16] = c;
+              for (int i = 0; i < PARTS; ++i) {
+                const uint8_t c = to_e4m3(x);
+                x = (x - from_e4m3(c)) * 16.f;
+                const int col = i * RT + r;
+                mem[L::Q0 + (col / 8) * (D * 8) + (d / 16) * 128 + (col % 8) * 16 + d % 16] = c;
+              }
             }
           }
           fence_async_smem();
@@ -477,25 +529,22 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : D <= 128 ? 3 : 1)
         float ks, vs;
         scales_of(page, ks, vs);
 
-        // adds the sums of tile j, which are relative to the reference after it
-        const auto add_sums = [&](uint32_t j, const float (&c)[RT]) {
+        const auto add_sums = [&](uint32_t j) {
           bar_wait(ofull + 8 * (j & 1), (j >> 1) & 1, kErrSoft, abort_flag);
           tc_fence_after();
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-            for (int r = 0; r < RT; ++r) o[mt][r] *= c[r];
+          for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int n = 0; n < N; n += 16) {
               uint32_t w[16];
               tmem_ld(tmem_o + my_lanes + ((j & 1) * MT + mt) * N + n, w);
               tmem_wait(w);
 #pragma unroll
-              for (int e = 0; e < 16; ++e)
-                if (n + e < RT * PARTS)
-                  o[mt][(n + e) % RT] = fmaf(__uint_as_float(w[e]), part_scale[(n + e) / RT], o[mt][(n + e) % RT]);
+              for (int q = 0; q < 16 / RT; ++q)
+                if (n / RT + q < PARTS)
+                  fma_rows(o[mt], [&](int r) { return __uint_as_float(w[(RT * q + r) % 16]); },
+                           [&](int) { return part_scale(n / RT + q); }, [&](int r) { return o[mt][r]; });
             }
-          }
         };
 
         for (int i = 0; i < tiles; ++i) {
@@ -506,10 +555,9 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : D <= 128 ? 3 : 1)
           page = page1;
           scales_of(page, ks, vs);
           page1 = page_of(key + 2 * UNIT);
-          // ---- scores ----
-          float x[RT];
-#pragma unroll
-          for (int r = 0; r < RT; ++r) x[r] = 0.f;
+          // ---- scores, less the reference ----
+          float y[RT], fk[RT];
+          mul_rows(fk, [&](int r) { return f[r]; }, [&](int) { return ks_i; });
           bar_wait(sfull + 8 * (j & 1), (j >> 1) & 1, kErrSoft, abort_flag);
           tc_fence_after();
 #pragma unroll
@@ -518,58 +566,99 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : D <= 128 ? 3 : 1)
             tmem_ld(tmem_s + my_lanes + (j & 1) * N + n, w);
             tmem_wait(w);
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (n + e < RT * PARTS)
-                x[(n + e) % RT] = fmaf(__uint_as_float(w[e]), part_scale[(n + e) / RT], x[(n + e) % RT]);
-          }
-          const bool alike = k0 >= p.all_lo && min(k0 + UNIT, p.tb) <= p.all_hi;   // rows see the same of these keys
+            for (int q = 0; q < 16 / RT; ++q) {
+              const int part = n / RT + q;
+              if (part == 0) {
 #pragma unroll
-          for (int r = 0; r < RT; ++r) x[r] = there ? x[r] * (f[r] * ks_i) : -INFINITY;
-          if (!alike) {
+                for (int r = 0; r < RT; ++r) y[r] = __uint_as_float(w[r % 16]);
+              } else if (part < PARTS) {
+                fma_rows(y, [&](int r) { return __uint_as_float(w[(RT * q + r) % 16]); },
+                         [&](int) { return part_scale(part); }, [&](int r) { return y[r]; });
+              }
+            }
+          }
+          fma_rows(y, [&](int r) { return y[r]; }, [&](int r) { return fk[r]; }, [&](int r) { return nm[r]; });
+          const bool alike = k0 >= p.all_lo && min(k0 + UNIT, p.tb) <= p.all_hi;   // rows see the same of these keys
+          if (__builtin_expect(!there, 0)) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r) y[r] = -INFINITY;
+          }
+          if (__builtin_expect(!alike, 0)) {
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
               const int pos = p.pos0 + (p.row0 + r) / a.G;
-              if (key > pos || (a.window > 0 && key <= pos - a.window)) x[r] = -INFINITY;
+              if (key > pos || (a.window > 0 && key <= pos - a.window)) y[r] = -INFINITY;
             }
           }
-          // ---- reference ----
-          const float lv = fmaxf(__log2f(vs_i), -60.f);
-          float top[RT];
+          // ---- the reference, if a key exceeds it by more than a factor of 2 ----
+          const float lv = fmaxf(lg2(vs_i), -60.f);
+          float over = y[0];
 #pragma unroll
-          for (int r = 0; r < RT; ++r) top[r] = x[r] + lv;
-          over_keys(top, buf, [](float s, float t) { return fmaxf(s, t); });
-          buf ^= 1;
-          float c[RT], pw[RT];
-          const float fold = vs_i * kPScale;
+          for (int r = 1; r < RT; ++r) over = fmaxf(over, y[r]);
+          bool added = i == 0;
+          if (any_of(over + lv > 1.f) || fresh) {
+            if (!added) add_sums(j - 1);
+            added = true;
 #pragma unroll
-          for (int r = 0; r < RT; ++r) {
-            const float mn = fmaxf(m[r], top[r]), ref = mn == -INFINITY ? 0.f : mn;
-            c[r] = ex2(m[r] - ref);
-            m[r] = mn;
-            const float w = ex2(x[r] - ref);
-            l[r] = fmaf(l[r], c[r], w);
-            pw[r] = w * fold;
+            for (int r = 0; r < RT; ++r) {
+              const float top = warp_max(y[r] + lv);
+              if (lane == 0) red[r][warp] = top;
+            }
+            named_barrier_sync(1, 32 * kSoftWarps);
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+              const float4 w = *reinterpret_cast<const float4*>(red[r]);
+              const float top = fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w));
+              const bool first = fresh & (1u << r);      // l and o are zero then
+              if (first && top == -INFINITY) continue;   // the row has seen no key
+              const float up = first ? top : fmaxf(top, 0.f), c = first ? 1.f : ex2(-up);
+              fresh &= ~(1u << r);
+              nm[r] -= up;
+              y[r] -= up;
+              l[r] *= c;
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) o[mt][r] *= c;
+            }
+            named_barrier_sync(1, 32 * kSoftWarps);   // red may be written again
           }
           // ---- weights to shared memory ----
-          uint32_t w[N / 8][2];
+          float pw[RT];
 #pragma unroll
-          for (int r = 0; r < RT; r += 4) {
-            float v[4] = {pw[r], pw[r + 1], pw[r + 2], pw[r + 3]};
-#pragma unroll
-            for (int q = 0; q < N / RT; ++q) {
-              if (q < PARTS - 1) w[q][r / 4] = take_e4m3(v);
-              else if (q < PARTS) w[q][r / 4] = to_e4m3x2(v[0], v[1]) | (to_e4m3x2(v[2], v[3]) << 16);
-              else w[q][r / 4] = 0;
-            }
-          }
+          for (int r = 0; r < RT; ++r) pw[r] = ex2(y[r]);
+          add_rows(l, [&](int r) { return l[r]; }, [&](int r) { return pw[r]; });
+          const float fold = vs_i * kPScale;
+          mul_rows(pw, [&](int r) { return pw[r]; }, [&](int) { return fold; });
           uint8_t* pb = mem + L::P0 + (j & 1) * L::P;
+          if constexpr (RT >= 4) {
+            uint32_t w[N / RT][RT / 4];
 #pragma unroll
-          for (int n = 0; n < N / 16; ++n)
-            *reinterpret_cast<uint4*>(pb + n * UNIT * 16 + tid * 16) =
-                make_uint4(w[2 * n][0], w[2 * n][1], w[2 * n + 1][0], w[2 * n + 1][1]);
+            for (int r = 0; r < RT; r += 4) {
+              float v[4] = {pw[r], pw[r + 1], pw[r + 2], pw[r + 3]};
+#pragma unroll
+              for (int q = 0; q < N / RT; ++q) {
+                if (q < PARTS - 1) w[q][r / 4] = take_e4m3(v);
+                else if (q < PARTS) w[q][r / 4] = to_e4m3x2(v[0], v[1]) | (to_e4m3x2(v[2], v[3]) << 16);
+                else w[q][r / 4] = 0;
+              }
+            }
+            const uint32_t* all = &w[0][0];
+#pragma unroll
+            for (int n = 0; n < N / 16; ++n)
+              *reinterpret_cast<uint4*>(pb + n * UNIT * 16 + tid * 16) = make_uint4(all[4 * n], all[4 * n + 1], all[4 * n + 2], all[4 * n + 3]);
+          } else {
+            // one row: its parts are the first columns, the others zeros
+            uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q) {
+              const uint32_t c = to_e4m3(pw[0]);
+              pw[0] = (pw[0] - from_e4m3((uint8_t)c)) * 16.f;
+              w[q / 4] |= c << (8 * (q % 4));
+            }
+            *reinterpret_cast<uint4*>(pb + tid * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
           // ---- values that must not reach a sum, where 0 * NaN is not 0 ----
           uint8_t* vt = mem + L::V0 + (j % ST) * L::TILE;
-          if (!__all_sync(0xffffffffu, there)) {
+          if (__builtin_expect(!__all_sync(0xffffffffu, there), 0)) {
             // rows of no key of the sequence: whatever their page holds becomes 0
             bar_wait(vfull + 8 * (j % ST), (j / ST) & 1, kErrSoft, abort_flag);
             if (!there) {
@@ -580,7 +669,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : D <= 128 ? 3 : 1)
                   *reinterpret_cast<uint4*>(vt + s * L::SUB + tid * L::INNER + e) = make_uint4(0, 0, 0, 0);
             }
           }
-          if (!alike) {
+          if (__builtin_expect(!alike, 0)) {
             // a NaN code reaches only the rows that see its key: it is put into their sums by hand, and becomes 0
             bar_wait(vfull + 8 * (j % ST), (j / ST) & 1, kErrSoft, abort_flag);
             named_barrier_sync(1, 32 * kSoftWarps);   // the zeros above
@@ -589,9 +678,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : D <= 128 ? 3 : 1)
               const uint32_t y = *reinterpret_cast<const uint32_t*>(vt + at);
               found |= ((y & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
             }
-            int any;
-            asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, %2, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
-                         : "=r"(any) : "r"(found), "r"(32 * kSoftWarps) : "memory");
+            const bool any = any_of(found != 0);
             if (any) {
               for (int kk = 0; kk < UNIT && k0 + kk < p.tb; ++kk)
 #pragma unroll
@@ -617,20 +704,28 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : D <= 128 ? 3 : 1)
           tc_fence_before();
           __syncwarp();
           if (lane == 0) bar_arrive(pfull + 8 * (j & 1));
-          // ---- the tile before ----
-          if (i > 0) add_sums(j - 1, corr);
-#pragma unroll
-          for (int r = 0; r < RT; ++r) corr[r] = c[r];
+          if (!added) add_sums(j - 1);
         }
-        add_sums(it + tiles - 1, corr);
+        add_sums(it + tiles - 1);
         it += tiles;
         ++seg;
       }
       // ---- the part's result ----
-      over_keys(l, buf, [](float s, float t) { return s + t; });
-      buf ^= 1;
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+#pragma unroll
+        for (int o2 = 16; o2; o2 >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o2);
+        if (lane == 0) red[r][warp] = l[r];
+      }
+      named_barrier_sync(1, 32 * kSoftWarps);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        const float4 w = *reinterpret_cast<const float4*>(red[r]);
+        l[r] = (w.x + w.y) + (w.z + w.w);
+      }
+      named_barrier_sync(1, 32 * kSoftWarps);   // red may be written again
       const bool begins = u == p.seg0, ends = p.u1 == p.seg1;
-      float* part = a.part + ((size_t)cta * 2 + (begins ? 1 : 0)) * RT * (D + 2);
+      float* part = a.part + ((size_t)cta * 2 + (begins ? 1 : 0)) * kMaxRows * (D + 2);
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
         const int row = p.row0 + r;
@@ -647,10 +742,10 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : D <= 128 ? 3 : 1)
         }
         if (tid == 0) {
           if (!(begins && ends)) {
-            part[RT * D + 2 * r] = m[r];
+            part[RT * D + 2 * r] = fresh & (1u << r) ? kNone : -nm[r];
             part[RT * D + 2 * r + 1] = l[r];
           } else if (a.lse) {
-            a.lse[th] = l[r] == 0.f ? -INFINITY : m[r] * kLn2 + logf(l[r]);
+            a.lse[th] = l[r] == 0.f ? -INFINITY : -nm[r] * kLn2 + logf(l[r]);
           }
         }
       }
@@ -675,7 +770,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : D <= 128 ? 3 : 1)
 }
 
 // One block for each (CTA that began a divided tile, row of it): the parts by the same rule, in order.
-template <int D>
+template <int D, int RT>
 __global__ void __launch_bounds__(D) paged_attention_merge_kernel(const AttnArgs a) {
   griddep_launch_dependents();
   griddep_wait();
@@ -683,15 +778,15 @@ __global__ void __launch_bounds__(D) paged_attention_merge_kernel(const AttnArgs
   const int parts = dsc[0], row = blockIdx.y, q_row = dsc[3] + row;
   if (parts == 0 || q_row > dsc[4]) return;
   const auto part = [&](int i) {
-    return a.part + ((size_t)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * RT * (D + 2);
+    return a.part + ((size_t)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * kMaxRows * (D + 2);
   };
-  float M = -INFINITY;
+  float M = kNone;
   for (int i = 0; i < parts; ++i) M = fmaxf(M, part(i)[RT * D + 2 * row]);
   float A = 0.f, Ls = 0.f;
 #pragma unroll 4
   for (int i = 0; i < parts; ++i) {
     const float* p = part(i);
-    const float c = M == -INFINITY ? 0.f : ex2(p[RT * D + 2 * row] - M);
+    const float c = ex2(p[RT * D + 2 * row] - M);
     A += p[row * D + threadIdx.x] * c;
     Ls += p[RT * D + 2 * row + 1] * c;
   }
@@ -700,9 +795,9 @@ __global__ void __launch_bounds__(D) paged_attention_merge_kernel(const AttnArgs
   if (threadIdx.x == 0 && a.lse) a.lse[th] = Ls == 0.f ? -INFINITY : M * kLn2 + logf(Ls);
 }
 
-template <int D, int PARTS>
+template <int D, int PARTS, int RT>
 int launch(const AttnArgs& a, cudaStream_t st) {
-  using L = Lay<D, PARTS>;
+  using L = Lay<D, PARTS, RT>;
   const sf_paged_cache& c = a.c;
   const uint64_t rows = (uint64_t)c.num_pages * c.n_kv_heads * c.page_size;
   if (rows > 0x7fffffffull) return fail(SF_ERR_UNSUPPORTED, "the cache has more than 2^31 - 1 rows");
@@ -714,7 +809,7 @@ int launch(const AttnArgs& a, cudaStream_t st) {
   if (!make_tensor_map(&mk, CU_TENSOR_MAP_DATA_TYPE_UINT8, c.k_codes, D, rows, D, L::INNER, box, swz) ||
       !make_tensor_map(&mv, CU_TENSOR_MAP_DATA_TYPE_UINT8, c.v_codes, D, rows, D, L::INNER, box, swz))
     return fail(SF_ERR_CUDA, "cuTensorMapEncodeTiled failed for the cache");
-  auto* fn = paged_attention_kernel<D, PARTS>;
+  auto* fn = paged_attention_kernel<D, PARTS, RT>;
   const size_t smem = L::smem(c.batch);
   if (smem > (size_t)device_info().smem_optin && device_info().smem_optin > 0)
     return fail(SF_ERR_UNSUPPORTED, "batch %d is too large for head_dim %d", c.batch, D);
@@ -742,7 +837,7 @@ int launch(const AttnArgs& a, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, paged_attention_merge_kernel<D>, a);
+  e = cudaLaunchKernelEx(&cfg, paged_attention_merge_kernel<D, RT>, a);
   if (e != cudaSuccess) return cuda_fail(e, "paged_attention_merge_kernel launch");
   g_launches.fetch_add(2, std::memory_order_relaxed);
   return SF_OK;
@@ -758,7 +853,7 @@ extern "C" {
 size_t sf_paged_attention_workspace_bytes(int head_dim) {
   if (head_dim <= 0) return 0;
   const size_t ctas = (size_t)device_info().sms * kMaxCtasPerSm;
-  return ctas * (2 * RT * ((size_t)head_dim + 2) * 4 + 32);
+  return ctas * (2 * kMaxRows * ((size_t)head_dim + 2) * 4 + 32);
 }
 
 int sf_paged_attention(const sf_paged_cache* cache, const void* q, int q_dtype, long long qts, long long qhs, void* out,
@@ -784,7 +879,9 @@ int sf_paged_attention(const sf_paged_cache* cache, const void* q, int q_dtype, 
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const auto go = [&](auto d) {
     constexpr int DD = decltype(d)::value;
-    return q_dtype == SF_BF16 ? launch<DD, 2>(a, st) : q_dtype == SF_F16 ? launch<DD, 3>(a, st) : launch<DD, 6>(a, st);
+    if ((long long)T * a.G <= cache->batch)
+      return q_dtype == SF_BF16 ? launch<DD, 2, 1>(a, st) : q_dtype == SF_F16 ? launch<DD, 3, 1>(a, st) : launch<DD, 6, 1>(a, st);
+    return q_dtype == SF_BF16 ? launch<DD, 2, 8>(a, st) : q_dtype == SF_F16 ? launch<DD, 3, 8>(a, st) : launch<DD, 6, 8>(a, st);
   };
   return D == 64    ? go(std::integral_constant<int, 64>())
          : D == 96  ? go(std::integral_constant<int, 96>())

@@ -252,7 +252,6 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : D <= 128 ? 3 : 1)
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(mem + L::CTL + 256);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(mem + L::CTL + 264);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  griddep_launch_dependents();
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
       bar_init(kfull + 8 * s, 1);
@@ -761,6 +760,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : D <= 128 ? 3 : 1)
       u = p.u1;
     }
   }
+  griddep_launch_dependents();   // not before: the merge's blocks would wait in the place of the next call's
   tc_fence_before();
   __syncthreads();
   if (warp == kMmaWarp) {
@@ -772,7 +772,6 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : D <= 128 ? 3 : 1)
 // One block for each (CTA that began a divided tile, row of it): the parts by the same rule, in order.
 template <int D, int RT>
 __global__ void __launch_bounds__(D) paged_attention_merge_kernel(const AttnArgs a) {
-  griddep_launch_dependents();
   griddep_wait();
   const int* dsc = a.desc + 8 * blockIdx.x;
   const int parts = dsc[0], row = blockIdx.y, q_row = dsc[3] + row;

@@ -30,78 +30,194 @@ struct NormArgs {
   float eps;
 };
 
-__device__ __forceinline__ float load_w(const NormArgs& a, int k) {
-  if (!a.w) return 1.f;
-  if (a.w_dtype == SF_F32) return static_cast<const float*>(a.w)[k];
-  if (a.w_dtype == SF_F16) return __half2float(static_cast<const __half*>(a.w)[k]);
-  return __bfloat162float(static_cast<const __nv_bfloat16*>(a.w)[k]);
+// The 8 weights of columns k .. k + 7.
+template <bool VEC>
+__device__ __forceinline__ void load_weights(const NormArgs& a, int k, float (&w)[8]) {
+  const auto from = [&](auto* p) {
+    if constexpr (VEC) {
+      load8(p + k, w);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = k + e < a.K ? to_f32(p[k + e]) : 0.f;
+    }
+  };
+  if (!a.w) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = 1.f;
+  } else if (a.w_dtype == SF_F32) {
+    from(static_cast<const float*>(a.w));
+  } else if (a.w_dtype == SF_F16) {
+    from(static_cast<const __half*>(a.w));
+  } else {
+    from(static_cast<const __nv_bfloat16*>(a.w));
+  }
 }
 
-// One block per row; a thread takes 8 columns at a time, so that 16 neighbouring lanes hold one 128-column group.
-template <typename TX>
-__global__ void __launch_bounds__(256) rms_norm_kernel(const NormArgs a) {
-  __shared__ float part[8];
-  const size_t row = blockIdx.x;
-  const TX* x = static_cast<const TX*>(a.x) + row * a.ldx;
-  const TX* r = a.r ? static_cast<const TX*>(a.r) + row * a.ldr : nullptr;
-  float rstd = 1.f;
-  if (a.norm) {
-    float ss = 0.f;
-    for (int k = threadIdx.x; k < a.K; k += 256) {
-      const float h = to_f32(x[k]) + (r ? to_f32(r[k]) : 0.f);
-      ss = fmaf(h, h, ss);
-    }
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_cols(const T* p, int k, int K, float (&v)[8]) {
+  if constexpr (VEC) {
+    if (k < K) {
+      load8(p + k, v);
+    } else {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = ss;
-    __syncthreads();
-    ss = 0.f;
-    for (int i = 0; i < 8; ++i) ss += part[i];
-    rstd = 1.f / sqrtf(ss / (float)a.K + a.eps);
+      for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = k + e < K ? to_f32(p[k + e]) : 0.f;
   }
-  const int G = (a.K + 127) / 128;
-  for (int base = 0; base < a.K; base += 256 * 8) {
-    const int k0 = base + 8 * threadIdx.x;
-    float y[8];
-    uint32_t amax = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int k = k0 + e;
-      float h = 0.f;
-      if (k < a.K) h = to_f32(x[k]) + (r ? to_f32(r[k]) : 0.f);
-      if (k < a.K && a.h) static_cast<TX*>(a.h)[row * a.K + k] = from_f32<TX>(h);
-      y[e] = k < a.K && a.norm ? h * rstd * load_w(a, k) : h;
-      amax = max(amax, __float_as_uint(y[e]) & 0x7fffffffu);
-    }
-    if (a.y_dtype != SF_E4M3) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if (k0 + e >= a.K) continue;
-        const size_t o = row * a.ldy + k0 + e;
-        if (a.y_dtype == SF_F32) static_cast<float*>(a.y)[o] = y[e];
-        else if (a.y_dtype == SF_F16) static_cast<__half*>(a.y)[o] = __float2half_rn(y[e]);
-        else static_cast<__nv_bfloat16*>(a.y)[o] = __float2bfloat16_rn(y[e]);
-      }
-      continue;
-    }
-    // the largest magnitude as an integer: infinities and NaN win, and spoil only their own group
-#pragma unroll
-    for (int o = 8; o; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    float scale = amax ? __uint_as_float(amax) / kE4m3Max : 1.f;
-    if (scale < FLT_MIN) scale = FLT_MIN;
-    if ((threadIdx.x & 15) == 0 && k0 < a.K) a.scales[row * G + k0 / 128] = scale;
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_cols(T* p, int k, int K, const float (&v)[8]) {
+  if constexpr (VEC) {
+    store8(p + k, v);
+  } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (k0 + e < a.K) static_cast<uint8_t*>(a.y)[row * a.ldy + k0 + e] = to_e4m3(y[e] / scale);
+      if (k + e < K) p[k + e] = from_f32<T>(v[e]);
+  }
+}
+
+// y of 8 columns to memory, in its type or as codes.  16 neighbouring lanes hold one 128-column group; every lane of
+// the warp calls this, with k >= K where it has no columns.
+template <bool VEC>
+__device__ __forceinline__ void put_columns(const NormArgs& a, size_t row, int k, const float (&y)[8]) {
+  if (a.y_dtype == SF_E4M3) {
+    // the largest magnitude as an integer: infinities and NaN win, and spoil only their own group
+    uint32_t amax = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) amax = max(amax, __float_as_uint(y[e]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 8; o; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if (k >= a.K) return;
+    float scale = amax ? __uint_as_float(amax) / kE4m3Max : 1.f;
+    if (scale < FLT_MIN) scale = FLT_MIN;
+    const float inv = 1.f / scale;
+    if ((threadIdx.x & 15) == 0) a.scales[row * ((a.K + 127) / 128) + k / 128] = scale;
+    float c[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c[e] = y[e] * inv;
+    uint8_t* out = static_cast<uint8_t*>(a.y) + row * a.ldy + k;
+    if (VEC) {
+      *reinterpret_cast<uint2*>(out) = to_e4m3x8(c);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (k + e < a.K) out[e] = to_e4m3(c[e]);
+    }
+    return;
+  }
+  if (k >= a.K) return;
+  if (a.y_dtype == SF_F32) store_cols<float, VEC>(static_cast<float*>(a.y) + row * a.ldy, k, a.K, y);
+  else if (a.y_dtype == SF_F16) store_cols<__half, VEC>(static_cast<__half*>(a.y) + row * a.ldy, k, a.K, y);
+  else store_cols<__nv_bfloat16, VEC>(static_cast<__nv_bfloat16*>(a.y) + row * a.ldy, k, a.K, y);
+}
+
+// blockDim.x threads a row (whole warps), blockDim.y rows a block (several only where one warp takes a row).  A thread
+// keeps CH x 8 columns of h, blockDim.x x 8 apart; with CH = 0 it reads them again for the output instead (rows longer
+// than 1024 threads keep).  VEC: every row starts at 16 bytes and K is a multiple of 8.
+// Memory-bound: 4096 x 8192 bf16 with the residual and e4m3 output moves 236 MB.
+template <typename TX, int CH, bool VEC>
+__global__ void __launch_bounds__(1024) rms_norm_kernel(const NormArgs a) {
+  __shared__ float part[32];
+  griddep_wait();
+  const size_t row = (size_t)blockIdx.x * blockDim.y + threadIdx.y;
+  if (row >= (size_t)a.T) return;   // whole warps
+  const int step = blockDim.x * 8, k0 = threadIdx.x * 8;
+  const TX* x = static_cast<const TX*>(a.x) + row * a.ldx;
+  const TX* r = a.r ? static_cast<const TX*>(a.r) + row * a.ldr : nullptr;
+  TX* h_out = static_cast<TX*>(a.h) + (a.h ? row * a.K : 0);
+  const auto load_h = [&](int k, float (&h)[8]) {
+    load_cols<TX, VEC>(x, k, a.K, h);
+    if (r) {
+      float v[8];
+      load_cols<TX, VEC>(r, k, a.K, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) h[e] += v[e];
+    }
+  };
+  constexpr int KEEP = CH > 0 ? CH : 1;
+  float h[KEEP][8], ss = 0.f;
+  if constexpr (CH > 0) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) load_h(k0 + c * step, h[c]);
+    griddep_launch_dependents();
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss = fmaf(h[c][e], h[c][e], ss);
+  } else {
+    for (int k = k0; k < a.K; k += step) {
+      load_h(k, h[0]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss = fmaf(h[0][e], h[0][e], ss);
+    }
+  }
+  float rstd = 1.f;
+  if (a.norm) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (blockDim.x > 32) {
+      if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = ss;
+      __syncthreads();
+      ss = (threadIdx.x & 31) < blockDim.x / 32 ? part[threadIdx.x & 31] : 0.f;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    }
+    rstd = 1.f / sqrtf(ss / (float)a.K + a.eps);
+  }
+  const auto finish = [&](int k, float (&v)[8]) {
+    if (k < a.K && a.h) store_cols<TX, VEC>(h_out, k, a.K, v);
+    if (a.norm && k < a.K) {
+      float w[8];
+      load_weights<VEC>(a, k, w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = k + e < a.K ? v[e] * rstd * w[e] : 0.f;
+    }
+    put_columns<VEC>(a, row, k, v);
+  };
+  if constexpr (CH > 0) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+      if (c == 0 || c * step < a.K) finish(k0 + c * step, h[c]);
+  } else {
+    for (int base = 0; base < a.K; base += step) {
+      load_h(k0 + base, h[0]);
+      finish(k0 + base, h[0]);
+    }
   }
 }
 
 int run_norm(const NormArgs& a, int x_dtype, cudaStream_t st) {
   if (a.T == 0) return SF_OK;
+  const size_t xe = x_dtype == SF_F32 ? 4 : 2, ye = a.y_dtype == SF_E4M3 ? 1 : a.y_dtype == SF_F32 ? 4 : 2;
+  const auto at16 = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+  const bool vec = a.K % 8 == 0 && at16(a.x) && at16(a.r) && at16(a.h) && at16(a.w) && at16(a.y) &&
+                   a.ldx * xe % 16 == 0 && a.ldr * xe % 16 == 0 && (size_t)a.K * xe % 16 == 0 && a.ldy * ye % (a.y_dtype == SF_E4M3 ? 8 : 16) == 0;
+  // Few rows: as many threads as the row has chunks, for the shortest chain of loads.  Many rows: 4 chunks a thread
+  // keep more loads in flight with less to reduce.
+  const int chunks = (a.K + 7) / 8;
+  const bool few = a.T <= 2 * device_info().sms;
+  int ch = few ? 1 : 4;
+  while (ch <= 4 && (chunks + ch - 1) / ch > 1024) ch *= 2;
+  const int nt = ch > 4 ? 1024 : ((chunks + ch - 1) / ch + 31) / 32 * 32;
+  const int rows = nt == 32 ? 4 : 1;
   const cudaError_t e = with_type(x_dtype, [&](auto* t) {
     using TX = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
-    rms_norm_kernel<TX><<<(unsigned)a.T, 256, 0, st>>>(a);
-    return cudaGetLastError();
+    auto* fn = ch == 1   ? (vec ? rms_norm_kernel<TX, 1, true> : rms_norm_kernel<TX, 1, false>)
+               : ch == 2 ? (vec ? rms_norm_kernel<TX, 2, true> : rms_norm_kernel<TX, 2, false>)
+               : ch == 4 ? (vec ? rms_norm_kernel<TX, 4, true> : rms_norm_kernel<TX, 4, false>)
+                         : (vec ? rms_norm_kernel<TX, 0, true> : rms_norm_kernel<TX, 0, false>);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(((long long)a.T + rows - 1) / rows));
+    cfg.blockDim = dim3((unsigned)nt, (unsigned)rows);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, fn, a);
   });
   if (e != cudaSuccess) return cuda_fail(e, "rms_norm_kernel launch");
   g_launches.fetch_add(1, std::memory_order_relaxed);

@@ -52,41 +52,68 @@ __device__ __forceinline__ void load_w(const TX* p, float (&v)[Piece<VEC>::W]) {
   else v[0] = to_f32(*p);
 }
 
-// `trow` is the table's row of the token's position.
-template <typename TX, bool VEC>
-__device__ __forceinline__ void turn_item(const TX* x, int item, const Turn& t, const float* trow, bool pos_ok,
-                                          Piece<VEC>& p) {
+// Cosines and sines of an item's pairs, from the table's row of the token's position (NaN without one).
+template <bool VEC>
+struct Angles {
+  static constexpr int W = Piece<VEC>::W;
+  float c[W], s[W];
+};
+template <bool VEC>
+__device__ __forceinline__ void load_angles(const Turn& t, int item, const float* trow, bool ok, Angles<VEC>& a) {
   constexpr int W = Piece<VEC>::W;
-  const int nt = turned_items<VEC>(t), half = t.rot / 2;
+  if (item >= turned_items<VEC>(t)) return;
+  if (!ok) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) a.c[i] = a.s[i] = __int_as_float(0x7fffffff);
+    return;
+  }
+  const int half = t.rot / 2;
+  if constexpr (VEC) {
+    const int n = t.interleaved ? 4 : 8;   // pairs of an item
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+      if (i >= n) break;
+      *reinterpret_cast<float4*>(a.c + i) = __ldg(reinterpret_cast<const float4*>(trow + n * item + i));
+      *reinterpret_cast<float4*>(a.s + i) = __ldg(reinterpret_cast<const float4*>(trow + half + n * item + i));
+    }
+  } else {
+    a.c[0] = __ldg(trow + item);
+    a.s[0] = __ldg(trow + half + item);
+  }
+}
+
+template <typename TX, bool VEC>
+__device__ __forceinline__ void load_item(const TX* x, int item, const Turn& t, Piece<VEC>& p) {
+  constexpr int W = Piece<VEC>::W;
+  const int nt = turned_items<VEC>(t);
   p.db = -1;
   if (item >= nt) {
     p.da = t.rot + (item - nt) * W;
-    load_w<TX, VEC>(x + p.da, p.a);
-    return;
-  }
-  const float nan = __int_as_float(0x7fffffff);
-  if (VEC && t.interleaved) {
+  } else if (VEC && t.interleaved) {
     p.da = 8 * item;
-    load_w<TX, VEC>(x + p.da, p.a);
-#pragma unroll
-    for (int i = 0; i < W / 2; ++i) {
-      const float c = pos_ok ? trow[4 * item + i] : nan, s = pos_ok ? trow[half + 4 * item + i] : nan;
-      const float a = p.a[2 * i], b = p.a[2 * i + 1];
-      p.a[2 * i] = a * c - b * s;
-      p.a[2 * i + 1] = a * s + b * c;
-    }
-    return;
+  } else {
+    p.da = t.interleaved ? 2 * item : W * item;
+    p.db = t.interleaved ? 2 * item + 1 : t.rot / 2 + W * item;
+    load_w<TX, VEC>(x + p.db, p.b);
   }
-  p.da = t.interleaved ? 2 * item : W * item;
-  p.db = t.interleaved ? 2 * item + 1 : half + W * item;
   load_w<TX, VEC>(x + p.da, p.a);
-  load_w<TX, VEC>(x + p.db, p.b);
+}
+template <bool VEC>
+__device__ __forceinline__ void turn_item(Piece<VEC>& p, int item, const Turn& t, const Angles<VEC>& w) {
+  if (p.db >= 0) {
 #pragma unroll
-  for (int i = 0; i < W; ++i) {
-    const float c = pos_ok ? trow[W * item + i] : nan, s = pos_ok ? trow[half + W * item + i] : nan;
-    const float a = p.a[i], b = p.b[i];
-    p.a[i] = a * c - b * s;
-    p.b[i] = a * s + b * c;
+    for (int i = 0; i < Piece<VEC>::W; ++i) {
+      const float a = p.a[i], b = p.b[i];
+      p.a[i] = a * w.c[i] - b * w.s[i];
+      p.b[i] = a * w.s[i] + b * w.c[i];
+    }
+  } else if (VEC && item < turned_items<VEC>(t)) {   // four pairs side by side
+#pragma unroll
+    for (int i = 0; i < Piece<VEC>::W / 2; ++i) {
+      const float a = p.a[2 * i], b = p.a[2 * i + 1];
+      p.a[2 * i] = a * w.c[i] - b * w.s[i];
+      p.a[2 * i + 1] = a * w.s[i] + b * w.c[i];
+    }
   }
 }
 
@@ -103,18 +130,29 @@ __device__ __forceinline__ void turn_token(const TX* x, long long xhs, TX* out, 
   if (!ok && threadIdx.x == 0) atomicOr(&g_dev_error, kErrIndex);
   const float* trow = t.table + (ok ? pos * t.rot : 0);
   const int per = head_items<VEC>(t, D);
-  for (int i = threadIdx.x; i < H * per; i += blockDim.x) {
-    const int h = i / per;
-    Piece<VEC> p;
-    turn_item<TX, VEC>(x + h * xhs, i % per, t, trow, ok, p);
-    store_w<TX, VEC>(out + h * ohs + p.da, p.a);
-    if (p.db >= 0) store_w<TX, VEC>(out + h * ohs + p.db, p.b);
+  // a thread takes one item of every (blockDim / per)-th head, so that its angles are loaded once
+  const int lanes = per < (int)blockDim.x ? (int)blockDim.x / per * per : (int)blockDim.x;
+  if ((int)threadIdx.x >= lanes) return;
+  for (int item = threadIdx.x % per; item < per; item += blockDim.x) {
+    Angles<VEC> w;
+    load_angles<VEC>(t, item, trow, ok, w);
+    const int heads = per < (int)blockDim.x ? lanes / per : 1;
+#pragma unroll 2
+    for (int h = per < (int)blockDim.x ? (int)threadIdx.x / per : 0; h < H; h += heads) {
+      Piece<VEC> p;
+      load_item<TX, VEC>(x + h * xhs, item, t, p);
+      turn_item<VEC>(p, item, t, w);
+      store_w<TX, VEC>(out + h * ohs + p.da, p.a);
+      if (p.db >= 0) store_w<TX, VEC>(out + h * ohs + p.db, p.b);
+    }
   }
 }
 
 template <typename TX, bool VEC>
 __global__ void __launch_bounds__(256) rotary_kernel(const Rows x, void* out, long long ots, long long ohs,
                                                      const void* positions, int pos64, const Turn t, int H, int D) {
+  griddep_launch_dependents();
+  griddep_wait();
   const size_t tok = blockIdx.x;
   const long long pos = pos64 ? static_cast<const long long*>(positions)[tok] : static_cast<const int*>(positions)[tok];
   turn_token<TX, VEC>(static_cast<const TX*>(x.p) + tok * x.ts, x.hs, static_cast<TX*>(out) + tok * ots, ohs, H, D, t,
@@ -129,19 +167,21 @@ struct AppendArgs {
   int H, T, units;      // units: an upper bound of the pages that the call touches
 };
 
-// One warp writes one (page, kv head, keys or values): first the largest magnitude of its new rows, then the codes.
-template <typename TX, bool VEC>
-__device__ void append_unit(const AppendArgs& a, int unit, int h, int which) {
-  const int lane = threadIdx.x & 31, D = a.c.head_dim, BS = a.c.page_size;
+// WARPS warps write one (page, kv head, keys or values): the largest magnitude of its new rows, then the codes.  A
+// thread keeps what it loaded where it has at most KEEP items, else it loads them again.
+template <typename TX, bool VEC, int WARPS>
+__device__ void append_unit(const AppendArgs& a, int unit, int h, int which, uint32_t* red) {
+  constexpr int KEEP = VEC ? 4 : 8, THREADS = 32 * WARPS;
+  const int tid = threadIdx.x % THREADS, lane = threadIdx.x & 31, D = a.c.head_dim, BS = a.c.page_size;
   const SeqSpan s = unit_span(a.c, a.T, unit);
   if (!s.ok) {
-    if (lane == 0) atomicOr(&g_dev_error, kErrIndex);
+    if (tid == 0) atomicOr(&g_dev_error, kErrIndex);
     return;
   }
   if (s.lo >= s.hi) return;
   const int page = s.page < a.c.pages_per_seq ? a.c.block_table[(size_t)s.b * a.c.pages_per_seq + s.page] : -1;
   if (page < 0 || page >= a.c.num_pages) {
-    if (lane == 0) atomicOr(&g_dev_error, kErrIndex);
+    if (tid == 0) atomicOr(&g_dev_error, kErrIndex);
     return;
   }
   const Rows& src = which ? a.v : a.k;
@@ -150,51 +190,68 @@ __device__ void append_unit(const AppendArgs& a, int unit, int h, int which) {
   uint8_t* codes = (which ? a.c.v_codes : a.c.k_codes) + ((size_t)page * a.c.n_kv_heads + h) * BS * D;
   float* scale_at = (which ? a.c.v_scales : a.c.k_scales) + (size_t)page * a.c.n_kv_heads + h;
   const TX* x0 = static_cast<const TX*>(src.p) + (size_t)(s.row + s.lo) * src.ts + h * src.hs;
-  const int slot0 = s.lo - s.page * BS, rows = s.hi - s.lo, per = head_items<VEC>(t, D);
+  const int slot0 = s.lo - s.page * BS, per = head_items<VEC>(t, D), items = (s.hi - s.lo) * per;
   const bool turned = t.rot > 0;
-  auto each = [&](auto&& fn) {
-    for (int i = lane; i < rows * per; i += 32) {
-      const int r = i / per, pos = s.lo + r;
-      const bool ok = !turned || pos < t.max_pos;
-      Piece<VEC> p;
-      turn_item<TX, VEC>(x0 + r * src.ts, i % per, t, t.table + (turned && ok ? (size_t)pos * t.rot : 0), ok, p);
-      fn(r, p);
-    }
+  const float old = slot0 > 0 ? *scale_at : 0.f;
+  const auto load = [&](int i, Piece<VEC>& p) {
+    const int r = i / per, item = i % per, pos = s.lo + r;
+    const bool ok = !turned || pos < t.max_pos;
+    Angles<VEC> w;
+    load_angles<VEC>(t, item, t.table + (turned && ok ? (size_t)pos * t.rot : 0), ok, w);
+    load_item<TX, VEC>(x0 + r * src.ts, item, t, p);
+    turn_item<VEC>(p, item, t, w);
   };
-  if (turned && s.hi > t.max_pos && lane == 0) atomicOr(&g_dev_error, kErrIndex);
+  if (turned && s.hi > t.max_pos && tid == 0) atomicOr(&g_dev_error, kErrIndex);
   uint32_t top = 0;   // bits of the largest finite magnitude
-  auto see = [&](float v) {
-    const uint32_t u = __float_as_uint(v) & 0x7fffffffu;
-    if (u < 0x7f800000u) top = max(top, u);
-  };
-  each([&](int, const Piece<VEC>& p) {
+  const auto see = [&](const Piece<VEC>& p) {
 #pragma unroll
     for (int i = 0; i < Piece<VEC>::W; ++i) {
-      see(p.a[i]);
-      if (p.db >= 0) see(p.b[i]);
+      const uint32_t u = __float_as_uint(p.a[i]) & 0x7fffffffu, v = p.db >= 0 ? __float_as_uint(p.b[i]) & 0x7fffffffu : 0u;
+      if (u < 0x7f800000u) top = max(top, u);
+      if (v < 0x7f800000u) top = max(top, v);
     }
-  });
+  };
+  Piece<VEC> kept[KEEP];
+  const bool keep = items <= KEEP * THREADS;
+  if (keep) {
+#pragma unroll
+    for (int c = 0; c < KEEP; ++c)
+      if (tid + c * THREADS < items) load(tid + c * THREADS, kept[c]);
+#pragma unroll
+    for (int c = 0; c < KEEP; ++c)
+      if (tid + c * THREADS < items) see(kept[c]);
+  } else {
+#pragma unroll 2
+    for (int i = tid; i < items; i += THREADS) {
+      Piece<VEC> p;
+      load(i, p);
+      see(p);
+    }
+  }
   top = __reduce_max_sync(0xffffffffu, top);
+  if constexpr (WARPS > 1) {
+    if (lane == 0) red[threadIdx.x >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) top = max(top, red[w]);
+  }
   int e = (int)(top >> 23) - 127 - ((top & 0x7fffffu) <= 0x600000u ? 8 : 7);   // 448 = 1.75 * 2^8
   if (e < -64) e = -64;
   float scale = __int_as_float((e + 127) << 23);
-  if (slot0 > 0) {
-    const float old = *scale_at;
-    if (old >= scale) {
-      scale = old;
-    } else {
-      const float ratio = old / scale;
-      for (int i = lane; i < slot0 * D / 16; i += 32) {
-        uint4 u = reinterpret_cast<uint4*>(codes)[i];
-        uint8_t* c = reinterpret_cast<uint8_t*>(&u);
+  if (old >= scale) {
+    scale = old;
+  } else if (slot0 > 0) {
+    const float ratio = old / scale;
+    for (int i = tid; i < slot0 * D / 16; i += THREADS) {
+      uint4 u = reinterpret_cast<uint4*>(codes)[i];
+      uint8_t* c = reinterpret_cast<uint8_t*>(&u);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) c[j] = to_e4m3(from_e4m3(c[j]) * ratio);
-        reinterpret_cast<uint4*>(codes)[i] = u;
-      }
+      for (int j = 0; j < 16; ++j) c[j] = to_e4m3(from_e4m3(c[j]) * ratio);
+      reinterpret_cast<uint4*>(codes)[i] = u;
     }
   }
   const float inv = 1.f / scale;
-  auto put = [&](int r, int d, const float (&v)[Piece<VEC>::W]) {
+  const auto put = [&](int r, int d, const float (&v)[Piece<VEC>::W]) {
     uint8_t* o = codes + (size_t)(slot0 + r) * D + d;
     if constexpr (VEC) {
       float w[8];
@@ -205,17 +262,31 @@ __device__ void append_unit(const AppendArgs& a, int unit, int h, int which) {
       *o = to_e4m3(v[0] * inv);
     }
   };
-  each([&](int r, const Piece<VEC>& p) {
-    put(r, p.da, p.a);
-    if (p.db >= 0) put(r, p.db, p.b);
-  });
-  __syncwarp();
-  if (lane == 0) *scale_at = scale;
+  const auto store = [&](int i, const Piece<VEC>& p) {
+    put(i / per, p.da, p.a);
+    if (p.db >= 0) put(i / per, p.db, p.b);
+  };
+  if (keep) {
+#pragma unroll
+    for (int c = 0; c < KEEP; ++c)
+      if (tid + c * THREADS < items) store(tid + c * THREADS, kept[c]);
+  } else {
+#pragma unroll 2
+    for (int i = tid; i < items; i += THREADS) {
+      Piece<VEC> p;
+      load(i, p);
+      store(i, p);
+    }
+  }
+  if (tid == 0) *scale_at = scale;   // every thread has read the old one: before the block's barrier, or in this warp
 }
 
-// The first blocks turn one query token each; each warp of the others writes one (page, kv head, keys or values).
-template <typename TX, bool VEC>
+// The first blocks turn one query token each; of the others, 8 / WARPS units a block.
+template <typename TX, bool VEC, int WARPS>
 __global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a, int q_blocks) {
+  __shared__ uint32_t red[8];
+  griddep_launch_dependents();
+  griddep_wait();
   if ((int)blockIdx.x < q_blocks) {
     const int tok = blockIdx.x;
     const TokenAt at = token_at(a.c, a.T, tok);
@@ -225,17 +296,17 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a, i
                         a.turn, at.ok ? max(at.pos, 0) : -1);
     return;
   }
-  const long long w = (long long)(blockIdx.x - q_blocks) * 8 + (threadIdx.x >> 5);
+  const long long w = (long long)(blockIdx.x - q_blocks) * (8 / WARPS) + threadIdx.x / (32 * WARPS);
   const long long heads = w >> 1;
   if (heads >= (long long)a.units * a.c.n_kv_heads) return;
-  append_unit<TX, VEC>(a, (int)(heads / a.c.n_kv_heads), (int)(heads % a.c.n_kv_heads), (int)(w & 1));
+  append_unit<TX, VEC, WARPS>(a, (int)(heads / a.c.n_kv_heads), (int)(heads % a.c.n_kv_heads), (int)(w & 1), red);
 }
 
-bool rows_vec(const void* p, long long ts, long long hs, int dtype) {
+bool rows_vec(const void* p, long long ts, long long hs) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ts % 8 == 0 && hs % 8 == 0;
 }
-bool turn_vec(int rot, int interleaved, int D) {
-  return D % 8 == 0 && rot % (interleaved ? 8 : 16) == 0;
+bool turn_vec(const float* table, int rot, int interleaved, int D) {
+  return D % 8 == 0 && rot % (interleaved ? 8 : 16) == 0 && reinterpret_cast<uintptr_t>(table) % 16 == 0;
 }
 
 int check_turn(const float* table, int max_pos, int rot, int D) {
@@ -260,14 +331,13 @@ int sf_rotary(const void* x, int dtype, long long xts, long long xhs, void* out,
   if (T == 0 || H == 0) return SF_OK;
   if (!x || !out || !positions) return fail(SF_ERR_NULL, "null pointer argument");
   const Turn t{table, max_pos, rot, interleaved};
-  const bool vec = turn_vec(rot, interleaved, D) && rows_vec(x, xts, xhs, dtype) && rows_vec(out, ots, ohs, dtype);
+  const bool vec = turn_vec(table, rot, interleaved, D) && rows_vec(x, xts, xhs) && rows_vec(out, ots, ohs);
   const Rows rows{x, xts, xhs};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = with_type(dtype, [&](auto* p) {
     using TX = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
     auto* fn = vec ? rotary_kernel<TX, true> : rotary_kernel<TX, false>;
-    fn<<<(unsigned)T, 256, 0, st>>>(rows, out, ots, ohs, positions, pos64, t, H, D);
-    return cudaGetLastError();
+    return launch_kernel(fn, T, 256, 0, st, true, rows, out, ots, ohs, positions, pos64, t, H, D);
   });
   if (e != cudaSuccess) return cuda_fail(e, "rotary_kernel launch");
   g_launches.fetch_add(1, std::memory_order_relaxed);
@@ -298,18 +368,20 @@ int sf_paged_append(const sf_paged_cache* cache, const void* k, long long kts, l
   a.H = H;
   a.T = T;
   a.units = max_units(*cache, T);
-  const bool vec = turn_vec(rot, interleaved, D) && rows_vec(k, kts, khs, dtype) && rows_vec(v, vts, vhs, dtype) &&
-                   (!q || (rows_vec(q, qts, qhs, dtype) && rows_vec(q_out, D, D, dtype)));
+  const bool vec = turn_vec(table, rot, interleaved, D) && rows_vec(k, kts, khs) && rows_vec(v, vts, vhs) &&
+                   (!q || (rows_vec(q, qts, qhs) && rows_vec(q_out, D, D)));
   const int q_blocks = q ? T : 0;
-  const long long warps = 2ll * a.units * cache->n_kv_heads;
-  const long long blocks = q_blocks + (warps + 7) / 8;
+  // a warp for the few rows of a decode step, a block for a page of a prompt
+  const bool wide = T / cache->batch > 4;
+  const long long work = 2ll * a.units * cache->n_kv_heads;
+  const long long blocks = q_blocks + (wide ? work : (work + 7) / 8);
   if (blocks > 0x7fffffffll) return fail(SF_ERR_UNSUPPORTED, "too many tokens in one call");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = with_type(dtype, [&](auto* p) {
     using TX = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
-    auto* fn = vec ? paged_append_kernel<TX, true> : paged_append_kernel<TX, false>;
-    fn<<<(unsigned)blocks, 256, 0, st>>>(a, q_blocks);
-    return cudaGetLastError();
+    auto* fn = wide ? (vec ? paged_append_kernel<TX, true, 8> : paged_append_kernel<TX, false, 8>)
+                    : (vec ? paged_append_kernel<TX, true, 1> : paged_append_kernel<TX, false, 1>);
+    return launch_kernel(fn, (int)blocks, 256, 0, st, true, a, q_blocks);
   });
   if (e != cudaSuccess) return cuda_fail(e, "paged_append_kernel launch");
   g_launches.fetch_add(1, std::memory_order_relaxed);

@@ -50,23 +50,6 @@ struct Fp8Params {
 // 32 bytes of the start address.
 __device__ __forceinline__ uint64_t rows128_desc(uint32_t saddr) { return smem_desc(saddr, 16, 1024, kSw128); }
 
-// Two fp32 lanes per instruction.
-__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
-  uint64_t v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
-  return v;
-}
-__device__ __forceinline__ float2 unpack2(uint64_t v) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-  return f;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -311,8 +294,9 @@ __global__ void __launch_bounds__(Plan<SPLIT>::THREADS, SPLIT ? 2 : 1)
             for (int j = 0; j < 8; ++j) {
               uint32_t w[4];
               if (per == 32) {
-                const float2 f0 = unpack2(acc[16 * g + 2 * j]), f1 = unpack2(acc[16 * g + 2 * j + 1]);
-                float v[4] = {f0.x, f0.y, f1.x, f1.y};
+                float v[4];
+                unpack2(acc[16 * g + 2 * j], v[0], v[1]);
+                unpack2(acc[16 * g + 2 * j + 1], v[2], v[3]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                   const int n = n0 + c0 + 32 * g + 4 * j + e;
@@ -322,7 +306,8 @@ __global__ void __launch_bounds__(Plan<SPLIT>::THREADS, SPLIT ? 2 : 1)
               } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                  float2 f = unpack2(acc[(16 * g + 4 * j + e) % (L::CW / 2)]);
+                  float2 f;
+                  unpack2(acc[(16 * g + 4 * j + e) % (L::CW / 2)], f.x, f.y);
                   const int n = n0 + c0 + 32 * g + 8 * j + 2 * e;
                   if (p.bias && n < p.N) f.x += __ldg(p.bias + n);
                   if (p.bias && n + 1 < p.N) f.y += __ldg(p.bias + n + 1);
@@ -340,7 +325,8 @@ __global__ void __launch_bounds__(Plan<SPLIT>::THREADS, SPLIT ? 2 : 1)
         } else if (t < p.T) {
 #pragma unroll
           for (int i = 0; i < L::CW / 2; ++i) {
-            const float2 f = unpack2(acc[i]);
+            float2 f;
+            unpack2(acc[i], f.x, f.y);
             const int n = n0 + c0 + 2 * i;
             if (n < p.N) store_y(p.Y, (size_t)t * p.N + n, f.x + (p.bias ? __ldg(p.bias + n) : 0.f), p.y_dtype);
             if (n + 1 < p.N) store_y(p.Y, (size_t)t * p.N + n + 1, f.y + (p.bias ? __ldg(p.bias + n + 1) : 0.f), p.y_dtype);
@@ -358,7 +344,8 @@ __global__ void __launch_bounds__(Plan<SPLIT>::THREADS, SPLIT ? 2 : 1)
 #pragma unroll
       for (int i = 0; i < CW; ++i) {
         const int c = c0 + i;
-        const float2 f = unpack2(acc[i / 2]);
+        float2 f;
+        unpack2(acc[i / 2], f.x, f.y);
         const uint32_t o = at + (uint32_t)(rank * cols + (c & (cols - 1))) * pitch;
         if (p.split > 1) st_cluster(o, (uint32_t)(c >> lg_cols), i & 1 ? f.y : f.x);
         else asm volatile("st.shared.f32 [%0], %1;" ::"r"(o), "f"(i & 1 ? f.y : f.x) : "memory");

@@ -102,22 +102,12 @@ __device__ __forceinline__ bool any_of(bool p) {
   return any;
 }
 // d = a * b + c and d = a + b over rows, two to an instruction
-__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
-  uint64_t v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
-  return v;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
 template <int R, typename A, typename B, typename C>
 __device__ __forceinline__ void fma_rows(float (&d)[R], A&& a, B&& b, C&& c) {
   if constexpr (R % 2 == 0) {
 #pragma unroll
     for (int r = 0; r < R; r += 2) {
-      uint64_t v;
-      asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(pack2(a(r), a(r + 1))), "l"(pack2(b(r), b(r + 1))), "l"(pack2(c(r), c(r + 1))));
-      unpack2(v, d[r], d[r + 1]);
+      unpack2(fma2(pack2(a(r), a(r + 1)), pack2(b(r), b(r + 1)), pack2(c(r), c(r + 1))), d[r], d[r + 1]);
     }
   } else {
 #pragma unroll
@@ -129,9 +119,7 @@ __device__ __forceinline__ void mul_rows(float (&d)[R], A&& a, B&& b) {
   if constexpr (R % 2 == 0) {
 #pragma unroll
     for (int r = 0; r < R; r += 2) {
-      uint64_t v;
-      asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(pack2(a(r), a(r + 1))), "l"(pack2(b(r), b(r + 1))));
-      unpack2(v, d[r], d[r + 1]);
+      unpack2(mul2(pack2(a(r), a(r + 1)), pack2(b(r), b(r + 1))), d[r], d[r + 1]);
     }
   } else {
 #pragma unroll
@@ -143,9 +131,7 @@ __device__ __forceinline__ void add_rows(float (&d)[R], A&& a, B&& b) {
   if constexpr (R % 2 == 0) {
 #pragma unroll
     for (int r = 0; r < R; r += 2) {
-      uint64_t v;
-      asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(pack2(a(r), a(r + 1))), "l"(pack2(b(r), b(r + 1))));
-      unpack2(v, d[r], d[r + 1]);
+      unpack2(add2(pack2(a(r), a(r + 1)), pack2(b(r), b(r + 1))), d[r], d[r + 1]);
     }
   } else {
 #pragma unroll

@@ -78,25 +78,32 @@ __device__ __forceinline__ void store_cols(T* p, int k, int K, const float (&v)[
   }
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
 // y of 8 columns to memory, in its type or as codes.  16 neighbouring lanes hold one 128-column group; every lane of
 // the warp calls this, with k >= K where it has no columns.
 template <bool VEC>
 __device__ __forceinline__ void put_columns(const NormArgs& a, size_t row, int k, const float (&y)[8]) {
   if (a.y_dtype == SF_E4M3) {
-    // the largest magnitude as an integer: infinities and NaN win, and spoil only their own group
-    uint32_t amax = 0;
+    // infinities and NaN win, and spoil only their own group
+    float amax = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) amax = max(amax, __float_as_uint(y[e]) & 0x7fffffffu);
+    for (int e = 0; e < 8; ++e) amax = max_nan(amax, fabsf(y[e]));
 #pragma unroll
-    for (int o = 8; o; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    for (int o = 8; o; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     if (k >= a.K) return;
-    float scale = amax ? __uint_as_float(amax) / kE4m3Max : 1.f;
+    float scale = amax == 0.f ? 1.f : amax * (1.f / kE4m3Max);
     if (scale < FLT_MIN) scale = FLT_MIN;
-    const float inv = 1.f / scale;
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
     if ((threadIdx.x & 15) == 0) a.scales[row * ((a.K + 127) / 128) + k / 128] = scale;
     float c[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) c[e] = y[e] * inv;
+    for (int e = 0; e < 8; e += 2) unpack2(mul2(pack2(y[e], y[e + 1]), pack2(inv, inv)), c[e], c[e + 1]);
     uint8_t* out = static_cast<uint8_t*>(a.y) + row * a.ldy + k;
     if (VEC) {
       *reinterpret_cast<uint2*>(out) = to_e4m3x8(c);
@@ -114,11 +121,11 @@ __device__ __forceinline__ void put_columns(const NormArgs& a, size_t row, int k
 }
 
 // blockDim.x threads a row (whole warps), blockDim.y rows a block (several only where one warp takes a row).  A thread
-// keeps CH x 8 columns of h, blockDim.x x 8 apart; with CH = 0 it reads them again for the output instead (rows longer
-// than 1024 threads keep).  VEC: every row starts at 16 bytes and K is a multiple of 8.
+// keeps CH x 8 columns of h, blockDim.x x 8 apart; with CH = 0 it reads them again for the output instead (rows of more
+// than 32768).  VEC: every row starts at 16 bytes and K is a multiple of 8.
 // Memory-bound: 4096 x 8192 bf16 with the residual and e4m3 output moves 236 MB.
 template <typename TX, int CH, bool VEC>
-__global__ void __launch_bounds__(1024) rms_norm_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(CH == 4 || CH == 8 ? 512 : 1024) rms_norm_kernel(const NormArgs a) {
   __shared__ float part[32];
   griddep_wait();
   const size_t row = (size_t)blockIdx.x * blockDim.y + threadIdx.y;
@@ -139,13 +146,28 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const NormArgs a) {
   constexpr int KEEP = CH > 0 ? CH : 1;
   float h[KEEP][8], ss = 0.f;
   if constexpr (CH > 0) {
+    // every load of the thread before the first use
 #pragma unroll
-    for (int c = 0; c < CH; ++c) load_h(k0 + c * step, h[c]);
+    for (int c = 0; c < CH; ++c) load_cols<TX, VEC>(x, k0 + c * step, a.K, h[c]);
+    if (r) {
+      float v[CH][8];
+#pragma unroll
+      for (int c = 0; c < CH; ++c) load_cols<TX, VEC>(r, k0 + c * step, a.K, v[c]);
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; e += 2)
+          unpack2(add2(pack2(h[c][e], h[c][e + 1]), pack2(v[c][e], v[c][e + 1])), h[c][e], h[c][e + 1]);
+    }
     griddep_launch_dependents();
+    uint64_t sq = 0;
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(h[c][e], h[c][e], ss);
+      for (int e = 0; e < 8; e += 2) sq = fma2(pack2(h[c][e], h[c][e + 1]), pack2(h[c][e], h[c][e + 1]), sq);
+    float lo, hi;
+    unpack2(sq, lo, hi);
+    ss = lo + hi;
   } else {
     for (int k = k0; k < a.K; k += step) {
       load_h(k, h[0]);
@@ -172,7 +194,8 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const NormArgs a) {
       float w[8];
       load_weights<VEC>(a, k, w);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = k + e < a.K ? v[e] * rstd * w[e] : 0.f;
+      for (int e = 0; e < 8; e += 2)
+        unpack2(mul2(mul2(pack2(v[e], v[e + 1]), pack2(rstd, rstd)), pack2(w[e], w[e + 1])), v[e], v[e + 1]);
     }
     put_columns<VEC>(a, row, k, v);
   };
@@ -198,15 +221,15 @@ int run_norm(const NormArgs& a, int x_dtype, cudaStream_t st) {
   // keep more loads in flight with less to reduce.
   const int chunks = (a.K + 7) / 8;
   const bool few = a.T <= 2 * device_info().sms;
-  int ch = few ? 1 : 4;
-  while (ch <= 4 && (chunks + ch - 1) / ch > 1024) ch *= 2;
-  const int nt = ch > 4 ? 1024 : ((chunks + ch - 1) / ch + 31) / 32 * 32;
+  const int ch = few && chunks <= 1024 ? 1 : few && chunks <= 2048 ? 2 : chunks <= 2048 ? 4 : chunks <= 4096 ? 8 : 0;
+  const int nt = ch == 0 ? 1024 : ((chunks + ch - 1) / ch + 31) / 32 * 32;
   const int rows = nt == 32 ? 4 : 1;
   const cudaError_t e = with_type(x_dtype, [&](auto* t) {
     using TX = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
     auto* fn = ch == 1   ? (vec ? rms_norm_kernel<TX, 1, true> : rms_norm_kernel<TX, 1, false>)
                : ch == 2 ? (vec ? rms_norm_kernel<TX, 2, true> : rms_norm_kernel<TX, 2, false>)
                : ch == 4 ? (vec ? rms_norm_kernel<TX, 4, true> : rms_norm_kernel<TX, 4, false>)
+               : ch == 8 ? (vec ? rms_norm_kernel<TX, 8, true> : rms_norm_kernel<TX, 8, false>)
                          : (vec ? rms_norm_kernel<TX, 0, true> : rms_norm_kernel<TX, 0, false>);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(((long long)a.T + rows - 1) / rows));

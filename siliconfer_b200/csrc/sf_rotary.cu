@@ -28,21 +28,21 @@ struct Rows {
   long long ts, hs;     // token and head strides
 };
 
-// One head's D elements are cut into items: a turned one (8 pairs, or with VEC = false one pair) or a copied one
-// (8 elements, or one).  VEC needs every stride and offset it meets to be a multiple of 8 elements.
+// One head's D elements are cut into items of 16 elements (VEC: two runs of 8) or 2: the pairs of a turned item, or
+// what is copied beyond them.  VEC needs every stride and offset it meets to be a multiple of 8 elements.
 template <bool VEC>
 __device__ __forceinline__ int turned_items(const Turn& t) {
-  return VEC ? (t.interleaved ? t.rot / 8 : t.rot / 16) : t.rot / 2;
+  return t.rot / (VEC ? 16 : 2);
 }
 template <bool VEC>
 __device__ __forceinline__ int head_items(const Turn& t, int D) {
-  return turned_items<VEC>(t) + (D - t.rot) / (VEC ? 8 : 1);
+  return turned_items<VEC>(t) + (D - t.rot + (VEC ? 15 : 1)) / (VEC ? 16 : 2);
 }
 
 template <bool VEC>
 struct Piece {
   static constexpr int W = VEC ? 8 : 1;
-  int da, db;           // first element of a; of b, or -1 when there is none
+  int da, db;           // first element of a; of b, or -1 where the head ends before it
   float a[W], b[W];
 };
 
@@ -69,12 +69,10 @@ __device__ __forceinline__ void load_angles(const Turn& t, int item, const float
   }
   const int half = t.rot / 2;
   if constexpr (VEC) {
-    const int n = t.interleaved ? 4 : 8;   // pairs of an item
 #pragma unroll
     for (int i = 0; i < 8; i += 4) {
-      if (i >= n) break;
-      *reinterpret_cast<float4*>(a.c + i) = __ldg(reinterpret_cast<const float4*>(trow + n * item + i));
-      *reinterpret_cast<float4*>(a.s + i) = __ldg(reinterpret_cast<const float4*>(trow + half + n * item + i));
+      *reinterpret_cast<float4*>(a.c + i) = __ldg(reinterpret_cast<const float4*>(trow + 8 * item + i));
+      *reinterpret_cast<float4*>(a.s + i) = __ldg(reinterpret_cast<const float4*>(trow + half + 8 * item + i));
     }
   } else {
     a.c[0] = __ldg(trow + item);
@@ -83,36 +81,38 @@ __device__ __forceinline__ void load_angles(const Turn& t, int item, const float
 }
 
 template <typename TX, bool VEC>
-__device__ __forceinline__ void load_item(const TX* x, int item, const Turn& t, Piece<VEC>& p) {
+__device__ __forceinline__ void load_item(const TX* x, int item, const Turn& t, int D, Piece<VEC>& p) {
   constexpr int W = Piece<VEC>::W;
   const int nt = turned_items<VEC>(t);
-  p.db = -1;
-  if (item >= nt) {
-    p.da = t.rot + (item - nt) * W;
-  } else if (VEC && t.interleaved) {
-    p.da = 8 * item;
+  if (item < nt && !t.interleaved) {
+    p.da = W * item;
+    p.db = t.rot / 2 + W * item;
   } else {
-    p.da = t.interleaved ? 2 * item : W * item;
-    p.db = t.interleaved ? 2 * item + 1 : t.rot / 2 + W * item;
-    load_w<TX, VEC>(x + p.db, p.b);
+    p.da = item < nt ? 2 * W * item : t.rot + (item - nt) * 2 * W;
+    p.db = p.da + W < D ? p.da + W : -1;
   }
   load_w<TX, VEC>(x + p.da, p.a);
+  if (p.db >= 0) load_w<TX, VEC>(x + p.db, p.b);
 }
 template <bool VEC>
 __device__ __forceinline__ void turn_item(Piece<VEC>& p, int item, const Turn& t, const Angles<VEC>& w) {
-  if (p.db >= 0) {
+  if (item >= turned_items<VEC>(t)) return;
+  if (VEC && t.interleaved) {   // pairs side by side: four in a, four in b
+#pragma unroll
+    for (int i = 0; i < Piece<VEC>::W / 2; ++i) {
+      const float a = p.a[2 * i], b = p.a[2 * i + 1], c = p.b[2 * i], d = p.b[2 * i + 1];
+      constexpr int H = Piece<VEC>::W / 2;
+      p.a[2 * i] = a * w.c[i] - b * w.s[i];
+      p.a[2 * i + 1] = a * w.s[i] + b * w.c[i];
+      p.b[2 * i] = c * w.c[H + i] - d * w.s[H + i];
+      p.b[2 * i + 1] = c * w.s[H + i] + d * w.c[H + i];
+    }
+  } else {
 #pragma unroll
     for (int i = 0; i < Piece<VEC>::W; ++i) {
       const float a = p.a[i], b = p.b[i];
       p.a[i] = a * w.c[i] - b * w.s[i];
       p.b[i] = a * w.s[i] + b * w.c[i];
-    }
-  } else if (VEC && item < turned_items<VEC>(t)) {   // four pairs side by side
-#pragma unroll
-    for (int i = 0; i < Piece<VEC>::W / 2; ++i) {
-      const float a = p.a[2 * i], b = p.a[2 * i + 1];
-      p.a[2 * i] = a * w.c[i] - b * w.s[i];
-      p.a[2 * i + 1] = a * w.s[i] + b * w.c[i];
     }
   }
 }
@@ -123,27 +123,36 @@ __device__ __forceinline__ void store_w(TX* p, const float (&v)[Piece<VEC>::W]) 
   else *p = from_f32<TX>(v[0]);
 }
 
-template <typename TX, bool VEC>
+template <typename TX, bool VEC, typename Position>
 __device__ __forceinline__ void turn_token(const TX* x, long long xhs, TX* out, long long ohs, int H, int D,
-                                           const Turn& t, long long pos) {
-  const bool ok = t.rot == 0 || (pos >= 0 && pos < t.max_pos);
-  if (!ok && threadIdx.x == 0) atomicOr(&g_dev_error, kErrIndex);
-  const float* trow = t.table + (ok ? pos * t.rot : 0);
-  const int per = head_items<VEC>(t, D);
-  // a thread takes one item of every (blockDim / per)-th head, so that its angles are loaded once
-  const int lanes = per < (int)blockDim.x ? (int)blockDim.x / per * per : (int)blockDim.x;
-  if ((int)threadIdx.x >= lanes) return;
+                                           const Turn& t, Position&& position) {
+  // A thread takes one item of every (blockDim / per)-th head, two heads at a time: their elements are asked for first,
+  // the angles, which hang on the position, once.
+  const int per = head_items<VEC>(t, D), lanes = per < (int)blockDim.x ? (int)blockDim.x / per * per : (int)blockDim.x;
+  const int heads = per < (int)blockDim.x ? lanes / per : 1, h0 = per < (int)blockDim.x ? (int)threadIdx.x / per : 0;
   for (int item = threadIdx.x % per; item < per; item += blockDim.x) {
     Angles<VEC> w;
-    load_angles<VEC>(t, item, trow, ok, w);
-    const int heads = per < (int)blockDim.x ? lanes / per : 1;
-#pragma unroll 2
-    for (int h = per < (int)blockDim.x ? (int)threadIdx.x / per : 0; h < H; h += heads) {
-      Piece<VEC> p;
-      load_item<TX, VEC>(x + h * xhs, item, t, p);
-      turn_item<VEC>(p, item, t, w);
-      store_w<TX, VEC>(out + h * ohs + p.da, p.a);
-      if (p.db >= 0) store_w<TX, VEC>(out + h * ohs + p.db, p.b);
+    bool ok = true, first = true;
+    for (int h = h0; h < H || first; h += 2 * heads) {
+      Piece<VEC> p[2];
+      const bool in0 = h < H && (int)threadIdx.x < lanes, in1 = h + heads < H && (int)threadIdx.x < lanes;
+      if (in0) load_item<TX, VEC>(x + h * xhs, item, t, D, p[0]);
+      if (in1) load_item<TX, VEC>(x + (h + heads) * xhs, item, t, D, p[1]);
+      if (first) {
+        const long long pos = position();   // by whole warps
+        ok = t.rot == 0 || (pos >= 0 && pos < t.max_pos);
+        if (!ok && threadIdx.x == 0) atomicOr(&g_dev_error, kErrIndex);
+        load_angles<VEC>(t, item, t.table + (ok ? pos * t.rot : 0), ok, w);
+        first = false;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (!(i ? in1 : in0)) continue;
+        turn_item<VEC>(p[i], item, t, w);
+        TX* o = out + (h + i * heads) * ohs;
+        store_w<TX, VEC>(o + p[i].da, p[i].a);
+        if (p[i].db >= 0) store_w<TX, VEC>(o + p[i].db, p[i].b);
+      }
     }
   }
 }
@@ -154,9 +163,9 @@ __global__ void __launch_bounds__(256) rotary_kernel(const Rows x, void* out, lo
   griddep_launch_dependents();
   griddep_wait();
   const size_t tok = blockIdx.x;
-  const long long pos = pos64 ? static_cast<const long long*>(positions)[tok] : static_cast<const int*>(positions)[tok];
-  turn_token<TX, VEC>(static_cast<const TX*>(x.p) + tok * x.ts, x.hs, static_cast<TX*>(out) + tok * ots, ohs, H, D, t,
-                      pos);
+  turn_token<TX, VEC>(static_cast<const TX*>(x.p) + tok * x.ts, x.hs, static_cast<TX*>(out) + tok * ots, ohs, H, D, t, [&] {
+    return pos64 ? static_cast<const long long*>(positions)[tok] : (long long)static_cast<const int*>(positions)[tok];
+  });
 }
 
 struct AppendArgs {
@@ -171,7 +180,7 @@ struct AppendArgs {
 // thread keeps what it loaded where it has at most KEEP items, else it loads them again.
 template <typename TX, bool VEC, int WARPS>
 __device__ void append_unit(const AppendArgs& a, int unit, int h, int which, uint32_t* red) {
-  constexpr int KEEP = VEC ? 4 : 8, THREADS = 32 * WARPS;
+  constexpr int KEEP = 2, THREADS = 32 * WARPS;
   const int tid = threadIdx.x % THREADS, lane = threadIdx.x & 31, D = a.c.head_dim, BS = a.c.page_size;
   const SeqSpan s = unit_span(a.c, a.T, unit);
   if (!s.ok) {
@@ -198,7 +207,7 @@ __device__ void append_unit(const AppendArgs& a, int unit, int h, int which, uin
     const bool ok = !turned || pos < t.max_pos;
     Angles<VEC> w;
     load_angles<VEC>(t, item, t.table + (turned && ok ? (size_t)pos * t.rot : 0), ok, w);
-    load_item<TX, VEC>(x0 + r * src.ts, item, t, p);
+    load_item<TX, VEC>(x0 + r * src.ts, item, t, D, p);
     turn_item<VEC>(p, item, t, w);
   };
   if (turned && s.hi > t.max_pos && tid == 0) atomicOr(&g_dev_error, kErrIndex);
@@ -283,17 +292,18 @@ __device__ void append_unit(const AppendArgs& a, int unit, int h, int which, uin
 
 // The first blocks turn one query token each; of the others, 8 / WARPS units a block.
 template <typename TX, bool VEC, int WARPS>
-__global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a, int q_blocks) {
+__global__ void __launch_bounds__(256, 3) paged_append_kernel(const AppendArgs a, int q_blocks) {
   __shared__ uint32_t red[8];
   griddep_launch_dependents();
   griddep_wait();
   if ((int)blockIdx.x < q_blocks) {
     const int tok = blockIdx.x;
-    const TokenAt at = token_at(a.c, a.T, tok);
-    if (!at.ok && threadIdx.x == 0) atomicOr(&g_dev_error, kErrIndex);
     turn_token<TX, VEC>(static_cast<const TX*>(a.q.p) + tok * a.q.ts, a.q.hs,
                         static_cast<TX*>(a.q_out) + (size_t)tok * a.H * a.c.head_dim, a.c.head_dim, a.H, a.c.head_dim,
-                        a.turn, at.ok ? max(at.pos, 0) : -1);
+                        a.turn, [&] {
+      const TokenAt at = token_at(a.c, a.T, tok);
+      return at.ok ? (long long)max(at.pos, 0) : -1ll;
+    });
     return;
   }
   const long long w = (long long)(blockIdx.x - q_blocks) * (8 / WARPS) + threadIdx.x / (32 * WARPS);
@@ -305,8 +315,8 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a, i
 bool rows_vec(const void* p, long long ts, long long hs) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ts % 8 == 0 && hs % 8 == 0;
 }
-bool turn_vec(const float* table, int rot, int interleaved, int D) {
-  return D % 8 == 0 && rot % (interleaved ? 8 : 16) == 0 && reinterpret_cast<uintptr_t>(table) % 16 == 0;
+bool turn_vec(const float* table, int rot, int D) {
+  return D % 8 == 0 && rot % 16 == 0 && reinterpret_cast<uintptr_t>(table) % 16 == 0;
 }
 
 int check_turn(const float* table, int max_pos, int rot, int D) {
@@ -331,7 +341,7 @@ int sf_rotary(const void* x, int dtype, long long xts, long long xhs, void* out,
   if (T == 0 || H == 0) return SF_OK;
   if (!x || !out || !positions) return fail(SF_ERR_NULL, "null pointer argument");
   const Turn t{table, max_pos, rot, interleaved};
-  const bool vec = turn_vec(table, rot, interleaved, D) && rows_vec(x, xts, xhs) && rows_vec(out, ots, ohs);
+  const bool vec = turn_vec(table, rot, D) && rows_vec(x, xts, xhs) && rows_vec(out, ots, ohs);
   const Rows rows{x, xts, xhs};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = with_type(dtype, [&](auto* p) {
@@ -368,7 +378,7 @@ int sf_paged_append(const sf_paged_cache* cache, const void* k, long long kts, l
   a.H = H;
   a.T = T;
   a.units = max_units(*cache, T);
-  const bool vec = turn_vec(table, rot, interleaved, D) && rows_vec(k, kts, khs) && rows_vec(v, vts, vhs) &&
+  const bool vec = turn_vec(table, rot, D) && rows_vec(k, kts, khs) && rows_vec(v, vts, vhs) &&
                    (!q || (rows_vec(q, qts, qhs) && rows_vec(q_out, D, D)));
   const int q_blocks = q ? T : 0;
   // a warp for the few rows of a decode step, a block for a page of a prompt

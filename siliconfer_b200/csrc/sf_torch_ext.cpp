@@ -10,6 +10,7 @@
 // computation happens here.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <climits>
@@ -131,9 +132,13 @@ at::Tensor like_rows(const at::Tensor& t, const at::Tensor& x) {
   sizes.back() = t.size(1);
   return t.view(sizes);
 }
+// Uninitialised tensors on ref's device.
+at::Tensor empty_on(at::IntArrayRef sizes, at::ScalarType dtype, const at::Tensor& ref) {
+  return at::detail::empty_cuda(sizes, dtype, ref.device(), c10::nullopt);
+}
 // Code rows that start at multiples of 16 bytes.
 at::Tensor empty_codes(int64_t T, int64_t K, const at::Tensor& ref) {
-  return at::empty_strided({T, K}, {(K + 15) / 16 * 16, 1}, ref.options().dtype(at::kFloat8_e4m3fn));
+  return at::detail::empty_strided_cuda({T, K}, {(K + 15) / 16 * 16, 1}, at::kFloat8_e4m3fn, ref.device());
 }
 
 std::tuple<at::Tensor, OptTensor, OptTensor> rms_norm(const at::Tensor& x, const OptTensor& weight, double eps,
@@ -157,16 +162,16 @@ std::tuple<at::Tensor, OptTensor, OptTensor> rms_norm(const at::Tensor& x, const
   }
   const int xdt = dtype_code(x.scalar_type()), wdt = w.defined() ? dtype_code(w.scalar_type()) : SF_F32;
   OptTensor h, scales;
-  if (r.t.defined()) h = at::empty({v.rows, v.K}, x.options());
+  if (r.t.defined()) h = empty_on({v.rows, v.K}, x.scalar_type(), x);
   at::Tensor y;
   int ydt = SF_E4M3;
   if (e4m3) {
     y = empty_codes(v.rows, v.K, x);
-    scales = at::empty({v.rows, (v.K + 127) / 128}, x.options().dtype(at::kFloat));
+    scales = empty_on({v.rows, (v.K + 127) / 128}, at::kFloat, x);
   } else {
     const at::ScalarType yt = out_dtype.value_or(x.scalar_type());
     ydt = dtype_code(yt);
-    y = at::empty({v.rows, v.K}, x.options().dtype(yt));
+    y = empty_on({v.rows, v.K}, yt, x);
   }
   check(sf_rms_norm(v.t.data_ptr(), xdt, v.ld, r.t.defined() ? r.t.data_ptr() : nullptr, r.ld,
                     h ? h->data_ptr() : nullptr, w.defined() ? w.data_ptr() : nullptr, wdt, (float)eps, y.data_ptr(), ydt,
@@ -182,7 +187,7 @@ std::tuple<at::Tensor, at::Tensor> quantize_e4m3(const at::Tensor& x) {
   const c10::cuda::CUDAGuard guard(x.device());
   const RowView v = rows_of(x, "x");
   at::Tensor y = empty_codes(v.rows, v.K, x);
-  at::Tensor scales = at::empty({v.rows, (v.K + 127) / 128}, x.options().dtype(at::kFloat));
+  at::Tensor scales = empty_on({v.rows, (v.K + 127) / 128}, at::kFloat, x);
   check(sf_quantize_e4m3(v.t.data_ptr(), dtype_code(x.scalar_type()), v.ld, static_cast<uint8_t*>(y.data_ptr()),
                          (v.K + 15) / 16 * 16, scales.data_ptr<float>(), (int)v.rows, (int)v.K, stream_of(x)));
   return {like_rows(y, x), like_rows(scales, x)};
@@ -213,7 +218,7 @@ at::Tensor fp8_linear(const at::Tensor& X, const at::Tensor& xs, const at::Tenso
     TORCH_CHECK(bias->scalar_type() == at::kFloat && bias->dim() == 1 && bias->size(0) == N, "bias must be fp32 [N]");
     b = bias->contiguous();
   }
-  at::Tensor Y = at::empty({x.rows, N}, X.options().dtype(out_dtype));
+  at::Tensor Y = empty_on({x.rows, N}, out_dtype, X);
   // a single row's stride has no meaning: the kernel is told one that its loads accept
   const int64_t ldx = x.rows > 1 ? x.ld : (x.K + 15) / 16 * 16, ldw = N > 1 ? W.stride(0) : (x.K + 15) / 16 * 16;
   check(sf_fp8_linear(static_cast<const uint8_t*>(x.t.data_ptr()), ldx, xsc.data_ptr<float>(),
@@ -250,7 +255,7 @@ at::Tensor rotary(const at::Tensor& x, const at::Tensor& positions, const at::Te
     TORCH_CHECK(y.stride(2) == 1 || D == 1, "out's heads must be contiguous");
   }
   const at::Tensor xi = x.stride(2) == 1 || D == 1 ? x : x.contiguous();
-  if (!y.defined()) y = at::empty({T, H, D}, x.options());
+  if (!y.defined()) y = empty_on({T, H, D}, x.scalar_type(), x);
   TORCH_CHECK(y.data_ptr() != xi.data_ptr() || y.strides() == xi.strides(),
               "out may be x itself, but no other view of x's memory");
   const at::Tensor pos = positions.contiguous();
@@ -330,7 +335,7 @@ OptTensor paged_append(const at::Tensor& k, const at::Tensor& v, const at::Tenso
                     q->scalar_type() == k.scalar_type(),
                 "q must be [T, heads, head_dim] of k's dtype");
     qi = head_rows(*q);
-    qo = at::empty(q->sizes(), q->options());
+    qo = empty_on(q->sizes(), q->scalar_type(), k);
   }
   if (given(table)) check_table(*table, k, c.head_dim);
   check(sf_paged_append(&c, ki.data_ptr(), ki.stride(0), ki.stride(1), vi.data_ptr(), vi.stride(0), vi.stride(1),
@@ -356,11 +361,11 @@ std::tuple<at::Tensor, OptTensor> paged_attention(const at::Tensor& q, const at:
   const c10::cuda::CUDAGuard guard(q.device());
   const at::Tensor qi = head_rows(q);
   const at::ScalarType ot = out_dtype.value_or(q.scalar_type());
-  at::Tensor out = at::empty(q.sizes(), q.options().dtype(ot));
+  at::Tensor out = empty_on(q.sizes(), ot, q);
   OptTensor lse;
-  if (return_lse) lse = at::empty({q.size(0), q.size(1)}, q.options().dtype(at::kFloat));
+  if (return_lse) lse = empty_on({q.size(0), q.size(1)}, at::kFloat, q);
   const size_t bytes = sf_paged_attention_workspace_bytes(c.head_dim);
-  at::Tensor ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+  at::Tensor ws = empty_on({(int64_t)bytes}, at::kByte, q);
   const double s = scale.has_value() ? *scale : 1.0 / std::sqrt((double)c.head_dim);
   check(sf_paged_attention(&c, qi.data_ptr(), dtype_code(q.scalar_type()), qi.stride(0), qi.stride(1), out.data_ptr(),
                            dtype_code(ot), return_lse ? lse->data_ptr<float>() : nullptr, (int)q.size(1), (int)q.size(0),

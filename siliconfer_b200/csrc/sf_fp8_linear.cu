@@ -46,10 +46,6 @@ struct Fp8Params {
   int tma_store;
 };
 
-// K-major tile of 128-byte rows in the 128-byte swizzle (8-row atoms of 1024 bytes); 32 k further inside the atom are
-// 32 bytes of the start address.
-__device__ __forceinline__ uint64_t rows128_desc(uint32_t saddr) { return smem_desc(saddr, 16, 1024, kSw128); }
-
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -187,28 +183,39 @@ __global__ void __launch_bounds__(Plan<SPLIT>::THREADS, SPLIT ? 2 : 1)
       meet();
     } else if (warp == kMmaWarp) {
       // ---------------- MMA issuer ----------------
-      if (lane == 0) {
-        const uint32_t idesc = idesc_e4m3(128, BN);
-        uint32_t it = 0;
-        bool ok = true;
-        for (int tile = tile0; tile < ntiles && ok; tile += tile_step) {
-          for (int kb = kb0; kb < kb1; ++kb, ++it) {
-            const uint32_t s = it % S, ph = (it / S) & 1, b = it % NBUF, use = it / NBUF;
-            if (!bar_wait(acce0 + 8 * b, (use & 1) ^ 1, kErrMma, abort_flag) ||
-                !bar_wait(full0 + 8 * s, ph, kErrMma, abort_flag)) { ok = false; break; }
-            tc_fence_after();
-            const uint32_t st = base + s * stage_bytes;
-  #pragma unroll
+      constexpr uint32_t idesc = idesc_e4m3(128, BN), high = desc_high(1024, kSw128);
+      const uint32_t low = desc_low(base, 16), step = stage_bytes >> 4;
+      uint32_t s = 0, ph = 0, b = 0, use = 0;
+      bool ok = true;
+      for (int tile = tile0; tile < ntiles && ok; tile += tile_step) {
+        for (int kb = kb0; kb < kb1; ++kb) {
+          ok = bar_wait(acce0 + 8 * b, use ^ 1, kErrMma, abort_flag) && bar_wait(full0 + 8 * s, ph, kErrMma, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t x = low + s * step, w = x + (xbytes >> 4);
+#pragma unroll
             for (int kk = 0; kk < kBK / 32; ++kk)
-              mma_f8(tmem + b * BN, rows128_desc(st + kk * 32), rows128_desc(st + xbytes + kk * 32), idesc, kk != 0);
-            mma_commit(empty0 + 8 * s);
+              mma_f8(tmem + b * BN, desc_of(x + 2 * kk, high), desc_of(w + 2 * kk, high), idesc, kk != 0);
             mma_commit(accf0 + 8 * b);
+            mma_commit(empty0 + 8 * s);
+          }
+          __syncwarp();
+          if (++s == (uint32_t)S) {
+            s = 0;
+            ph ^= 1;
+          }
+          if (++b == NBUF) {
+            b = 0;
+            use ^= 1;
           }
         }
-        // every issued MMA has completed before TMEM is freed
-        mma_commit(drain);
-        bar_drain(drain, 0, kErrDrain);
       }
+      // every issued MMA has completed before TMEM is freed
+      if (elect_one()) mma_commit(drain);
+      __syncwarp();
+      bar_drain(drain, 0, kErrDrain);
       __syncwarp();
       meet();
     } else {

@@ -217,11 +217,11 @@ int run_norm(const NormArgs& a, int x_dtype, cudaStream_t st) {
   const auto at16 = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
   const bool vec = a.K % 8 == 0 && at16(a.x) && at16(a.r) && at16(a.h) && at16(a.w) && at16(a.y) &&
                    a.ldx * xe % 16 == 0 && a.ldr * xe % 16 == 0 && (size_t)a.K * xe % 16 == 0 && a.ldy * ye % (a.y_dtype == SF_E4M3 ? 8 : 16) == 0;
-  // Few rows: as many threads as the row has chunks, for the shortest chain of loads.  Many rows: 4 chunks a thread
-  // keep more loads in flight with less to reduce.
+  // Few rows: as many threads as the row has chunks, for the shortest chain of loads.  Many rows: 2 chunks a thread
+  // (4096 x 8192: 48 us; 1 chunk 60, 4 chunks 52, 8 chunks 69), more where the row is too long for 512 threads.
   const int chunks = (a.K + 7) / 8;
   const bool few = a.T <= 2 * device_info().sms;
-  const int ch = few && chunks <= 1024 ? 1 : few && chunks <= 2048 ? 2 : chunks <= 2048 ? 4 : chunks <= 4096 ? 8 : 0;
+  const int ch = few && chunks <= 1024 ? 1 : chunks <= 1024 || (few && chunks <= 2048) ? 2 : chunks <= 2048 ? 4 : chunks <= 4096 ? 8 : 0;
   const int nt = ch == 0 ? 1024 : ((chunks + ch - 1) / ch + 31) / 32 * 32;
   const int rows = nt == 32 ? 4 : 1;
   const cudaError_t e = with_type(x_dtype, [&](auto* t) {

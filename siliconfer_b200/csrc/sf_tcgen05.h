@@ -23,6 +23,18 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
+// The same without any wait in hardware, for a thread that looks at several barriers in turn.
+__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 // Bounded wait that also gives up when another role of the block raised the abort flag.
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, unsigned code, volatile int* abort_flag) {
   if (bar_try(bar, parity)) return true;
@@ -81,11 +93,35 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t leading, 
   return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(leading >> 4) << 16) | ((uint64_t)(stride >> 4) << 32) |
          ((uint64_t)1 << 46) | (swizzle << 61);
 }
+// The two words of such a descriptor for a thread that issues many: the upper one is a constant, and an operand n bytes
+// further adds n >> 4 to the lower one.
+__device__ __forceinline__ uint32_t desc_low(uint32_t saddr, uint32_t leading) {
+  return ((saddr & 0x3FFFFu) >> 4) | ((leading >> 4) << 16);
+}
+__host__ __device__ constexpr uint32_t desc_high(uint32_t stride, uint64_t swizzle) {
+  return (stride >> 4) | (1u << 14) | ((uint32_t)swizzle << 29);
+}
+__device__ __forceinline__ uint64_t desc_of(uint32_t low, uint32_t high) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(low), "r"(high));
+  return d;
+}
 // Instruction descriptor of kind::f8f6f4: D fp32 (bits 4-5 = 1), A and B e4m3 (0), transposed (MN-major) A and B in
 // bits 15 and 16, N >> 3 in bits 17-22, M >> 4 in bits 24-28.
 __host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N, bool a_mn = false, bool b_mn = false) {
   return (1u << 4) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(N >> 3) << 17) |
          ((uint32_t)(M >> 4) << 24);
+}
+// One lane of the (converged) warp.  A warp that issues MMAs runs its loop as a whole, with only the instructions under
+// this: descriptors, barriers and counters then live in uniform registers, where the MMA takes its operands.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(yes));
+  return yes != 0;
 }
 __device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(

@@ -8,10 +8,12 @@
 // times its scale is at most 2 and most tiles of keys need no reduction over the threads.
 //
 // A call's work is a list of units of 128 keys, for each (sequence, kv head, tile of RT query rows) in turn; a row is
-// one (new token, query head of the kv head's group), so that a group reads its keys once.  Every CTA takes an equal,
-// contiguous share of that list, whatever the sequences' lengths: it finds its place from a prefix sum over the
-// batch.  A CTA that holds all of a tile's units writes the result; the others leave their parts in the workspace,
-// which a second kernel merges.
+// one (new token, query head of the kv head's group), so that a group reads its keys once.  The list is cut into
+// contiguous shares, one per CTA, whatever the sequences' lengths: a CTA finds its place from a prefix sum over the
+// batch.  The SMs do not get memory at the same pace (with equal shares they were busy between 0.66 and 0.92 of the
+// kernel's time), so the CTAs that are resident at first share 4/5 of a long list, and as many small CTAs that follow
+// where an SM is through share the rest.  A CTA that holds all of a tile's units writes the result; the others leave
+// their parts in the workspace, which a second kernel merges.
 //
 // Both products run on the codes as they lie in the cache (kind::f8f6f4), and no code is ever converted:
 //  * S^T[key, column] = K Q^T: 128 keys are the MMA's rows.  A query row is scaled by a power of two to at most 256 and
@@ -57,7 +59,7 @@ struct AttnArgs {
   float* lse;
   float* part;          // [CTA][2][rows x D unnormalised sums, then rows x (m, l)], up to kMaxRows
   int* desc;            // [CTA][8]: the tile that this CTA began and others ended
-  int H, T, G, q_dtype, out_dtype, window, lg_page;
+  int H, T, G, q_dtype, out_dtype, window, lg_page, resident;
   float scale;
 };
 
@@ -184,6 +186,28 @@ __device__ __forceinline__ int keys_from(const AttnArgs& a, int len, int n) {
   return a.window > 0 ? max(0, len - n + 1 - a.window) & ~(UNIT - 1) : 0;
 }
 
+// A list is long at this many units for each resident CTA: at 80 (64 x 4096 keys, 32 kv heads) the small CTAs gain 0.13
+// of the time, at 18 (16 x 8192, 8 kv heads) their own beginnings cost 0.24 of it.
+constexpr int kLong = 40;
+// CTAs' shares of `total` units: `first` equal ones of the first `most` units, `small` ones of the rest.
+struct Shares {
+  long long total, most, first, small;
+  __device__ __forceinline__ Shares(long long total_, int resident, int grid) : total(total_) {
+    const bool two = grid >= 2 * resident && total >= (long long)kLong * resident;
+    first = min((long long)min(grid, resident), total);
+    small = two ? resident : 0;
+    most = two ? total * 4 / 5 : total;
+  }
+  __device__ __forceinline__ long long ctas() const { return first + small; }
+  __device__ __forceinline__ long long begin(long long cta) const {
+    return cta <= first ? (first ? most * cta / first : 0) : most + (total - most) * (cta - first) / small;
+  }
+  // the CTA that holds a unit
+  __device__ __forceinline__ long long holder(long long u) const {
+    return u < most ? ((u + 1) * first - 1) / most : first + ((u - most + 1) * small - 1) / (total - most);
+  }
+};
+
 // The part of a tile of query rows that begins at unit u and is this CTA's.
 struct Part {
   int b, kvh, row0, last_row, r_first, pos0;
@@ -301,13 +325,14 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : D <= 128 ? 3 : 1)
     if (b < B) info[b] = SeqInfo{before + incl - u, len, n};
     __syncthreads();
   }
-  const long long C = min((long long)gridDim.x, total), cta = blockIdx.x;   // CTAs with a share: at least a unit each
+  const long long cta = blockIdx.x;
+  const Shares shares(total, a.resident, (int)gridDim.x);
   if (threadIdx.x == 0) a.desc[8 * cta] = 0;
   long long u = 0, u_end = 0;
   int b = 0;
-  if (cta < C) {
-    u = total * cta / C;
-    u_end = total * (cta + 1) / C;
+  if (cta < shares.ctas()) {
+    u = shares.begin(cta);
+    u_end = shares.begin(cta + 1);
     for (int lo = 0, hi = B; hi - lo > 1;) {
       const int mid = (lo + hi) >> 1;
       if (info[mid].first <= u) lo = mid;
@@ -372,65 +397,71 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : D <= 128 ? 3 : 1)
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
-    // ---------------- MMAs ----------------
-    if (lane == 0) {
-      constexpr uint32_t idesc_s = idesc_e4m3(128, N), idesc_o = idesc_e4m3(128, N, true, true);
-      uint32_t it = 0, seg = 0;
-      bool ok = true;
-      const auto scores = [&](uint32_t j) {
-        const uint32_t s = j % ST, st = base + L::K0 + s * L::TILE;
-        if (!bar_wait(kfull + 8 * s, (j / ST) & 1, kErrMma, abort_flag)) return false;
-        tc_fence_after();
+    // ---------------- MMAs: the scores of a tile, then the sums of the one before ----------------
+    constexpr uint32_t idesc_s = idesc_e4m3(128, N), idesc_o = idesc_e4m3(128, N, true, true);
+    constexpr uint32_t hk = desc_high(8 * L::INNER, L::SWZ), hq = desc_high(D / 16 * 128, kSwNone),
+                       hv = desc_high(8 * L::INNER, L::SWZ), hp = desc_high(UNIT * 16, kSwNone);
+    const uint32_t dk = desc_low(base + L::K0, 16), dq = desc_low(base + L::Q0, 128), dv = desc_low(base + L::V0, L::SUB),
+                   dp = desc_low(base + L::P0, 128);
+    uint32_t it = 0, seg = 0;
+    bool ok = true;
+    const auto scores = [&](uint32_t j) {
+      const uint32_t s = j % ST;
+      if (!__all_sync(0xffffffffu, bar_wait(kfull + 8 * s, (j / ST) & 1, kErrMma, abort_flag))) return false;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t k0 = dk + s * (L::TILE >> 4), d = tmem_s + (j & 1) * N;
 #pragma unroll
         for (int k = 0; k < D / 32; ++k) {
-          const uint32_t at = L::INNER == 32 ? k * L::SUB : k / (L::INNER / 32) * L::SUB + k % (L::INNER / 32) * 32;
-          mma_f8(tmem_s + (j & 1) * N, smem_desc(st + at, 16, 8 * L::INNER, L::SWZ),
-                 smem_desc(base + L::Q0 + k * 256, 128, D / 16 * 128, kSwNone), idesc_s, k != 0);
+          constexpr int PER = L::INNER / 32;   // steps of a sub-tile
+          const uint32_t at = k / PER * L::SUB + k % PER * 32;
+          mma_f8(d, desc_of(k0 + (at >> 4), hk), desc_of(dq + k * 16, hq), idesc_s, k != 0);
         }
-        mma_commit(kempty + 8 * s);
         mma_commit(sfull + 8 * (j & 1));
-        return true;
-      };
-      const auto sums = [&](uint32_t j) {
-        const uint32_t s = j % ST, st = base + L::V0 + s * L::TILE, pb = base + L::P0 + (j & 1) * L::P;
-        if (!bar_wait(vfull + 8 * s, (j / ST) & 1, kErrMma, abort_flag) ||
-            !bar_wait(pfull + 8 * (j & 1), (j >> 1) & 1, kErrMma, abort_flag))
-          return false;
-        tc_fence_after();
+        mma_commit(kempty + 8 * s);
+      }
+      __syncwarp();
+      return true;
+    };
+    const auto sums = [&](uint32_t j) {
+      const uint32_t s = j % ST;
+      if (!__all_sync(0xffffffffu, bar_wait(vfull + 8 * s, (j / ST) & 1, kErrMma, abort_flag) &&
+                                       bar_wait(pfull + 8 * (j & 1), (j >> 1) & 1, kErrMma, abort_flag)))
+        return false;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t v0 = dv + s * (L::TILE >> 4), p0 = dp + (j & 1) * (L::P >> 4), d = tmem_o + (j & 1) * MT * N;
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
           for (int k = 0; k < UNIT / 32; ++k)
-            mma_f8(tmem_o + ((j & 1) * MT + m) * N,
-                   smem_desc(st + m * L::SUB + k * 32 * L::INNER, L::SUB, 8 * L::INNER, L::SWZ),
-                   smem_desc(pb + k * 512, 128, UNIT * 16, kSwNone), idesc_o, k != 0);
-        mma_commit(vempty + 8 * s);
+            mma_f8(d + m * N, desc_of(v0 + ((m * L::SUB + k * 32 * L::INNER) >> 4), hv), desc_of(p0 + k * 32, hp), idesc_o,
+                   k != 0);
         mma_commit(ofull + 8 * (j & 1));
-        return true;
-      };
-      while (u < u_end && ok) {
-        const Part p = part_at<RT>(a, info, u, u_end, b);
-        const int tiles = p.tb > p.ta ? (p.tb - p.ta + UNIT - 1) / UNIT : 0;
-        if (tiles > 0) {
-          ok = bar_wait(qfull, seg & 1, kErrMma, abort_flag);
-          ++seg;
-          if (ok) {
-            tc_fence_after();
-            ok = scores(it);
-          }
-          for (int i = 0; i < tiles && ok; ++i) {
-            if (i + 1 < tiles) ok = scores(it + i + 1);
-            if (ok) ok = sums(it + i);
-          }
-          it += tiles;
-        }
-        u = p.u1;
+        mma_commit(vempty + 8 * s);
       }
-      // every issued MMA has completed before TMEM is freed
-      mma_commit(drain);
-      bar_drain(drain, 0, kErrDrain);
+      __syncwarp();
+      return true;
+    };
+    while (u < u_end && ok) {
+      const Part p = part_at<RT>(a, info, u, u_end, b);
+      const int tiles = p.tb > p.ta ? (p.tb - p.ta + UNIT - 1) / UNIT : 0;
+      if (tiles > 0) {
+        ok = __all_sync(0xffffffffu, bar_wait(qfull, seg & 1, kErrMma, abort_flag));
+        ++seg;
+        if (ok) ok = scores(it);
+        for (int i = 0; i < tiles && ok; ++i) {
+          if (i + 1 < tiles) ok = scores(it + i + 1);
+          if (ok) ok = sums(it + i);
+        }
+        it += tiles;
+      }
+      u = p.u1;
     }
+    // every issued MMA has completed before TMEM is freed
+    if (elect_one()) mma_commit(drain);
     __syncwarp();
+    bar_drain(drain, 0, kErrDrain);
   } else {
     // ---------------- softmax and sums: a thread is key tid of a tile, and column tid of the head ----------------
     // After an expired wait these warps go on through their loops (every wait then returns at once), so that none of
@@ -737,7 +768,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : D <= 128 ? 3 : 1)
       if (begins && !ends && tid == 0) {
         // CTAs of the tile's parts: this one to the one that holds its last unit
         int* dsc = a.desc + 8 * cta;
-        dsc[0] = (int)((p.seg1 * C - 1) / total - cta + 1);
+        dsc[0] = (int)(shares.holder(p.seg1 - 1) - cta + 1);
         dsc[1] = p.r_first;
         dsc[2] = p.kvh;
         dsc[3] = p.row0;
@@ -781,7 +812,7 @@ __global__ void __launch_bounds__(D) paged_attention_merge_kernel(const AttnArgs
 }
 
 template <int D, int PARTS, int RT>
-int launch(const AttnArgs& a, cudaStream_t st) {
+int launch(AttnArgs a, cudaStream_t st) {
   using L = Lay<D, PARTS, RT>;
   const sf_paged_cache& c = a.c;
   const uint64_t rows = (uint64_t)c.num_pages * c.n_kv_heads * c.page_size;
@@ -809,8 +840,9 @@ int launch(const AttnArgs& a, cudaStream_t st) {
   // no more CTAs than units there may be
   const double cap = ((double)c.pages_per_seq * c.page_size + UNIT - 1) / UNIT;
   const double units = cap * ((double)a.T * a.G / RT + c.batch) * c.n_kv_heads;
-  int grid = device_info().sms * per_sm;
-  if (units < grid) grid = (int)units;
+  a.resident = device_info().sms * per_sm;
+  int grid = 2 * a.resident;
+  if (units < (double)kLong * a.resident) grid = units < a.resident ? (int)units : a.resident;
   e = launch_kernel(fn, grid, kThreads, smem, st, true, mk, mv, a);
   if (e != cudaSuccess) return cuda_fail(e, "paged_attention_kernel launch");
   cudaLaunchConfig_t cfg = {};
@@ -837,7 +869,7 @@ extern "C" {
 
 size_t sf_paged_attention_workspace_bytes(int head_dim) {
   if (head_dim <= 0) return 0;
-  const size_t ctas = (size_t)device_info().sms * kMaxCtasPerSm;
+  const size_t ctas = (size_t)device_info().sms * kMaxCtasPerSm * 2;
   return ctas * (2 * kMaxRows * ((size_t)head_dim + 2) * 4 + 32);
 }
 
@@ -856,7 +888,7 @@ int sf_paged_attention(const sf_paged_cache* cache, const void* q, int q_dtype, 
   AttnArgs a{};
   a.c = *cache; a.q = q; a.qts = qts; a.qhs = qhs; a.out = out; a.lse = lse;
   a.desc = static_cast<int*>(workspace);
-  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (size_t)device_info().sms * kMaxCtasPerSm * 32);
+  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (size_t)device_info().sms * kMaxCtasPerSm * 2 * 32);
   a.H = H; a.T = T; a.G = H / cache->n_kv_heads; a.q_dtype = q_dtype; a.out_dtype = out_dtype; a.window = window;
   a.lg_page = __builtin_ctz((unsigned)cache->page_size);
   a.scale = scale;

@@ -23,18 +23,6 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// The same without any wait in hardware, for a thread that looks at several barriers in turn.
-__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
 // Bounded wait that also gives up when another role of the block raised the abort flag.
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, unsigned code, volatile int* abort_flag) {
   if (bar_try(bar, parity)) return true;

@@ -507,3 +507,31 @@ def test_validation_without_gpu():
     assert app(t=F, mp=8, rot=65) == 2 and app(t=F, mp=0, rot=64) == 2
     assert lib.sf_paged_attention(None, F, 0, 512, 64, F, 0, None, 8, 1, 1.0, 0, F, big, None) == 1
     assert lib.sf_paged_attention_workspace_bytes(128) > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,page,rot,D", [(1, 16, 64, 64), (3, 64, 64, 64), (70, 64, 128, 128), (300, 256, 48, 96), (20, 32, 20, 64)])
+def test_append_infinite_keys(cuda, n, page, rot, D, dtype, interleaved):
+    """A turned infinity is infinite (NaN against another one), saturates, and does not set the page's scale."""
+    from siliconfer_b200.paged_kv import paged_append
+    from siliconfer_b200.rotary import rotary_table
+    b = Batch([n + 5, n + 40], [n, n], 2, 2, D, page, dtype, seed=n)
+    k = torch.randn(b.T, 2, D, generator=b.g, device="cuda").to(dtype)
+    k[0, 0, 3], k[n, 1, 1], k[n, 1, 0] = float("inf"), float("-inf"), float("nan")
+    k[b.T - 1, 0, 0] = k[b.T - 1, 0, rot // 2] = k[b.T - 1, 0, 1] = float("inf")
+    pos = torch.cat([torch.arange(l - c, l, device="cuda") for _, l, c, _ in b.rows()])
+    table = rotary_table(1000, rot)
+    c, s = (x[:, None] for x in table.double()[pos].split(rot // 2, 1))
+    i, j = (slice(0, rot, 2), slice(1, rot, 2)) if interleaved else (slice(0, rot // 2), slice(rot // 2, rot))
+    y = k.double()
+    x0, x1 = y[..., i].clone(), y[..., j].clone()
+    y[..., i], y[..., j] = x0 * c - x1 * s, x0 * s + x1 * c
+    kc, kscale = append_ref(b.k, b.ks, b, y)
+    paged_append(k, torch.zeros_like(k), *b.args(), starts=b.starts, table=table, interleaved=interleaved)
+    assert torch.equal(b.ks.double(), kscale)
+    got = b.k.double()
+    assert torch.equal(got.isnan(), kc.isnan()) and kc.isnan().any() and (kc.abs() == 448).any()
+    diff = (got - kc).nan_to_num()
+    assert (diff.abs() <= 0.1251 * kc.nan_to_num().abs() + 2.0 ** -9).all() and (diff != 0).double().mean() <= 1e-4

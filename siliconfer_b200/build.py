@@ -20,7 +20,7 @@ SOURCES = [PKG / "csrc" / "sf_q4.cu", PKG / "csrc" / "sf_q4_gemm_tc.cu", PKG / "
            PKG / "csrc" / "sf_q4_tp.cu", PKG / "csrc" / "sf_kv_attention.cu", PKG / "csrc" / "sf_rms_norm.cu",
            PKG / "csrc" / "sf_fp8_linear.cu", PKG / "csrc" / "sf_rotary.cu", PKG / "csrc" / "sf_paged_attention.cu"]
 HEADERS = [ROOT / "include" / "sf_q4.h", PKG / "csrc" / "sf_q4_internal.h", PKG / "csrc" / "sf_e4m3.h",
-           PKG / "csrc" / "sf_paged.h", PKG / "csrc" / "sf_tcgen05.h"]
+           PKG / "csrc" / "sf_paged.h", PKG / "csrc" / "sf_paged_prompt.h", PKG / "csrc" / "sf_tcgen05.h"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -102,6 +102,9 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 __device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
   return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
+__device__ __forceinline__ uint32_t to_e5m2x2(float lo, float hi) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E5M2);
+}
 __device__ __forceinline__ uint8_t to_e4m3(float v) { return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3); }
 __device__ __forceinline__ uint2 to_e4m3x8(const float (&v)[8]) {
   return make_uint2(to_e4m3x2(v[0], v[1]) | (to_e4m3x2(v[2], v[3]) << 16),

@@ -535,3 +535,100 @@ def test_append_infinite_keys(cuda, n, page, rot, D, dtype, interleaved):
     assert torch.equal(got.isnan(), kc.isnan()) and kc.isnan().any() and (kc.abs() == 448).any()
     diff = (got - kc).nan_to_num()
     assert (diff.abs() <= 0.1251 * kc.nan_to_num().abs() + 2.0 ** -9).all() and (diff != 0).double().mean() <= 1e-4
+
+
+# Long runs of bf16 queries take tiles of 256 rows.  The bounds are the same: weights in fp16, queries to 2^-17 of the
+# row's largest element.
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,Hkv,D,page", [(64, 8, 128, 64), (14, 2, 64, 16), (32, 32, 128, 256), (8, 8, 64, 128), (16, 1, 128, 32),
+                                          (40, 8, 64, 64)])
+def test_prompts(cuda, H, Hkv, D, page):
+    """Whole prompts, later chunks, runs that end anywhere in a tile; empty sequences and single tokens between."""
+    n = 256 * 40 * Hkv // (H * Hkv) + 900      # rows for a quarter of the SMs at least
+    for lens, news in (([n], [n]), ([n + 500, 0, 300, 70, 1], [n, 0, 290, 1, 1]), ([n, n - 3], [n - 128, n - 130]),
+                       ([2500, 2049], [n, 255])):
+        check_attention(Batch(lens, [min(a, b) for a, b in zip(news, lens)], H, Hkv, D, page, torch.bfloat16, seed=n))
+    check_attention(Batch([n + 40] * 3, [n // 2] * 3, H, Hkv, D, page, torch.bfloat16, ragged=False), out_dtype=torch.float32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window", [1, 40, 128, 300, 5000])
+def test_prompts_with_a_window(cuda, window):
+    check_attention(Batch([1500, 900], [1400, 300], 16, 8, 128, 64, torch.bfloat16), window=window, out_dtype=torch.float16)
+    check_attention(Batch([700, 600], [700, 600], 28, 4, 64, 16, torch.bfloat16), window=window, scale=-0.2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fill", [0x7f, 0xff, 0x7e])
+def test_prompts_beyond_the_end(cuda, fill):
+    check_attention(Batch([1001, 650, 0], [1001, 200, 0], 64, 8, 128, 64, torch.bfloat16, fill=fill))
+    check_attention(Batch([1500], [1490], 14, 2, 64, 16, torch.bfloat16, fill=fill))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_prompt_rows_keep_to_themselves(cuda, D):
+    """NaN and infinite queries, NaN keys and values that some rows see and others do not, with a window and without."""
+    from siliconfer_b200.paged_kv import paged_attention
+    for window in (0, 200):
+        b = Batch([900], [800], 32, 8, D, 16, torch.bfloat16)
+        ref, _, vmax = b.ref(window=window)
+        k, v = b.k.view(torch.uint8), b.v.view(torch.uint8)
+        marks = (40, 333, 640, 897)
+        for at in marks:
+            k[b.table[0, at // 16], 1, at % 16] = 0x7f
+            v[b.table[0, at // 16], 1, at % 16, 3] = 0xff
+            v[b.table[0, at // 16], 0, at % 16, D - 1] = 0x7f
+        b.q[300, 20, 5], b.q[301, 21, 0] = float("nan"), float("inf")
+        out = paged_attention(b.q, *b.args(), starts=b.starts, window=window)
+        pos = torch.arange(100, 900, device="cuda")
+        sees = torch.zeros(800, dtype=torch.bool, device="cuda")
+        for at in marks:
+            sees |= (pos >= at) & ((pos < at + window) if window else True)
+        bad = torch.zeros_like(out, dtype=torch.bool)
+        bad[sees, 4:8] = True
+        bad[sees, :4, D - 1] = True
+        bad[300, 20] = bad[301, 21] = True
+        assert torch.equal(out.isnan(), bad)
+        assert ((out.double() - ref).abs()[~bad] <= 2.0 ** -10 * vmax + 2.0 ** -8 * ref.abs()[~bad]).all()
+
+
+@pytest.mark.gpu
+def test_prompt_values_strides_and_padding(cuda):
+    from siliconfer_b200 import _lib
+    from siliconfer_b200.paged_kv import paged_attention
+    b = Batch([700, 800], [650, 800], 32, 8, 64, 16, torch.bfloat16)
+    first = check_attention(b)
+    for _ in range(3):
+        assert torch.equal(check_attention(b), first)
+    wide = torch.zeros(b.T, 35 * 64 + 1, device="cuda", dtype=torch.bfloat16)
+    q = b.q
+    for off in (0, 1, 72):
+        wide[:, off:off + 32 * 64] = q.reshape(b.T, -1)
+        b.q = wide[:, off:off + 32 * 64].view(b.T, 32, 64)
+        assert torch.equal(check_attention(b), first)
+    b.q = q.transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(check_attention(b), first)
+    # scores of rising size, so that references move; scales far apart, zero; queries of one size and of others
+    b.q = (q.float() * torch.linspace(0.01, 6, b.T, device="cuda")[:, None, None]).to(torch.bfloat16)
+    check_attention(b)
+    b.vs = torch.exp2(torch.randint(-40, 12, b.vs.shape, generator=b.g, device="cuda").float())
+    check_attention(b)
+    b.vs[::2] = 0
+    check_attention(b)
+    b.q = (q.float() * 2.0 ** 60).to(torch.bfloat16)
+    check_attention(b, scale=2.0 ** -63)
+    b.q = torch.zeros_like(q)
+    check_attention(b)
+    # fewer tokens than rows: padding rows in front give 0; a page number out of range is an error, its keys are not seen
+    b = Batch([600, 800], [600, 800], 32, 8, 64, 16, torch.bfloat16)
+    b.seq_lens[0] = 500
+    out, lse = paged_attention(b.q, *b.args(), starts=b.starts, return_lse=True)
+    assert (out[:100] == 0).all() and (lse[:100] == -math.inf).all() and torch.isfinite(lse[100:]).all()
+    assert _lib.load().sf_q4_check_device_error() == 0
+    b.seq_lens[0] = 600
+    b.table[0] = b.P + 5
+    out, lse = paged_attention(b.q, *b.args(), starts=b.starts, return_lse=True)
+    torch.cuda.synchronize()
+    assert _lib.load().sf_q4_check_device_error() != 0
+    assert (out[:600] == 0).all() and (lse[:600] == -math.inf).all() and torch.isfinite(out[600:].float()).all()

@@ -144,11 +144,19 @@ __global__ void __launch_bounds__(CH == 4 || CH == 8 ? 512 : 1024) rms_norm_kern
     }
   };
   constexpr int KEEP = CH > 0 ? CH : 1;
-  float h[KEEP][8], ss = 0.f;
+  // Few rows: the weights come with the row, not after its sum (1 x 4096, fp32 weights: 2.2 us, was 2.4).  With many
+  // rows other blocks fill that wait, and the registers cost more (8192 x 4096 with 2 chunks: 52 us so, 45 otherwise).
+  constexpr bool EARLY = CH == 1;
+  float h[KEEP][8], w_kept[EARLY ? CH : 1][8], ss = 0.f;
   if constexpr (CH > 0) {
     // every load of the thread before the first use
 #pragma unroll
     for (int c = 0; c < CH; ++c) load_cols<TX, VEC>(x, k0 + c * step, a.K, h[c]);
+    if constexpr (EARLY) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+        if (a.norm && k0 + c * step < a.K) load_weights<VEC>(a, k0 + c * step, w_kept[c]);
+    }
     if (r) {
       float v[CH][8];
 #pragma unroll
@@ -188,11 +196,16 @@ __global__ void __launch_bounds__(CH == 4 || CH == 8 ? 512 : 1024) rms_norm_kern
     }
     rstd = 1.f / sqrtf(ss / (float)a.K + a.eps);
   }
-  const auto finish = [&](int k, float (&v)[8]) {
+  const auto finish = [&](int c, int k, float (&v)[8]) {
     if (k < a.K && a.h) store_cols<TX, VEC>(h_out, k, a.K, v);
     if (a.norm && k < a.K) {
       float w[8];
-      load_weights<VEC>(a, k, w);
+      if constexpr (EARLY) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = w_kept[c][e];
+      } else {
+        load_weights<VEC>(a, k, w);
+      }
 #pragma unroll
       for (int e = 0; e < 8; e += 2)
         unpack2(mul2(mul2(pack2(v[e], v[e + 1]), pack2(rstd, rstd)), pack2(w[e], w[e + 1])), v[e], v[e + 1]);
@@ -202,11 +215,11 @@ __global__ void __launch_bounds__(CH == 4 || CH == 8 ? 512 : 1024) rms_norm_kern
   if constexpr (CH > 0) {
 #pragma unroll
     for (int c = 0; c < CH; ++c)
-      if (c == 0 || c * step < a.K) finish(k0 + c * step, h[c]);
+      if (c == 0 || c * step < a.K) finish(c, k0 + c * step, h[c]);
   } else {
     for (int base = 0; base < a.K; base += step) {
       load_h(k0 + base, h[0]);
-      finish(k0 + base, h[0]);
+      finish(0, k0 + base, h[0]);
     }
   }
 }

@@ -27,6 +27,10 @@
 //
 // Long runs of bf16 queries go to the kernel of sf_paged_prompt.h.
 //
+// Measured.  Bound by the cache's bytes: 16 sequences of 8192 tokens, 64 query and 8 kv heads of 128, 61 us, 4.4 TB/s;
+// 64 sequences of up to 4096 tokens, 32 heads, 203 us, 5.8 TB/s.  Bound by latency: one sequence of 1000 tokens, 12 us,
+// of which the merge is 4.
+//
 // Warps 0-3: softmax and sums.  Warp 4: TMA copies of pages.  Warp 5: MMAs.  Every wait is bounded: on expiry the
 // kernel records it in the device error word and raises a flag on which the other roles stop waiting.
 #include <algorithm>

@@ -6,6 +6,10 @@
 //
 // h stays in registers in fp32 between the sum and the output, so x and the residual are read once and the sum is
 // rounded only where it is stored.
+//
+// Memory-bound: 4096 x 8192 bf16 with the residual and e4m3 output, 236 MB, takes 48 us = 4.9 TB/s, 8192 x 4096 45 us;
+// one row of 4096 2.2 us, a launch.  Rows whose length is no multiple of 8 take loads of one element (4096 x 4097:
+// 75 us).
 #include <atomic>
 #include <cfloat>
 #include <cstdint>

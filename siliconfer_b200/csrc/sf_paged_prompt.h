@@ -167,25 +167,28 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     for (int i = 0; i < items && ok; ++i) {
       const PromptItem p = item_at(i);
       // lane l: page of box l two tiles ahead, its scales one tile ahead
-      const auto page_of = [&](int key) { return lane < boxes && key < p.tb ? __ldg(p.pages + (key >> a.lg_page)) : -2; };
+      constexpr long long kNoKey = 1ll << 32;   // no page number, right or wrong
+      const auto page_of = [&](int key) -> long long {
+        return lane < boxes && key < p.tb ? __ldg(p.pages + (key >> a.lg_page)) : kNoKey;
+      };
       struct Box {
         int page;
         float ks, vs;
       };
-      const auto scales_of = [&](int page) {
+      const auto scales_of = [&](long long page) {
         Box x{-1, 0.f, 0.f};
         if (page >= 0 && page < a.c.num_pages) {
-          x.page = page;
+          x.page = (int)page;
           x.ks = __ldg(a.c.k_scales + (size_t)page * Hkv + p.kvh);
           x.vs = __ldg(a.c.v_scales + (size_t)page * Hkv + p.kvh);
-        } else if (page != -2) {
+        } else if (page != kNoKey) {
           atomicOr(&g_dev_error, kErrIndex);
         }
         return x;
       };
       int key = p.ta + lane * box;
       Box nxt = scales_of(page_of(key));
-      int page2 = page_of(key + UNIT);
+      long long page2 = page_of(key + UNIT);
       for (int k0 = p.ta; k0 < p.tb && ok; k0 += UNIT, ++it, key += UNIT) {
         const Box cur = nxt;
         nxt = scales_of(page2);

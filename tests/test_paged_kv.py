@@ -632,3 +632,20 @@ def test_prompt_values_strides_and_padding(cuda):
     torch.cuda.synchronize()
     assert _lib.load().sf_q4_check_device_error() != 0
     assert (out[:600] == 0).all() and (lse[:600] == -math.inf).all() and torch.isfinite(out[600:].float()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [-1, -2, -(2 ** 31), 2 ** 31 - 1])
+@pytest.mark.parametrize("n", [1, 600])
+def test_page_numbers_out_of_range_are_reported(cuda, n, page):
+    """For single tokens and for prompts; the other sequence's rows are what they were."""
+    from siliconfer_b200 import _lib
+    from siliconfer_b200.paged_kv import paged_attention
+    b = Batch([700, 800], [n, n], 32, 8, 64, 16, torch.bfloat16)
+    good = check_attention(b)
+    b.table[0, 3] = page
+    out = paged_attention(b.q, *b.args(), starts=b.starts)
+    torch.cuda.synchronize()
+    assert _lib.load().sf_q4_check_device_error() != 0
+    assert torch.equal(out[n:], good[n:]) and torch.isfinite(out.float()).all()
+    assert _lib.load().sf_q4_check_device_error() == 0

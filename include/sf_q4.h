@@ -289,7 +289,7 @@ int sf_kv_attention_decode(const void* q, int q_dtype, const int8_t* k_codes, co
  * when residual is.  y of y_dtype [T, K], row stride ldy; for SF_E4M3, y holds
  * codes and scales [T, ceil(K/128)] receives, for each row and 128 columns,
  * max|y| / 448 (1 where that is 0, at least 2^-126), codes the e4m3 values
- * nearest to y / scale.  A group that holds an infinity or NaN decodes to NaN.
+ * nearest to y / scale, a quotient rounded to fp32.  A group that holds an infinity or NaN decodes to NaN.
  * sf_quantize_e4m3: the same codes and scales of x itself. */
 int sf_rms_norm(const void* x, int x_dtype, long long ldx, const void* residual, long long ldr, void* h_out,
                 const void* weight, int w_dtype, float eps, void* y, int y_dtype, long long ldy, float* scales,

@@ -2,14 +2,14 @@
 // and 128 columns.
 //
 //   h = x + residual,  y = h / sqrt(mean(h^2) + eps) * weight
-//   scale = max|y| / 448 over 128 columns,  code = e4m3(y / scale)
+//   scale = max|y| / 448 over 128 columns,  code = e4m3(y / scale)   (both quotients rounded once, to fp32)
 //
 // h stays in registers in fp32 between the sum and the output, so x and the residual are read once and the sum is
 // rounded only where it is stored.
 //
-// Memory-bound: 4096 x 8192 bf16 with the residual and e4m3 output, 236 MB, takes 48 us = 4.9 TB/s, 8192 x 4096 45 us;
-// one row of 4096 2.2 us, a launch.  Rows whose length is no multiple of 8 take loads of one element (4096 x 4097:
-// 75 us).
+// Memory-bound: 4096 x 8192 bf16 with the residual and e4m3 output, 236 MB, takes 52 us = 4.6 TB/s, 8192 x 4096 49 us;
+// one row of 4096 2.3 us, a launch.  Codes by one product with the reciprocal, which may be a step off near a tie, took
+// 48, 46 and 2.1 us.  Rows whose length is no multiple of 8 take loads of one element (4096 x 4097: 70 us).
 #include <atomic>
 #include <cfloat>
 #include <cstdint>
@@ -88,6 +88,29 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return d;
 }
 
+// A code is e4m3(y / scale), the quotient rounded to fp32 first: where y and the group's largest are in a simple ratio the
+// quotient of their exact values is a tie between two codes, which this rounding restores (of 67 million codes of a norm
+// 787 then differ from the exact values', 1150 by the unrounded quotient).  y times the reciprocal is off by at most 2^-22
+// of itself (2^-23 of the reciprocal, 2^-24 of each product), so the products with a reciprocal 2^-21 smaller and larger
+// have the quotient between them, and 8 columns are divided only where these round to different codes.
+__device__ __forceinline__ uint2 quotient_codes(const float (&y)[8], float scale) {
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
+  const float near = inv * (1 - 0x1p-21f), far = inv * (1 + 0x1p-21f);
+  float lo[8], hi[8];
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    unpack2(mul2(pack2(y[e], y[e + 1]), pack2(near, near)), lo[e], lo[e + 1]);
+    unpack2(mul2(pack2(y[e], y[e + 1]), pack2(far, far)), hi[e], hi[e + 1]);
+  }
+  const uint2 code = to_e4m3x8(lo), other = to_e4m3x8(hi);
+  if (code.x == other.x && code.y == other.y) return code;
+  float q[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) q[e] = __fdiv_rn(y[e], scale);
+  return to_e4m3x8(q);
+}
+
 // y of 8 columns to memory, in its type or as codes.  16 neighbouring lanes hold one 128-column group; every lane of
 // the warp calls this, with k >= K where it has no columns.
 template <bool VEC>
@@ -100,21 +123,17 @@ __device__ __forceinline__ void put_columns(const NormArgs& a, size_t row, int k
 #pragma unroll
     for (int o = 8; o; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     if (k >= a.K) return;
-    float scale = amax == 0.f ? 1.f : amax * (1.f / kE4m3Max);
+    float scale = amax == 0.f ? 1.f : amax / kE4m3Max;
     if (scale < FLT_MIN) scale = FLT_MIN;
-    float inv;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
     if ((threadIdx.x & 15) == 0) a.scales[row * ((a.K + 127) / 128) + k / 128] = scale;
-    float c[8];
-#pragma unroll
-    for (int e = 0; e < 8; e += 2) unpack2(mul2(pack2(y[e], y[e + 1]), pack2(inv, inv)), c[e], c[e + 1]);
+    const uint2 codes = quotient_codes(y, scale);
     uint8_t* out = static_cast<uint8_t*>(a.y) + row * a.ldy + k;
     if (VEC) {
-      *reinterpret_cast<uint2*>(out) = to_e4m3x8(c);
+      *reinterpret_cast<uint2*>(out) = codes;
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (k + e < a.K) out[e] = to_e4m3(c[e]);
+        if (k + e < a.K) out[e] = (uint8_t)((e < 4 ? codes.x : codes.y) >> 8 * (e % 4));
     }
     return;
   }
@@ -127,9 +146,10 @@ __device__ __forceinline__ void put_columns(const NormArgs& a, size_t row, int k
 // blockDim.x threads a row (whole warps), blockDim.y rows a block (several only where one warp takes a row).  A thread
 // keeps CH x 8 columns of h, blockDim.x x 8 apart; with CH = 0 it reads them again for the output instead (rows of more
 // than 32768).  VEC: every row starts at 16 bytes and K is a multiple of 8.
-// Memory-bound: 4096 x 8192 bf16 with the residual and e4m3 output moves 236 MB.
-template <typename TX, int CH, bool VEC>
-__global__ void __launch_bounds__(CH == 4 || CH == 8 ? 512 : 1024) rms_norm_kernel(const NormArgs a) {
+// Memory-bound: 4096 x 8192 bf16 with the residual and e4m3 output moves 236 MB.  NT: the most threads; rows of 2 chunks a
+// thread keep to 40 registers so that 3 blocks of 512 fit an SM (that case 52 us; with 50 registers and 2 blocks 61).
+template <typename TX, int CH, bool VEC, int NT>
+__global__ void __launch_bounds__(NT, CH == 2 && NT == 512 ? 3 : 1) rms_norm_kernel(const NormArgs a) {
   __shared__ float part[32];
   griddep_wait();
   const size_t row = (size_t)blockIdx.x * blockDim.y + threadIdx.y;
@@ -235,7 +255,7 @@ int run_norm(const NormArgs& a, int x_dtype, cudaStream_t st) {
   const bool vec = a.K % 8 == 0 && at16(a.x) && at16(a.r) && at16(a.h) && at16(a.w) && at16(a.y) &&
                    a.ldx * xe % 16 == 0 && a.ldr * xe % 16 == 0 && (size_t)a.K * xe % 16 == 0 && a.ldy * ye % (a.y_dtype == SF_E4M3 ? 8 : 16) == 0;
   // Few rows: as many threads as the row has chunks, for the shortest chain of loads.  Many rows: 2 chunks a thread
-  // (4096 x 8192: 48 us; 1 chunk 60, 4 chunks 52, 8 chunks 69), more where the row is too long for 512 threads.
+  // (4096 x 8192, codes by one product: 48 us; 1 chunk 60, 4 chunks 52, 8 chunks 69), more where the row is too long for 512 threads.
   const int chunks = (a.K + 7) / 8;
   const bool few = a.T <= 2 * device_info().sms;
   const int ch = few && chunks <= 1024 ? 1 : chunks <= 1024 || (few && chunks <= 2048) ? 2 : chunks <= 2048 ? 4 : chunks <= 4096 ? 8 : 0;
@@ -243,11 +263,12 @@ int run_norm(const NormArgs& a, int x_dtype, cudaStream_t st) {
   const int rows = nt == 32 ? 4 : 1;
   const cudaError_t e = with_type(x_dtype, [&](auto* t) {
     using TX = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
-    auto* fn = ch == 1   ? (vec ? rms_norm_kernel<TX, 1, true> : rms_norm_kernel<TX, 1, false>)
-               : ch == 2 ? (vec ? rms_norm_kernel<TX, 2, true> : rms_norm_kernel<TX, 2, false>)
-               : ch == 4 ? (vec ? rms_norm_kernel<TX, 4, true> : rms_norm_kernel<TX, 4, false>)
-               : ch == 8 ? (vec ? rms_norm_kernel<TX, 8, true> : rms_norm_kernel<TX, 8, false>)
-                         : (vec ? rms_norm_kernel<TX, 0, true> : rms_norm_kernel<TX, 0, false>);
+    auto* fn = ch == 1   ? (vec ? rms_norm_kernel<TX, 1, true, 1024> : rms_norm_kernel<TX, 1, false, 1024>)
+               : ch == 2 ? (nt <= 512 ? (vec ? rms_norm_kernel<TX, 2, true, 512> : rms_norm_kernel<TX, 2, false, 512>)
+                                      : (vec ? rms_norm_kernel<TX, 2, true, 1024> : rms_norm_kernel<TX, 2, false, 1024>))
+               : ch == 4 ? (vec ? rms_norm_kernel<TX, 4, true, 512> : rms_norm_kernel<TX, 4, false, 512>)
+               : ch == 8 ? (vec ? rms_norm_kernel<TX, 8, true, 512> : rms_norm_kernel<TX, 8, false, 512>)
+                         : (vec ? rms_norm_kernel<TX, 0, true, 1024> : rms_norm_kernel<TX, 0, false, 1024>);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(((long long)a.T + rows - 1) / rows));
     cfg.blockDim = dim3((unsigned)nt, (unsigned)rows);

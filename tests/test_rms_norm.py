@@ -177,3 +177,38 @@ def test_norm_validation_without_gpu():
     assert call(T=0, x=None) == 0
     q = lambda **k: lib.sf_quantize_e4m3(*{**dict(x=F, xdt=0, ldx=64, y=F, ldy=64, s=F, T=1, K=64, st=None), **k}.values())
     assert q(K=0) == 2 and q(xdt=3) == 3 and q(s=None) == 1 and q(ldy=1) == 2 and q(T=0) == 0
+
+
+def _check_quotients(codes, scales, y):
+    """Scales that are max|y| / 448 rounded once, and codes that are y / scale rounded to fp32 and to e4m3: no bound."""
+    T, K = y.shape
+    G = -(-K // 128)
+    amax = torch.nn.functional.pad(y.abs(), (0, G * 128 - K)).view(T, G, 128).amax(2)
+    want = torch.where(amax == 0, torch.ones_like(amax), (amax.double() / 448).float().clamp_min(2.0 ** -126))
+    assert torch.equal(scales, want)
+    q = (y.double() / scales.double().repeat_interleave(128, 1)[:, :K]).float()
+    assert torch.equal(codes.float(), q.clamp(-448, 448).to(torch.float8_e4m3fn).float())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("T,K", [(1, 4096), (600, 1024), (333, 901), (40, 20000)])
+def test_scales_and_codes_are_rounded_quotients(cuda, T, K, dtype):
+    from siliconfer_b200.norm import quantize_e4m3, rms_norm, rms_norm_e4m3
+    x, r, w = _inputs(T, K, dtype, seed=5)
+    _check_quotients(*quantize_e4m3(x), x.float())
+    for res in (None, r):
+        y = rms_norm(x, w, residual=res, out_dtype=torch.float32)
+        _check_quotients(*rms_norm_e4m3(x, w, residual=res)[:2], y if res is None else y[0])
+
+
+@pytest.mark.gpu
+def test_codes_at_ties(cuda):
+    """All midpoints of two codes and their neighbours in fp32, under scales that divide them exactly and that do not."""
+    from siliconfer_b200.norm import quantize_e4m3
+    codes = torch.arange(0x7f, dtype=torch.uint8).view(torch.float8_e4m3fn).float()
+    mid = torch.nn.functional.pad((codes[1:] + codes[:-1]) / 2, (0, 1), value=448.0)    # 126 of them, and 448
+    rows = torch.stack([torch.nextafter(mid, mid * 0 + d) for d in (0.0, 1e9)] + [mid, -mid])
+    rows[:, -1] = 448
+    rows = torch.cat([rows * f for f in (1.0, 3.0, 7.0, 1.1, 0.3, 2.0 ** -100, 2.0 ** 100)]).cuda()
+    _check_quotients(*quantize_e4m3(rows), rows)

@@ -22,10 +22,13 @@
 //    row's largest lose what lies under 2^-17, 2^-21 or 2^-33 of it).
 //  * out^T[d, column] = V^T P^T: the head's columns are the MMA's rows, V is its transposed operand.  Weights are cut
 //    into as many parts as queries: 8, 12 or 24 bits, and no coarser than 2^-21 of the reference for bf16.
+// The finer of the queries' and the output's types decides the parts: an fp32 output of bf16 queries has six.  With two, a
+// weight is within 2^-8 of itself, which moves a bf16 output by 3e-4 to 5e-4 of its norm, a fifth to a third of what its
+// own rounding does (1.7e-3); a third part would cost the decode step half again as many columns and conversions.
 // Both scores and partial sums go to fresh TMEM buffers, two each; a thread is one key for the scores and one column d
 // for the sums, which it keeps in registers in fp32.
 //
-// Long runs of bf16 queries go to the kernel of sf_paged_prompt.h.
+// Long runs of bf16 queries with 16-bit outputs go to the kernel of sf_paged_prompt.h.
 //
 // Measured.  Bound by the cache's bytes: 16 sequences of 8192 tokens, 64 query and 8 kv heads of 128, 61 us, 4.4 TB/s;
 // 64 sequences of up to 4096 tokens, 32 heads, 203 us, 5.8 TB/s.  Bound by latency: one sequence of 1000 tokens, 12 us,
@@ -910,7 +913,8 @@ int sf_paged_attention(const sf_paged_cache* cache, const void* q, int q_dtype, 
   const long long items = ((long long)T * a.G / kPromptRows + cache->batch) * cache->n_kv_heads;
   const bool many = (long long)T * a.G >= 64ll * cache->batch &&
                     std::max((long long)T * a.G / kPromptRows, (long long)cache->batch) * cache->n_kv_heads >= device_info().sms / 8;
-  const bool prompt = q_dtype == SF_BF16 && (D == 64 || D == 128) && many && items <= 0x7fffffffll &&
+  const int type = std::min(q_dtype, out_dtype);   // the finer one
+  const bool prompt = q_dtype == SF_BF16 && out_dtype != SF_F32 && (D == 64 || D == 128) && many && items <= 0x7fffffffll &&
                       reinterpret_cast<uintptr_t>(out) % 16 == 0;
   if (prompt) {
     const bool q_vec = reinterpret_cast<uintptr_t>(q) % 16 == 0 && qts % 8 == 0 && qhs % 8 == 0;
@@ -919,8 +923,8 @@ int sf_paged_attention(const sf_paged_cache* cache, const void* q, int q_dtype, 
   const auto go = [&](auto d) {
     constexpr int DD = decltype(d)::value;
     if ((long long)T * a.G <= cache->batch)
-      return q_dtype == SF_BF16 ? launch<DD, 2, 1>(a, st) : q_dtype == SF_F16 ? launch<DD, 3, 1>(a, st) : launch<DD, 6, 1>(a, st);
-    return q_dtype == SF_BF16 ? launch<DD, 2, 8>(a, st) : q_dtype == SF_F16 ? launch<DD, 3, 8>(a, st) : launch<DD, 6, 8>(a, st);
+      return type == SF_BF16 ? launch<DD, 2, 1>(a, st) : type == SF_F16 ? launch<DD, 3, 1>(a, st) : launch<DD, 6, 1>(a, st);
+    return type == SF_BF16 ? launch<DD, 2, 8>(a, st) : type == SF_F16 ? launch<DD, 3, 8>(a, st) : launch<DD, 6, 8>(a, st);
   };
   return D == 64    ? go(std::integral_constant<int, 64>())
          : D == 96  ? go(std::integral_constant<int, 96>())

@@ -1,5 +1,5 @@
-// sf_paged_prompt.h -- attention over the paged e4m3 cache for long runs of bf16 queries (part of sf_paged_attention.cu,
-// whose formulas, reference and query scaling it shares).
+// sf_paged_prompt.h -- attention over the paged e4m3 cache for long runs of bf16 queries with 16-bit outputs (part of
+// sf_paged_attention.cu, whose formulas, reference and query scaling it shares).
 //
 // A CTA takes 256 query rows of a kv head's group (two tiles of 128, a thread for each row) through all their keys, 128
 // at a time:
@@ -552,8 +552,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         for (int e = 0; e < 16; e += 8) {
           if (!mine) break;
           const float z[8] = {x[e], x[e + 1], x[e + 2], x[e + 3], x[e + 4], x[e + 5], x[e + 6], x[e + 7]};
-          if (a.out_dtype == SF_F32) store8(static_cast<float*>(a.out) + th * D + c + e, z);
-          else if (a.out_dtype == SF_F16) store8(static_cast<__half*>(a.out) + th * D + c + e, z);
+          if (a.out_dtype == SF_F16) store8(static_cast<__half*>(a.out) + th * D + c + e, z);
           else store8(static_cast<__nv_bfloat16*>(a.out) + th * D + c + e, z);
         }
       }

@@ -39,7 +39,8 @@ def paged_attention(q, k_codes, k_scales, v_codes, v_scales, block_table, seq_le
     """q [T, heads, head_dim] -> softmax(scale * q . k) v over each row's own and earlier tokens.
 
     ``scale`` defaults to head_dim^-0.5; ``window`` > 0 limits a row to its
-    last ``window`` keys.  A row that sees no key gives 0.  ``return_lse`` adds
+    last ``window`` keys.  Weights are held as fine as the finer of q's type
+    and ``out_dtype`` (q's type by default).  A row that sees no key gives 0.  ``return_lse`` adds
     log sum e^(scale * q . k) [T, heads] (-inf for such a row)."""
     out, lse = _lib.ext().paged_attention(q, k_codes, k_scales, v_codes, v_scales, block_table, seq_lens, starts, scale,
                                           window, out_dtype, return_lse)

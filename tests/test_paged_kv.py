@@ -649,3 +649,30 @@ def test_page_numbers_out_of_range_are_reported(cuda, n, page):
     assert _lib.load().sf_q4_check_device_error() != 0
     assert torch.equal(out[n:], good[n:]) and torch.isfinite(out.float()).all()
     assert _lib.load().sf_q4_check_device_error() == 0
+
+
+def _mass(b, **kw):
+    """sum_j p_j |v_j| of every output."""
+    v, b.v = b.v, (b.v.view(torch.uint8) & 0x7f).view(torch.float8_e4m3fn)
+    out = b.ref(**kw)[0]
+    b.v = v
+    return out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,out_dtype", [(torch.bfloat16, torch.float32), (torch.float16, torch.float32),
+                                             (torch.bfloat16, torch.float16), (torch.float32, torch.float16)])
+@pytest.mark.parametrize("H,Hkv,D,n", [(64, 8, 128, 1), (14, 2, 64, 1), (8, 8, 256, 1), (4, 4, 96, 3), (64, 8, 128, 300),
+                                       (16, 16, 64, 600)])
+def test_weights_are_as_fine_as_the_output(cuda, H, Hkv, D, n, dtype, out_dtype):
+    """The finer of the queries' and the output's types.  Few keys and queries exact in their type, so that a weight's own
+    rounding shows: fp32 within 2e-5 of itself, and its share of the sum, 5e-5 of sum p |v| in all; fp16 2^-11 more, and
+    half a unit of the output."""
+    from siliconfer_b200.paged_kv import paged_attention
+    b = Batch([n + 1, n + 2, n + 5, n + 30], [n] * 4, H, Hkv, D, 16, dtype)
+    out = paged_attention(b.q, *b.args(), starts=b.starts, out_dtype=out_dtype)
+    ref, mass = b.ref()[0], _mass(b)
+    bound = 5e-5 * mass
+    if out_dtype == torch.float16:
+        bound = bound + 2.0 ** -11 * mass + 2.0 ** -11 * ref.abs() + 2.0 ** -24
+    assert ((out.double() - ref).abs() <= bound).all()

@@ -8,7 +8,7 @@
 //
 // Every element is read and written once, and a page's rows wait in registers for the page's largest value.  A decode
 // step (8 tokens, 32 heads) takes 3.9 us, most of it the launch.  4096 tokens with 64 query and 8 kv heads of 128 take
-// 42.5 us, 3.8 TB/s: queries pass at the memory's rate, the pages' part is held by its instructions (a maximum, a turn,
+// 43.0 us, 3.8 TB/s: queries pass at the memory's rate, the pages' part is held by its instructions (a maximum, a turn,
 // a conversion for each element), so it runs first.  With a division for every item instead of a fixed item for a
 // thread, that call took 49 us.
 #include <atomic>
@@ -188,10 +188,13 @@ template <typename TX, bool VEC, typename Position>
 __device__ __forceinline__ void turn_token(int tid, int threads, const TX* x, long long xhs, TX* out, long long ohs, int H,
                                            int D, const Turn& t, Position&& position) {
   // A thread takes one item of every (threads / per)-th head, some heads at a time: their elements are asked for first,
-  // the angles, which hang on the position, once.
+  // the angles, which hang on the position, once.  The position is found in the first pass of both loops, the only one
+  // that every lane of a warp makes.
   constexpr int M = kAtOnce<TX>;
   const int per = head_items<VEC>(t, D), heads = per < threads ? threads / per : 1, lanes = per < threads ? heads * per : threads;
   const int h0 = per < threads ? tid / per : 0;
+  long long pos = 0;
+  bool known = false, ok = true;
   for (int item = per < threads ? tid - h0 * per : tid; item < per; item += threads) {
     const Place at = place_of<VEC>(item, t, D);
     Angles<VEC> w;
@@ -201,10 +204,13 @@ __device__ __forceinline__ void turn_token(int tid, int threads, const TX* x, lo
 #pragma unroll
       for (int i = 0; i < M; ++i)
         if (h + i * heads < H && tid < lanes) load_item<TX, VEC>(x + (h + i * heads) * xhs, at, raw[i]);
-      if (first) {
-        const long long pos = position();   // by whole warps
-        const bool ok = t.rot == 0 || (pos >= 0 && pos < t.max_pos);
+      if (!known) {
+        known = true;
+        pos = position();   // by whole warps
+        ok = t.rot == 0 || (pos >= 0 && pos < t.max_pos);
         if (!ok && tid == 0) atomicOr(&g_dev_error, kErrIndex);
+      }
+      if (first) {
         load_angles<VEC>(t, item, t.table + (ok ? pos * t.rot : 0), ok, w);
         first = false;
       }

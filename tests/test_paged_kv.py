@@ -676,3 +676,15 @@ def test_weights_are_as_fine_as_the_output(cuda, H, Hkv, D, n, dtype, out_dtype)
     if out_dtype == torch.float16:
         bound = bound + 2.0 ** -11 * mass + 2.0 ** -11 * ref.abs() + 2.0 ** -24
     assert ((out.double() - ref).abs() <= bound).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,dtype", [(2, torch.bfloat16), (2, torch.float16), (1, torch.float32), (1, torch.bfloat16)])
+@pytest.mark.parametrize("n,interleaved", [(64, False), (61, True)])
+def test_append_heads_of_more_items_than_threads(cuda, H, dtype, n, interleaved):
+    """48 items a head and 32 threads a token: many tokens of few heads, among more sequences than a search probes at once."""
+    lens = [n + 5 * b for b in range(40)]
+    b = Batch(lens, [n] * 40, H, 1, 96, 32, dtype, seed=H)
+    check_append(b, dtype, rot=20, interleaved=interleaved)
+    b = Batch(lens, [n] * 40, H, 1, 96, 32, dtype, seed=H)
+    check_append(b, dtype, rot=96, interleaved=interleaved, strided=True)

@@ -192,9 +192,14 @@ struct Lay {
   static_assert(TMEM_USED <= 512, "TMEM plan");
 };
 
+// First key that a row sees which sees none from `end` on.  Rows before their sequence have an `end` below zero, which
+// must not be taken from a window near 2^31.
+__device__ __forceinline__ int first_seen(const AttnArgs& a, int end) {
+  return a.window > 0 ? max(0, max(0, end) - a.window) : 0;
+}
 // First key that the sequence's units cover, a multiple of UNIT.
 __device__ __forceinline__ int keys_from(const AttnArgs& a, int len, int n) {
-  return a.window > 0 ? max(0, len - n + 1 - a.window) & ~(UNIT - 1) : 0;
+  return first_seen(a, len - n + 1) & ~(UNIT - 1);
 }
 
 // A list is long at this many units for each resident CTA: at 80 (64 x 4096 keys, 32 kv heads) the small CTAs gain 0.13
@@ -246,8 +251,8 @@ __device__ __forceinline__ Part part_at(const AttnArgs& a, const SeqInfo* info, 
   p.last_row = min(p.row0 + RT, s.n * a.G) - 1;
   const int tile_hi = p.pos0 + p.last_row / a.G + 1;
   p.all_hi = p.pos0 + p.row0 / a.G + 1;
-  p.tile_lo = a.window > 0 ? max(0, p.all_hi - a.window) : 0;
-  p.all_lo = a.window > 0 ? max(0, tile_hi - a.window) : 0;
+  p.tile_lo = first_seen(a, p.all_hi);
+  p.all_lo = first_seen(a, tile_hi);
   // tiles of keys without one that some row sees are left out
   p.ta = max(from + j0 * UNIT, p.tile_lo & ~(UNIT - 1));
   p.tb = (int)min((long long)tile_hi, from + (long long)(j0 + (p.u1 - u)) * UNIT);
@@ -614,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : D <= 128 ? 3 : 1)
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
               const int pos = p.pos0 + (p.row0 + r) / a.G;
-              if (key > pos || (a.window > 0 && key <= pos - a.window)) y[r] = -INFINITY;
+              if (key > pos || key < first_seen(a, pos + 1)) y[r] = -INFINITY;
             }
           }
           // ---- the reference, if a key exceeds it by more than a factor of 2 ----
@@ -719,7 +724,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : D <= 128 ? 3 : 1)
 #pragma unroll
                   for (int r = 0; r < RT; ++r) {
                     const int pos = p.pos0 + (p.row0 + r) / a.G;
-                    if (k0 + kk <= pos && (a.window <= 0 || k0 + kk > pos - a.window)) o[mt][r] = __int_as_float(0x7fffffff);
+                    if (k0 + kk <= pos && k0 + kk >= first_seen(a, pos + 1)) o[mt][r] = __int_as_float(0x7fffffff);
                   }
                 }
               named_barrier_sync(1, 32 * kSoftWarps);
@@ -902,7 +907,8 @@ int sf_paged_attention(const sf_paged_cache* cache, const void* q, int q_dtype, 
   a.c = *cache; a.q = q; a.qts = qts; a.qhs = qhs; a.out = out; a.lse = lse;
   a.desc = static_cast<int*>(workspace);
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (size_t)device_info().sms * kMaxCtasPerSm * 2 * 32);
-  a.H = H; a.T = T; a.G = H / cache->n_kv_heads; a.q_dtype = q_dtype; a.out_dtype = out_dtype; a.window = window;
+  a.H = H; a.T = T; a.G = H / cache->n_kv_heads; a.q_dtype = q_dtype; a.out_dtype = out_dtype;
+  a.window = window < (long long)cache->pages_per_seq * cache->page_size ? window : 0;   // a wider one hides nothing
   a.lg_page = __builtin_ctz((unsigned)cache->page_size);
   a.scale = scale;
   if ((long long)T * a.G > 0x7fffffffll) return fail(SF_ERR_UNSUPPORTED, "too many query rows");

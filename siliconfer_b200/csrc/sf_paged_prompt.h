@@ -60,8 +60,8 @@ __device__ __forceinline__ PromptItem prompt_item(const AttnArgs& a, const int* 
   p.pos0 = len - n;
   p.all_hi = p.pos0 + p.row0 / a.G + 1;
   p.tb = p.pos0 + p.last_row / a.G + 1;
-  p.ta = a.window > 0 ? max(0, p.all_hi - a.window) & ~(UNIT - 1) : 0;
-  p.all_lo = a.window > 0 ? max(0, p.tb - a.window) : 0;
+  p.ta = first_seen(a, p.all_hi) & ~(UNIT - 1);
+  p.all_lo = first_seen(a, p.tb);
   p.pages = a.c.block_table + (size_t)b * a.c.pages_per_seq;
   return p;
 }
@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
               over = fmaxf(over, fmaxf(m0, m1) + sc.z);
             }
           } else {
-            const int hi = pos - k0, lo = a.window > 0 ? hi - a.window : -1;
+            const int hi = pos - k0, lo = first_seen(a, pos + 1) - k0;
 #pragma unroll
             for (int c = 0; c < UNIT / 16; ++c) {
               const float4 sc = scales[c * 16 >> lg_box];
@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
               float m = -INFINITY;
 #pragma unroll
               for (int e = 16 * c; e < 16 * c + 16; ++e) {
-                y[e] = e > to || e <= lo ? -INFINITY : y[e] * fk;
+                y[e] = e > to || e < lo ? -INFINITY : y[e] * fk;
                 m = fmaxf(m, y[e]);
               }
               over = fmaxf(over, m + sc.z);
@@ -508,7 +508,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             if (!whole && any_of<256>(nan != 0)) {
               for (int kk = 0; kk < UNIT && k0 + kk < p.tb; ++kk) {
                 if (scales[kk >> lg_box].w == 0.f) continue;
-                const bool sees = k0 + kk <= pos && (a.window <= 0 || k0 + kk > pos - a.window);
+                const bool sees = k0 + kk <= pos && k0 + kk >= first_seen(a, pos + 1);
                 for (int d = 0; d < D; ++d) {
                   if ((mem[L::V0 + swizzle(kk * L::INNER + d, L::INNER)] & 0x7fu) != 0x7fu) continue;
                   uint32_t w;

@@ -688,3 +688,19 @@ def test_append_heads_of_more_items_than_threads(cuda, H, dtype, n, interleaved)
     check_append(b, dtype, rot=20, interleaved=interleaved)
     b = Batch(lens, [n] * 40, H, 1, 96, 32, dtype, seed=H)
     check_append(b, dtype, rot=96, interleaved=interleaved, strided=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 100, 2 ** 30, 1024])
+@pytest.mark.parametrize("n,D", [(4, 64), (400, 128)])
+def test_windows_wider_than_the_sequences(cuda, n, D, window):
+    """They hide nothing, from sequences with fewer tokens than rows either."""
+    from siliconfer_b200 import _lib
+    from siliconfer_b200.paged_kv import paged_attention
+    b = Batch([n, n, n + 500, n], [n] * 4, 32, 8, D, 16, torch.bfloat16)
+    b.seq_lens.copy_(torch.tensor([1, n // 2, n + 500, 0]))
+    want, lse = paged_attention(b.q, *b.args(), starts=b.starts, return_lse=True)
+    out, l2 = paged_attention(b.q, *b.args(), starts=b.starts, return_lse=True, window=window)
+    assert torch.equal(out, want) and torch.equal(l2, lse)
+    assert torch.isfinite(l2[n - 1]).all() and (out[:n - 1] == 0).all()
+    assert _lib.load().sf_q4_check_device_error() == 0

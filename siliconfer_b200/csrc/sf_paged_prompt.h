@@ -37,7 +37,7 @@ __device__ __forceinline__ uint32_t swizzle(uint32_t at, int inner) { return at 
 
 // The 256 rows of a work item, and the keys that some of them see.
 struct PromptItem {
-  int kvh, row0, last_row, r_first, pos0, ta, tb, all_lo, all_hi;
+  int kvh, row0, last_row, r_first, pos0, ta, tb, lo, all_lo, all_hi;   // lo: the first key that some row sees; ta: its tile's
   const int* pages;
 };
 __device__ __forceinline__ PromptItem prompt_item(const AttnArgs& a, const int* first, int i) {
@@ -60,7 +60,8 @@ __device__ __forceinline__ PromptItem prompt_item(const AttnArgs& a, const int* 
   p.pos0 = len - n;
   p.all_hi = p.pos0 + p.row0 / a.G + 1;
   p.tb = p.pos0 + p.last_row / a.G + 1;
-  p.ta = first_seen(a, p.all_hi) & ~(UNIT - 1);
+  p.lo = first_seen(a, p.all_hi);
+  p.ta = p.lo & ~(UNIT - 1);
   p.all_lo = first_seen(a, p.tb);
   p.pages = a.c.block_table + (size_t)b * a.c.pages_per_seq;
   return p;
@@ -168,8 +169,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const PromptItem p = item_at(i);
       // lane l: page of box l two tiles ahead, its scales one tile ahead
       constexpr long long kNoKey = 1ll << 32;   // no page number, right or wrong
-      const auto page_of = [&](int key) -> long long {
-        return lane < boxes && key < p.tb ? __ldg(p.pages + (key >> a.lg_page)) : kNoKey;
+      const auto page_of = [&](int key) -> long long {   // a page that ends before the first key may have been given up
+        return lane < boxes && key < p.tb && key + box > p.lo ? __ldg(p.pages + (key >> a.lg_page)) : kNoKey;
       };
       struct Box {
         int page;

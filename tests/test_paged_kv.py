@@ -704,3 +704,20 @@ def test_windows_wider_than_the_sequences(cuda, n, D, window):
     assert torch.equal(out, want) and torch.equal(l2, lse)
     assert torch.isfinite(l2[n - 1]).all() and (out[:n - 1] == 0).all()
     assert _lib.load().sf_q4_check_device_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 600])
+@pytest.mark.parametrize("D,page", [(64, 16), (128, 32), (64, 128)])
+def test_pages_that_a_window_has_given_up(cuda, D, page, n):
+    """Page numbers before a sequence's first key in the window are not looked at, for single tokens and for prompts."""
+    from siliconfer_b200 import _lib
+    from siliconfer_b200.paged_kv import paged_attention
+    b = Batch([1500, 905], [n, n], 32, 8, D, page, torch.bfloat16)
+    good = check_attention(b, window=200)
+    for s, l, _, _ in b.rows():
+        b.table[s, :max(0, l - n + 1 - 200) // page] = -1
+    out = paged_attention(b.q, *b.args(), starts=b.starts, window=200)
+    torch.cuda.synchronize()
+    assert _lib.load().sf_q4_check_device_error() == 0
+    assert torch.equal(out, good)

@@ -328,10 +328,14 @@ int sf_rotary(const void* x, int dtype, long long xts, long long xhs, void* out,
  * rows starts[b] .. starts[b+1]-1 (starts NULL: T / batch rows each), and are
  * the sequence's last tokens.  A sequence with fewer tokens than rows has padding
  * rows in front: nothing of them is written, their query is turned as at
- * position 0, and they see no key.  page_size 16, 32, 64, 128 or 256; head_dim 64, 96,
+ * position 0, and they see no key.  So have rows before starts[0] and from
+ * starts[batch] on, which are no sequence's (a captured step replayed with fewer
+ * tokens).  page_size 16, 32, 64, 128 or 256; head_dim 64, 96,
  * 128 or 256; batch <= 4096.  block_table, seq_lens and starts are int32 device
- * arrays; a page, length or position outside its tensor is skipped and reported
- * as SF_ERR_INDEX by sf_q4_check_device_error. */
+ * arrays; a page or length outside its tensor is skipped and reported as
+ * SF_ERR_INDEX by sf_q4_check_device_error.  So are starts that fall or leave
+ * the T rows: an append skips the sequences concerned, and attention gives 0 for
+ * the whole call. */
 typedef struct {
   uint8_t* k_codes;
   float* k_scales;

@@ -36,14 +36,16 @@ struct TokenAt {
   bool ok;
   int b, pos;
 };
-// Sequence and position of row `tok` (negative for a padding row); called by whole warps.
+// Sequence and position of row `tok` (negative for a padding row and for a row of no sequence, before the first one's or
+// behind the last one's); called by whole warps.
 __device__ __forceinline__ TokenAt token_at(const sf_paged_cache& c, int T, int tok) {
   const int b = c.starts ? warp_last_le(c.batch, tok, [&](int i) { return (long long)c.starts[i]; })
                          : tok / (T / c.batch);
   const int r0 = first_row(c, T, b), r1 = first_row(c, T, b + 1);
+  const bool rows_ok = r0 >= 0 && r0 <= r1 && r1 <= T;
+  if (rows_ok && ((b == 0 && tok < r0) || (b == c.batch - 1 && tok >= r1))) return {true, b, -1};
   const int len = c.seq_lens[b];
-  const bool ok = r0 >= 0 && r0 <= tok && tok < r1 && r1 <= T && len_ok(c, len);
-  return {ok, b, len - r1 + tok};
+  return {rows_ok && r0 <= tok && tok < r1 && len_ok(c, len), b, len - r1 + tok};
 }
 
 // Work units of an append: one for each page that a sequence's new rows may touch.  Sequence b's units start at

@@ -259,6 +259,17 @@ __device__ __forceinline__ Part part_at(const AttnArgs& a, const SeqInfo* info, 
   return p;
 }
 
+// Result of the call's rows that no sequence holds, [0, from) and [to, T), each written by one CTA.
+__device__ __forceinline__ void clear_rows(const AttnArgs& a, int from, int to) {
+  const size_t width = (size_t)a.H * a.c.head_dim;
+  for (int i = blockIdx.x; i < from + (a.T - to); i += gridDim.x) {
+    const size_t row = i < from ? i : to + (i - from);
+    for (size_t e = threadIdx.x; e < width; e += blockDim.x) store_out(a, row * width + e, 0.f);
+    if (a.lse)
+      for (int h = threadIdx.x; h < a.H; h += blockDim.x) a.lse[row * a.H + h] = -INFINITY;
+  }
+}
+
 template <int D, int PARTS, int RT>
 __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : D <= 128 ? 3 : 1)
     paged_attention_kernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV,
@@ -304,17 +315,21 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : D <= 128 ? 3 : 1)
 
   // ---- the batch's units, and this CTA's share ----
   const int B = a.c.batch, Hkv = a.c.n_kv_heads, page_size = a.c.page_size;
+  // with starts that are none (below 0, falling, past T) no row is a sequence's
+  const int rows0 = first_row(a.c, a.T, 0), rows1 = first_row(a.c, a.T, B);
   long long total = 0;
+  int bad = 0;
   for (int at = 0; at < B; at += kThreads) {
     const int b = at + threadIdx.x;
     long long u = 0;
-    int len = 0, n = 0;
+    int len = 0, n = 0, off = 0;
     if (b < B) {
       const int r0 = first_row(a.c, a.T, b), r1 = first_row(a.c, a.T, b + 1);
       len = a.c.seq_lens[b];
       n = r1 - r0;
       if (r0 < 0 || n < 0 || r1 > a.T) {
         n = 0;
+        off = 1;
         atomicOr(&g_dev_error, kErrIndex);
       }
       if (!len_ok(a.c, len)) {
@@ -339,8 +354,10 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : D <= 128 ? 3 : 1)
       total += wsum[w];
     }
     if (b < B) info[b] = SeqInfo{before + incl - u, len, n};
-    __syncthreads();
+    bad |= __syncthreads_or(off);
   }
+  if (bad) total = 0;
+  clear_rows(a, bad ? 0 : rows0, bad ? 0 : rows1);
   const long long cta = blockIdx.x;
   const Shares shares(total, a.resident, (int)gridDim.x);
   if (threadIdx.x == 0) a.desc[8 * cta] = 0;

@@ -109,15 +109,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 
   // ---- items before each sequence's ----
   const int B = a.c.batch, Hkv = a.c.n_kv_heads, page_size = a.c.page_size;
-  int total = 0;
+  const int rows0 = first_row(a.c, a.T, 0), rows1 = first_row(a.c, a.T, B);
+  int total = 0, bad = 0;
   for (int at = 0; at < B; at += kPromptThreads) {
     const int b = at + threadIdx.x;
-    int u = 0;
+    int u = 0, off = 0;
     if (b < B) {
       const int r0 = first_row(a.c, a.T, b), r1 = first_row(a.c, a.T, b + 1);
       int n = r1 - r0;
       if (r0 < 0 || n < 0 || r1 > a.T) {
         n = 0;
+        off = 1;
         atomicOr(&g_dev_error, kErrIndex);
       }
       if (!len_ok(a.c, a.c.seq_lens[b])) atomicOr(&g_dev_error, kErrIndex);
@@ -138,8 +140,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       total += wsum[w];
     }
     if (b < B) first[b] = before + incl - u;
-    __syncthreads();
+    bad |= __syncthreads_or(off);
   }
+  if (bad) total = 0;
+  clear_rows(a, bad ? 0 : rows0, bad ? 0 : rows1);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();

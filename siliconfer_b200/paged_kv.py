@@ -13,7 +13,9 @@ starts[b + 1] - 1 of q, k and v (without ``starts``: the same number for every
 sequence), and are the last of its seq_lens[b] tokens.  Token j of sequence b
 is slot j % page_size of page block_table[b, j // page_size].  A sequence with
 fewer tokens than rows has padding rows in front, which are not written and see
-no key (a waiting slot of a decode batch: length 0 and one row).
+no key (a waiting slot of a decode batch: length 0 and one row).  Rows before
+starts[0] and from starts[batch] on are no sequence's and are treated alike (a
+captured step replayed with fewer tokens).
 """
 from __future__ import annotations
 

@@ -721,3 +721,60 @@ def test_pages_that_a_window_has_given_up(cuda, D, page, n):
     torch.cuda.synchronize()
     assert _lib.load().sf_q4_check_device_error() == 0
     assert torch.equal(out, good)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [2, 400])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_of_no_sequence(cuda, n, dtype):
+    """Rows before the first sequence's and behind the last one's: turned as at position 0, not written, and they see nothing;
+    starts that fall or leave the rows: an error, and 0 for all of them."""
+    from siliconfer_b200 import _lib
+    from siliconfer_b200.paged_kv import paged_append, paged_attention
+    from siliconfer_b200.rotary import rotary_table
+    H, Hkv, D, before, after = 32, 8, 64, 3, 5
+    b = Batch([700, n, 30], [n, n, 3], H, Hkv, D, 16, dtype)
+    q = torch.randn(before + b.T + after, H, D, device="cuda").to(dtype)
+    inside = torch.zeros(q.shape[0], dtype=torch.bool, device="cuda")
+    inside[before:before + b.T] = True
+    q[inside] = b.q
+
+    def attend(starts):
+        junk = [torch.full(s, 7.0, device="cuda", dtype=d) for s, d in (((q.shape), dtype), ((q.shape[:2]), torch.float32)) * 4]
+        del junk   # what the call's outputs may be made of
+        return paged_attention(q, *b.args(), starts=starts, return_lse=True)
+
+    def check(out, lse):
+        ref, lref, vmax = b.ref()
+        bound = 3e-5 * vmax if dtype == torch.float32 else 2.0 ** -10 * vmax + 2.0 ** -8 * ref.abs()
+        assert ((out[inside].double() - ref).abs() <= bound).all()
+        assert ((lse[inside].double() - lref).abs() <= 4e-5 + 2e-6 * lref.abs()).all()
+        assert (out[~inside] == 0).all() and (lse[~inside] == -math.inf).all()
+
+    starts = b.starts + before
+    check(*attend(starts))
+    # a captured step, replayed with fewer tokens
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, l2 = paged_attention(q, *b.args(), starts=starts, return_lse=True)
+    graph.replay()
+    starts[-1] -= 2
+    b.seq_lens[-1] -= 2
+    graph.replay()
+    inside[before + b.T - 2:] = False
+    b.lens, b.news, b.T, b.q = [700, n, 28], [n, n, 1], b.T - 2, b.q[:-2]
+    check(out, l2)
+    # the append: the same rows alone, into a copy of the cache
+    kv = torch.randn(q.shape[0], Hkv, D, device="cuda").to(dtype)
+    table = rotary_table(701, D)
+    caches = [t.clone() for t in (b.k, b.ks, b.v, b.vs)]
+    want = paged_append(kv[inside], kv[inside], *caches, b.table, b.seq_lens, starts=starts - before, q=q[inside], table=table)
+    turned = paged_append(kv, kv, *b.args(), starts=starts, q=q, table=table)
+    assert torch.equal(turned[inside], want) and torch.equal(turned[~inside], q[~inside])
+    for a, c in zip(b.args(), caches):
+        assert torch.equal(a.view(torch.uint8), c.view(torch.uint8))
+    assert _lib.load().sf_q4_check_device_error() == 0
+    for bad in ([0, 5, 4, 9], [0, 5, 6, q.shape[0] + 1], [-1, 5, 6, 9]):
+        out, l2 = attend(torch.tensor(bad, dtype=torch.int32, device="cuda"))
+        assert (out == 0).all() and (l2 == -math.inf).all()
+        assert _lib.load().sf_q4_check_device_error() == 10

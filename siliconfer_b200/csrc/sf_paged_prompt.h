@@ -30,7 +30,7 @@ struct PromptLay {
   static constexpr uint32_t CTL = W0 + V16, SCALES = CTL + 512, FIRST = CTL + 1024;
   static constexpr uint64_t SWZ = INNER == 128 ? kSw128 : kSw64;
   static constexpr uint32_t TMEM_COLS = 512, O0 = 256;       // scores of two tiles, sums of two tiles
-  static size_t smem(int batch) { return 1024 + FIRST + (size_t)(batch + 1) * 4; }
+  static constexpr size_t smem(int batch) { return 1024 + FIRST + (size_t)batch * 4; }
 };
 
 __device__ __forceinline__ uint32_t swizzle(uint32_t at, int inner) { return at ^ ((at >> 3) & (inner == 128 ? 0x70 : 0x30)); }
@@ -587,6 +587,7 @@ int launch_prompt(const AttnArgs& a, long long items, bool q_vec, cudaStream_t s
     return fail(SF_ERR_CUDA, "cuTensorMapEncodeTiled failed for the cache");
   auto* fn = paged_prompt_kernel<D>;
   const size_t smem = L::smem(c.batch);
+  static_assert(L::smem(4096) + 1024 <= 232448, "shared memory plan: with the static arrays, 227 KB for any batch");
   cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return cuda_fail(e, "paged_prompt_kernel shared memory");
   const int sms = device_info().sms;

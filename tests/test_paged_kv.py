@@ -778,3 +778,17 @@ def test_rows_of_no_sequence(cuda, n, dtype):
         out, l2 = attend(torch.tensor(bad, dtype=torch.int32, device="cuda"))
         assert (out == 0).all() and (l2 == -math.inf).all()
         assert _lib.load().sf_q4_check_device_error() == 10
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_the_largest_batch(cuda, D):
+    """4096 sequences, as single tokens and as short runs: nothing is refused, and the last ones' rows are their own."""
+    from siliconfer_b200 import _lib
+    from siliconfer_b200.paged_kv import paged_attention
+    for H, n in ((2, 1), (16, 8)):
+        b = Batch([n + k % 40 for k in range(4096)], [n] * 4096, H, 1, D, 16, torch.bfloat16, ragged=False)
+        out = paged_attention(b.q, *b.args())
+        ref, _, vmax = b.ref()
+        assert ((out.double() - ref).abs() <= 2.0 ** -10 * vmax + 2.0 ** -8 * ref.abs()).all()
+        assert _lib.load().sf_q4_check_device_error() == 0

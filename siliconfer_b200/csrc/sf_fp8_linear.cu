@@ -400,7 +400,8 @@ cudaError_t launch(const CUtensorMap& mx, const CUtensorMap& mw, const CUtensorM
                    cudaStream_t st) {
   auto* fn = fp8_linear_kernel<SPLIT>;
   const size_t smem = Plan<SPLIT>::bytes(p.rows, p.stages);
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  // the limit is the process's: the same for calls of every size, or another thread's could lower it before this launch
+  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);

@@ -9,6 +9,8 @@
 
 namespace sf {
 
+constexpr int kMaxBatch = 4096;
+
 // Greatest b in [0, n) with f(b) <= v, for a non-decreasing f with f(0) <= v; the warp probes 32 places at a time.
 template <typename F>
 __device__ __forceinline__ int warp_last_le(int n, long long v, F&& f) {
@@ -90,7 +92,7 @@ inline int check_paged(const sf_paged_cache* c, int T) {
   if (!c) return fail(SF_ERR_NULL, "null pointer argument");
   if (T < 0 || c->batch < 1 || c->n_kv_heads < 1 || c->num_pages < 1 || c->pages_per_seq < 1)
     return fail(SF_ERR_SHAPE, "need T >= 0 and batch, n_kv_heads, num_pages, pages_per_seq >= 1");
-  if (c->batch > 4096) return fail(SF_ERR_UNSUPPORTED, "batch %d is above 4096", c->batch);
+  if (c->batch > kMaxBatch) return fail(SF_ERR_UNSUPPORTED, "batch %d is above %d", c->batch, kMaxBatch);
   if (!c->starts && T % c->batch) return fail(SF_ERR_SHAPE, "without starts, T must be a multiple of batch");
   if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1)))
     return fail(SF_ERR_UNSUPPORTED, "page_size %d not built (16, 32, 64, 128, 256)", c->page_size);

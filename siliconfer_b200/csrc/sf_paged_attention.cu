@@ -56,6 +56,7 @@ constexpr int UNIT = 128;            // keys of a tile
 constexpr int kMaxRows = 8;          // query rows of a tile: 8, or 1 where no sequence has more
 constexpr int kSoftWarps = 4, kProdWarp = 4, kMmaWarp = 5, kThreads = 192;
 constexpr int kMaxCtasPerSm = 4;
+constexpr size_t kBlockSmem = 232448;   // 227 KB: dynamic and static arrays of a block
 constexpr float kPScale = 128.f;     // of a weight: at most 256, within e4m3
 constexpr float kNone = -1e30f;      // the reference of a part without a key
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -862,9 +863,9 @@ int launch(AttnArgs a, cudaStream_t st) {
     return fail(SF_ERR_CUDA, "cuTensorMapEncodeTiled failed for the cache");
   auto* fn = paged_attention_kernel<D, PARTS, RT>;
   const size_t smem = L::smem(c.batch);
-  if (smem > (size_t)device_info().smem_optin && device_info().smem_optin > 0)
-    return fail(SF_ERR_UNSUPPORTED, "batch %d is too large for head_dim %d", c.batch, D);
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  // the limit is the process's: the same for calls of every batch, or another thread's could lower it before this launch
+  static_assert(L::smem(kMaxBatch) + 1024 <= kBlockSmem, "shared memory plan");
+  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::smem(kMaxBatch));
   if (e != cudaSuccess) return cuda_fail(e, "paged_attention_kernel shared memory");
   // what shared memory, TMEM and registers let an SM hold
   int per_sm = (int)(228 * 1024 / (smem + 2048));

@@ -587,8 +587,8 @@ int launch_prompt(const AttnArgs& a, long long items, bool q_vec, cudaStream_t s
     return fail(SF_ERR_CUDA, "cuTensorMapEncodeTiled failed for the cache");
   auto* fn = paged_prompt_kernel<D>;
   const size_t smem = L::smem(c.batch);
-  static_assert(L::smem(4096) + 1024 <= 232448, "shared memory plan: with the static arrays, 227 KB for any batch");
-  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static_assert(L::smem(kMaxBatch) + 1024 <= kBlockSmem, "shared memory plan");
+  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::smem(kMaxBatch));
   if (e != cudaSuccess) return cuda_fail(e, "paged_prompt_kernel shared memory");
   const int sms = device_info().sms;
   e = launch_kernel(fn, items < sms ? (int)items : sms, kPromptThreads, smem, st, true, mk, mv, a, (int)q_vec);

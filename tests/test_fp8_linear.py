@@ -198,3 +198,35 @@ def test_weight_quantizer_on_cpu():
     assert codes.shape == w.shape and codes.stride(0) % 16 == 0 and scales.shape == (2, 3)
     assert scales[0, 0] == 1 and (codes[:128, :128].float() == 0).all()
     assert torch.allclose(scales[1, 2], w[128:, 256:].abs().max() / 448)
+
+
+@pytest.mark.gpu
+def test_calls_of_different_sizes_from_two_threads(cuda):
+    """A launch's shared memory hangs on its tokens; the calls of one thread leave the other's alone."""
+    import threading
+
+    from siliconfer_b200 import _lib
+    lib, refused = _lib.load(), []
+
+    def work(T):
+        x, xs, w, ws, _ = _case(T, 256, 512, seed=T)
+        ref = torch.empty(T, 256, device="cuda")
+        y, stream = torch.zeros_like(ref), torch.cuda.Stream()
+        torch.cuda.synchronize()
+        for out, n in ((ref, 1), (y, 4000)):
+            for _ in range(n):
+                rc = lib.sf_fp8_linear(x.data_ptr(), x.stride(0), xs.data_ptr(), w.data_ptr(), w.stride(0), ws.data_ptr(), None,
+                                       out.data_ptr(), 0, T, 256, 512, stream.cuda_stream)
+                if rc:
+                    refused.append((T, rc))
+                    return
+            stream.synchronize()
+        if not torch.equal(y, ref):
+            refused.append((T, "result"))
+
+    threads = [threading.Thread(target=work, args=(T,)) for T in (16, 100)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not refused

@@ -792,3 +792,43 @@ def test_the_largest_batch(cuda, D):
         ref, _, vmax = b.ref()
         assert ((out.double() - ref).abs() <= 2.0 ** -10 * vmax + 2.0 ** -8 * ref.abs()).all()
         assert _lib.load().sf_q4_check_device_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 64])
+def test_batches_of_different_sizes_from_two_threads(cuda, n):
+    """A launch's shared memory hangs on its batch; the calls of one thread leave the other's alone."""
+    import ctypes
+    import threading
+
+    from siliconfer_b200 import _lib
+    lib, refused = _lib.load(), []
+    H, Hkv, D = 8, 8, 64
+
+    def work(batch):
+        b = Batch([n] * batch, [n] * batch, H, Hkv, D, 16, torch.bfloat16, ragged=False, seed=batch)
+        cache = _lib.PagedCache(k_codes=b.k.data_ptr(), k_scales=b.ks.data_ptr(), v_codes=b.v.data_ptr(), v_scales=b.vs.data_ptr(),
+                                block_table=b.table.data_ptr(), seq_lens=b.seq_lens.data_ptr(), starts=None, num_pages=b.P,
+                                n_kv_heads=Hkv, page_size=16, head_dim=D, batch=batch, pages_per_seq=b.table.shape[1])
+        size = lib.sf_paged_attention_workspace_bytes(D)
+        ws, stream = torch.empty(size, dtype=torch.uint8, device="cuda"), torch.cuda.Stream()
+        ref = torch.empty(b.T, H, D, dtype=torch.bfloat16, device="cuda")
+        out = torch.zeros_like(ref)
+        torch.cuda.synchronize()
+        for y, times in ((ref, 1), (out, 2000)):
+            for _ in range(times):
+                rc = lib.sf_paged_attention(ctypes.byref(cache), b.q.data_ptr(), 2, H * D, D, y.data_ptr(), 2, None, H, b.T, 0.125, 0,
+                                            ws.data_ptr(), size, stream.cuda_stream)
+                if rc:
+                    refused.append((batch, rc))
+                    return
+            stream.synchronize()
+        if not torch.equal(out, ref):
+            refused.append((batch, "result"))
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in (20, 300)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not refused

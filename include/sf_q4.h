@@ -331,7 +331,7 @@ int sf_rotary(const void* x, int dtype, long long xts, long long xhs, void* out,
  * position 0, and they see no key.  So have rows before starts[0] and from
  * starts[batch] on, which are no sequence's (a captured step replayed with fewer
  * tokens).  page_size 16, 32, 64, 128 or 256; head_dim 64, 96,
- * 128 or 256; batch <= 4096.  block_table, seq_lens and starts are int32 device
+ * 128 or 256; batch <= 4096; pages_per_seq * page_size <= 2^31 - 1024.  block_table, seq_lens and starts are int32 device
  * arrays; a page or length outside its tensor is skipped and reported as
  * SF_ERR_INDEX by sf_q4_check_device_error.  So are starts that fall or leave
  * the T rows: an append skips the sequences concerned, and attention gives 0 for

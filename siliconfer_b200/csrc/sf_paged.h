@@ -98,8 +98,9 @@ inline int check_paged(const sf_paged_cache* c, int T) {
     return fail(SF_ERR_UNSUPPORTED, "page_size %d not built (16, 32, 64, 128, 256)", c->page_size);
   if (!(c->head_dim == 64 || c->head_dim == 96 || c->head_dim == 128 || c->head_dim == 256))
     return fail(SF_ERR_UNSUPPORTED, "head_dim %d not built (64, 96, 128, 256)", c->head_dim);
-  if ((long long)c->pages_per_seq * c->page_size > 0x7fffffffll)
-    return fail(SF_ERR_SHAPE, "a sequence may hold at most 2^31 - 1 tokens");
+  // the kernels look up to 3 tiles of 128 keys beyond a sequence's last one, in 32 bits
+  if ((long long)c->pages_per_seq * c->page_size > 0x7fffffffll - 1023)
+    return fail(SF_ERR_SHAPE, "a sequence may hold at most 2^31 - 1024 tokens");
   if (T == 0) return SF_OK;
   if (!c->k_codes || !c->k_scales || !c->v_codes || !c->v_scales || !c->block_table || !c->seq_lens)
     return fail(SF_ERR_NULL, "null pointer argument");

@@ -832,3 +832,19 @@ def test_batches_of_different_sizes_from_two_threads(cuda, n):
     for t in threads:
         t.join()
     assert not refused
+
+
+def test_sequences_near_31_bits_are_refused_without_gpu():
+    """Positions are 32-bit and tiles of keys are looked at ahead: the last 1023 positions are not for use."""
+    import ctypes
+
+    from siliconfer_b200 import _lib
+    lib, F = _lib.load(), 0x1000
+    for page in (16, 64, 256):
+        for pages, want in ((2 ** 31 // page - 1024 // page, 0), (2 ** 31 // page - 1024 // page + 1, 2), (2 ** 31 // page - 1, 2),
+                            (2 ** 31 // page, 2)):
+            c = ctypes.byref(_lib.PagedCache(k_codes=F, k_scales=F, v_codes=F, v_scales=F, block_table=F, seq_lens=F, starts=None,
+                                             num_pages=4, n_kv_heads=2, page_size=page, head_dim=64, batch=1, pages_per_seq=pages))
+            # no rows: validated, not launched
+            assert lib.sf_paged_attention(c, F, 0, 512, 64, F, 0, None, 8, 0, 1.0, 0, F, 1 << 30, None) == want
+            assert lib.sf_paged_append(c, F, 128, 64, F, 128, 64, None, 0, 0, None, 0, 0, 0, None, 0, 0, 0, None) == want

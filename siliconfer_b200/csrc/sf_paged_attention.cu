@@ -38,6 +38,7 @@
 // kernel records it in the device error word and raises a flag on which the other roles stop waiting.
 #include <algorithm>
 #include <atomic>
+#include <climits>
 #include <cmath>
 #include <cstdint>
 
@@ -931,12 +932,23 @@ int sf_paged_attention(const sf_paged_cache* cache, const void* q, int q_dtype, 
   a.scale = scale;
   if ((long long)T * a.G > 0x7fffffffll) return fail(SF_ERR_UNSUPPORTED, "too many query rows");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // Tiles of 256 rows where the sequences have 64 rows on average and the tiles an eighth of the SMs: 16 sequences of 64
-  // rows over 2048 keys take 57 us so and 95 otherwise, of 128 rows 57 and 181; 16 tiles (1 sequence of 256 rows, 8 kv
-  // heads, 2048 keys) about as long either way, 32 tiles 62 and 95.
+  // Tiles of 256 rows: an SM takes 3 us for 128 keys of a tile, however many of its rows are in use, and some 6 us before
+  // and after.  Tiles of 8 rows: all SMs together take 0.5 ns for 128 keys of a row, and 4 ns more a row (7 at head_dim 64).
+  // So the rows of a round of tiles decide, fewer where the sequences are short; of the lengths the host knows only the
+  // block table's.
+  // Measured, head_dim 128, tiles of 256 and of 8 rows, in us: 18 sequences of 64 rows, 256 keys 15 and 15, 2048 keys 54
+  // and 30, 32768 keys 727 and 155; 64 tiles of 64 rows 17 and 25, 56 and 54, 734 and 556; 128 such 18 and 37, 58 and 90,
+  // 739 and 1187; 256 rows of 64 heads 21 and 69, 63 and 175, 758 and 1174.  Head_dim 64: 64 tiles of 64 rows 14 and 27, 50
+  // and 59, 671 and 401.
+  // One long sequence among many short ones is not seen here: 32 sequences of 64 rows and 8 kv heads, one of 16384 keys and
+  // 31 of 300, take 383 so and 134 otherwise.
   const long long items = ((long long)T * a.G / kPromptRows + cache->batch) * cache->n_kv_heads;
-  const bool many = (long long)T * a.G >= 64ll * cache->batch &&
-                    std::max((long long)T * a.G / kPromptRows, (long long)cache->batch) * cache->n_kv_heads >= device_info().sms / 8;
+  const int sms = device_info().sms;
+  const long long keys = std::min((long long)cache->pages_per_seq * cache->page_size,
+                                  a.window > 0 ? (long long)a.window + kPromptRows : LLONG_MAX);
+  const long long tiles = std::max(((long long)T * a.G + kPromptRows - 1) / kPromptRows, (long long)cache->batch) * cache->n_kv_heads,
+                  rounds = (tiles + sms - 1) / sms, key_tiles = (keys + UNIT - 1) / UNIT;
+  const bool many = (double)T * H * (key_tiles + (D == 64 ? 14 : 7)) >= 5800.0 * rounds * (key_tiles + 2);
   const int type = std::min(q_dtype, out_dtype);   // the finer one
   const bool prompt = q_dtype == SF_BF16 && out_dtype != SF_F32 && (D == 64 || D == 128) && many && items <= 0x7fffffffll &&
                       reinterpret_cast<uintptr_t>(out) % 16 == 0;

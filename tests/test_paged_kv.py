@@ -848,3 +848,19 @@ def test_sequences_near_31_bits_are_refused_without_gpu():
             # no rows: validated, not launched
             assert lib.sf_paged_attention(c, F, 0, 512, 64, F, 0, None, 8, 0, 1.0, 0, F, 1 << 30, None) == want
             assert lib.sf_paged_append(c, F, 128, 64, F, 128, 64, None, 0, 0, None, 0, 0, 0, None, 0, 0, 0, None) == want
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,n,H,Hkv,length,launches", [
+    (18, 1, 64, 1, 32768, 2), (3, 8, 64, 8, 32768, 2), (18, 1, 64, 1, 2048, 2), (8, 8, 64, 8, 32768, 2), (2, 32, 64, 8, 32768, 2),
+    (16, 8, 64, 8, 2048, 1), (16, 8, 64, 8, 32768, 1), (1, 256, 64, 8, 32768, 1), (2, 32, 64, 8, 256, 1), (64, 4, 64, 4, 2048, 1)])
+def test_few_rows_share_the_keys_of_long_sequences(cuda, B, n, H, Hkv, length, launches):
+    """A kernel with a CTA for 256 rows (one launch) where a round of such tiles has rows enough, else keys are shared by all
+    SMs (two launches), whichever was measured to be faster."""
+    from siliconfer_b200 import _lib
+    from siliconfer_b200.paged_kv import paged_attention
+    b = Batch([length] + [n + 40] * (B - 1), [n] * B, H, Hkv, 128, 64, torch.bfloat16, ragged=False)
+    before = _lib.launch_count()
+    paged_attention(b.q, *b.args())
+    assert _lib.launch_count() - before == launches
+    check_attention(b)

@@ -638,7 +638,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : D <= 128 ? 3 : 1)
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
               const int pos = p.pos0 + (p.row0 + r) / a.G;
-              if (key > pos || key < first_seen(a, pos + 1)) y[r] = -INFINITY;
+              if (key > pos || (a.window > 0 && key <= pos - a.window)) y[r] = -INFINITY;
             }
           }
           // ---- the reference, if a key exceeds it by more than a factor of 2 ----
@@ -743,7 +743,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : D <= 128 ? 3 : 1)
 #pragma unroll
                   for (int r = 0; r < RT; ++r) {
                     const int pos = p.pos0 + (p.row0 + r) / a.G;
-                    if (k0 + kk <= pos && k0 + kk >= first_seen(a, pos + 1)) o[mt][r] = __int_as_float(0x7fffffff);
+                    if (k0 + kk <= pos && (a.window <= 0 || k0 + kk > pos - a.window)) o[mt][r] = __int_as_float(0x7fffffff);
                   }
                 }
               named_barrier_sync(1, 32 * kSoftWarps);

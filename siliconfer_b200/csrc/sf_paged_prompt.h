@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
               over = fmaxf(over, fmaxf(m0, m1) + sc.z);
             }
           } else {
-            const int hi = pos - k0, lo = first_seen(a, pos + 1) - k0;
+            const int hi = max(pos - k0, -1), lo = a.window > 0 ? hi - a.window : -1;
 #pragma unroll
             for (int c = 0; c < UNIT / 16; ++c) {
               const float4 sc = scales[c * 16 >> lg_box];
@@ -418,7 +418,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
               float m = -INFINITY;
 #pragma unroll
               for (int e = 16 * c; e < 16 * c + 16; ++e) {
-                y[e] = e > to || e < lo ? -INFINITY : y[e] * fk;
+                y[e] = e > to || e <= lo ? -INFINITY : y[e] * fk;
                 m = fmaxf(m, y[e]);
               }
               over = fmaxf(over, m + sc.z);
@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             if (!whole && any_of<256>(nan != 0)) {
               for (int kk = 0; kk < UNIT && k0 + kk < p.tb; ++kk) {
                 if (scales[kk >> lg_box].w == 0.f) continue;
-                const bool sees = k0 + kk <= pos && k0 + kk >= first_seen(a, pos + 1);
+                const bool sees = k0 + kk <= pos && (a.window <= 0 || k0 + kk > pos - a.window);
                 for (int d = 0; d < D; ++d) {
                   if ((mem[L::V0 + swizzle(kk * L::INNER + d, L::INNER)] & 0x7fu) != 0x7fu) continue;
                   uint32_t w;

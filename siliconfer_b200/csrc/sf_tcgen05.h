@@ -77,12 +77,7 @@ __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.a
 // Shared-memory matrix descriptor: start address >> 4 in bits 0-13, leading and stride byte offsets >> 4 in bits
 // 16-29 and 32-45, version 1 at bit 46, swizzle in bits 61-63.
 enum : uint64_t { kSwNone = 0, kSw128 = 2, kSw64 = 4, kSw32 = 6 };
-__device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t leading, uint32_t stride, uint64_t swizzle) {
-  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(leading >> 4) << 16) | ((uint64_t)(stride >> 4) << 32) |
-         ((uint64_t)1 << 46) | (swizzle << 61);
-}
-// The two words of such a descriptor for a thread that issues many: the upper one is a constant, and an operand n bytes
-// further adds n >> 4 to the lower one.
+// Its two words: the upper one is a constant, and an operand n bytes further adds n >> 4 to the lower one.
 __device__ __forceinline__ uint32_t desc_low(uint32_t saddr, uint32_t leading) {
   return ((saddr & 0x3FFFFu) >> 4) | ((leading >> 4) << 16);
 }

@@ -289,7 +289,8 @@ int sf_kv_attention_decode(const void* q, int q_dtype, const int8_t* k_codes, co
  * when residual is.  y of y_dtype [T, K], row stride ldy; for SF_E4M3, y holds
  * codes and scales [T, ceil(K/128)] receives, for each row and 128 columns,
  * max|y| / 448 (1 where that is 0, at least 2^-126), codes the e4m3 values
- * nearest to y / scale, a quotient rounded to fp32.  A group that holds an infinity or NaN decodes to NaN.
+ * nearest to y / scale, a quotient rounded to fp32.  A group that holds an
+ * infinity or NaN decodes to NaN.
  * sf_quantize_e4m3: the same codes and scales of x itself. */
 int sf_rms_norm(const void* x, int x_dtype, long long ldx, const void* residual, long long ldr, void* h_out,
                 const void* weight, int w_dtype, float eps, void* y, int y_dtype, long long ldy, float* scales,
@@ -330,10 +331,10 @@ int sf_rotary(const void* x, int dtype, long long xts, long long xhs, void* out,
  * rows in front: nothing of them is written, their query is turned as at
  * position 0, and they see no key.  So have rows before starts[0] and from
  * starts[batch] on, which are no sequence's (a captured step replayed with fewer
- * tokens).  page_size 16, 32, 64, 128 or 256; head_dim 64, 96,
- * 128 or 256; batch <= 4096; pages_per_seq * page_size <= 2^31 - 1024.  block_table, seq_lens and starts are int32 device
- * arrays; a page or length outside its tensor is skipped and reported as
- * SF_ERR_INDEX by sf_q4_check_device_error.  So are starts that fall or leave
+ * tokens).  page_size 16, 32, 64, 128 or 256; head_dim 64, 96, 128 or 256;
+ * batch <= 4096; pages_per_seq * page_size <= 2^31 - 1024.  block_table, seq_lens
+ * and starts are int32 device arrays; a page or length outside its tensor is
+ * skipped and reported as SF_ERR_INDEX by sf_q4_check_device_error.  So are starts that fall or leave
  * the T rows: an append skips the sequences concerned, and attention gives 0 for
  * the whole call. */
 typedef struct {
@@ -354,7 +355,8 @@ typedef struct {
  * largest finite value is <= 448 * 2^e.  When rows are added to a page that holds
  * tokens and they need a larger e, its older codes are rewritten for it (exact
  * but where they become subnormal).  Infinities are stored as +-448 * 2^e, NaN as
- * NaN, and neither counts for the scale.  Two sequences of one call must not
+ * NaN, and neither counts for the scale.  A position past the table's end is
+ * turned to NaN and reported as SF_ERR_INDEX.  Two sequences of one call must not
  * write to the same page. */
 int sf_paged_append(const sf_paged_cache* cache, const void* k, long long kts, long long khs, const void* v,
                     long long vts, long long vhs, const void* q, long long qts, long long qhs, void* q_out, int dtype,
@@ -364,7 +366,9 @@ int sf_paged_append(const sf_paged_cache* cache, const void* k, long long kts, l
  * position p = seq_lens[b] - n + i and sees keys max(0, p - window + 1) .. p
  * (window <= 0: 0 .. p);
  *   out[t,h,:] = sum_j softmax_j(scale * q . k_j) v_j,  lse[t,h] = log sum_j e^(scale * q . k_j).
- * H % n_kv_heads == 0 (any group size).  A row that sees no key gives 0, and lse
+ * H % n_kv_heads == 0 (any group size).  Softmax weights are held as fine as the
+ * finer of q_dtype and out_dtype; v_scales up to 2^100, beyond which small weights
+ * leave fp32's range.  A row that sees no key gives 0, and lse
  * -inf.  out [T, H, D] of out_dtype, contiguous; lse [T, H] fp32 or NULL.  The
  * workspace belongs to the caller and needs
  * sf_paged_attention_workspace_bytes(head_dim) bytes, 16-byte aligned. */

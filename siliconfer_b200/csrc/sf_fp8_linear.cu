@@ -15,9 +15,10 @@
 //    the rows that exist are loaded; what the MMA reads above them ends in TMEM lanes that nothing looks at.
 //  * persistent: 128 x 256 tiles in turn on one CTA per SM, stored through shared memory by TMA.
 //
-// Measured (tokens x K x N).  Weight-bound: 16 x 8192 x 28672 46.8 us, 5.0 TB/s.  Bound by the sums, which leave TMEM
-// once for each k-block: 2048 x 4096 x 11008 120 us, 1536 TFLOP/s.  Bound by latency, the first copies and the
-// cluster's exchange: 1 x 4096 x 4096 8.7 us, 77 x 896 x 4864 10 us.
+// Measured (tokens x K x N) in a graph; called one after another 3 to 15 us more.  Weight-bound: 16 x 8192 x 28672 46.7 us,
+// 5.1 TB/s.  Bound by latency, the first copies and the cluster's exchange: 1 x 4096 x 4096 8.6 us, 77 x 896 x 4864 10 us.
+// 2048 x 4096 x 11008 120 us, 1540 TFLOP/s: the tensor pipe works 38 % of the time, issue slots 34 %; the summing warps wait
+// for TMEM (long scoreboard) and for their own chain, with two accumulator buffers to hide it.
 #include <atomic>
 #include <cstdint>
 #include <cstring>

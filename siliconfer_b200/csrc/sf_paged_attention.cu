@@ -23,15 +23,17 @@
 //  * out^T[d, column] = V^T P^T: the head's columns are the MMA's rows, V is its transposed operand.  Weights are cut
 //    into as many parts as queries: 8, 12 or 24 bits, and no coarser than 2^-21 of the reference for bf16.
 // The finer of the queries' and the output's types decides the parts: an fp32 output of bf16 queries has six.  With two, a
-// weight is within 2^-8 of itself, which moves a bf16 output by 3e-4 to 5e-4 of its norm, a fifth to a third of what its
-// own rounding does (1.7e-3); a third part would cost the decode step half again as many columns and conversions.
+// weight is within 2^-8 of itself, which moves a bf16 output by 3e-4 to 9e-4 of its norm; its own rounding does by 1.7e-3.
+// A third part costs a decode step of grouped heads up to 12 % (64 sequences of 2000 tokens, 64/8 heads: 73 us, 65 with
+// two), tiles of a prompt 44 % (8 x 256 tokens: 1008 and 700 us); six parts take 16 x 8192 tokens 66 us, two 61.
 // Both scores and partial sums go to fresh TMEM buffers, two each; a thread is one key for the scores and one column d
 // for the sums, which it keeps in registers in fp32.
 //
 // Long runs of bf16 queries with 16-bit outputs go to the kernel of sf_paged_prompt.h.
 //
-// Measured.  Bound by the cache's bytes: 16 sequences of 8192 tokens, 64 query and 8 kv heads of 128, 61 us, 4.4 TB/s;
-// 64 sequences of up to 4096 tokens, 32 heads, 203 us, 5.8 TB/s.  Bound by latency: one sequence of 1000 tokens, 12 us,
+// Measured in a graph.  Bound by the cache's bytes: 64 sequences of up to 4096 tokens, 32 heads, 204 us, 5.7 TB/s (one call
+// after another 205 to 211).  16 sequences of 8192 tokens, 64 query and 8 kv heads of 128, 61 us, 4.4 TB/s: DRAM 54 % and
+// issue slots 26 % in use, waits for loads first among the stalls.  Bound by latency: one sequence of 1000 tokens, 12 us,
 // of which the merge is 4.
 //
 // Warps 0-3: softmax and sums.  Warp 4: TMA copies of pages.  Warp 5: MMAs.  Every wait is bounded: on expiry the

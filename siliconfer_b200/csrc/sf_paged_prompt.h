@@ -13,7 +13,7 @@
 // take seven instructions, and widening V costs a thread 64 codes for its 128 keys.
 //
 // A key's bytes serve 256 rows here and 8 in paged_attention_kernel.  8 sequences of 256 tokens with 64 query heads over
-// up to 4000 keys: 196 us, 454 TFLOP/s (paged_attention_kernel: 700 us); a tile of 128 keys takes 3.2 us, of which the
+// up to 4000 keys: 197 us, 451 TFLOP/s (paged_attention_kernel: 700 us); a tile of 128 keys takes 3.2 us, of which the
 // tensor cores work 1.1.
 #pragma once
 

@@ -7,9 +7,10 @@
 // h stays in registers in fp32 between the sum and the output, so x and the residual are read once and the sum is
 // rounded only where it is stored.
 //
-// Memory-bound: 4096 x 8192 bf16 with the residual and e4m3 output, 236 MB, takes 52 us = 4.6 TB/s, 8192 x 4096 49 us;
-// one row of 4096 2.3 us, a launch.  Codes by one product with the reciprocal, which may be a step off near a tie, took
-// 48, 46 and 2.1 us.  Rows whose length is no multiple of 8 take loads of one element (4096 x 4097: 70 us).
+// 4096 x 8192 bf16 with the residual and e4m3 output, 236 MB, takes 52 us = 4.6 TB/s (issue slots 62 % and DRAM 45 % in use,
+// waits for loads first among the stalls), 8192 x 4096 49 us; one row of 4096 2.4 us, a launch; quantizing 8192 x 4096
+// 31 us.  Codes by one product with the reciprocal, which may be a step off near a tie, took 48, 46 and 2.2 us.  Rows whose
+// length is no multiple of 8 take loads of one element (4096 x 4097: 70 us).
 #include <atomic>
 #include <cfloat>
 #include <cstdint>
@@ -146,7 +147,7 @@ __device__ __forceinline__ void put_columns(const NormArgs& a, size_t row, int k
 // blockDim.x threads a row (whole warps), blockDim.y rows a block (several only where one warp takes a row).  A thread
 // keeps CH x 8 columns of h, blockDim.x x 8 apart; with CH = 0 it reads them again for the output instead (rows of more
 // than 32768).  VEC: every row starts at 16 bytes and K is a multiple of 8.
-// Memory-bound: 4096 x 8192 bf16 with the residual and e4m3 output moves 236 MB.  NT: the most threads; rows of 2 chunks a
+// NT: the most threads; rows of 2 chunks a
 // thread keep to 40 registers so that 3 blocks of 512 fit an SM (that case 52 us; with 50 registers and 2 blocks 61).
 template <typename TX, int CH, bool VEC, int NT>
 __global__ void __launch_bounds__(NT, CH == 2 && NT == 512 ? 3 : 1) rms_norm_kernel(const NormArgs a) {
@@ -168,7 +169,7 @@ __global__ void __launch_bounds__(NT, CH == 2 && NT == 512 ? 3 : 1) rms_norm_ker
     }
   };
   constexpr int KEEP = CH > 0 ? CH : 1;
-  // Few rows: the weights come with the row, not after its sum (1 x 4096, fp32 weights: 2.2 us, was 2.4).  With many
+  // Few rows: the weights come with the row, not after its sum (1 x 4096, fp32 weights: 0.2 us less).  With many
   // rows other blocks fill that wait, and the registers cost more (8192 x 4096 with 2 chunks: 52 us so, 45 otherwise).
   constexpr bool EARLY = CH == 1;
   float h[KEEP][8], w_kept[EARLY ? CH : 1][8], ss = 0.f;

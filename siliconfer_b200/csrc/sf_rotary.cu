@@ -7,8 +7,8 @@
 // code becomes subnormal), and costs a floating-point code no precision.
 //
 // Every element is read and written once, and a page's rows wait in registers for the page's largest value.  A decode
-// step (8 tokens, 32 heads) takes 3.9 us, most of it the launch.  4096 tokens with 64 query and 8 kv heads of 128 take
-// 43.0 us, 3.8 TB/s: queries pass at the memory's rate, the pages' part is held by its instructions (a maximum, a turn,
+// step (8 tokens, 32 heads) takes 3.8 us, most of it the launch.  4096 tokens with 64 query and 8 kv heads of 128 take
+// 43.7 us, 3.7 TB/s: queries pass at the memory's rate, the pages' part is held by its instructions (a maximum, a turn,
 // a conversion for each element), so it runs first.  With a division for every item instead of a fixed item for a
 // thread, that call took 49 us.
 #include <atomic>

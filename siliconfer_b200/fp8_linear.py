@@ -4,7 +4,8 @@ The 8-bit sibling of ``Q4Linear``: weights of one byte, products on the tensor
 cores in e4m3, sums in fp32.  Inputs are e4m3 rows with one scale for every
 128 columns, as ``rms_norm_e4m3`` and ``quantize_e4m3`` give them.  No
 counterpart in siliconfer (its weights are int4 or int2).  The kernel is in
-libsf_q4.so (``sf_fp8_linear``); there is no CPU fallback.
+libsf_q4.so (``sf_fp8_linear``); there is no CPU fallback, and no gradient:
+outputs are detached from inputs that require one.
 """
 from __future__ import annotations
 

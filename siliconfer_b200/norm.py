@@ -5,7 +5,8 @@
 codes whose rows start at multiples of 16 bytes, and a [..., ceil(K / 128)]
 fp32 scale, max|y| / 448 of each row's 128 columns.  No counterpart in
 siliconfer, which norms in fp32 through MLX.  The kernels are in libsf_q4.so
-(``sf_rms_norm``, ``sf_quantize_e4m3``); there is no CPU fallback.
+(``sf_rms_norm``, ``sf_quantize_e4m3``); there is no CPU fallback, and no
+gradient: outputs are detached from inputs that require one.
 """
 from __future__ import annotations
 

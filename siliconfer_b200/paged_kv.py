@@ -6,7 +6,7 @@ for each kv head, so that tokens can be added to a page, and its older codes
 moved to a larger scale, without losing what they hold.  Keys and values can
 be written together with the rotary positions of the step.  The kernels are in
 libsf_q4.so (``sf_paged_append``, ``sf_paged_attention``); there is no CPU
-fallback.
+fallback, and no gradient: outputs are detached from inputs that require one.
 
 A call's new tokens are packed: sequence b's are rows starts[b] ..
 starts[b + 1] - 1 of q, k and v (without ``starts``: the same number for every

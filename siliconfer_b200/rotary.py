@@ -3,7 +3,8 @@
 The angles come from a table of cosines and sines, built once on the host in
 64 bits, so that a position of a million turns as exactly as the first one.
 siliconfer applies its positions through MLX (siliconfer/model/layers.py).
-The kernel is in libsf_q4.so (``sf_rotary``); there is no CPU fallback.
+The kernel is in libsf_q4.so (``sf_rotary``); there is no CPU fallback, and no
+gradient: outputs are detached from inputs that require one.
 """
 from __future__ import annotations
 

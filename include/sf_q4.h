@@ -377,6 +377,63 @@ int sf_paged_attention(const sf_paged_cache* cache, const void* q, int q_dtype, 
                        int out_dtype, float* lse, int H, int T, float scale, int window, void* workspace,
                        size_t workspace_bytes, void* stream);
 
+/* ---- norms and rotary positions of query and key heads ----------------------------
+ *   y = x / sqrt(mean(x^2) + eps) * weight       over a head's D elements (eps < 0: y = x)
+ *   out = y with its first rot elements turned, pair by pair (sf_rotary's pairs), pair j
+ *   by the angle of table row positions[t][axes[j]]
+ * q [T, H, D] and k [T, Hkv, D] of dtype with token and head strides, q_out and k_out
+ * likewise (each may be its input itself); H or Hkv may be 0.  Weights [D] of w_dtype
+ * (NULL: ones).  positions [T, axes_n] int32 (pos64 = 0) or int64, contiguous; axes
+ * [rot / 2] uint8, may be NULL where axes_n is 1; axes_n at most 8.  fp32 arithmetic.
+ * D a multiple of 16 up to 512, of 8 up to 256, or of 4 up to 128.  A position outside
+ * [0, max_pos) or an axis outside [0, axes_n) gives NaN in the elements that it turns and
+ * SF_ERR_INDEX at the next error check. */
+int sf_qk_norm_rotary(const void* q, long long qts, long long qhs, void* q_out, long long qots, long long qohs, int H,
+                      const void* k, long long kts, long long khs, void* k_out, long long kots, long long kohs, int Hkv,
+                      int dtype, const void* q_weight, const void* k_weight, int w_dtype, float eps,
+                      const void* positions, int pos64, int axes_n, const uint8_t* axes, const float* table, int max_pos,
+                      int rot, int interleaved, int T, int D, void* stream);
+
+/* ---- a paged cache in 4 bits --------------------------------------------------------
+ * The e4m3 cache's tokens, pages and rules (sf_paged_cache), with another content:
+ * k_codes, v_codes uint8 [num_pages, n_kv_heads, page_size, head_dim / 2], 16-byte
+ * aligned, and k_scales, v_scales bf16 [num_pages, n_kv_heads, page_size, 4], 8-byte
+ * aligned, a scale for each quarter of a vector.  Element e of a vector lies in quarter
+ * c = e / (D / 4) at place r = e % (D / 4); its code is bits 4c .. 4c + 3 of the vector's
+ * 16-bit word r (low byte first) and stands for (code - 8) * scale[c].  Scales are at
+ * least 0; a vector that holds an infinity or a NaN has four NaN scales. */
+typedef struct {
+  uint8_t* k_codes;
+  void* k_scales;
+  uint8_t* v_codes;
+  void* v_scales;
+  const int* block_table; /* [batch, pages_per_seq] */
+  const int* seq_lens;    /* [batch] */
+  const int* starts;      /* [batch + 1] or NULL */
+  int num_pages, n_kv_heads, page_size, head_dim, batch, pages_per_seq;
+} sf_paged4_cache;
+
+/* sf_paged_append for this cache, with sf_qk_norm_rotary's norms, axes and positions for
+ * q and k on the way (positions NULL: a token's place in its sequence; a padding row's
+ * query is turned as at position 0 whatever positions says).  table NULL: nothing is
+ * turned; eps < 0: nothing is normed.  For each quarter of a vector
+ *   scale = max|y| / 7.5, rounded to fp32 and then to bf16, at least 2^-126
+ *   code  = y / scale, rounded to the nearest whole number (ties to even) and limited to
+ *           -8 .. 7, plus 8
+ * with y in fp64 for keys and values.  Two rows of one call must not be the same token. */
+int sf_paged4_append(const sf_paged4_cache* cache, const void* k, long long kts, long long khs, const void* v,
+                     long long vts, long long vhs, const void* q, long long qts, long long qhs, void* q_out, int dtype,
+                     int H, int T, const void* q_weight, const void* k_weight, int w_dtype, float eps,
+                     const void* positions, int pos64, int axes_n, const uint8_t* axes, const float* table, int max_pos,
+                     int rot, int interleaved, void* stream);
+
+/* sf_paged_attention over this cache.  Value scales up to 2^100.  A row that sees a key
+ * or value vector with NaN scales is NaN as a whole. */
+size_t sf_paged4_attention_workspace_bytes(int head_dim);
+int sf_paged4_attention(const sf_paged4_cache* cache, const void* q, int q_dtype, long long qts, long long qhs, void* out,
+                        int out_dtype, float* lse, int H, int T, float scale, int window, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
 /* Device dequant to fp32/fp16/bf16 [N, K].  fp32 output is bit-exact with
    dequantize_sym / dequantize_asym (siliconfer/quant/primitives.py:54-75,
    117-140); fp16/bf16 are that value rounded to nearest even. */

@@ -36,6 +36,11 @@ class PagedCache(ctypes.Structure):
                 ("head_dim", _I), ("batch", _I), ("pages_per_seq", _I)]
 
 
+class Paged4Cache(ctypes.Structure):
+    """Mirror of sf_paged4_cache (include/sf_q4.h)."""
+    _fields_ = PagedCache._fields_
+
+
 # name -> argtypes (restype is int unless listed in _RESTYPES)
 SIGNATURES = {
     "sf_status_string": [_I],
@@ -77,11 +82,18 @@ SIGNATURES = {
                         _I, _I, _P],
     "sf_paged_attention_workspace_bytes": [_I],
     "sf_paged_attention": [ctypes.POINTER(PagedCache), _P, _I, _LL, _LL, _P, _I, _P, _I, _I, _F, _I, _P, _SZ, _P],
+    "sf_qk_norm_rotary": [_P, _LL, _LL, _P, _LL, _LL, _I, _P, _LL, _LL, _P, _LL, _LL, _I, _I, _P, _P, _I, _F, _P, _I, _I,
+                          _P, _P, _I, _I, _I, _I, _I, _P],
+    "sf_paged4_append": [ctypes.POINTER(Paged4Cache), _P, _LL, _LL, _P, _LL, _LL, _P, _LL, _LL, _P, _I, _I, _I, _P, _P,
+                         _I, _F, _P, _I, _I, _P, _P, _I, _I, _I, _P],
+    "sf_paged4_attention_workspace_bytes": [_I],
+    "sf_paged4_attention": [ctypes.POINTER(Paged4Cache), _P, _I, _LL, _LL, _P, _I, _P, _I, _I, _F, _I, _P, _SZ, _P],
 }
 _RESTYPES = {"sf_status_string": ctypes.c_char_p, "sf_last_error": ctypes.c_char_p,
              "sf_q4_launch_count": _LL, "sf_q4_step_workspace_bytes": _SZ,
              "sf_q4_step_destroy": None, "sf_tp_handle_bytes": _SZ, "sf_tp_comm_destroy": None,
-             "sf_kv_attention_workspace_bytes": _SZ, "sf_paged_attention_workspace_bytes": _SZ}
+             "sf_kv_attention_workspace_bytes": _SZ, "sf_paged_attention_workspace_bytes": _SZ,
+             "sf_paged4_attention_workspace_bytes": _SZ}
 
 _lib = None
 

@@ -1,0 +1,514 @@
+// sf_norm_turn.cu -- norms and rotary positions of query and key heads, and keys and values into a 4-bit cache.
+//
+//   y = x / sqrt(mean(x^2) + eps) * weight        of a head's D elements
+//   pair (a, b), pair number j:  (a cos - b sin, a sin + b cos), cos and sin from row positions[axes[j]] of a table
+//   quarter c of a vector:  scale = bf16(max|y| / 7.5), at least 2^-126;  code = clamp(rint(y / scale), -8, 7) + 8
+//
+// A block takes one token: its angles, which hang on one or several positions, are brought to shared memory once and
+// serve all heads.  A group of lanes takes a vector, a lane the same W places of all four quarters: these hold both
+// elements of its rotary pairs, and the codes of a place are one 16-bit word.
+#include <atomic>
+#include <cstdint>
+#include <type_traits>
+
+#include "sf_e4m3.h"
+#include "sf_paged4.h"
+#include "sf_q4_internal.h"
+
+namespace sf {
+SF_DEFINE_ERROR_READER(take_dev_error_norm_turn)
+extern std::atomic<long long> g_launches;
+
+namespace {
+
+constexpr int kThreads = 256, kMaxDim = 512, kMaxAxes = 8;
+
+struct Vectors {
+  const void* p;
+  long long ts, hs;     // token and head strides
+};
+struct Out {
+  void* p;
+  long long ts, hs;
+};
+enum Pairs { kNoPairs, kHalves, kHalvesOfHalf, kNeighbours, kAnyPairs };
+
+struct HeadArgs {
+  Vectors q, k, v;
+  Out qo, ko;
+  const void *wq, *wk;  // norm weights or NULL
+  int w_dtype, norm;
+  float eps;
+  const float* table;   // [max_pos, rot]: cosines, then sines
+  int max_pos, rot, interleaved, pairs;
+  const void* positions;   // [T, axes_n] or NULL: a token's place in its sequence
+  int pos64, axes_n;
+  const uint8_t* axes;  // [rot / 2] or NULL: all pairs belong to axis 0
+  int H, Hkv, T, D;
+  int groups, rounds;   // groups of lanes of a block, vectors that one takes
+  // the cache's
+  sf_paged_cache c;
+  __nv_bfloat16 *ks, *vs;
+};
+
+__device__ __forceinline__ float load_weight(const void* w, int dtype, int i) {
+  if (dtype == SF_F32) return static_cast<const float*>(w)[i];
+  if (dtype == SF_F16) return __half2float(static_cast<const __half*>(w)[i]);
+  return __bfloat162float(static_cast<const __nv_bfloat16*>(w)[i]);
+}
+
+// W consecutive elements as they are loaded.
+template <typename TX, int W>
+struct Raw {
+  static constexpr int BYTES = W * (int)sizeof(TX);
+  using Word = std::conditional_t<BYTES == 16, uint4, std::conditional_t<BYTES == 8, uint2, std::conditional_t<BYTES == 4, uint32_t, uint16_t>>>;
+  union {
+    Word w;
+    TX e[W];
+  };
+  __device__ __forceinline__ Raw() {}
+};
+template <typename TX, int W, bool VEC>
+__device__ __forceinline__ void load_raw(const TX* x, Raw<TX, W>& r) {
+  if constexpr (VEC) {
+    r.w = *reinterpret_cast<const typename Raw<TX, W>::Word*>(x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; ++i) r.e[i] = x[i];
+  }
+}
+
+// A vector's elements: y[c][i] is element c * D/4 + r0 + i.
+// F: float, or double for keys on their way to codes.
+template <typename F>
+__device__ __forceinline__ void turn_pair(F& a, F& b, float c, float s) {
+  const F ya = fma(a, (F)c, -(b * (F)s)), yb = fma(b, (F)c, a * (F)s);
+  a = ya;
+  b = yb;
+}
+// cs, sn: pair j's cosine and sine; buf: a place in shared memory for the vector, used where a pair's two elements lie
+// in different lanes.  Called by whole warps; lanes with there = false turn nothing.
+template <typename F, int W>
+__device__ __forceinline__ void turn_vector(F (&y)[4][W], bool there, int r0, const HeadArgs& a, const float* cs,
+                                            const float* sn, F* buf) {
+  const int Q = a.D / 4, half = a.rot / 2;
+  if (a.pairs == kAnyPairs) {
+    __syncwarp();
+    if (there) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int i = 0; i < W; ++i) buf[c * Q + r0 + i] = y[c][i];
+    }
+    __syncwarp();
+    if (!there) return;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        const int e = c * Q + r0 + i;
+        if (e >= a.rot) continue;
+        const bool second = a.interleaved ? e & 1 : e >= half;
+        const int j = a.interleaved ? e / 2 : second ? e - half : e;
+        const int other = a.interleaved ? e ^ 1 : second ? e - half : e + half;
+        const F s = (F)sn[j];
+        y[c][i] = fma(y[c][i], (F)cs[j], buf[other] * (second ? s : -s));
+      }
+    return;
+  }
+  if (!there) return;
+  if (a.pairs == kHalves) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int i = 0; i < W; ++i) turn_pair<F>(y[c][i], y[c + 2][i], cs[c * Q + r0 + i], sn[c * Q + r0 + i]);
+  } else if (a.pairs == kHalvesOfHalf) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) turn_pair<F>(y[0][i], y[1][i], cs[r0 + i], sn[r0 + i]);
+  } else if (a.pairs == kNeighbours) {
+    if constexpr (W > 1) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int i = 0; i < W; i += 2) {
+          const int e = c * Q + r0 + i;
+          if (e < a.rot) turn_pair<F>(y[c][i], y[c][i + 1], cs[e / 2], sn[e / 2]);
+        }
+    }
+  }
+}
+
+// y -> its code less 8, for a scale s; z is y in fp64.  The quotient is taken in fp32; where that leaves it within 2^-18
+// of a tie, what z / s and the code differ by decides, which is exact but for one rounding in fp64.
+__device__ __forceinline__ int code_of(double z, float y, float s, float inv) {
+  const float t = y * inv;
+  float r = rintf(t);
+  if (fabsf(t - r) > 0.5f - 0x1p-18f) {
+    const double d = fma(-(double)r, (double)s, z), twice = 2.0 * fabs(d);
+    if (twice > (double)s || (twice == (double)s && ((int)r & 1))) r += d > 0 ? 1.f : -1.f;
+  }
+  return (int)fminf(fmaxf(r, -8.f), 7.f);
+}
+
+struct TokenPlace {
+  bool put;        // the row is a sequence's token, and its page is there
+  int pos;         // -1: none; -2: a padding row
+  long long slot;  // (page * n_kv_heads) * page_size + slot
+};
+
+template <typename TX, int W, int GP, bool VEC, bool CACHE>
+__global__ void __launch_bounds__(kThreads) norm_turn_kernel(const HeadArgs a) {
+  constexpr int M = sizeof(TX) == 2 ? 4 : 2;   // vectors of a group under way
+  extern __shared__ __align__(16) double exchange[];
+  __shared__ __align__(16) float cs[kMaxDim / 2], sn[kMaxDim / 2], wsm[2][kMaxDim];
+  __shared__ TokenPlace place;
+  griddep_launch_dependents();
+  griddep_wait();
+  const int tok = blockIdx.x, tid = threadIdx.x, g = tid / GP, r0 = tid % GP * W, D = a.D, Q = D / 4;
+  const bool mine = g < a.groups && r0 < Q;
+  const int nv = a.Hkv * (CACHE ? 2 : 1) + a.H;
+  // vectors in order: keys, values (with a cache), queries
+  const auto source = [&](int v, int& kind, int& h) {
+    kind = v < a.Hkv ? 1 : CACHE && v < 2 * a.Hkv ? 2 : 0;
+    h = kind == 0 ? v - a.Hkv * (CACHE ? 2 : 1) : kind == 1 ? v : v - a.Hkv;
+    const Vectors& s = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
+    return static_cast<const TX*>(s.p) + (long long)tok * s.ts + h * s.hs;
+  };
+  Raw<TX, W> raw[M][4];
+  const auto load = [&](int round) {
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      const int v = g + a.groups * (round + m + a.rounds * (int)blockIdx.y);
+      if (!mine || round + m >= a.rounds || v >= nv) continue;
+      int kind, h;
+      const TX* x = source(v, kind, h);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) load_raw<TX, W, VEC>(x + c * Q + r0, raw[m][c]);
+    }
+  };
+  load(0);
+
+  // ---- the token's place, angles and the norms' weights ----
+  if (CACHE) {
+    if (tid < 32) {
+      const TokenAt at = token_at(a.c, a.T, tok);
+      if (tid == 0) {
+        TokenPlace p{false, -1, 0};
+        if (!at.ok) {
+          atomicOr(&g_dev_error, kErrIndex);
+        } else if (at.pos < 0) {
+          p.pos = -2;
+        } else {
+          p.pos = at.pos;
+          const int page = a.c.block_table[(size_t)at.b * a.c.pages_per_seq + at.pos / a.c.page_size];
+          p.put = page >= 0 && page < a.c.num_pages;
+          if (p.put) p.slot = (long long)page * a.c.n_kv_heads * a.c.page_size + at.pos % a.c.page_size;
+          else atomicOr(&g_dev_error, kErrIndex);
+        }
+        place = p;
+      }
+    }
+    __syncthreads();
+  }
+  const int half = a.rot / 2;
+  for (int j = tid; j < half; j += blockDim.x) {
+    long long p;
+    if (CACHE && place.pos == -2) {
+      p = 0;   // a padding row's positions are nobody's
+    } else if (a.positions) {
+      const int axis = a.axes ? a.axes[j] : 0;
+      const long long at = (long long)tok * a.axes_n + axis;
+      p = axis >= a.axes_n ? -1
+          : a.pos64        ? static_cast<const long long*>(a.positions)[at]
+                           : (long long)static_cast<const int*>(a.positions)[at];
+    } else {
+      p = place.pos;
+    }
+    const bool ok = p >= 0 && p < a.max_pos;
+    if (!ok) atomicOr(&g_dev_error, kErrIndex);
+    const float nan = __int_as_float(0x7fffffff);
+    cs[j] = ok ? __ldg(a.table + p * a.rot + j) : nan;
+    sn[j] = ok ? __ldg(a.table + p * a.rot + half + j) : nan;
+  }
+  if (a.norm) {
+    for (int i = tid; i < 2 * D; i += blockDim.x) {
+      const int which = i >= D, e = which ? i - D : i;
+      const void* w = which ? a.wk : a.wq;
+      wsm[which][e] = w ? load_weight(w, a.w_dtype, e) : 1.f;
+    }
+  }
+  __syncthreads();
+  // this vector's place in its warp's part of the exchange, room for 128 W doubles
+  double* buf64 = exchange + (tid / 32) * (128 * W) + (tid % 32) / GP * D;
+  float* buf32 = reinterpret_cast<float*>(exchange + (tid / 32) * (128 * W)) + (tid % 32) / GP * D;
+
+  for (int round = 0; round < a.rounds; round += M) {
+    if (round > 0) load(round);
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      if (round + m >= a.rounds) break;
+      const int v = g + a.groups * (round + m + a.rounds * (int)blockIdx.y);
+      const bool there = mine && v < nv;
+      int kind = 0, h = 0;
+      if (there) source(v, kind, h);
+      // whole warps go through both parts, since sums and maxima are shuffled; a warp's groups may differ in kind
+      if (CACHE && __any_sync(0xffffffffu, there && kind != 0)) {
+        // ---- a key or a value to its codes ----
+        const bool put = there && kind != 0 && place.put, key = put && kind == 1;
+        double z[4][W];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < W; ++i) z[c][i] = there ? (double)to_f32(raw[m][c].e[i]) : 0.0;
+        if (a.norm) {
+          double ss = 0;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < W; ++i) ss = fma(z[c][i], z[c][i], ss);
+#pragma unroll
+          for (int o = GP / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          const double r = 1.0 / sqrt(ss / D + (double)a.eps);
+          if (key) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int i = 0; i < W; ++i) z[c][i] = z[c][i] * r * (double)wsm[1][c * Q + r0 + i];
+          }
+        }
+        turn_vector<double, W>(z, key, r0, a, cs, sn, buf64);
+        uint32_t top[4], most = 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          top[c] = 0;
+#pragma unroll
+          for (int i = 0; i < W; ++i) top[c] = max(top[c], __float_as_uint((float)z[c][i]) & 0x7fffffffu);
+#pragma unroll
+          for (int o = GP / 2; o; o >>= 1) top[c] = max(top[c], __shfl_xor_sync(0xffffffffu, top[c], o));
+          most = max(most, top[c]);
+        }
+        const bool finite = most < 0x7f800000u;
+        uint32_t words[W] = {}, scale_bits[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float s = __fdiv_rn(__uint_as_float(top[c]), 7.5f);
+          // within 4 last places of a tie of two scales: from the largest magnitude in fp64
+          const bool near = ((__float_as_uint(s) - 0x7ffcu) & 0xffffu) <= 8u;
+          if (__any_sync(0xffffffffu, near)) {
+            double big = 0;
+#pragma unroll
+            for (int i = 0; i < W; ++i) big = fmax(big, fabs(z[c][i]));
+#pragma unroll
+            for (int o = GP / 2; o; o >>= 1) big = fmax(big, __shfl_xor_sync(0xffffffffu, big, o));
+            if (near) s = (float)(big / 7.5);
+          }
+          const __nv_bfloat16 sb = finite ? __float2bfloat16_rn(fmaxf(s, 0x1p-126f)) : __float2bfloat16_rn(__int_as_float(0x7fffffff));
+          scale_bits[c] = __bfloat16_as_ushort(sb);
+          s = __bfloat162float(sb);
+          const float inv = 1.f / s;
+#pragma unroll
+          for (int i = 0; i < W; ++i) {
+            const int n = finite ? code_of(z[c][i], (float)z[c][i], s, inv) + 8 : 8;
+            words[i] |= (uint32_t)n << (4 * c);
+          }
+        }
+        if (put) {
+          const long long vec = place.slot + (long long)h * a.c.page_size;
+          uint8_t* codes = (kind == 1 ? a.c.k_codes : a.c.v_codes) + vec * (D / 2) + 2 * r0;
+          static_assert(!CACHE || W == 4, "a lane's words are stored as 8 bytes");
+          *reinterpret_cast<uint2*>(codes) = make_uint2(words[0] | words[1 % W] << 16, words[2 % W] | words[3 % W] << 16);
+          if (r0 == 0)
+            *reinterpret_cast<uint2*>((kind == 1 ? a.ks : a.vs) + vec * 4) =
+                make_uint2(scale_bits[0] | scale_bits[1] << 16, scale_bits[2] | scale_bits[3] << 16);
+        }
+      }
+      const bool out = there && (kind == 0 || !CACHE);
+      if (!CACHE || __any_sync(0xffffffffu, out)) {
+        // ---- a query, or a key that stays one, to its own type ----
+        float y[4][W];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < W; ++i) y[c][i] = there ? to_f32(raw[m][c].e[i]) : 0.f;
+        if (a.norm) {
+          float ss = 0;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < W; ++i) ss = fmaf(y[c][i], y[c][i], ss);
+#pragma unroll
+          for (int o = GP / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          const float r = rsqrtf(ss / (float)D + a.eps);
+          if (out) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int i = 0; i < W; ++i) y[c][i] = y[c][i] * r * wsm[kind][c * Q + r0 + i];
+          }
+        }
+        turn_vector<float, W>(y, out, r0, a, cs, sn, buf32);
+        if (out) {
+          const Out& d = kind == 0 ? a.qo : a.ko;
+          TX* o = static_cast<TX*>(d.p) + (long long)tok * d.ts + h * d.hs + r0;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            Raw<TX, W> w;
+#pragma unroll
+            for (int i = 0; i < W; ++i) w.e[i] = from_f32<TX>(y[c][i]);
+            if constexpr (VEC) {
+              *reinterpret_cast<typename Raw<TX, W>::Word*>(o + c * Q) = w.w;
+            } else {
+#pragma unroll
+              for (int i = 0; i < W; ++i) o[c * Q + i] = w.e[i];
+            }
+          }
+        }
+      }
+    }
+  }
+}
+
+bool aligned_rows(const void* p, int dtype, long long ts, long long hs, int W) {
+  const int size = dtype == SF_F32 ? 4 : 2;
+  return reinterpret_cast<uintptr_t>(p) % (size * W) == 0 && ts % W == 0 && hs % W == 0;
+}
+
+int check_args(const HeadArgs& a, int dtype) {
+  if (dtype < 0 || dtype > 2 || a.w_dtype < 0 || a.w_dtype > 2) return fail(SF_ERR_DTYPE, "unknown dtype code");
+  if (a.rot < 0 || a.rot % 2 || a.rot > a.D) return fail(SF_ERR_SHAPE, "rot must be even and at most head_dim");
+  if (a.rot > 0 && (!a.table || a.max_pos < 1)) return fail(SF_ERR_SHAPE, "the rotary table is missing or empty");
+  if (a.positions && (a.axes_n < 1 || a.axes_n > kMaxAxes || (a.axes_n > 1 && !a.axes)))
+    return fail(SF_ERR_SHAPE, "need 1 to %d axes, and with more than one the axis of each pair", kMaxAxes);
+  if (a.norm && !(a.eps >= 0.f)) return fail(SF_ERR_SHAPE, "eps must not be negative");
+  return SF_OK;
+}
+
+// Vectors of a token to groups of lanes: one each where the tokens are few, else up to 4 (2 of fp32).
+template <typename TX, int W, bool CACHE>
+cudaError_t launch(HeadArgs& a, bool vec, cudaStream_t st) {
+  const int lanes = a.D / 4 / W, nv = a.Hkv * (CACHE ? 2 : 1) + a.H;
+  const auto go = [&](auto gp) -> cudaError_t {
+    constexpr int GP = decltype(gp)::value;
+    constexpr int most = kThreads / GP, M = sizeof(TX) == 2 ? 4 : 2;
+    int rounds = 1;
+    if ((long long)a.T * nv * GP > 1024ll * device_info().sms) rounds = (nv + most - 1) / most < M ? (nv + most - 1) / most : M;
+    a.rounds = rounds;
+    a.groups = (nv + rounds - 1) / rounds;
+    if (a.groups > most) a.groups = most;
+    const int per_warp = 32 / GP, threads = (a.groups + per_warp - 1) / per_warp * 32;
+    a.groups = threads / GP;
+    const int parts = (nv + a.groups * rounds - 1) / (a.groups * rounds);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)a.T, (unsigned)parts);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = a.pairs == kAnyPairs ? (size_t)threads / 32 * 128 * W * sizeof(double) : 0;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    auto* fn = vec ? norm_turn_kernel<TX, W, GP, true, CACHE> : norm_turn_kernel<TX, W, GP, false, CACHE>;
+    return cudaLaunchKernelEx(&cfg, fn, a);
+  };
+  if (lanes <= 4) return go(std::integral_constant<int, 4>());
+  if (lanes <= 8) return go(std::integral_constant<int, 8>());
+  if (lanes <= 16) return go(std::integral_constant<int, 16>());
+  return go(std::integral_constant<int, 32>());
+}
+
+// Which of a head's elements make its pairs, as the lanes hold them (W places of every quarter).
+int pairs_of(const HeadArgs& a, int W) {
+  if (a.rot == 0) return kNoPairs;
+  if (a.interleaved) return W > 1 ? kNeighbours : kAnyPairs;
+  return a.rot == a.D ? kHalves : 2 * a.rot == a.D ? kHalvesOfHalf : kAnyPairs;
+}
+
+}  // namespace
+}  // namespace sf
+
+using namespace sf;
+
+extern "C" {
+
+int sf_qk_norm_rotary(const void* q, long long qts, long long qhs, void* q_out, long long qots, long long qohs, int H,
+                      const void* k, long long kts, long long khs, void* k_out, long long kots, long long kohs, int Hkv,
+                      int dtype, const void* q_weight, const void* k_weight, int w_dtype, float eps,
+                      const void* positions, int pos64, int axes_n, const uint8_t* axes, const float* table, int max_pos,
+                      int rot, int interleaved, int T, int D, void* stream) {
+  if (T < 0 || H < 0 || Hkv < 0) return fail(SF_ERR_SHAPE, "need T, H, Hkv >= 0");
+  if (D < 4 || D % 4 || D > (D % 16 == 0 ? 512 : D % 8 == 0 ? 256 : 128))
+    return fail(SF_ERR_UNSUPPORTED, "head_dim %d not built (multiples of 16 up to 512, of 8 up to 256, of 4 up to 128)", D);
+  HeadArgs a{};
+  a.q = Vectors{q, qts, qhs};
+  a.k = Vectors{k, kts, khs};
+  a.qo = Out{q_out, qots, qohs};
+  a.ko = Out{k_out, kots, kohs};
+  a.wq = q_weight; a.wk = k_weight; a.w_dtype = w_dtype;
+  a.norm = eps >= 0.f;
+  a.eps = eps;
+  a.table = table; a.max_pos = max_pos; a.rot = rot; a.interleaved = interleaved;
+  a.positions = positions; a.pos64 = pos64; a.axes_n = axes_n; a.axes = axes;
+  a.H = H; a.Hkv = Hkv; a.T = T; a.D = D;
+  if (int rc = check_args(a, dtype)) return rc;
+  if (T == 0 || H + Hkv == 0) return SF_OK;
+  if ((H && (!q || !q_out)) || (Hkv && (!k || !k_out)) || (rot && !positions)) return fail(SF_ERR_NULL, "null pointer argument");
+  if ((long long)H + Hkv > 0xffff) return fail(SF_ERR_UNSUPPORTED, "more than 65535 heads");
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = with_type(dtype, [&](auto* p) {
+    using TX = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
+    const auto go = [&](auto w) {
+      constexpr int W = decltype(w)::value;
+      a.pairs = pairs_of(a, W);
+      const bool vec = (!H || (aligned_rows(q, dtype, qts, qhs, W) && aligned_rows(q_out, dtype, qots, qohs, W))) &&
+                       (!Hkv || (aligned_rows(k, dtype, kts, khs, W) && aligned_rows(k_out, dtype, kots, kohs, W)));
+      return launch<TX, W, false>(a, vec, st);
+    };
+    return D % 16 == 0  ? go(std::integral_constant<int, 4>())
+           : D % 8 == 0 ? go(std::integral_constant<int, 2>())
+                        : go(std::integral_constant<int, 1>());
+  });
+  if (e != cudaSuccess) return cuda_fail(e, "norm_turn_kernel launch");
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return SF_OK;
+}
+
+int sf_paged4_append(const sf_paged4_cache* cache, const void* k, long long kts, long long khs, const void* v,
+                     long long vts, long long vhs, const void* q, long long qts, long long qhs, void* q_out, int dtype,
+                     int H, int T, const void* q_weight, const void* k_weight, int w_dtype, float eps,
+                     const void* positions, int pos64, int axes_n, const uint8_t* axes, const float* table, int max_pos,
+                     int rot, int interleaved, void* stream) {
+  HeadArgs a{};
+  if (int rc = check_paged4(cache, T, a.c)) return rc;
+  const int D = cache->head_dim;
+  a.q = Vectors{q, qts, qhs};
+  a.k = Vectors{k, kts, khs};
+  a.v = Vectors{v, vts, vhs};
+  a.qo = Out{q_out, (long long)H * D, D};
+  a.wq = q_weight; a.wk = k_weight; a.w_dtype = w_dtype;
+  a.norm = eps >= 0.f;
+  a.eps = eps;
+  a.table = table; a.max_pos = max_pos; a.rot = table ? rot : 0; a.interleaved = interleaved;
+  a.positions = positions; a.pos64 = pos64; a.axes_n = axes_n; a.axes = axes;
+  a.H = q ? H : 0; a.Hkv = cache->n_kv_heads; a.T = T; a.D = D;
+  a.ks = static_cast<__nv_bfloat16*>(cache->k_scales);
+  a.vs = static_cast<__nv_bfloat16*>(cache->v_scales);
+  if (int rc = check_args(a, dtype)) return rc;
+  if (T == 0) return SF_OK;
+  if (!k || !v || (q && !q_out)) return fail(SF_ERR_NULL, "null pointer argument");
+  if (q && H < 1) return fail(SF_ERR_SHAPE, "need H >= 1 query heads");
+  if ((long long)a.H + 2ll * a.Hkv > 0xffff) return fail(SF_ERR_UNSUPPORTED, "more than 65535 heads");
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = with_type(dtype, [&](auto* p) {
+    using TX = std::remove_const_t<std::remove_pointer_t<decltype(p)>>;
+    a.pairs = pairs_of(a, 4);
+    const bool vec = aligned_rows(k, dtype, kts, khs, 4) && aligned_rows(v, dtype, vts, vhs, 4) &&
+                     (!q || (aligned_rows(q, dtype, qts, qhs, 4) && aligned_rows(q_out, dtype, D, D, 4)));
+    return launch<TX, 4, true>(a, vec, st);
+  });
+  if (e != cudaSuccess) return cuda_fail(e, "norm_turn_kernel launch");
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return SF_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,604 @@
+// sf_paged4_attention.cu -- attention over the pages of a 4-bit cache.
+//
+//   p_j = softmax_j(scale * q . k_j),  out = sum_j p_j v_j,  element = (code - 8) * scale of its vector's quarter
+//
+// The softmax keeps a running reference m and sum l of e^(score - m): keys in order, out and l are multiplied by
+// e^(m - m') when the reference moves to m'.  Parts of a row's keys, a warp's, a CTA's, merge by the same rule.  m is a
+// largest score plus the logarithm of its value vector's largest scale; it moves only when a key would exceed it by a
+// factor of 2, so that a weight times a scale is bounded and most keys need no reduction over the lanes.
+//
+// One row of a kv head's group is one (new token, query head); a tile has 8 rows, so that a group reads its keys once.
+// Both products are mma.sync m16n8k16 in fp16 with the codes as the larger operand and the 8 rows as columns:
+//  * S^T[key, row] = K Q^T: 16 keys are the MMA's rows; each quarter of the head has sums of its own, which are added
+//    times the key's scale in fp32.  For bf16 queries and outputs a pair of codes is a pair of fp16 subnormals n * 2^-24
+//    after one mask, and the sums begin at -8 times the sum of the quarter's queries.  The tensor cores align a subnormal
+//    as it stands, which leaves such sums 2^-17 of their largest product (measured on sums of one key); for the finer types
+//    the codes become the numbers n - 8, at two instructions a pair more.  A query row is brought to at most 2^14 by a
+//    power of two; fp16 then holds a bf16 or fp16 row as it is, and two parts an fp32 row.
+//  * out^T[d, row] += V^T P^T: a quarter's weights are the softmax's times the key's scale of that quarter, in fp16 (two
+//    parts for the finer types, 22 bits), codes the numbers n - 8.
+#include <algorithm>
+#include <atomic>
+#include <climits>
+#include <cmath>
+#include <cstdint>
+
+#include "sf_e4m3.h"
+#include "sf_paged4.h"
+#include "sf_paged_work.h"
+#include "sf_q4_internal.h"
+
+namespace sf {
+SF_DEFINE_ERROR_READER(take_dev_error_paged4)
+extern std::atomic<long long> g_launches;
+
+namespace {
+
+constexpr int kWarps = 4, kThreads = 32 * kWarps, kStages = 4, kBlock = 16;   // keys of a warp's step
+constexpr float kTopLog = 13.f;      // log2 of a weight times its scale, at most one above it
+
+struct Attn4Args : AttnArgs {
+  const __nv_bfloat16 *ks, *vs;      // [pages, n_kv_heads, page_size, 4]
+};
+
+__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(b0));
+}
+// an 8 x 8 matrix of 16-bit elements, transposed over the warp
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 half2_floats(uint32_t b) { return __half22float2(*reinterpret_cast<const __half2*>(&b)); }
+__device__ __forceinline__ uint32_t add_half2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("add.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+// quarter C's pair of codes of a word: fp16 numbers n * 2^-24 (C even) or n * 2^-20
+template <int C>
+__device__ __forceinline__ uint32_t codes_of(uint32_t w) {
+  return (C >= 2 ? w >> 8 : w) & (C % 2 ? 0x00f000f0u : 0x000f000fu);
+}
+// the codes less 8, times 1 or 16: the lowest bits of 1024 + n or 1024 + 16 n
+template <int C>
+__device__ __forceinline__ uint32_t centred(uint32_t w) {
+  return add_half2(codes_of<C>(w) | 0x64006400u, C % 2 ? 0xe480e480u : 0xe408e408u);
+}
+// four bf16 scales
+__device__ __forceinline__ void scales_of(uint2 u, float (&s)[4]) {
+  s[0] = __uint_as_float(u.x << 16), s[1] = __uint_as_float(u.x & 0xffff0000u);
+  s[2] = __uint_as_float(u.y << 16), s[3] = __uint_as_float(u.y & 0xffff0000u);
+}
+
+// A lane (g = lane / 4, t = lane % 4) reads KW words of keys g and g + 8, words t * KW .. of the vector; and of the
+// values of keys 2t, 2t + 1, 2t + 8, 2t + 9 the VW words that lane group g turns into rows of V^T.  It reads back only
+// what it copied, so the copies need no barrier.
+template <int D>
+struct Lay4 {
+  static constexpr int Q = D / 4, WORDS = D / 8, KW = WORDS / 4, VW = (WORDS + 7) / 8;
+  static constexpr int KCHUNK = KW % 4 == 0 ? 16 : KW % 2 == 0 ? 8 : 4, KCHUNKS = KW * 4 / KCHUNK;
+  static constexpr int VCHUNK = D == 96 ? 4 : VW * 4, VCHUNKS = VW * 4 / VCHUNK;
+  static constexpr uint32_t K0 = 0, V0 = 2 * KW * 128, S0 = V0 + 4 * VW * 128, STAGE = S0 + 4 * 256;
+  static constexpr uint32_t RING = kWarps * kStages * STAGE, JOIN = kWarps * 8 * (D + 4) * 4;
+  static constexpr uint32_t INFO = RING > JOIN ? RING : JOIN;
+  static constexpr size_t smem(int batch) { return INFO + (size_t)batch * sizeof(SeqInfo); }
+  // first element of a lane group's pair of places: word of set s
+  __device__ static __forceinline__ int word(int s, int g) { return D == 96 ? 8 * s + g : g * VW + s; }
+};
+
+template <int D, int QP, int PP>
+__global__ void __launch_bounds__(kThreads, D <= 128 ? 4 : 2) paged4_attention_kernel(const Attn4Args a, int q_pairs) {
+  using L = Lay4<D>;
+  constexpr int RT = 8, KW = L::KW, VW = L::VW, Q = L::Q;
+  constexpr bool FINE = PP == 2;   // keys' codes less 8, as the values'
+  extern __shared__ __align__(16) uint8_t mem[];
+  __shared__ long long wsum[kWarps];
+  __shared__ float wm[kWarps][RT], wl[kWarps][RT];
+  SeqInfo* info = reinterpret_cast<SeqInfo*>(mem + L::INFO);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  griddep_wait();
+
+  // ---- the batch's units, and this CTA's share ----
+  const int B = a.c.batch, Hkv = a.c.n_kv_heads, page_size = a.c.page_size;
+  const int rows0 = first_row(a.c, a.T, 0), rows1 = first_row(a.c, a.T, B);
+  long long total = 0;
+  int bad = 0;
+  for (int at = 0; at < B; at += kThreads) {
+    const int b = at + threadIdx.x;
+    long long u = 0;
+    int len = 0, n = 0, off = 0;
+    if (b < B) {
+      const int r0 = first_row(a.c, a.T, b), r1 = first_row(a.c, a.T, b + 1);
+      len = a.c.seq_lens[b];
+      n = r1 - r0;
+      if (r0 < 0 || n < 0 || r1 > a.T) {
+        n = 0;
+        off = 1;
+        atomicOr(&g_dev_error, kErrIndex);
+      }
+      if (!len_ok(a.c, len)) {
+        len = 0;
+        atomicOr(&g_dev_error, kErrIndex);
+      }
+      const int tiles = (int)(((long long)n * a.G + RT - 1) / RT);
+      u = (long long)tiles * Hkv * max(1, (len - keys_from(a, len, n) + UNIT - 1) / UNIT);
+    }
+    long long incl = u;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += x;
+    }
+    if (lane == 31) wsum[warp] = incl;
+    __syncthreads();
+    long long before = total;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += wsum[w];
+      total += wsum[w];
+    }
+    if (b < B) info[b] = SeqInfo{before + incl - u, len, n};
+    bad |= __syncthreads_or(off);
+  }
+  if (bad) total = 0;
+  clear_rows(a, bad ? 0 : rows0, bad ? 0 : rows1);
+  const long long cta = blockIdx.x;
+  const Shares shares(total, a.resident, (int)gridDim.x);
+  if (threadIdx.x == 0) a.desc[8 * cta] = 0;
+  long long u = 0, u_end = 0;
+  int b = 0;
+  if (cta < shares.ctas()) {
+    u = shares.begin(cta);
+    u_end = shares.begin(cta + 1);
+    for (int lo = 0, hi = B; hi - lo > 1;) {
+      const int mid = (lo + hi) >> 1;
+      if (info[mid].first <= u) lo = mid;
+      else hi = mid;
+      b = lo;
+    }
+  }
+
+  while (u < u_end) {
+    const Part p = part_at<RT>(a, info, u, u_end, b);
+    const int blocks = p.tb > p.ta ? (p.tb - p.ta + kBlock - 1) / kBlock : 0;   // of all warps
+    const int mine = blocks > warp ? (blocks - warp - 1) / kWarps + 1 : 0;
+    const int* pages = a.c.block_table + (size_t)p.b * a.c.pages_per_seq;
+    // ---- copies: this warp's block i is the part's block warp + kWarps * i ----
+    const auto key_of = [&](int i) { return p.ta + kBlock * (warp + kWarps * i); };
+    // Page of a block, -1 where it has none; a page that ends before the first key in sight may have been given up.
+    const auto page_of = [&](int i) {
+      const int k0 = key_of(i);
+      if (i >= mine || k0 + kBlock <= p.tile_lo) return -1;
+      const int page = __ldg(pages + (k0 >> a.lg_page));
+      if (page >= 0 && page < a.c.num_pages) return page;
+      atomicOr(&g_dev_error, kErrIndex);
+      return -1;
+    };
+    int page_l = page_of(lane);            // lane i's: block i of the current 32
+    uint32_t there = 0;                    // bit i % 32: the block has a page
+    const uint32_t ring = smem_u32(mem) + warp * kStages * L::STAGE;
+    const auto copy = [&](int i) {
+      if (i < mine) {
+        if (i % 32 == 0 && i > 0) page_l = page_of(i + lane);
+        const int page = __shfl_sync(0xffffffffu, page_l, i % 32);
+        there = (there & ~(1u << (i % 32))) | (page >= 0 ? 1u << (i % 32) : 0u);
+        if (page >= 0) {
+          const size_t vec = ((size_t)page * Hkv + p.kvh) * page_size + (key_of(i) & (page_size - 1));
+          const uint32_t st = ring + (i % kStages) * L::STAGE;
+          const uint8_t* kc = a.c.k_codes + (vec + g) * (D / 2) + t * KW * 4;
+          const uint8_t* vc = a.c.v_codes + (vec + 2 * t) * (D / 2);
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+#pragma unroll
+            for (int c = 0; c < L::KCHUNKS; ++c)
+              copy_async<L::KCHUNK>(st + L::K0 + (r * L::KCHUNKS + c) * (32 * L::KCHUNK) + lane * L::KCHUNK,
+                                    kc + r * 8 * (D / 2) + c * L::KCHUNK);
+            copy_async<8>(st + L::S0 + r * 256 + lane * 8, a.ks + (vec + g + 8 * r) * 4);
+            copy_async<8>(st + L::S0 + (2 + r) * 256 + lane * 8, a.vs + (vec + g + 8 * r) * 4);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int c = 0; c < L::VCHUNKS; ++c)
+              if (L::word(c * (L::VCHUNK / 4), g) < L::WORDS)
+                copy_async<L::VCHUNK>(st + L::V0 + (e * L::VCHUNKS + c) * (32 * L::VCHUNK) + lane * L::VCHUNK,
+                                      vc + ((e & 1) + (e >> 1) * 8) * (D / 2) + 4 * L::word(c * (L::VCHUNK / 4), g));
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) copy(i);
+
+    // ---- query fragments: column g's elements of this lane's words ----
+    uint32_t qf[4][KW][QP];
+    float f[2], init[4][2];
+    {
+      const int row = p.row0 + g;
+      const bool real = row <= p.last_row;
+      const long long qo = (long long)(p.r_first + row / a.G) * a.qts + (long long)(p.kvh * a.G + row % a.G) * a.qhs + 2 * t * KW;
+      float v[4][2 * KW];
+      uint32_t top = 0;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int e = 0; e < 2 * KW; e += 2) {
+          const long long at = qo + c * Q + e;
+          if (!real) {
+            v[c][e] = v[c][e + 1] = 0.f;
+          } else if (q_pairs && a.q_dtype == SF_BF16) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const __nv_bfloat16*>(a.q) + at);
+            v[c][e] = __uint_as_float(w << 16);
+            v[c][e + 1] = __uint_as_float(w & 0xffff0000u);
+          } else if (q_pairs && a.q_dtype == SF_F16) {
+            const float2 w = half2_floats(*reinterpret_cast<const uint32_t*>(static_cast<const __half*>(a.q) + at));
+            v[c][e] = w.x;
+            v[c][e + 1] = w.y;
+          } else {
+            v[c][e] = load_q(a, at);
+            v[c][e + 1] = load_q(a, at + 1);
+          }
+          top = max(top, max(__float_as_uint(v[c][e]) & 0x7fffffffu, __float_as_uint(v[c][e + 1]) & 0x7fffffffu));
+        }
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // the row's largest value to [2^13, 2^14) by a power of two
+      const int ex = min(max((int)(top >> 23) - 140, -126), 113);
+      const float down = __int_as_float((127 - ex) << 23);
+      // an infinity or a NaN: the row is NaN
+      const float f_row = top >= 0x7f800000u ? __int_as_float(0x7fffffff)
+                                             : __int_as_float((127 + ex) << 23) * (a.scale * kLog2e) * (FINE ? 1.f : 0x1p24f);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < KW; ++i) {
+          // the codes of odd quarters lie four bits higher
+          float x = v[c][2 * i] * down * (c % 2 ? 0.0625f : 1.f), y = v[c][2 * i + 1] * down * (c % 2 ? 0.0625f : 1.f);
+#pragma unroll
+          for (int part = 0; part < QP; ++part) {
+            qf[c][i][part] = half2_bits(x, y);
+            const float2 h = half2_floats(qf[c][i][part]);
+            sum += h.x + h.y;
+            x -= h.x;
+            y -= h.y;
+          }
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) init[c][e] = FINE ? 0.f : __shfl_sync(0xffffffffu, sum, (2 * t + e) * 4) * (c % 2 ? -0x1p-17f : -0x1p-21f);
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) f[e] = __shfl_sync(0xffffffffu, f_row, (2 * t + e) * 4);
+    }
+
+    float nm[2] = {0.f, 0.f}, l[2] = {0.f, 0.f};   // minus the reference, and the sum, of columns 2t and 2t + 1
+    bool fresh[2] = {true, true};                  // no key yet
+    float o[VW][4][4];                             // sums: rows 2 * word (+ 1) of quarter c, columns 2t, 2t + 1
+#pragma unroll
+    for (int s = 0; s < VW; ++s)
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[s][c][e] = 0.f;
+
+    for (int i = 0; i < mine; ++i) {
+      copy(i + kStages - 1);
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+      if (!(there >> (i % 32) & 1)) continue;
+      const int k0 = key_of(i);
+      const uint8_t* st = mem + (warp * kStages + i % kStages) * L::STAGE;
+      // ---- scores ----
+      float y[4] = {0.f, 0.f, 0.f, 0.f};           // keys g, g, g + 8, g + 8; columns 2t, 2t + 1
+      {
+        uint32_t w[2][KW];
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int c = 0; c < L::KCHUNKS; ++c) {
+            const uint8_t* at = st + L::K0 + (r * L::KCHUNKS + c) * (32 * L::KCHUNK) + lane * L::KCHUNK;
+            if constexpr (L::KCHUNK == 16) *reinterpret_cast<uint4*>(&w[r][4 * c]) = *reinterpret_cast<const uint4*>(at);
+            else if constexpr (L::KCHUNK == 8) *reinterpret_cast<uint2*>(&w[r][2 * c]) = *reinterpret_cast<const uint2*>(at);
+            else w[r][c] = *reinterpret_cast<const uint32_t*>(at);
+          }
+        float ks[2][4];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) scales_of(*reinterpret_cast<const uint2*>(st + L::S0 + r * 256 + lane * 8), ks[r]);
+        const auto quarter = [&](auto cc) {
+          constexpr int C = decltype(cc)::value;
+          float s[4] = {init[C][0], init[C][1], init[C][0], init[C][1]};
+          const auto codes = [&](uint32_t x) { return FINE ? centred<C>(x) : codes_of<C>(x); };
+#pragma unroll
+          for (int j = 0; j + 1 < KW; j += 2) {
+            const uint32_t a0 = codes(w[0][j]), a1 = codes(w[1][j]), a2 = codes(w[0][j + 1]), a3 = codes(w[1][j + 1]);
+#pragma unroll
+            for (int part = 0; part < QP; ++part) mma16(s, a0, a1, a2, a3, qf[C][j][part], qf[C][j + 1][part]);
+          }
+          if constexpr (KW % 2) {
+#pragma unroll
+            for (int part = 0; part < QP; ++part)
+              mma8(s, codes(w[0][KW - 1]), codes(w[1][KW - 1]), qf[C][KW - 1][part]);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = fmaf(s[e], ks[e >> 1][C], y[e]);
+        };
+        quarter(std::integral_constant<int, 0>());
+        quarter(std::integral_constant<int, 1>());
+        quarter(std::integral_constant<int, 2>());
+        quarter(std::integral_constant<int, 3>());
+      }
+      float vs[2][4], lv[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        scales_of(*reinterpret_cast<const uint2*>(st + L::S0 + (2 + r) * 256 + lane * 8), vs[r]);
+        lv[r] = fmaxf(lg2(fmaxf(fmaxf(vs[r][0], vs[r][1]), fmaxf(vs[r][2], vs[r][3]))), -60.f);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = fmaf(y[e], f[e & 1], nm[e & 1]);
+      const bool alike = k0 >= p.all_lo && k0 + kBlock <= min(p.all_hi, p.tb);   // every row sees all of these keys
+      bool hidden[4] = {false, false, false, false};
+      if (!alike) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = k0 + g + 8 * (e >> 1), pos = p.pos0 + (p.row0 + 2 * t + (e & 1)) / a.G;
+          hidden[e] = key >= p.tb || key > pos || (a.window > 0 && key <= pos - a.window);
+          if (hidden[e]) y[e] = -INFINITY;
+        }
+      }
+      // ---- the reference, if a key exceeds it by more than a factor of 2 ----
+      const float over = fmaxf(fmaxf(y[0], y[1]) + lv[0], fmaxf(y[2], y[3]) + lv[1]);
+      if (__any_sync(0xffffffffu, over > kTopLog + 1.f || fresh[0] || fresh[1])) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float top = fmaxf(y[e] + lv[0], y[e + 2] + lv[1]);
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+          if (fresh[e] && top == -INFINITY) continue;   // the row has seen no key
+          const float up = fresh[e] ? top - kTopLog : fmaxf(top - kTopLog, 0.f), c = fresh[e] ? 1.f : ex2(-up);
+          fresh[e] = false;
+          nm[e] -= up;
+          y[e] -= up;
+          y[e + 2] -= up;
+          l[e] *= c;
+#pragma unroll
+          for (int s = 0; s < VW; ++s)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              o[s][q][e] *= c;
+              o[s][q][e + 2] *= c;
+            }
+        }
+      }
+      // ---- weights, times each quarter's scale, as the second operand ----
+      float pw[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) pw[e] = ex2(y[e]);
+      l[0] += pw[0] + pw[2];
+      l[1] += pw[1] + pw[3];
+      uint32_t pf[4][PP][2];
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float x = pw[2 * r] * vs[r][c], z = pw[2 * r + 1] * vs[r][c];
+          if (!alike) {   // 0 times a NaN scale is not 0
+            if (hidden[2 * r]) x = 0.f;
+            if (hidden[2 * r + 1]) z = 0.f;
+          }
+#pragma unroll
+          for (int part = 0; part < PP; ++part) {
+            const uint32_t h = half2_bits(x, z);
+            pf[c][part][r] = transpose8(h);
+            const float2 w = half2_floats(h);
+            x -= w.x;
+            z -= w.y;
+          }
+        }
+      // ---- sums ----
+      uint32_t w[4][VW];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int c = 0; c < L::VCHUNKS; ++c) {
+          const uint8_t* at = st + L::V0 + (e * L::VCHUNKS + c) * (32 * L::VCHUNK) + lane * L::VCHUNK;
+          if constexpr (L::VCHUNK == 16) *reinterpret_cast<uint4*>(&w[e][4 * c]) = *reinterpret_cast<const uint4*>(at);
+          else if constexpr (L::VCHUNK == 8) *reinterpret_cast<uint2*>(&w[e][2 * c]) = *reinterpret_cast<const uint2*>(at);
+          else w[e][c] = *reinterpret_cast<const uint32_t*>(at);
+        }
+#pragma unroll
+      for (int s = 0; s < VW; ++s) {
+        // both tokens' half-words of a place side by side
+        const uint32_t lo0 = __byte_perm(w[0][s], w[1][s], 0x5410), hi0 = __byte_perm(w[0][s], w[1][s], 0x7632),
+                       lo1 = __byte_perm(w[2][s], w[3][s], 0x5410), hi1 = __byte_perm(w[2][s], w[3][s], 0x7632);
+        const auto quarter = [&](auto cc) {
+          constexpr int C = decltype(cc)::value;
+          const uint32_t a0 = centred<C>(lo0), a1 = centred<C>(hi0), a2 = centred<C>(lo1), a3 = centred<C>(hi1);
+#pragma unroll
+          for (int part = 0; part < PP; ++part) mma16(o[s][C], a0, a1, a2, a3, pf[C][part][0], pf[C][part][1]);
+        };
+        quarter(std::integral_constant<int, 0>());
+        quarter(std::integral_constant<int, 1>());
+        quarter(std::integral_constant<int, 2>());
+        quarter(std::integral_constant<int, 3>());
+      }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+    // ---- the warps' parts ----
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], x);
+      if (g == 0) {
+        wm[warp][2 * t + e] = fresh[e] ? kNone : -nm[e];
+        wl[warp][2 * t + e] = l[e];
+      }
+    }
+    __syncthreads();   // the rings are free, too
+    float* join = reinterpret_cast<float*>(mem);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int col = 2 * t + e;
+      const float M = fmaxf(fmaxf(wm[0][col], wm[1][col]), fmaxf(wm[2][col], wm[3][col]));
+      const float c = ex2(wm[warp][col] - M);
+      float* to = join + (warp * RT + col) * (D + 4);
+#pragma unroll
+      for (int s = 0; s < VW; ++s) {
+        const int word = L::word(s, g);
+        if (word >= L::WORDS) continue;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<float2*>(to + q * Q + 2 * word) =
+              make_float2(o[s][q][e] * c * (q % 2 ? 0.0625f : 1.f), o[s][q][e + 2] * c * (q % 2 ? 0.0625f : 1.f));
+      }
+    }
+    __syncthreads();
+    const bool begins = u == p.seg0, ends = p.u1 == p.seg1;
+    float* part = a.part + ((size_t)cta * 2 + (begins ? 1 : 0)) * kMaxRows * (D + 2);
+    for (int x = threadIdx.x; x < RT * D; x += kThreads) {
+      const int r = x / D, d = x % D, row = p.row0 + r;
+      if (row > p.last_row) break;
+      const float M = fmaxf(fmaxf(wm[0][r], wm[1][r]), fmaxf(wm[2][r], wm[3][r]));
+      float A = 0.f, Ls = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        A += join[(w * RT + r) * (D + 4) + d];
+        Ls += wl[w][r] * ex2(wm[w][r] - M);
+      }
+      const size_t th = (size_t)(p.r_first + row / a.G) * a.H + p.kvh * a.G + row % a.G;
+      if (begins && ends) store_out(a, th * D + d, Ls == 0.f ? 0.f : A / Ls);
+      else part[r * D + d] = A;
+      if (d == 0) {
+        if (!(begins && ends)) {
+          part[RT * D + 2 * r] = M;
+          part[RT * D + 2 * r + 1] = Ls;
+        } else if (a.lse) {
+          a.lse[th] = Ls == 0.f ? -INFINITY : M * kLn2 + logf(Ls);
+        }
+      }
+    }
+    if (begins && !ends && threadIdx.x == 0) {
+      // CTAs of the tile's parts: this one to the one that holds its last unit
+      int* dsc = a.desc + 8 * cta;
+      dsc[0] = (int)(shares.holder(p.seg1 - 1) - cta + 1);
+      dsc[1] = p.r_first;
+      dsc[2] = p.kvh;
+      dsc[3] = p.row0;
+      dsc[4] = p.last_row;
+    }
+    __syncthreads();   // the join's place is the next part's rings
+    u = p.u1;
+  }
+  griddep_launch_dependents();   // not before: the merge's blocks would wait in the place of the next call's
+}
+
+template <int D, int QP, int PP>
+int launch4(Attn4Args a, cudaStream_t st) {
+  using L = Lay4<D>;
+  const sf_paged_cache& c = a.c;
+  auto* fn = paged4_attention_kernel<D, QP, PP>;
+  const size_t smem = L::smem(c.batch);
+  // the limit is the process's: the same for calls of every batch, or another thread's could lower it before this launch
+  static_assert(L::smem(kMaxBatch) + 2048 <= kBlockSmem, "shared memory plan");
+  cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::smem(kMaxBatch));
+  if (e != cudaSuccess) return cuda_fail(e, "paged4_attention_kernel shared memory");
+  int per_sm = (int)(228 * 1024 / (smem + 2048));
+  const int most = D <= 128 ? 4 : 2;
+  if (per_sm > most) per_sm = most;
+  if (per_sm < 1) per_sm = 1;
+  // no more CTAs than units there may be
+  const double cap = ((double)c.pages_per_seq * c.page_size + UNIT - 1) / UNIT;
+  const double units = cap * ((double)a.T * a.G / 8 + c.batch) * c.n_kv_heads;
+  a.resident = device_info().sms * per_sm;
+  int grid = 2 * a.resident;
+  if (units < (double)kLong * a.resident) grid = units < a.resident ? (int)units : a.resident;
+  const size_t size = a.q_dtype == SF_F32 ? 4 : 2;
+  const int pairs = reinterpret_cast<uintptr_t>(a.q) % (2 * size) == 0 && a.qts % 2 == 0 && a.qhs % 2 == 0;
+  e = launch_kernel(fn, grid, kThreads, smem, st, true, a, pairs);
+  if (e != cudaSuccess) return cuda_fail(e, "paged4_attention_kernel launch");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid, 8);
+  cfg.blockDim = dim3(D);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, paged_attention_merge_kernel<D, 8>, static_cast<const AttnArgs&>(a));
+  if (e != cudaSuccess) return cuda_fail(e, "paged_attention_merge_kernel launch");
+  g_launches.fetch_add(2, std::memory_order_relaxed);
+  return SF_OK;
+}
+
+constexpr int kMaxCtasPerSm = 4;
+
+}  // namespace
+}  // namespace sf
+
+using namespace sf;
+
+extern "C" {
+
+size_t sf_paged4_attention_workspace_bytes(int head_dim) {
+  if (head_dim <= 0) return 0;
+  const size_t ctas = (size_t)device_info().sms * kMaxCtasPerSm * 2;
+  return ctas * (2 * kMaxRows * ((size_t)head_dim + 2) * 4 + 32);
+}
+
+int sf_paged4_attention(const sf_paged4_cache* cache, const void* q, int q_dtype, long long qts, long long qhs, void* out,
+                        int out_dtype, float* lse, int H, int T, float scale, int window, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+  Attn4Args a{};
+  if (int rc = check_paged4(cache, T, a.c)) return rc;
+  if (q_dtype < 0 || q_dtype > 2 || out_dtype < 0 || out_dtype > 2) return fail(SF_ERR_DTYPE, "unknown dtype code");
+  if (H < 1 || H % cache->n_kv_heads) return fail(SF_ERR_SHAPE, "H must be a positive multiple of n_kv_heads");
+  if (T == 0) return SF_OK;
+  if (!q || !out || !workspace) return fail(SF_ERR_NULL, "null pointer argument");
+  const int D = cache->head_dim;
+  const size_t need = sf_paged4_attention_workspace_bytes(D);
+  if (workspace_bytes < need) return fail(SF_ERR_SHAPE, "workspace too small: need %zu bytes", need);
+  if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail(SF_ERR_ALIGN, "workspace must be 16-byte aligned");
+  a.q = q; a.qts = qts; a.qhs = qhs; a.out = out; a.lse = lse;
+  a.ks = static_cast<const __nv_bfloat16*>(cache->k_scales);
+  a.vs = static_cast<const __nv_bfloat16*>(cache->v_scales);
+  a.desc = static_cast<int*>(workspace);
+  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (size_t)device_info().sms * kMaxCtasPerSm * 2 * 32);
+  a.H = H; a.T = T; a.G = H / cache->n_kv_heads; a.q_dtype = q_dtype; a.out_dtype = out_dtype;
+  a.window = window < (long long)cache->pages_per_seq * cache->page_size ? window : 0;   // a wider one hides nothing
+  a.lg_page = __builtin_ctz((unsigned)cache->page_size);
+  a.scale = scale;
+  if ((long long)T * a.G > 0x7fffffffll) return fail(SF_ERR_UNSUPPORTED, "too many query rows");
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool fine = std::min(q_dtype, out_dtype) != SF_BF16;   // the finer of the types
+  const auto go = [&](auto d) {
+    constexpr int DD = decltype(d)::value;
+    if (q_dtype == SF_F32) return launch4<DD, 2, 2>(a, st);
+    return fine ? launch4<DD, 1, 2>(a, st) : launch4<DD, 1, 1>(a, st);
+  };
+  return D == 64    ? go(std::integral_constant<int, 64>())
+         : D == 96  ? go(std::integral_constant<int, 96>())
+         : D == 128 ? go(std::integral_constant<int, 128>())
+                    : go(std::integral_constant<int, 256>());
+}
+
+}  // extern "C"

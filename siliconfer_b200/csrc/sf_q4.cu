@@ -383,17 +383,18 @@ int sf_q4_quantize_pack(const float* W, uint8_t* packed, float* scales, float* z
 int sf_q4_check_device_error(void) {
   const unsigned int a = take_dev_error_gemv(), b = take_dev_error_tc(),
                      c = take_dev_error_tile() | take_dev_error_tp(), d = take_dev_error_fp8(),
-                     e = take_dev_error_rotary(), f = take_dev_error_paged();
+                     e = take_dev_error_rotary(), f = take_dev_error_paged(), g = take_dev_error_norm_turn(),
+                     h = take_dev_error_paged4();
   if (a == 0xffffffffu || b == 0xffffffffu || c == 0xffffffffu || d == 0xffffffffu || e == 0xffffffffu ||
-      f == 0xffffffffu)
+      f == 0xffffffffu || g == 0xffffffffu || h == 0xffffffffu)
     return fail(SF_ERR_CUDA, "reading the device error word failed");
   if ((a | b | c) & kErrPoisoned)
     return fail(SF_ERR_COMM,
                 "a tensor-parallel exchange met a poisoned communicator (a rank's bounded wait expired in an "
                 "earlier call; create the communicator again) (code %u)", a | b | c);
-  const unsigned int waits = (a | b | c | d | e | f) & ~kErrIndex;
+  const unsigned int waits = (a | b | c | d | e | f | g | h) & ~kErrIndex;
   if (waits) return fail(SF_ERR_TIMEOUT, "a device-side wait expired (code %u)", waits);
-  if (d | e | f)
+  if (d | e | f | g | h)
     return fail(SF_ERR_INDEX, "a kernel met a page, position or length outside its tensor and skipped the access");
   return SF_OK;
 }

@@ -67,6 +67,8 @@ unsigned int take_dev_error_tp();
 unsigned int take_dev_error_fp8();
 unsigned int take_dev_error_rotary();
 unsigned int take_dev_error_paged();
+unsigned int take_dev_error_norm_turn();
+unsigned int take_dev_error_paged4();
 
 // Carves one exchange region for a pushed task from a tensor-parallel
 // communicator's arena (same order on every rank, so the same offsets):

@@ -373,6 +373,222 @@ std::tuple<at::Tensor, OptTensor> paged_attention(const at::Tensor& q, const at:
   return {out, lse};
 }
 
+// ---- norms of heads, and the 4-bit cache -------------------------------------
+
+// Norm weights and positions as the C entry points take them; `keep` holds copies alive that had to be made.
+struct TurnArgs {
+  const void *wq = nullptr, *wk = nullptr, *positions = nullptr;
+  const uint8_t* axes = nullptr;
+  const float* table = nullptr;
+  float eps = -1.f;
+  int w_dtype = SF_F32, pos64 = 0, axes_n = 1, max_pos = 0, rot = 0;
+};
+TurnArgs turn_args(const OptTensor& table, const OptTensor& positions, const OptTensor& axes, const OptTensor& wq,
+                   const OptTensor& wk, c10::optional<double> eps, const at::Tensor& ref, int64_t T, int64_t D,
+                   std::vector<at::Tensor>& keep) {
+  TurnArgs a;
+  if (given(table)) {
+    check_table(*table, ref, D);
+    a.table = table->data_ptr<float>();
+    a.max_pos = (int)table->size(0);
+    a.rot = (int)table->size(1);
+  }
+  if (given(positions)) {
+    on_device(*positions, ref, "positions");
+    TORCH_CHECK(given(table), "positions need a rotary table");
+    TORCH_CHECK((positions->dim() == 1 || positions->dim() == 2) && positions->size(0) == T,
+                "positions must be [T] or [T, axes]");
+    TORCH_CHECK(positions->scalar_type() == at::kInt || positions->scalar_type() == at::kLong,
+                "positions must be int32 or int64");
+    const int64_t n = positions->dim() == 2 ? positions->size(1) : 1;
+    TORCH_CHECK(n >= 1 && n <= 8, "positions may have 1 to 8 axes");
+    keep.push_back(positions->contiguous());
+    a.positions = keep.back().data_ptr();
+    a.pos64 = positions->scalar_type() == at::kLong;
+    a.axes_n = (int)n;
+  }
+  if (given(axes)) {
+    on_device(*axes, ref, "axes");
+    TORCH_CHECK(given(positions), "axes need positions");
+    TORCH_CHECK(axes->scalar_type() == at::kByte && axes->dim() == 1 && axes->size(0) == a.rot / 2,
+                "axes must be uint8 [rot / 2]");
+    keep.push_back(axes->contiguous());
+    a.axes = keep.back().data_ptr<uint8_t>();
+  }
+  TORCH_CHECK(a.axes_n == 1 || a.axes, "positions of several axes need the axis of each pair (axes)");
+  if (eps.has_value()) {
+    TORCH_CHECK(*eps >= 0, "eps must not be negative");
+    a.eps = (float)*eps;
+  }
+  const auto weight = [&](const OptTensor& w, const char* name) -> const void* {
+    if (!given(w)) return nullptr;
+    on_device(*w, ref, name);
+    TORCH_CHECK(eps.has_value(), name, " needs eps");
+    TORCH_CHECK(w->dim() == 1 && w->size(0) == D, name, " must be [head_dim]");
+    keep.push_back(w->contiguous());
+    a.w_dtype = dtype_code(w->scalar_type());
+    return keep.back().data_ptr();
+  };
+  a.wq = weight(wq, "q_weight");
+  a.wk = weight(wk, "k_weight");
+  TORCH_CHECK(!a.wq || !a.wk || wq->scalar_type() == wk->scalar_type(), "q_weight and k_weight must have one dtype");
+  return a;
+}
+
+std::tuple<at::Tensor, OptTensor> qk_norm_rotary(const at::Tensor& q, const OptTensor& k, const OptTensor& positions,
+                                                 const OptTensor& table, const OptTensor& wq, const OptTensor& wk,
+                                                 c10::optional<double> eps, bool interleaved, const OptTensor& axes,
+                                                 const OptTensor& out) {
+  TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor");
+  TORCH_CHECK(q.dim() == 3 && q.size(2) >= 1, "q must be [T, heads, head_dim]");
+  const int64_t T = q.size(0), D = q.size(2);
+  TORCH_CHECK(T <= INT_MAX && q.size(1) <= INT_MAX && D <= INT_MAX, "q is too large");
+  if (given(k)) {
+    on_device(*k, q, "k");
+    TORCH_CHECK(k->dim() == 3 && k->size(0) == T && k->size(2) == D && k->scalar_type() == q.scalar_type(),
+                "k must be [T, n_kv_heads, head_dim] of q's dtype");
+    TORCH_CHECK(k->size(1) <= INT_MAX, "k is too large");
+  }
+  TORCH_CHECK(!given(table) || given(positions), "the rotary table needs positions");
+  const c10::cuda::CUDAGuard guard(q.device());
+  std::vector<at::Tensor> keep;
+  const TurnArgs a = turn_args(table, positions, axes, wq, wk, eps, q, T, D, keep);
+  const at::Tensor qi = head_rows(q);
+  at::Tensor qo, ki, ko;
+  if (given(out)) {
+    qo = *out;
+    on_device(qo, q, "out");
+    TORCH_CHECK(qo.sizes() == q.sizes() && qo.scalar_type() == q.scalar_type(), "out must have x's shape and dtype");
+    TORCH_CHECK(qo.stride(2) == 1 || D == 1, "out's heads must be contiguous");
+    TORCH_CHECK(qo.data_ptr() != qi.data_ptr() || qo.strides() == qi.strides(),
+                "out may be x itself, but no other view of x's memory");
+  } else {
+    qo = empty_on(q.sizes(), q.scalar_type(), q);
+  }
+  if (given(k)) {
+    ki = head_rows(*k);
+    ko = empty_on(k->sizes(), k->scalar_type(), q);
+  }
+  const bool has = ki.defined();
+  check(sf_qk_norm_rotary(qi.data_ptr(), qi.stride(0), qi.stride(1), qo.data_ptr(), qo.stride(0), qo.stride(1),
+                          (int)q.size(1), has ? ki.data_ptr() : nullptr, has ? ki.stride(0) : 0, has ? ki.stride(1) : 0,
+                          has ? ko.data_ptr() : nullptr, has ? ko.stride(0) : 0, has ? ko.stride(1) : 0,
+                          has ? (int)ki.size(1) : 0, dtype_code(q.scalar_type()), a.wq, a.wk, a.w_dtype, a.eps,
+                          a.positions, a.pos64, a.axes_n, a.axes, a.table, a.max_pos, a.rot, interleaved, (int)T, (int)D,
+                          stream_of(q)));
+  return {qo, has ? OptTensor(ko) : OptTensor()};
+}
+
+sf_paged4_cache paged4_cache(const at::Tensor& kc, const at::Tensor& ks, const at::Tensor& vc, const at::Tensor& vs,
+                             const at::Tensor& bt, const at::Tensor& lens, const OptTensor& starts, const at::Tensor& ref,
+                             std::vector<at::Tensor>& keep) {
+  on_device(kc, ref, "k_codes");
+  on_device(vc, ref, "v_codes");
+  on_device(ks, ref, "k_scales");
+  on_device(vs, ref, "v_scales");
+  on_device(bt, ref, "block_table");
+  on_device(lens, ref, "seq_lens");
+  TORCH_CHECK(kc.scalar_type() == at::kByte && vc.scalar_type() == at::kByte && kc.dim() == 4 && kc.sizes() == vc.sizes() &&
+                  kc.is_contiguous() && vc.is_contiguous(),
+              "k_codes and v_codes must be contiguous uint8 [pages, n_kv_heads, page_size, head_dim / 2]");
+  const bool fits = ks.dim() == 4 && ks.size(0) == kc.size(0) && ks.size(1) == kc.size(1) && ks.size(2) == kc.size(2) &&
+                    ks.size(3) == 4 && vs.sizes() == ks.sizes();
+  TORCH_CHECK(fits && ks.scalar_type() == at::kBFloat16 && vs.scalar_type() == at::kBFloat16 && ks.is_contiguous() &&
+                  vs.is_contiguous(),
+              "k_scales and v_scales must be contiguous bf16 [pages, n_kv_heads, page_size, 4]");
+  TORCH_CHECK(bt.scalar_type() == at::kInt && bt.dim() == 2, "block_table must be int32 [batch, pages_per_seq]");
+  TORCH_CHECK(lens.scalar_type() == at::kInt && lens.dim() == 1 && lens.size(0) == bt.size(0),
+              "seq_lens must be int32 [batch]");
+  for (int i = 0; i < 4; ++i) TORCH_CHECK(kc.size(i) <= INT_MAX / 2, "the cache is too large");
+  TORCH_CHECK(bt.size(1) <= INT_MAX && bt.size(0) <= INT_MAX, "block_table is too large");
+  sf_paged4_cache c{};
+  c.k_codes = static_cast<uint8_t*>(kc.data_ptr());
+  c.k_scales = ks.data_ptr();
+  c.v_codes = static_cast<uint8_t*>(vc.data_ptr());
+  c.v_scales = vs.data_ptr();
+  keep.push_back(bt.contiguous());
+  c.block_table = keep.back().data_ptr<int>();
+  keep.push_back(lens.contiguous());
+  c.seq_lens = keep.back().data_ptr<int>();
+  if (given(starts)) {
+    on_device(*starts, ref, "starts");
+    TORCH_CHECK(starts->scalar_type() == at::kInt && starts->dim() == 1 && starts->size(0) == bt.size(0) + 1,
+                "starts must be int32 [batch + 1]");
+    keep.push_back(starts->contiguous());
+    c.starts = keep.back().data_ptr<int>();
+  }
+  c.num_pages = (int)kc.size(0);
+  c.n_kv_heads = (int)kc.size(1);
+  c.page_size = (int)kc.size(2);
+  c.head_dim = (int)(2 * kc.size(3));
+  c.batch = (int)bt.size(0);
+  c.pages_per_seq = (int)bt.size(1);
+  return c;
+}
+
+OptTensor paged4_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& kc, const at::Tensor& ks,
+                        const at::Tensor& vc, const at::Tensor& vs, const at::Tensor& bt, const at::Tensor& lens,
+                        const OptTensor& starts, const OptTensor& q, const OptTensor& table, bool interleaved,
+                        const OptTensor& positions, const OptTensor& axes, const OptTensor& wq, const OptTensor& wk,
+                        c10::optional<double> eps) {
+  TORCH_CHECK(k.is_cuda(), "k must be a CUDA tensor");
+  on_device(v, k, "v");
+  std::vector<at::Tensor> keep;
+  const sf_paged4_cache c = paged4_cache(kc, ks, vc, vs, bt, lens, starts, k, keep);
+  TORCH_CHECK(k.dim() == 3 && k.size(1) == c.n_kv_heads && k.size(2) == c.head_dim && v.sizes() == k.sizes() &&
+                  v.scalar_type() == k.scalar_type(),
+              "k and v must be [T, n_kv_heads, head_dim] of one dtype");
+  TORCH_CHECK(k.size(0) <= INT_MAX, "k is too large");
+  const c10::cuda::CUDAGuard guard(k.device());
+  const TurnArgs a = turn_args(table, positions, axes, wq, wk, eps, k, k.size(0), c.head_dim, keep);
+  TORCH_CHECK(given(q) || !a.wq, "q_weight without q");
+  const at::Tensor ki = head_rows(k), vi = head_rows(v);
+  at::Tensor qi, qo;
+  if (given(q)) {
+    on_device(*q, k, "q");
+    TORCH_CHECK(given(table) || eps.has_value(), "q is only normed and turned: it needs eps or a rotary table");
+    TORCH_CHECK(q->dim() == 3 && q->size(0) == k.size(0) && q->size(2) == c.head_dim &&
+                    q->scalar_type() == k.scalar_type(),
+                "q must be [T, heads, head_dim] of k's dtype");
+    TORCH_CHECK(q->size(1) <= INT_MAX, "q is too large");
+    qi = head_rows(*q);
+    qo = empty_on(q->sizes(), q->scalar_type(), k);
+  }
+  const bool has = qi.defined();
+  check(sf_paged4_append(&c, ki.data_ptr(), ki.stride(0), ki.stride(1), vi.data_ptr(), vi.stride(0), vi.stride(1),
+                         has ? qi.data_ptr() : nullptr, has ? qi.stride(0) : 0, has ? qi.stride(1) : 0,
+                         has ? qo.data_ptr() : nullptr, dtype_code(k.scalar_type()), has ? (int)qi.size(1) : 0,
+                         (int)k.size(0), a.wq, a.wk, a.w_dtype, a.eps, a.positions, a.pos64, a.axes_n, a.axes, a.table,
+                         a.max_pos, a.rot, interleaved, stream_of(k)));
+  return has ? OptTensor(qo) : OptTensor();
+}
+
+std::tuple<at::Tensor, OptTensor> paged4_attention(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& ks,
+                                                   const at::Tensor& vc, const at::Tensor& vs, const at::Tensor& bt,
+                                                   const at::Tensor& lens, const OptTensor& starts,
+                                                   c10::optional<double> scale, int64_t window,
+                                                   c10::optional<at::ScalarType> out_dtype, bool return_lse) {
+  TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor");
+  std::vector<at::Tensor> keep;
+  const sf_paged4_cache c = paged4_cache(kc, ks, vc, vs, bt, lens, starts, q, keep);
+  TORCH_CHECK(q.dim() == 3 && q.size(2) == c.head_dim, "q must be [T, heads, head_dim]");
+  TORCH_CHECK(q.size(0) <= INT_MAX && q.size(1) <= INT_MAX, "q is too large");
+  TORCH_CHECK(window <= INT_MAX, "window is too large");
+  const c10::cuda::CUDAGuard guard(q.device());
+  const at::Tensor qi = head_rows(q);
+  const at::ScalarType ot = out_dtype.value_or(q.scalar_type());
+  at::Tensor out = empty_on(q.sizes(), ot, q);
+  OptTensor lse;
+  if (return_lse) lse = empty_on({q.size(0), q.size(1)}, at::kFloat, q);
+  const size_t bytes = sf_paged4_attention_workspace_bytes(c.head_dim);
+  at::Tensor ws = empty_on({(int64_t)bytes}, at::kByte, q);
+  const double s = scale.has_value() ? *scale : 1.0 / std::sqrt((double)c.head_dim);
+  check(sf_paged4_attention(&c, qi.data_ptr(), dtype_code(q.scalar_type()), qi.stride(0), qi.stride(1), out.data_ptr(),
+                            dtype_code(ot), return_lse ? lse->data_ptr<float>() : nullptr, (int)q.size(1), (int)q.size(0),
+                            (float)s, window > 0 ? (int)window : 0, ws.data_ptr(), bytes, stream_of(q)));
+  return {out, lse};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -389,4 +605,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rotary", &rotary, "rotary positions");
   m.def("paged_append", &paged_append, "rotary positions, and keys and values into the pages of an e4m3 cache");
   m.def("paged_attention", &paged_attention, "attention over the pages of an e4m3 cache -> (out, lse or None)");
+  m.def("qk_norm_rotary", &qk_norm_rotary, "norms and rotary positions of query and key heads -> (q, k or None)");
+  m.def("paged4_append", &paged4_append, "norms, rotary positions, and keys and values into the pages of a 4-bit cache");
+  m.def("paged4_attention", &paged4_attention, "attention over the pages of a 4-bit cache -> (out, lse or None)");
 }

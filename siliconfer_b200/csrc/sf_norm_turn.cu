@@ -7,6 +7,7 @@
 // A block takes one token: its angles, which hang on one or several positions, are brought to shared memory once and
 // serve all heads.  A group of lanes takes a vector, a lane the same W places of all four quarters: these hold both
 // elements of its rotary pairs, and the codes of a place are one 16-bit word.
+#include <algorithm>
 #include <atomic>
 #include <cstdint>
 #include <type_traits>
@@ -81,16 +82,26 @@ __device__ __forceinline__ void load_raw(const TX* x, Raw<TX, W>& r) {
 // A vector's elements: y[c][i] is element c * D/4 + r0 + i.
 // F: float, or double for keys on their way to codes.
 template <typename F>
-__device__ __forceinline__ void turn_pair(F& a, F& b, float c, float s) {
-  const F ya = fma(a, (F)c, -(b * (F)s)), yb = fma(b, (F)c, a * (F)s);
+__device__ __forceinline__ void turn_pair(F& a, F& b, F c, F s) {
+  const F ya = fma(a, c, -(b * s)), yb = fma(b, c, a * s);
   a = ya;
   b = yb;
+}
+template <int W, typename F>
+__device__ __forceinline__ void load_angles(const F* p, F (&v)[W]) {
+  if constexpr (W == 4 && sizeof(F) == 4) {
+    const float4 u = *reinterpret_cast<const float4*>(p);
+    v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; ++i) v[i] = p[i];
+  }
 }
 // cs, sn: pair j's cosine and sine; buf: a place in shared memory for the vector, used where a pair's two elements lie
 // in different lanes.  Called by whole warps; lanes with there = false turn nothing.
 template <typename F, int W>
-__device__ __forceinline__ void turn_vector(F (&y)[4][W], bool there, int r0, const HeadArgs& a, const float* cs,
-                                            const float* sn, F* buf) {
+__device__ __forceinline__ void turn_vector(F (&y)[4][W], bool there, int r0, const HeadArgs& a, const F* cs,
+                                            const F* sn, F* buf) {
   const int Q = a.D / 4, half = a.rot / 2;
   if (a.pairs == kAnyPairs) {
     __syncwarp();
@@ -111,20 +122,27 @@ __device__ __forceinline__ void turn_vector(F (&y)[4][W], bool there, int r0, co
         const bool second = a.interleaved ? e & 1 : e >= half;
         const int j = a.interleaved ? e / 2 : second ? e - half : e;
         const int other = a.interleaved ? e ^ 1 : second ? e - half : e + half;
-        const F s = (F)sn[j];
-        y[c][i] = fma(y[c][i], (F)cs[j], buf[other] * (second ? s : -s));
+        const F s = sn[j];
+        y[c][i] = fma(y[c][i], cs[j], buf[other] * (second ? s : -s));
       }
     return;
   }
   if (!there) return;
   if (a.pairs == kHalves) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
+    for (int c = 0; c < 2; ++c) {
+      F cw[W], sw[W];
+      load_angles<W>(cs + c * Q + r0, cw);
+      load_angles<W>(sn + c * Q + r0, sw);
 #pragma unroll
-      for (int i = 0; i < W; ++i) turn_pair<F>(y[c][i], y[c + 2][i], cs[c * Q + r0 + i], sn[c * Q + r0 + i]);
+      for (int i = 0; i < W; ++i) turn_pair<F>(y[c][i], y[c + 2][i], cw[i], sw[i]);
+    }
   } else if (a.pairs == kHalvesOfHalf) {
+    F cw[W], sw[W];
+    load_angles<W>(cs + r0, cw);
+    load_angles<W>(sn + r0, sw);
 #pragma unroll
-    for (int i = 0; i < W; ++i) turn_pair<F>(y[0][i], y[1][i], cs[r0 + i], sn[r0 + i]);
+    for (int i = 0; i < W; ++i) turn_pair<F>(y[0][i], y[1][i], cw[i], sw[i]);
   } else if (a.pairs == kNeighbours) {
     if constexpr (W > 1) {
 #pragma unroll
@@ -138,16 +156,37 @@ __device__ __forceinline__ void turn_vector(F (&y)[4][W], bool there, int r0, co
   }
 }
 
-// y -> its code less 8, for a scale s; z is y in fp64.  The quotient is taken in fp32; where that leaves it within 2^-18
-// of a tie, what z / s and the code differ by decides, which is exact but for one rounding in fp64.
-__device__ __forceinline__ int code_of(double z, float y, float s, float inv) {
-  const float t = y * inv;
-  float r = rintf(t);
-  if (fabsf(t - r) > 0.5f - 0x1p-18f) {
-    const double d = fma(-(double)r, (double)s, z), twice = 2.0 * fabs(d);
-    if (twice > (double)s || (twice == (double)s && ((int)r & 1))) r += d > 0 ? 1.f : -1.f;
+// y / s to the nearest whole number (ties to even), limited to -8 .. 7, plus 8; inv = 1 / s in fp32.  A first guess is at
+// most one off, and what y and guess * s differ by, which is exact (in fp64 but for one rounding of y's last place), says so.
+__device__ __forceinline__ uint32_t code_of(float y, float s, float inv) {
+  const float m = fmaf(y, inv, 12582912.f), r = m - 12582912.f, d = fmaf(-r, s, y), over = fmaf(fabsf(d), 2.f, -s);
+  int n = __float_as_int(m) - 0x4b400000;
+  if (over > 0.f || (over == 0.f && (n & 1))) n += d > 0.f ? 1 : -1;
+  return (uint32_t)(min(max(n, -8), 7) + 8);
+}
+__device__ __forceinline__ uint32_t code_of(double y, double s, double inv) {
+  const double m = fma(y, inv, 6755399441055744.0), r = m - 6755399441055744.0, d = fma(-r, s, y), over = fma(fabs(d), 2.0, -s);
+  int n = __double2loint(m);
+  if (over > 0.0 || (over == 0.0 && (n & 1))) n += __double2hiint(d) >= 0 ? 1 : -1;
+  return (uint32_t)(min(max(n, -8), 7) + 8);
+}
+// Largest magnitude of each quarter over a vector's lanes, as bits (an infinity or a NaN is above every number).
+template <int GP, int W>
+__device__ __forceinline__ uint32_t quarter_tops(const float (&y)[4][W], uint32_t (&top)[4]) {
+  uint32_t most = 0;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    top[c] = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) top[c] = max(top[c], __float_as_uint(y[c][i]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = GP / 2; o; o >>= 1) top[c] = max(top[c], __shfl_xor_sync(0xffffffffu, top[c], o));
+    most = max(most, top[c]);
   }
-  return (int)fminf(fmaxf(r, -8.f), 7.f);
+  return most;
+}
+__device__ __forceinline__ uint32_t scale_bits(float s, bool finite) {
+  return finite ? __bfloat16_as_ushort(__float2bfloat16_rn(fmaxf(s, 0x1p-126f))) : 0x7fc0u;
 }
 
 struct TokenPlace {
@@ -155,18 +194,28 @@ struct TokenPlace {
   int pos;         // -1: none; -2: a padding row
   long long slot;  // (page * n_kv_heads) * page_size + slot
 };
+// A lane's words and, from a vector's first lane, its scales.
+__device__ __forceinline__ void store_codes(const HeadArgs& a, const TokenPlace& place, int kind, int h, int r0,
+                                            const uint32_t (&words)[4], const uint32_t (&sb)[4]) {
+  const long long vec = place.slot + (long long)h * a.c.page_size;
+  uint8_t* codes = (kind == 1 ? a.c.k_codes : a.c.v_codes) + vec * (a.D / 2) + 2 * r0;
+  *reinterpret_cast<uint2*>(codes) = make_uint2(words[0] | words[1] << 16, words[2] | words[3] << 16);
+  if (r0 == 0)
+    *reinterpret_cast<uint2*>((kind == 1 ? a.ks : a.vs) + vec * 4) = make_uint2(sb[0] | sb[1] << 16, sb[2] | sb[3] << 16);
+}
 
 template <typename TX, int W, int GP, bool VEC, bool CACHE>
-__global__ void __launch_bounds__(kThreads) norm_turn_kernel(const HeadArgs a) {
-  constexpr int M = sizeof(TX) == 2 ? 4 : 2;   // vectors of a group under way
+__global__ void __launch_bounds__(kThreads, CACHE ? 3 : 4) norm_turn_kernel(const __grid_constant__ HeadArgs a) {
+  static_assert(!CACHE || W == 4, "a lane's words are stored as 8 bytes");
   extern __shared__ __align__(16) double exchange[];
   __shared__ __align__(16) float cs[kMaxDim / 2], sn[kMaxDim / 2], wsm[2][kMaxDim];
+  __shared__ __align__(16) double cs64[CACHE ? 128 : 1], sn64[CACHE ? 128 : 1], w64[CACHE ? 256 : 1];   // for keys
   __shared__ TokenPlace place;
   griddep_launch_dependents();
   griddep_wait();
   const int tok = blockIdx.x, tid = threadIdx.x, g = tid / GP, r0 = tid % GP * W, D = a.D, Q = D / 4;
   const bool mine = g < a.groups && r0 < Q;
-  const int nv = a.Hkv * (CACHE ? 2 : 1) + a.H;
+  const int nv = a.Hkv * (CACHE ? 2 : 1) + a.H, first = g + a.groups * a.rounds * (int)blockIdx.y;
   // vectors in order: keys, values (with a cache), queries
   const auto source = [&](int v, int& kind, int& h) {
     kind = v < a.Hkv ? 1 : CACHE && v < 2 * a.Hkv ? 2 : 0;
@@ -174,17 +223,14 @@ __global__ void __launch_bounds__(kThreads) norm_turn_kernel(const HeadArgs a) {
     const Vectors& s = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
     return static_cast<const TX*>(s.p) + (long long)tok * s.ts + h * s.hs;
   };
-  Raw<TX, W> raw[M][4];
+  Raw<TX, W> next[4];
   const auto load = [&](int round) {
+    const int v = first + a.groups * round;
+    if (!mine || round >= a.rounds || v >= nv) return;
+    int kind, h;
+    const TX* x = source(v, kind, h);
 #pragma unroll
-    for (int m = 0; m < M; ++m) {
-      const int v = g + a.groups * (round + m + a.rounds * (int)blockIdx.y);
-      if (!mine || round + m >= a.rounds || v >= nv) continue;
-      int kind, h;
-      const TX* x = source(v, kind, h);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) load_raw<TX, W, VEC>(x + c * Q + r0, raw[m][c]);
-    }
+    for (int c = 0; c < 4; ++c) load_raw<TX, W, VEC>(x + c * Q + r0, next[c]);
   };
   load(0);
 
@@ -229,12 +275,17 @@ __global__ void __launch_bounds__(kThreads) norm_turn_kernel(const HeadArgs a) {
     const float nan = __int_as_float(0x7fffffff);
     cs[j] = ok ? __ldg(a.table + p * a.rot + j) : nan;
     sn[j] = ok ? __ldg(a.table + p * a.rot + half + j) : nan;
+    if constexpr (CACHE) cs64[j] = cs[j], sn64[j] = sn[j];
   }
   if (a.norm) {
     for (int i = tid; i < 2 * D; i += blockDim.x) {
       const int which = i >= D, e = which ? i - D : i;
       const void* w = which ? a.wk : a.wq;
-      wsm[which][e] = w ? load_weight(w, a.w_dtype, e) : 1.f;
+      const float x = w ? load_weight(w, a.w_dtype, e) : 1.f;
+      wsm[which][e] = x;
+      if constexpr (CACHE) {
+        if (which) w64[e] = x;
+      }
     }
   }
   __syncthreads();
@@ -242,24 +293,26 @@ __global__ void __launch_bounds__(kThreads) norm_turn_kernel(const HeadArgs a) {
   double* buf64 = exchange + (tid / 32) * (128 * W) + (tid % 32) / GP * D;
   float* buf32 = reinterpret_cast<float*>(exchange + (tid / 32) * (128 * W)) + (tid % 32) / GP * D;
 
-  for (int round = 0; round < a.rounds; round += M) {
-    if (round > 0) load(round);
+#pragma unroll 1
+  for (int round = 0; round < a.rounds; ++round) {
+    const int v = first + a.groups * round;
+    const bool there = mine && v < nv;
+    int kind = 0, h = 0;
+    if (there) source(v, kind, h);
+    Raw<TX, W> raw[4];
 #pragma unroll
-    for (int m = 0; m < M; ++m) {
-      if (round + m >= a.rounds) break;
-      const int v = g + a.groups * (round + m + a.rounds * (int)blockIdx.y);
-      const bool there = mine && v < nv;
-      int kind = 0, h = 0;
-      if (there) source(v, kind, h);
-      // whole warps go through both parts, since sums and maxima are shuffled; a warp's groups may differ in kind
-      if (CACHE && __any_sync(0xffffffffu, there && kind != 0)) {
-        // ---- a key or a value to its codes ----
-        const bool put = there && kind != 0 && place.put, key = put && kind == 1;
+    for (int c = 0; c < 4; ++c) raw[c] = next[c];
+    load(round + 1);
+    // whole warps go through each part that some lane needs, since sums and maxima are shuffled
+    if constexpr (CACHE) {
+      if (__any_sync(0xffffffffu, there && kind == 1)) {
+        // ---- a key, in fp64, to its codes ----
+        const bool key = there && kind == 1;
         double z[4][W];
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int i = 0; i < W; ++i) z[c][i] = there ? (double)to_f32(raw[m][c].e[i]) : 0.0;
+          for (int i = 0; i < W; ++i) z[c][i] = key ? (double)to_f32(raw[c].e[i]) : 0.0;
         if (a.norm) {
           double ss = 0;
 #pragma unroll
@@ -273,94 +326,101 @@ __global__ void __launch_bounds__(kThreads) norm_turn_kernel(const HeadArgs a) {
 #pragma unroll
             for (int c = 0; c < 4; ++c)
 #pragma unroll
-              for (int i = 0; i < W; ++i) z[c][i] = z[c][i] * r * (double)wsm[1][c * Q + r0 + i];
+              for (int i = 0; i < W; ++i) z[c][i] = z[c][i] * r * w64[c * Q + r0 + i];
           }
         }
-        turn_vector<double, W>(z, key, r0, a, cs, sn, buf64);
-        uint32_t top[4], most = 0;
+        turn_vector<double, W>(z, key, r0, a, cs64, sn64, buf64);
+        uint32_t top[4], words[4] = {}, sb[4];
+        {
+          float y[4][W];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          top[c] = 0;
+          for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int i = 0; i < W; ++i) top[c] = max(top[c], __float_as_uint((float)z[c][i]) & 0x7fffffffu);
+            for (int i = 0; i < W; ++i) y[c][i] = (float)z[c][i];
+          const bool finite = quarter_tops<GP, W>(y, top) < 0x7f800000u;
 #pragma unroll
-          for (int o = GP / 2; o; o >>= 1) top[c] = max(top[c], __shfl_xor_sync(0xffffffffu, top[c], o));
-          most = max(most, top[c]);
-        }
-        const bool finite = most < 0x7f800000u;
-        uint32_t words[W] = {}, scale_bits[4];
+          for (int c = 0; c < 4; ++c) {
+            float s = __fdiv_rn(__uint_as_float(top[c]), 7.5f);
+            // within 4 last places of a tie of two scales: from the largest magnitude in fp64
+            const bool near = ((__float_as_uint(s) - 0x7ffcu) & 0xffffu) <= 8u;
+            if (__any_sync(0xffffffffu, near)) {
+              double big = 0;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float s = __fdiv_rn(__uint_as_float(top[c]), 7.5f);
-          // within 4 last places of a tie of two scales: from the largest magnitude in fp64
-          const bool near = ((__float_as_uint(s) - 0x7ffcu) & 0xffffu) <= 8u;
-          if (__any_sync(0xffffffffu, near)) {
-            double big = 0;
+              for (int i = 0; i < W; ++i) big = fmax(big, fabs(z[c][i]));
 #pragma unroll
-            for (int i = 0; i < W; ++i) big = fmax(big, fabs(z[c][i]));
+              for (int o = GP / 2; o; o >>= 1) big = fmax(big, __shfl_xor_sync(0xffffffffu, big, o));
+              if (near) s = (float)(big / 7.5);
+            }
+            sb[c] = scale_bits(s, finite);
+            s = __uint_as_float(sb[c] << 16);
+            const double s64 = s, inv = 1.f / s;
 #pragma unroll
-            for (int o = GP / 2; o; o >>= 1) big = fmax(big, __shfl_xor_sync(0xffffffffu, big, o));
-            if (near) s = (float)(big / 7.5);
-          }
-          const __nv_bfloat16 sb = finite ? __float2bfloat16_rn(fmaxf(s, 0x1p-126f)) : __float2bfloat16_rn(__int_as_float(0x7fffffff));
-          scale_bits[c] = __bfloat16_as_ushort(sb);
-          s = __bfloat162float(sb);
-          const float inv = 1.f / s;
-#pragma unroll
-          for (int i = 0; i < W; ++i) {
-            const int n = finite ? code_of(z[c][i], (float)z[c][i], s, inv) + 8 : 8;
-            words[i] |= (uint32_t)n << (4 * c);
+            for (int i = 0; i < W; ++i) words[i] |= (finite ? code_of(z[c][i], s64, inv) : 8u) << (4 * c);
           }
         }
-        if (put) {
-          const long long vec = place.slot + (long long)h * a.c.page_size;
-          uint8_t* codes = (kind == 1 ? a.c.k_codes : a.c.v_codes) + vec * (D / 2) + 2 * r0;
-          static_assert(!CACHE || W == 4, "a lane's words are stored as 8 bytes");
-          *reinterpret_cast<uint2*>(codes) = make_uint2(words[0] | words[1 % W] << 16, words[2 % W] | words[3 % W] << 16);
-          if (r0 == 0)
-            *reinterpret_cast<uint2*>((kind == 1 ? a.ks : a.vs) + vec * 4) =
-                make_uint2(scale_bits[0] | scale_bits[1] << 16, scale_bits[2] | scale_bits[3] << 16);
-        }
+        if (key && place.put) store_codes(a, place, 1, h, r0, words, sb);
       }
-      const bool out = there && (kind == 0 || !CACHE);
-      if (!CACHE || __any_sync(0xffffffffu, out)) {
-        // ---- a query, or a key that stays one, to its own type ----
+      if (__any_sync(0xffffffffu, there && kind == 2)) {
+        // ---- a value, exact as it is, to its codes ----
         float y[4][W];
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int i = 0; i < W; ++i) y[c][i] = there ? to_f32(raw[m][c].e[i]) : 0.f;
-        if (a.norm) {
-          float ss = 0;
+          for (int i = 0; i < W; ++i) y[c][i] = there && kind == 2 ? to_f32(raw[c].e[i]) : 0.f;
+        uint32_t top[4], words[4] = {}, sb[4];
+        const bool finite = quarter_tops<GP, W>(y, top) < 0x7f800000u;
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 4; ++c) {
+          sb[c] = scale_bits(__fdiv_rn(__uint_as_float(top[c]), 7.5f), finite);
+          const float s = __uint_as_float(sb[c] << 16), inv = 1.f / s;
 #pragma unroll
-            for (int i = 0; i < W; ++i) ss = fmaf(y[c][i], y[c][i], ss);
-#pragma unroll
-          for (int o = GP / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-          const float r = rsqrtf(ss / (float)D + a.eps);
-          if (out) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-              for (int i = 0; i < W; ++i) y[c][i] = y[c][i] * r * wsm[kind][c * Q + r0 + i];
-          }
+          for (int i = 0; i < W; ++i) words[i] |= (finite ? code_of(y[c][i], s, inv) : 8u) << (4 * c);
         }
-        turn_vector<float, W>(y, out, r0, a, cs, sn, buf32);
+        if (there && kind == 2 && place.put) store_codes(a, place, 2, h, r0, words, sb);
+      }
+    }
+    const bool out = there && (kind == 0 || !CACHE);
+    if (!CACHE || __any_sync(0xffffffffu, out)) {
+      // ---- a query, or a key that stays one, to its own type ----
+      float y[4][W];
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int i = 0; i < W; ++i) y[c][i] = out ? to_f32(raw[c].e[i]) : 0.f;
+      if (a.norm) {
+        float ss = 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < W; ++i) ss = fmaf(y[c][i], y[c][i], ss);
+#pragma unroll
+        for (int o = GP / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float r = rsqrtf(ss / (float)D + a.eps);
         if (out) {
-          const Out& d = kind == 0 ? a.qo : a.ko;
-          TX* o = static_cast<TX*>(d.p) + (long long)tok * d.ts + h * d.hs + r0;
+          const float* w = wsm[kind] + r0;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            Raw<TX, W> w;
+            float u[W];
+            load_angles<W>(w + c * Q, u);
 #pragma unroll
-            for (int i = 0; i < W; ++i) w.e[i] = from_f32<TX>(y[c][i]);
-            if constexpr (VEC) {
-              *reinterpret_cast<typename Raw<TX, W>::Word*>(o + c * Q) = w.w;
-            } else {
+            for (int i = 0; i < W; ++i) y[c][i] *= r * u[i];
+          }
+        }
+      }
+      turn_vector<float, W>(y, out, r0, a, cs, sn, buf32);
+      if (out) {
+        const Out& d = kind == 0 ? a.qo : a.ko;
+        TX* o = static_cast<TX*>(d.p) + (long long)tok * d.ts + h * d.hs + r0;
 #pragma unroll
-              for (int i = 0; i < W; ++i) o[c * Q + i] = w.e[i];
-            }
+        for (int c = 0; c < 4; ++c) {
+          Raw<TX, W> w;
+#pragma unroll
+          for (int i = 0; i < W; ++i) w.e[i] = from_f32<TX>(y[c][i]);
+          if constexpr (VEC) {
+            *reinterpret_cast<typename Raw<TX, W>::Word*>(o + c * Q) = w.w;
+          } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i) o[c * Q + i] = w.e[i];
           }
         }
       }
@@ -383,18 +443,17 @@ int check_args(const HeadArgs& a, int dtype) {
   return SF_OK;
 }
 
-// Vectors of a token to groups of lanes: one each where the tokens are few, else up to 4 (2 of fp32).
+// Vectors of a token to groups of lanes: one each where the tokens are few, else up to 4 in turn, the next one's elements
+// under way.
 template <typename TX, int W, bool CACHE>
 cudaError_t launch(HeadArgs& a, bool vec, cudaStream_t st) {
   const int lanes = a.D / 4 / W, nv = a.Hkv * (CACHE ? 2 : 1) + a.H;
   const auto go = [&](auto gp) -> cudaError_t {
-    constexpr int GP = decltype(gp)::value;
-    constexpr int most = kThreads / GP, M = sizeof(TX) == 2 ? 4 : 2;
+    constexpr int GP = decltype(gp)::value, most = kThreads / GP;
     int rounds = 1;
-    if ((long long)a.T * nv * GP > 1024ll * device_info().sms) rounds = (nv + most - 1) / most < M ? (nv + most - 1) / most : M;
+    if ((long long)a.T * nv * GP > 1024ll * device_info().sms) rounds = std::min((nv + most - 1) / most, 4);
     a.rounds = rounds;
-    a.groups = (nv + rounds - 1) / rounds;
-    if (a.groups > most) a.groups = most;
+    a.groups = std::min((nv + rounds - 1) / rounds, most);
     const int per_warp = 32 / GP, threads = (a.groups + per_warp - 1) / per_warp * 32;
     a.groups = threads / GP;
     const int parts = (nv + a.groups * rounds - 1) / (a.groups * rounds);
@@ -411,10 +470,16 @@ cudaError_t launch(HeadArgs& a, bool vec, cudaStream_t st) {
     auto* fn = vec ? norm_turn_kernel<TX, W, GP, true, CACHE> : norm_turn_kernel<TX, W, GP, false, CACHE>;
     return cudaLaunchKernelEx(&cfg, fn, a);
   };
-  if (lanes <= 4) return go(std::integral_constant<int, 4>());
-  if (lanes <= 8) return go(std::integral_constant<int, 8>());
-  if (lanes <= 16) return go(std::integral_constant<int, 16>());
-  return go(std::integral_constant<int, 32>());
+  if constexpr (W == 4) {
+    if (lanes <= 4) return go(std::integral_constant<int, 4>());
+    if (lanes <= 8) return go(std::integral_constant<int, 8>());
+    if (CACHE || lanes <= 16) return go(std::integral_constant<int, 16>());
+  }
+  if constexpr (W == 2) {
+    if (lanes <= 16) return go(std::integral_constant<int, 16>());
+  }
+  if constexpr (CACHE) return cudaErrorInvalidValue;   // a head of the cache has at most 256 elements
+  else return go(std::integral_constant<int, 32>());
 }
 
 // Which of a head's elements make its pairs, as the lanes hold them (W places of every quarter).

@@ -4,9 +4,9 @@
 //   pair (a, b), pair number j:  (a cos - b sin, a sin + b cos), cos and sin from row positions[axes[j]] of a table
 //   quarter c of a vector:  scale = bf16(max|y| / 7.5), at least 2^-126;  code = clamp(rint(y / scale), -8, 7) + 8
 //
-// A block takes one token: its angles, which hang on one or several positions, are brought to shared memory once and
-// serve all heads.  A group of lanes takes a vector, a lane the same W places of all four quarters: these hold both
-// elements of its rotary pairs, and the codes of a place are one 16-bit word.
+// A block takes one token and some of its heads: the angles, which hang on one or several positions, are brought to shared
+// memory once.  A group of lanes takes a vector at a time, the next one's elements under way; a lane the same W places of
+// all four quarters: these hold both elements of its rotary pairs, and the codes of a place are one 16-bit word.
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
@@ -22,7 +22,7 @@ extern std::atomic<long long> g_launches;
 
 namespace {
 
-constexpr int kThreads = 256, kMaxDim = 512, kMaxAxes = 8;
+constexpr int kRounds = 6, kThreads = 256, kMaxDim = 512, kMaxAxes = 8;
 
 struct Vectors {
   const void* p;
@@ -46,7 +46,7 @@ struct HeadArgs {
   int pos64, axes_n;
   const uint8_t* axes;  // [rot / 2] or NULL: all pairs belong to axis 0
   int H, Hkv, T, D;
-  int groups, rounds;   // groups of lanes of a block, vectors that one takes
+  int w_vec;            // weights may be loaded four at a time
   // the cache's
   sf_paged_cache c;
   __nv_bfloat16 *ks, *vs;
@@ -87,9 +87,16 @@ __device__ __forceinline__ void turn_pair(F& a, F& b, F c, F s) {
   a = ya;
   b = yb;
 }
-template <int W, typename F>
-__device__ __forceinline__ void load_angles(const F* p, F (&v)[W]) {
-  if constexpr (W == 4 && sizeof(F) == 4) {
+// two pairs at once
+__device__ __forceinline__ void turn_pairs(float& a0, float& a1, float& b0, float& b1, float c0, float c1, float s0, float s1) {
+  const uint64_t a = pack2(a0, a1), b = pack2(b0, b1), c = pack2(c0, c1), s = pack2(s0, s1), n = pack2(-s0, -s1);
+  unpack2(fma2(a, c, mul2(b, n)), a0, a1);
+  unpack2(fma2(b, c, mul2(a, s)), b0, b1);
+}
+
+template <int W>
+__device__ __forceinline__ void load_angles(const float* p, float (&v)[W]) {
+  if constexpr (W == 4) {
     const float4 u = *reinterpret_cast<const float4*>(p);
     v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
   } else {
@@ -100,8 +107,8 @@ __device__ __forceinline__ void load_angles(const F* p, F (&v)[W]) {
 // cs, sn: pair j's cosine and sine; buf: a place in shared memory for the vector, used where a pair's two elements lie
 // in different lanes.  Called by whole warps; lanes with there = false turn nothing.
 template <typename F, int W>
-__device__ __forceinline__ void turn_vector(F (&y)[4][W], bool there, int r0, const HeadArgs& a, const F* cs,
-                                            const F* sn, F* buf) {
+__device__ __forceinline__ void turn_vector(F (&y)[4][W], bool there, int r0, const HeadArgs& a, const float* cs,
+                                            const float* sn, F* buf) {
   const int Q = a.D / 4, half = a.rot / 2;
   if (a.pairs == kAnyPairs) {
     __syncwarp();
@@ -122,27 +129,29 @@ __device__ __forceinline__ void turn_vector(F (&y)[4][W], bool there, int r0, co
         const bool second = a.interleaved ? e & 1 : e >= half;
         const int j = a.interleaved ? e / 2 : second ? e - half : e;
         const int other = a.interleaved ? e ^ 1 : second ? e - half : e + half;
-        const F s = sn[j];
-        y[c][i] = fma(y[c][i], cs[j], buf[other] * (second ? s : -s));
+        y[c][i] = fma(y[c][i], (F)cs[j], buf[other] * (F)(second ? sn[j] : -sn[j]));
       }
     return;
   }
   if (!there) return;
-  if (a.pairs == kHalves) {
+  // W pairs (x[i], z[i])
+  const auto run = [&](F (&x)[W], F (&z)[W], int j) {
+    float c[W], s[W];
+    load_angles<W>(cs + j, c);
+    load_angles<W>(sn + j, s);
+    if constexpr (W > 1 && sizeof(F) == 4) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      F cw[W], sw[W];
-      load_angles<W>(cs + c * Q + r0, cw);
-      load_angles<W>(sn + c * Q + r0, sw);
+      for (int i = 0; i < W; i += 2) turn_pairs(x[i], x[i + 1], z[i], z[i + 1], c[i], c[i + 1], s[i], s[i + 1]);
+    } else {
 #pragma unroll
-      for (int i = 0; i < W; ++i) turn_pair<F>(y[c][i], y[c + 2][i], cw[i], sw[i]);
+      for (int i = 0; i < W; ++i) turn_pair<F>(x[i], z[i], c[i], s[i]);
     }
+  };
+  if (a.pairs == kHalves) {
+    run(y[0], y[2], r0);
+    run(y[1], y[3], Q + r0);
   } else if (a.pairs == kHalvesOfHalf) {
-    F cw[W], sw[W];
-    load_angles<W>(cs + r0, cw);
-    load_angles<W>(sn + r0, sw);
-#pragma unroll
-    for (int i = 0; i < W; ++i) turn_pair<F>(y[0][i], y[1][i], cw[i], sw[i]);
+    run(y[0], y[1], r0);
   } else if (a.pairs == kNeighbours) {
     if constexpr (W > 1) {
 #pragma unroll
@@ -189,52 +198,76 @@ __device__ __forceinline__ uint32_t scale_bits(float s, bool finite) {
   return finite ? __bfloat16_as_ushort(__float2bfloat16_rn(fmaxf(s, 0x1p-126f))) : 0x7fc0u;
 }
 
-struct TokenPlace {
-  bool put;        // the row is a sequence's token, and its page is there
-  int pos;         // -1: none; -2: a padding row
-  long long slot;  // (page * n_kv_heads) * page_size + slot
-};
 // A lane's words and, from a vector's first lane, its scales.
-__device__ __forceinline__ void store_codes(const HeadArgs& a, const TokenPlace& place, int kind, int h, int r0,
+__device__ __forceinline__ void store_codes(const HeadArgs& a, long long slot, int kind, int h, int r0,
                                             const uint32_t (&words)[4], const uint32_t (&sb)[4]) {
-  const long long vec = place.slot + (long long)h * a.c.page_size;
+  const long long vec = slot + (long long)h * a.c.page_size;   // slot: (page * n_kv_heads) * page_size + slot
   uint8_t* codes = (kind == 1 ? a.c.k_codes : a.c.v_codes) + vec * (a.D / 2) + 2 * r0;
   *reinterpret_cast<uint2*>(codes) = make_uint2(words[0] | words[1] << 16, words[2] | words[3] << 16);
   if (r0 == 0)
     *reinterpret_cast<uint2*>((kind == 1 ? a.ks : a.vs) + vec * 4) = make_uint2(sb[0] | sb[1] << 16, sb[2] | sb[3] << 16);
 }
 
+// W weights of a lane's quarter c, 1 without any.
+template <int W>
+__device__ __forceinline__ void load_weights(const HeadArgs& a, const void* w, int e, float (&v)[W]) {
+#pragma unroll
+  for (int i = 0; i < W; ++i) v[i] = 1.f;
+  if (!w) return;
+  if (W == 4 && a.w_vec) {
+    if (a.w_dtype == SF_F32) {
+      const float4 u = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(w) + e));
+      v[0] = u.x, v[1 % W] = u.y, v[2 % W] = u.z, v[3 % W] = u.w;
+    } else {
+      const uint2 u = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(w) + e));
+      const uint32_t h[4] = {u.x & 0xffffu, u.x >> 16, u.y & 0xffffu, u.y >> 16};
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        v[i] = a.w_dtype == SF_BF16 ? __uint_as_float(h[i] << 16) : __half2float(__ushort_as_half((unsigned short)h[i]));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; ++i) v[i] = load_weight(w, a.w_dtype, e + i);
+  }
+}
+
+struct TokenPlace {
+  bool put;        // the row is a sequence's token, and its page is there
+  int pos;         // -1: none; -2: a padding row
+  long long slot;  // (page * n_kv_heads) * page_size + slot
+};
+
 template <typename TX, int W, int GP, bool VEC, bool CACHE>
-__global__ void __launch_bounds__(kThreads, CACHE ? 3 : 4) norm_turn_kernel(const __grid_constant__ HeadArgs a) {
+__global__ void __launch_bounds__(kThreads, CACHE ? 2 : 4) norm_turn_kernel(const __grid_constant__ HeadArgs a) {
   static_assert(!CACHE || W == 4, "a lane's words are stored as 8 bytes");
+  constexpr int AT = 32 / GP;   // vectors of a warp at a time
   extern __shared__ __align__(16) double exchange[];
-  __shared__ __align__(16) float cs[kMaxDim / 2], sn[kMaxDim / 2], wsm[2][kMaxDim];
-  __shared__ __align__(16) double cs64[CACHE ? 128 : 1], sn64[CACHE ? 128 : 1], w64[CACHE ? 256 : 1];   // for keys
+  __shared__ __align__(16) float cs[kMaxDim / 2], sn[kMaxDim / 2];
   __shared__ TokenPlace place;
   griddep_launch_dependents();
   griddep_wait();
-  const int tok = blockIdx.x, tid = threadIdx.x, g = tid / GP, r0 = tid % GP * W, D = a.D, Q = D / 4;
-  const bool mine = g < a.groups && r0 < Q;
-  const int nv = a.Hkv * (CACHE ? 2 : 1) + a.H, first = g + a.groups * a.rounds * (int)blockIdx.y;
-  // vectors in order: keys, values (with a cache), queries
+  const int D = a.D, Q = D / 4, tid = threadIdx.x, lane = tid & 31, r0 = lane % GP * W, tok = blockIdx.x;
+  // vectors in order: keys, values (with a cache), queries; this warp's are v0, v0 + step, ...
+  const int nv = a.Hkv * (CACHE ? 2 : 1) + a.H, step = (int)(blockDim.x / 32 * gridDim.y) * AT,
+            v0 = (int)(blockIdx.y * (blockDim.x / 32) + tid / 32) * AT + lane / GP;
+  const bool mine = r0 < Q;
   const auto source = [&](int v, int& kind, int& h) {
     kind = v < a.Hkv ? 1 : CACHE && v < 2 * a.Hkv ? 2 : 0;
     h = kind == 0 ? v - a.Hkv * (CACHE ? 2 : 1) : kind == 1 ? v : v - a.Hkv;
     const Vectors& s = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
-    return static_cast<const TX*>(s.p) + (long long)tok * s.ts + h * s.hs;
+    return static_cast<const TX*>(s.p) + (long long)tok * s.ts + h * s.hs + r0;
   };
   Raw<TX, W> next[4];
-  const auto load = [&](int round) {
-    const int v = first + a.groups * round;
-    if (!mine || round >= a.rounds || v >= nv) return;
+  const auto load = [&](int v) {
+    if (!mine || v >= nv) return;
     int kind, h;
     const TX* x = source(v, kind, h);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) load_raw<TX, W, VEC>(x + c * Q + r0, next[c]);
+    for (int c = 0; c < 4; ++c) load_raw<TX, W, VEC>(x + c * Q, next[c]);
   };
-  load(0);
+  load(v0);
 
-  // ---- the token's place, angles and the norms' weights ----
+  // ---- the token's place and angles ----
   if (CACHE) {
     if (tid < 32) {
       const TokenAt at = token_at(a.c, a.T, tok);
@@ -275,34 +308,23 @@ __global__ void __launch_bounds__(kThreads, CACHE ? 3 : 4) norm_turn_kernel(cons
     const float nan = __int_as_float(0x7fffffff);
     cs[j] = ok ? __ldg(a.table + p * a.rot + j) : nan;
     sn[j] = ok ? __ldg(a.table + p * a.rot + half + j) : nan;
-    if constexpr (CACHE) cs64[j] = cs[j], sn64[j] = sn[j];
-  }
-  if (a.norm) {
-    for (int i = tid; i < 2 * D; i += blockDim.x) {
-      const int which = i >= D, e = which ? i - D : i;
-      const void* w = which ? a.wk : a.wq;
-      const float x = w ? load_weight(w, a.w_dtype, e) : 1.f;
-      wsm[which][e] = x;
-      if constexpr (CACHE) {
-        if (which) w64[e] = x;
-      }
-    }
   }
   __syncthreads();
+  const bool put = CACHE && place.put;
+  const long long slot = CACHE ? place.slot : 0;
   // this vector's place in its warp's part of the exchange, room for 128 W doubles
-  double* buf64 = exchange + (tid / 32) * (128 * W) + (tid % 32) / GP * D;
-  float* buf32 = reinterpret_cast<float*>(exchange + (tid / 32) * (128 * W)) + (tid % 32) / GP * D;
+  double* buf64 = exchange + (tid / 32) * (128 * W) + lane / GP * D;
+  float* buf32 = reinterpret_cast<float*>(exchange + (tid / 32) * (128 * W)) + lane / GP * D;
 
 #pragma unroll 1
-  for (int round = 0; round < a.rounds; ++round) {
-    const int v = first + a.groups * round;
+  for (int v = v0; v - lane / GP < nv; v += step) {
     const bool there = mine && v < nv;
     int kind = 0, h = 0;
     if (there) source(v, kind, h);
     Raw<TX, W> raw[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) raw[c] = next[c];
-    load(round + 1);
+    load(v + step);
     // whole warps go through each part that some lane needs, since sums and maxima are shuffled
     if constexpr (CACHE) {
       if (__any_sync(0xffffffffu, there && kind == 1)) {
@@ -324,41 +346,42 @@ __global__ void __launch_bounds__(kThreads, CACHE ? 3 : 4) norm_turn_kernel(cons
           const double r = 1.0 / sqrt(ss / D + (double)a.eps);
           if (key) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+            for (int c = 0; c < 4; ++c) {
+              float w[W];
+              load_weights<W>(a, a.wk, c * Q + r0, w);
 #pragma unroll
-              for (int i = 0; i < W; ++i) z[c][i] = z[c][i] * r * w64[c * Q + r0 + i];
-          }
-        }
-        turn_vector<double, W>(z, key, r0, a, cs64, sn64, buf64);
-        uint32_t top[4], words[4] = {}, sb[4];
-        {
-          float y[4][W];
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int i = 0; i < W; ++i) y[c][i] = (float)z[c][i];
-          const bool finite = quarter_tops<GP, W>(y, top) < 0x7f800000u;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            float s = __fdiv_rn(__uint_as_float(top[c]), 7.5f);
-            // within 4 last places of a tie of two scales: from the largest magnitude in fp64
-            const bool near = ((__float_as_uint(s) - 0x7ffcu) & 0xffffu) <= 8u;
-            if (__any_sync(0xffffffffu, near)) {
-              double big = 0;
-#pragma unroll
-              for (int i = 0; i < W; ++i) big = fmax(big, fabs(z[c][i]));
-#pragma unroll
-              for (int o = GP / 2; o; o >>= 1) big = fmax(big, __shfl_xor_sync(0xffffffffu, big, o));
-              if (near) s = (float)(big / 7.5);
+              for (int i = 0; i < W; ++i) z[c][i] = z[c][i] * r * (double)w[i];
             }
-            sb[c] = scale_bits(s, finite);
-            s = __uint_as_float(sb[c] << 16);
-            const double s64 = s, inv = 1.f / s;
-#pragma unroll
-            for (int i = 0; i < W; ++i) words[i] |= (finite ? code_of(z[c][i], s64, inv) : 8u) << (4 * c);
           }
         }
-        if (key && place.put) store_codes(a, place, 1, h, r0, words, sb);
+        turn_vector<double, W>(z, key, r0, a, cs, sn, buf64);
+        uint32_t top[4], words[4] = {}, sb[4];
+        float y[4][W];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < W; ++i) y[c][i] = (float)z[c][i];
+        const bool finite = quarter_tops<GP, W>(y, top) < 0x7f800000u;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float s = __fdiv_rn(__uint_as_float(top[c]), 7.5f);
+          // within 4 last places of a tie of two scales: from the largest magnitude in fp64
+          const bool near = ((__float_as_uint(s) - 0x7ffcu) & 0xffffu) <= 8u;
+          if (__any_sync(0xffffffffu, near)) {
+            double big = 0;
+#pragma unroll
+            for (int i = 0; i < W; ++i) big = fmax(big, fabs(z[c][i]));
+#pragma unroll
+            for (int o = GP / 2; o; o >>= 1) big = fmax(big, __shfl_xor_sync(0xffffffffu, big, o));
+            if (near) s = (float)(big / 7.5);
+          }
+          sb[c] = scale_bits(s, finite);
+          s = __uint_as_float(sb[c] << 16);
+          const double s64 = s, inv = 1.f / s;
+#pragma unroll
+          for (int i = 0; i < W; ++i) words[i] |= (finite ? code_of(z[c][i], s64, inv) : 8u) << (4 * c);
+        }
+        if (key && put) store_codes(a, slot, 1, h, r0, words, sb);
       }
       if (__any_sync(0xffffffffu, there && kind == 2)) {
         // ---- a value, exact as it is, to its codes ----
@@ -376,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, CACHE ? 3 : 4) norm_turn_kernel(cons
 #pragma unroll
           for (int i = 0; i < W; ++i) words[i] |= (finite ? code_of(y[c][i], s, inv) : 8u) << (4 * c);
         }
-        if (there && kind == 2 && place.put) store_codes(a, place, 2, h, r0, words, sb);
+        if (there && kind == 2 && put) store_codes(a, slot, 2, h, r0, words, sb);
       }
     }
     const bool out = there && (kind == 0 || !CACHE);
@@ -397,11 +420,11 @@ __global__ void __launch_bounds__(kThreads, CACHE ? 3 : 4) norm_turn_kernel(cons
         for (int o = GP / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         const float r = rsqrtf(ss / (float)D + a.eps);
         if (out) {
-          const float* w = wsm[kind] + r0;
+          const void* w = kind == 1 ? a.wk : a.wq;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             float u[W];
-            load_angles<W>(w + c * Q, u);
+            load_weights<W>(a, w, c * Q + r0, u);
 #pragma unroll
             for (int i = 0; i < W; ++i) y[c][i] *= r * u[i];
           }
@@ -443,24 +466,22 @@ int check_args(const HeadArgs& a, int dtype) {
   return SF_OK;
 }
 
-// Vectors of a token to groups of lanes: one each where the tokens are few, else up to 4 in turn, the next one's elements
-// under way.
+// Warps of a block and blocks of a token: a warp takes its vectors at once where the tokens are few, else 6 times in turn.
 template <typename TX, int W, bool CACHE>
 cudaError_t launch(HeadArgs& a, bool vec, cudaStream_t st) {
   const int lanes = a.D / 4 / W, nv = a.Hkv * (CACHE ? 2 : 1) + a.H;
+  const size_t wsize = a.w_dtype == SF_F32 ? 16 : 8;
+  a.w_vec = reinterpret_cast<uintptr_t>(a.wq) % wsize == 0 && reinterpret_cast<uintptr_t>(a.wk) % wsize == 0;
   const auto go = [&](auto gp) -> cudaError_t {
-    constexpr int GP = decltype(gp)::value, most = kThreads / GP;
-    int rounds = 1;
-    if ((long long)a.T * nv * GP > 1024ll * device_info().sms) rounds = std::min((nv + most - 1) / most, 4);
-    a.rounds = rounds;
-    a.groups = std::min((nv + rounds - 1) / rounds, most);
-    const int per_warp = 32 / GP, threads = (a.groups + per_warp - 1) / per_warp * 32;
-    a.groups = threads / GP;
-    const int parts = (nv + a.groups * rounds - 1) / (a.groups * rounds);
+    constexpr int GP = decltype(gp)::value, AT = 32 / GP;
+    const int passes = (nv + AT - 1) / AT;
+    const long long fill = 32ll * device_info().sms;   // warps
+    const int rounds = (int)std::min<long long>(kRounds, std::max<long long>(1, (long long)a.T * passes / fill));
+    const int warps = (passes + rounds - 1) / rounds, parts = (warps + kThreads / 32 - 1) / (kThreads / 32);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)a.T, (unsigned)parts);
-    cfg.blockDim = dim3((unsigned)threads);
-    cfg.dynamicSmemBytes = a.pairs == kAnyPairs ? (size_t)threads / 32 * 128 * W * sizeof(double) : 0;
+    cfg.blockDim = dim3((unsigned)((warps + parts - 1) / parts * 32));
+    cfg.dynamicSmemBytes = a.pairs == kAnyPairs ? (size_t)cfg.blockDim.x / 32 * 128 * W * sizeof(double) : 0;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

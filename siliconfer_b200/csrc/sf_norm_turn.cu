@@ -39,14 +39,13 @@ struct HeadArgs {
   Out qo, ko;
   const void *wq, *wk;  // norm weights or NULL
   int w_dtype, norm;
-  float eps;
+  float eps, inv_d;     // 1 / D
   const float* table;   // [max_pos, rot]: cosines, then sines
   int max_pos, rot, interleaved, pairs;
   const void* positions;   // [T, axes_n] or NULL: a token's place in its sequence
   int pos64, axes_n;
   const uint8_t* axes;  // [rot / 2] or NULL: all pairs belong to axis 0
   int H, Hkv, T, D;
-  int w_vec;            // weights may be loaded four at a time
   // the cache's
   sf_paged_cache c;
   __nv_bfloat16 *ks, *vs;
@@ -95,7 +94,7 @@ __device__ __forceinline__ void turn_pairs(float& a0, float& a1, float& b0, floa
 }
 
 template <int W>
-__device__ __forceinline__ void load_angles(const float* p, float (&v)[W]) {
+__device__ __forceinline__ void load_floats(const float* p, float (&v)[W]) {
   if constexpr (W == 4) {
     const float4 u = *reinterpret_cast<const float4*>(p);
     v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
@@ -137,8 +136,8 @@ __device__ __forceinline__ void turn_vector(F (&y)[4][W], bool there, int r0, co
   // W pairs (x[i], z[i])
   const auto run = [&](F (&x)[W], F (&z)[W], int j) {
     float c[W], s[W];
-    load_angles<W>(cs + j, c);
-    load_angles<W>(sn + j, s);
+    load_floats<W>(cs + j, c);
+    load_floats<W>(sn + j, s);
     if constexpr (W > 1 && sizeof(F) == 4) {
 #pragma unroll
       for (int i = 0; i < W; i += 2) turn_pairs(x[i], x[i + 1], z[i], z[i + 1], c[i], c[i + 1], s[i], s[i + 1]);
@@ -200,35 +199,13 @@ __device__ __forceinline__ uint32_t scale_bits(float s, bool finite) {
 
 // A lane's words and, from a vector's first lane, its scales.
 __device__ __forceinline__ void store_codes(const HeadArgs& a, long long slot, int kind, int h, int r0,
-                                            const uint32_t (&words)[4], const uint32_t (&sb)[4]) {
+                                            bool finite, const uint32_t (&words)[4], const uint32_t (&sb)[4]) {
   const long long vec = slot + (long long)h * a.c.page_size;   // slot: (page * n_kv_heads) * page_size + slot
   uint8_t* codes = (kind == 1 ? a.c.k_codes : a.c.v_codes) + vec * (a.D / 2) + 2 * r0;
-  *reinterpret_cast<uint2*>(codes) = make_uint2(words[0] | words[1] << 16, words[2] | words[3] << 16);
+  *reinterpret_cast<uint2*>(codes) = finite ? make_uint2(words[0] | words[1] << 16, words[2] | words[3] << 16)
+                                            : make_uint2(0x88888888u, 0x88888888u);
   if (r0 == 0)
     *reinterpret_cast<uint2*>((kind == 1 ? a.ks : a.vs) + vec * 4) = make_uint2(sb[0] | sb[1] << 16, sb[2] | sb[3] << 16);
-}
-
-// W weights of a lane's quarter c, 1 without any.
-template <int W>
-__device__ __forceinline__ void load_weights(const HeadArgs& a, const void* w, int e, float (&v)[W]) {
-#pragma unroll
-  for (int i = 0; i < W; ++i) v[i] = 1.f;
-  if (!w) return;
-  if (W == 4 && a.w_vec) {
-    if (a.w_dtype == SF_F32) {
-      const float4 u = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(w) + e));
-      v[0] = u.x, v[1 % W] = u.y, v[2 % W] = u.z, v[3 % W] = u.w;
-    } else {
-      const uint2 u = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(w) + e));
-      const uint32_t h[4] = {u.x & 0xffffu, u.x >> 16, u.y & 0xffffu, u.y >> 16};
-#pragma unroll
-      for (int i = 0; i < W; ++i)
-        v[i] = a.w_dtype == SF_BF16 ? __uint_as_float(h[i] << 16) : __half2float(__ushort_as_half((unsigned short)h[i]));
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < W; ++i) v[i] = load_weight(w, a.w_dtype, e + i);
-  }
 }
 
 struct TokenPlace {
@@ -242,30 +219,36 @@ __global__ void __launch_bounds__(kThreads, CACHE ? 2 : 4) norm_turn_kernel(cons
   static_assert(!CACHE || W == 4, "a lane's words are stored as 8 bytes");
   constexpr int AT = 32 / GP;   // vectors of a warp at a time
   extern __shared__ __align__(16) double exchange[];
-  __shared__ __align__(16) float cs[kMaxDim / 2], sn[kMaxDim / 2];
+  __shared__ __align__(16) float cs[kMaxDim / 2], sn[kMaxDim / 2], weights[2][kMaxDim];
   __shared__ TokenPlace place;
   griddep_launch_dependents();
   griddep_wait();
   const int D = a.D, Q = D / 4, tid = threadIdx.x, lane = tid & 31, r0 = lane % GP * W, tok = blockIdx.x;
-  // vectors in order: keys, values (with a cache), queries; this warp's are v0, v0 + step, ...
-  const int nv = a.Hkv * (CACHE ? 2 : 1) + a.H, step = (int)(blockDim.x / 32 * gridDim.y) * AT,
-            v0 = (int)(blockIdx.y * (blockDim.x / 32) + tid / 32) * AT + lane / GP;
-  const bool mine = r0 < Q;
-  const auto source = [&](int v, int& kind, int& h) {
-    kind = v < a.Hkv ? 1 : CACHE && v < 2 * a.Hkv ? 2 : 0;
-    h = kind == 0 ? v - a.Hkv * (CACHE ? 2 : 1) : kind == 1 ? v : v - a.Hkv;
-    const Vectors& s = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
-    return static_cast<const TX*>(s.p) + (long long)tok * s.ts + h * s.hs + r0;
+  // A pass is a kind of vectors (1 keys, 2 values, 0 queries, in that order) and AT of its heads; this warp's are first,
+  // first + step, ...
+  const int k_passes = (a.Hkv + AT - 1) / AT, kv_passes = k_passes * (CACHE ? 2 : 1), passes = kv_passes + (a.H + AT - 1) / AT;
+  const int step = (int)(blockDim.x / 32 * gridDim.y),
+            first = __shfl_sync(0xffffffffu, (int)(blockIdx.y * (blockDim.x / 32) + tid / 32), 0);
+  const auto kind_of = [&](int p) { return p < k_passes ? 1 : CACHE && p < kv_passes ? 2 : 0; };
+  const auto head_of = [&](int p, int kind) {
+    return (p - (kind == 1 ? 0 : kind == 2 ? k_passes : kv_passes)) * AT + lane / GP;
   };
+  const auto there_of = [&](int h, int kind) { return r0 < Q && h < (kind == 0 ? a.H : a.Hkv); };
   Raw<TX, W> next[4];
-  const auto load = [&](int v) {
-    if (!mine || v >= nv) return;
-    int kind, h;
-    const TX* x = source(v, kind, h);
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+#pragma unroll
+    for (int i = 0; i < W; ++i) next[c].e[i] = TX(0.f);   // lanes beyond a vector's end add nothing to its sums
+  const auto load = [&](int p) {
+    if (p >= passes) return;
+    const int kind = kind_of(p), h = head_of(p, kind);
+    if (!there_of(h, kind)) return;
+    const Vectors& s = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
+    const TX* x = static_cast<const TX*>(s.p) + (long long)tok * s.ts + h * s.hs + r0;
 #pragma unroll
     for (int c = 0; c < 4; ++c) load_raw<TX, W, VEC>(x + c * Q, next[c]);
   };
-  load(v0);
+  load(first);
 
   // ---- the token's place and angles ----
   if (CACHE) {
@@ -309,6 +292,13 @@ __global__ void __launch_bounds__(kThreads, CACHE ? 2 : 4) norm_turn_kernel(cons
     cs[j] = ok ? __ldg(a.table + p * a.rot + j) : nan;
     sn[j] = ok ? __ldg(a.table + p * a.rot + half + j) : nan;
   }
+  if (a.norm) {
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      const void* w = which ? a.wk : a.wq;
+      for (int i = tid; i < D; i += blockDim.x) weights[which][i] = w ? load_weight(w, a.w_dtype, i) : 1.f;
+    }
+  }
   __syncthreads();
   const bool put = CACHE && place.put;
   const long long slot = CACHE ? place.slot : 0;
@@ -317,24 +307,22 @@ __global__ void __launch_bounds__(kThreads, CACHE ? 2 : 4) norm_turn_kernel(cons
   float* buf32 = reinterpret_cast<float*>(exchange + (tid / 32) * (128 * W)) + lane / GP * D;
 
 #pragma unroll 1
-  for (int v = v0; v - lane / GP < nv; v += step) {
-    const bool there = mine && v < nv;
-    int kind = 0, h = 0;
-    if (there) source(v, kind, h);
+  for (int p = first; p < passes; p += step) {
+    const int kind = kind_of(p), h = head_of(p, kind);
+    const bool there = there_of(h, kind);
     Raw<TX, W> raw[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) raw[c] = next[c];
-    load(v + step);
-    // whole warps go through each part that some lane needs, since sums and maxima are shuffled
+    load(p + step);
+    // whole warps go through it, since sums and maxima are shuffled
     if constexpr (CACHE) {
-      if (__any_sync(0xffffffffu, there && kind == 1)) {
-        // ---- a key, in fp64, to its codes ----
-        const bool key = there && kind == 1;
+      if (kind == 1) {
+        // ---- keys, in fp64, to their codes ----
         double z[4][W];
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int i = 0; i < W; ++i) z[c][i] = key ? (double)to_f32(raw[c].e[i]) : 0.0;
+          for (int i = 0; i < W; ++i) z[c][i] = (double)to_f32(raw[c].e[i]);
         if (a.norm) {
           double ss = 0;
 #pragma unroll
@@ -344,17 +332,17 @@ __global__ void __launch_bounds__(kThreads, CACHE ? 2 : 4) norm_turn_kernel(cons
 #pragma unroll
           for (int o = GP / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
           const double r = 1.0 / sqrt(ss / D + (double)a.eps);
-          if (key) {
+          if (there) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               float w[W];
-              load_weights<W>(a, a.wk, c * Q + r0, w);
+              load_floats<W>(weights[1] + c * Q + r0, w);
 #pragma unroll
               for (int i = 0; i < W; ++i) z[c][i] = z[c][i] * r * (double)w[i];
             }
           }
         }
-        turn_vector<double, W>(z, key, r0, a, cs, sn, buf64);
+        turn_vector<double, W>(z, there, r0, a, cs, sn, buf64);
         uint32_t top[4], words[4] = {}, sb[4];
         float y[4][W];
 #pragma unroll
@@ -379,17 +367,18 @@ __global__ void __launch_bounds__(kThreads, CACHE ? 2 : 4) norm_turn_kernel(cons
           s = __uint_as_float(sb[c] << 16);
           const double s64 = s, inv = 1.f / s;
 #pragma unroll
-          for (int i = 0; i < W; ++i) words[i] |= (finite ? code_of(z[c][i], s64, inv) : 8u) << (4 * c);
+          for (int i = 0; i < W; ++i) words[i] |= code_of(z[c][i], s64, inv) << (4 * c);
         }
-        if (key && put) store_codes(a, slot, 1, h, r0, words, sb);
+        if (there && put) store_codes(a, slot, 1, h, r0, finite, words, sb);
+        continue;
       }
-      if (__any_sync(0xffffffffu, there && kind == 2)) {
-        // ---- a value, exact as it is, to its codes ----
+      if (kind == 2) {
+        // ---- values, exact as they are, to their codes ----
         float y[4][W];
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int i = 0; i < W; ++i) y[c][i] = there && kind == 2 ? to_f32(raw[c].e[i]) : 0.f;
+          for (int i = 0; i < W; ++i) y[c][i] = to_f32(raw[c].e[i]);
         uint32_t top[4], words[4] = {}, sb[4];
         const bool finite = quarter_tops<GP, W>(y, top) < 0x7f800000u;
 #pragma unroll
@@ -397,54 +386,57 @@ __global__ void __launch_bounds__(kThreads, CACHE ? 2 : 4) norm_turn_kernel(cons
           sb[c] = scale_bits(__fdiv_rn(__uint_as_float(top[c]), 7.5f), finite);
           const float s = __uint_as_float(sb[c] << 16), inv = 1.f / s;
 #pragma unroll
-          for (int i = 0; i < W; ++i) words[i] |= (finite ? code_of(y[c][i], s, inv) : 8u) << (4 * c);
+          for (int i = 0; i < W; ++i) words[i] |= code_of(y[c][i], s, inv) << (4 * c);
         }
-        if (there && kind == 2 && put) store_codes(a, slot, 2, h, r0, words, sb);
+        if (there && put) store_codes(a, slot, 2, h, r0, finite, words, sb);
+        continue;
       }
     }
-    const bool out = there && (kind == 0 || !CACHE);
-    if (!CACHE || __any_sync(0xffffffffu, out)) {
-      // ---- a query, or a key that stays one, to its own type ----
-      float y[4][W];
+    // ---- queries, or keys that stay ones, to their own type ----
+    float y[4][W];
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int i = 0; i < W; ++i) y[c][i] = to_f32(raw[c].e[i]);
+    if (a.norm) {
+      float ss = 0;
 #pragma unroll
       for (int c = 0; c < 4; ++c)
 #pragma unroll
-        for (int i = 0; i < W; ++i) y[c][i] = out ? to_f32(raw[c].e[i]) : 0.f;
-      if (a.norm) {
-        float ss = 0;
+        for (int i = 0; i < W; ++i) ss = fmaf(y[c][i], y[c][i], ss);
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+      for (int o = GP / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const float r = rsqrtf(fmaf(ss, a.inv_d, a.eps));
+      if (there) {
+        const float* w = weights[kind] + r0;
 #pragma unroll
-          for (int i = 0; i < W; ++i) ss = fmaf(y[c][i], y[c][i], ss);
+        for (int c = 0; c < 4; ++c) {
+          float u[W];
+          load_floats<W>(w + c * Q, u);
+          if constexpr (W > 1) {
 #pragma unroll
-        for (int o = GP / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float r = rsqrtf(ss / (float)D + a.eps);
-        if (out) {
-          const void* w = kind == 1 ? a.wk : a.wq;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            float u[W];
-            load_weights<W>(a, w, c * Q + r0, u);
-#pragma unroll
-            for (int i = 0; i < W; ++i) y[c][i] *= r * u[i];
+            for (int i = 0; i < W; i += 2)
+              unpack2(mul2(pack2(y[c][i], y[c][i + 1]), mul2(pack2(r, r), pack2(u[i], u[i + 1]))), y[c][i], y[c][i + 1]);
+          } else {
+            y[c][0] *= r * u[0];
           }
         }
       }
-      turn_vector<float, W>(y, out, r0, a, cs, sn, buf32);
-      if (out) {
-        const Out& d = kind == 0 ? a.qo : a.ko;
-        TX* o = static_cast<TX*>(d.p) + (long long)tok * d.ts + h * d.hs + r0;
+    }
+    turn_vector<float, W>(y, there, r0, a, cs, sn, buf32);
+    if (there) {
+      const Out& d = kind == 0 ? a.qo : a.ko;
+      TX* o = static_cast<TX*>(d.p) + (long long)tok * d.ts + h * d.hs + r0;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          Raw<TX, W> w;
+      for (int c = 0; c < 4; ++c) {
+        Raw<TX, W> w;
 #pragma unroll
-          for (int i = 0; i < W; ++i) w.e[i] = from_f32<TX>(y[c][i]);
-          if constexpr (VEC) {
-            *reinterpret_cast<typename Raw<TX, W>::Word*>(o + c * Q) = w.w;
-          } else {
+        for (int i = 0; i < W; ++i) w.e[i] = from_f32<TX>(y[c][i]);
+        if constexpr (VEC) {
+          *reinterpret_cast<typename Raw<TX, W>::Word*>(o + c * Q) = w.w;
+        } else {
 #pragma unroll
-            for (int i = 0; i < W; ++i) o[c * Q + i] = w.e[i];
-          }
+          for (int i = 0; i < W; ++i) o[c * Q + i] = w.e[i];
         }
       }
     }
@@ -469,12 +461,11 @@ int check_args(const HeadArgs& a, int dtype) {
 // Warps of a block and blocks of a token: a warp takes its vectors at once where the tokens are few, else 6 times in turn.
 template <typename TX, int W, bool CACHE>
 cudaError_t launch(HeadArgs& a, bool vec, cudaStream_t st) {
-  const int lanes = a.D / 4 / W, nv = a.Hkv * (CACHE ? 2 : 1) + a.H;
-  const size_t wsize = a.w_dtype == SF_F32 ? 16 : 8;
-  a.w_vec = reinterpret_cast<uintptr_t>(a.wq) % wsize == 0 && reinterpret_cast<uintptr_t>(a.wk) % wsize == 0;
+  const int lanes = a.D / 4 / W;
+  a.inv_d = 1.f / (float)a.D;
   const auto go = [&](auto gp) -> cudaError_t {
     constexpr int GP = decltype(gp)::value, AT = 32 / GP;
-    const int passes = (nv + AT - 1) / AT;
+    const int passes = (a.Hkv + AT - 1) / AT * (CACHE ? 2 : 1) + (a.H + AT - 1) / AT;
     const long long fill = 32ll * device_info().sms;   // warps
     const int rounds = (int)std::min<long long>(kRounds, std::max<long long>(1, (long long)a.T * passes / fill));
     const int warps = (passes + rounds - 1) / rounds, parts = (warps + kThreads / 32 - 1) / (kThreads / 32);

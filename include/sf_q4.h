@@ -396,9 +396,9 @@ int sf_qk_norm_rotary(const void* q, long long qts, long long qhs, void* q_out, 
 
 /* ---- a paged cache in 4 bits --------------------------------------------------------
  * The e4m3 cache's tokens, pages and rules (sf_paged_cache), with another content:
- * k_codes, v_codes uint8 [num_pages, n_kv_heads, page_size, head_dim / 2], 16-byte
- * aligned, and k_scales, v_scales bf16 [num_pages, n_kv_heads, page_size, 4], 8-byte
- * aligned, a scale for each quarter of a vector.  Element e of a vector lies in quarter
+ * k_codes, v_codes uint8 [num_pages, n_kv_heads, page_size, head_dim / 2] and k_scales,
+ * v_scales bf16 [num_pages, n_kv_heads, page_size, 4], a scale for each quarter of a
+ * vector, all 16-byte aligned.  Element e of a vector lies in quarter
  * c = e / (D / 4) at place r = e % (D / 4); its code is bits 4c .. 4c + 3 of the vector's
  * 16-bit word r (low byte first) and stands for (code - 8) * scale[c].  Scales are at
  * least 0; a vector that holds an infinity or a NaN has four NaN scales. */

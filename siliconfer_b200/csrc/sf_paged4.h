@@ -40,8 +40,8 @@ inline int check_paged4(const sf_paged4_cache* c, int T, sf_paged_cache& g) {
   if (!c) return fail(SF_ERR_NULL, "null pointer argument");
   g = geometry(*c);
   if (int rc = check_paged(&g, T)) return rc;
-  if (T > 0 && ((reinterpret_cast<uintptr_t>(c->k_scales) | reinterpret_cast<uintptr_t>(c->v_scales)) & 7))
-    return fail(SF_ERR_ALIGN, "k_scales and v_scales must be 8-byte aligned");
+  if (T > 0 && ((reinterpret_cast<uintptr_t>(c->k_scales) | reinterpret_cast<uintptr_t>(c->v_scales)) & 15))
+    return fail(SF_ERR_ALIGN, "k_scales and v_scales must be 16-byte aligned");
   return SF_OK;
 }
 

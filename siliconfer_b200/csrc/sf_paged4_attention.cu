@@ -27,6 +27,7 @@
 #include "sf_paged4.h"
 #include "sf_paged_work.h"
 #include "sf_q4_internal.h"
+#include "sf_tcgen05.h"
 
 namespace sf {
 SF_DEFINE_ERROR_READER(take_dev_error_paged4)
@@ -34,7 +35,8 @@ extern std::atomic<long long> g_launches;
 
 namespace {
 
-constexpr int kWarps = 4, kThreads = 32 * kWarps, kStages = 4, kBlock = 16;   // keys of a warp's step
+constexpr int kWarps = 4, kThreads = 32 * kWarps, kBlock = 16, kStep = 32;   // keys of an MMA, and of a warp's copy
+constexpr unsigned kErrCopy = 1u << 17;
 constexpr float kTopLog = 13.f;      // log2 of a weight times its scale, at most one above it
 
 struct Attn4Args : AttnArgs {
@@ -46,6 +48,13 @@ __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, u
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// d = a b + c, with c kept
+__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0,
+                                      float c1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+}
 __device__ __forceinline__ void mma8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
   asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -56,11 +65,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
-}
-template <int BYTES>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
-  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
 __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
@@ -80,40 +84,78 @@ __device__ __forceinline__ uint32_t codes_of(uint32_t w) {
 // the codes less 8, times 1 or 16: the lowest bits of 1024 + n or 1024 + 16 n
 template <int C>
 __device__ __forceinline__ uint32_t centred(uint32_t w) {
-  return add_half2(codes_of<C>(w) | 0x64006400u, C % 2 ? 0xe480e480u : 0xe408e408u);
+  uint32_t x;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(x) : "r"(C >= 2 ? w >> 8 : w), "r"(C % 2 ? 0x00f000f0u : 0x000f000fu), "r"(0x64006400u));
+  return add_half2(x, C % 2 ? 0xe480e480u : 0xe408e408u);
 }
 // four bf16 scales
 __device__ __forceinline__ void scales_of(uint2 u, float (&s)[4]) {
   s[0] = __uint_as_float(u.x << 16), s[1] = __uint_as_float(u.x & 0xffff0000u);
   s[2] = __uint_as_float(u.y << 16), s[3] = __uint_as_float(u.y & 0xffff0000u);
 }
+// the largest of four scales that are not negative, NaN above all numbers
+__device__ __forceinline__ float top_scale(uint2 u) {
+  const uint32_t m = __vmaxu2(u.x, u.y);
+  return __uint_as_float(max(m << 16, m & 0xffff0000u));
+}
+template <int N>
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int c = 0; c < N; c += 4) {
+      const uint4 u = *reinterpret_cast<const uint4*>(p + 4 * c);
+      w[c] = u.x, w[c + 1] = u.y, w[c + 2] = u.z, w[c + 3] = u.w;
+    }
+  } else if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int c = 0; c < N; c += 2) {
+      const uint2 u = *reinterpret_cast<const uint2*>(p + 4 * c);
+      w[c] = u.x, w[c + 1] = u.y;
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < N; ++c) w[c] = *reinterpret_cast<const uint32_t*>(p + 4 * c);
+  }
+}
 
-// A lane (g = lane / 4, t = lane % 4) reads KW words of keys g and g + 8, words t * KW .. of the vector; and of the
-// values of keys 2t, 2t + 1, 2t + 8, 2t + 9 the VW words that lane group g turns into rows of V^T.  It reads back only
-// what it copied, so the copies need no barrier.
+// A warp's copy is kStep keys as they lie in their pages: rows of D / 2 bytes of codes, and of 8 bytes of scales.  A lane
+// (g = lane / 4, t = lane % 4) reads KW words of two keys from word t * KW on, and the VW words of four values that lane
+// group g turns into rows of V^T.  An MMA's row m is the copy's row m ^ (m / 2 % 2): at D = 128 the rows that a phase of
+// loads touches lie in both halves of the banks then, for the keys' loads and for the values'.
 template <int D>
 struct Lay4 {
-  static constexpr int Q = D / 4, WORDS = D / 8, KW = WORDS / 4, VW = (WORDS + 7) / 8;
-  static constexpr int KCHUNK = KW % 4 == 0 ? 16 : KW % 2 == 0 ? 8 : 4, KCHUNKS = KW * 4 / KCHUNK;
-  static constexpr int VCHUNK = D == 96 ? 4 : VW * 4, VCHUNKS = VW * 4 / VCHUNK;
-  static constexpr uint32_t K0 = 0, V0 = 2 * KW * 128, S0 = V0 + 4 * VW * 128, STAGE = S0 + 4 * 256;
-  static constexpr uint32_t RING = kWarps * kStages * STAGE, JOIN = kWarps * 8 * (D + 4) * 4;
+  static constexpr int Q = D / 4, WORDS = D / 8, ROW = D / 2, KW = WORDS / 4, VW = (WORDS + 7) / 8;
+  static constexpr int STAGES = D == 64 ? 3 : 2;
+  static constexpr uint32_t K0 = 0, V0 = kStep * ROW, KS0 = 2 * V0, VS0 = KS0 + kStep * 8, STAGE = VS0 + kStep * 8;
+  static constexpr uint32_t RING = kWarps * STAGES * STAGE, JOIN = kWarps * 8 * (D + 4) * 4;
   static constexpr uint32_t INFO = RING > JOIN ? RING : JOIN;
   static constexpr size_t smem(int batch) { return INFO + (size_t)batch * sizeof(SeqInfo); }
-  // first element of a lane group's pair of places: word of set s
+  // the word that lane group g holds in set s
   __device__ static __forceinline__ int word(int s, int g) { return D == 96 ? 8 * s + g : g * VW + s; }
 };
 
 template <int D, int QP, int PP>
-__global__ void __launch_bounds__(kThreads, D <= 128 ? 4 : 2) paged4_attention_kernel(const Attn4Args a, int q_pairs) {
+#ifndef MINB
+#define MINB 4
+#endif
+__global__ void __launch_bounds__(kThreads, D <= 128 ? MINB : 2) paged4_attention_kernel(const __grid_constant__ Attn4Args a, int q_pairs) {
   using L = Lay4<D>;
-  constexpr int RT = 8, KW = L::KW, VW = L::VW, Q = L::Q;
+  constexpr int RT = 8, KW = L::KW, VW = L::VW, Q = L::Q, ST = L::STAGES;
   constexpr bool FINE = PP == 2;   // keys' codes less 8, as the values'
-  extern __shared__ __align__(16) uint8_t mem[];
+  extern __shared__ __align__(128) uint8_t mem[];
   __shared__ long long wsum[kWarps];
   __shared__ float wm[kWarps][RT], wl[kWarps][RT];
+  __shared__ __align__(8) uint64_t bars[kWarps][ST];
+  __shared__ int abort_word;
+  volatile int* abort_flag = &abort_word;
   SeqInfo* info = reinterpret_cast<SeqInfo*>(mem + L::INFO);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);
+  if (threadIdx.x == 0) {
+    for (int w = 0; w < kWarps; ++w)
+      for (int i = 0; i < ST; ++i) bar_init(smem_u32(&bars[w][i]), 1);
+    abort_word = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
   griddep_wait();
 
   // ---- the batch's units, and this CTA's share ----
@@ -176,57 +218,62 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 4 : 2) paged4_attention_k
     }
   }
 
+  // This lane's copy: keys' codes, values' codes, keys' scales or values' scales (lane % 4) of box lane / 4 of a step.
+  const int box = min(page_size, kStep), boxes = kStep / box, my_box = lane >> 2;
+  const uint32_t row_bytes = t < 2 ? L::ROW : 8, page_bytes = (uint32_t)(Hkv * page_size) * row_bytes;
+  const uint8_t* const src = t == 0   ? a.c.k_codes
+                             : t == 1 ? a.c.v_codes
+                                      : reinterpret_cast<const uint8_t*>(t == 2 ? a.ks : a.vs);
+  const uint32_t ring = smem_u32(mem) + warp * ST * L::STAGE, bar0 = smem_u32(&bars[warp][0]),
+                 dst = ring + (t == 0 ? L::K0 : t == 1 ? L::V0 : t == 2 ? L::KS0 : L::VS0) + my_box * box * row_bytes;
+  const uint32_t k_row = (g ^ (g >> 1 & 1)) * L::ROW + t * KW * 4, s_row = (g ^ (g >> 1 & 1)) * 8;
+  uint32_t slot = 0, phase = 0;   // of this warp's next step
+  bool ok = true;
+
   while (u < u_end) {
     const Part p = part_at<RT>(a, info, u, u_end, b);
-    const int blocks = p.tb > p.ta ? (p.tb - p.ta + kBlock - 1) / kBlock : 0;   // of all warps
-    const int mine = blocks > warp ? (blocks - warp - 1) / kWarps + 1 : 0;
+    // ---- copies: this warp takes the steps at p.ta + kStep * (warp + kWarps * i) ----
     const int* pages = a.c.block_table + (size_t)p.b * a.c.pages_per_seq;
-    // ---- copies: this warp's block i is the part's block warp + kWarps * i ----
-    const auto key_of = [&](int i) { return p.ta + kBlock * (warp + kWarps * i); };
-    // Page of a block, -1 where it has none; a page that ends before the first key in sight may have been given up.
-    const auto page_of = [&](int i) {
-      const int k0 = key_of(i);
-      if (i >= mine || k0 + kBlock <= p.tile_lo) return -1;
-      const int page = __ldg(pages + (k0 >> a.lg_page));
-      if (page >= 0 && page < a.c.num_pages) return page;
-      atomicOr(&g_dev_error, kErrIndex);
-      return -1;
-    };
-    int page_l = page_of(lane);            // lane i's: block i of the current 32
-    uint32_t there = 0;                    // bit i % 32: the block has a page
-    const uint32_t ring = smem_u32(mem) + warp * kStages * L::STAGE;
-    const auto copy = [&](int i) {
-      if (i < mine) {
-        if (i % 32 == 0 && i > 0) page_l = page_of(i + lane);
-        const int page = __shfl_sync(0xffffffffu, page_l, i % 32);
-        there = (there & ~(1u << (i % 32))) | (page >= 0 ? 1u << (i % 32) : 0u);
-        if (page >= 0) {
-          const size_t vec = ((size_t)page * Hkv + p.kvh) * page_size + (key_of(i) & (page_size - 1));
-          const uint32_t st = ring + (i % kStages) * L::STAGE;
-          const uint8_t* kc = a.c.k_codes + (vec + g) * (D / 2) + t * KW * 4;
-          const uint8_t* vc = a.c.v_codes + (vec + 2 * t) * (D / 2);
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-#pragma unroll
-            for (int c = 0; c < L::KCHUNKS; ++c)
-              copy_async<L::KCHUNK>(st + L::K0 + (r * L::KCHUNKS + c) * (32 * L::KCHUNK) + lane * L::KCHUNK,
-                                    kc + r * 8 * (D / 2) + c * L::KCHUNK);
-            copy_async<8>(st + L::S0 + r * 256 + lane * 8, a.ks + (vec + g + 8 * r) * 4);
-            copy_async<8>(st + L::S0 + (2 + r) * 256 + lane * 8, a.vs + (vec + g + 8 * r) * 4);
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int c = 0; c < L::VCHUNKS; ++c)
-              if (L::word(c * (L::VCHUNK / 4), g) < L::WORDS)
-                copy_async<L::VCHUNK>(st + L::V0 + (e * L::VCHUNKS + c) * (32 * L::VCHUNK) + lane * L::VCHUNK,
-                                      vc + ((e & 1) + (e >> 1) * 8) * (D / 2) + 4 * L::word(c * (L::VCHUNK / 4), g));
+    const uint32_t head = (uint32_t)(p.kvh * page_size);
+    int copy_key = p.ta + kStep * warp + my_box * box;   // first key of this lane's box of the next copy
+    // Page of the box at `key`, -1 where there is none; a page that ends before the first key in sight may have been given up.
+    const auto page_of = [&](int key) {
+      int page = -1;
+      if (my_box < boxes && key < p.tb && key + box > p.tile_lo) {
+        page = __ldg(pages + (key >> a.lg_page));
+        if ((unsigned)page >= (unsigned)a.c.num_pages) {
+          if (t == 0) atomicOr(&g_dev_error, kErrIndex);
+          page = -1;
         }
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
+      return page;
     };
+    int page = page_of(copy_key);
+    uint32_t there = 0;   // bits 2 s and 2 s + 1: the halves of the step in slot s that have a page
+    const auto copy = [&](uint32_t s) {
+      if (copy_key - my_box * box >= p.tb) return;
+      const int now = page, key = copy_key;
+      copy_key += kStep * kWarps;
+      page = page_of(copy_key);
+      const unsigned have = __ballot_sync(0xffffffffu, now >= 0);
+      there = (there & ~(3u << (2 * s))) | (boxes == 1 ? (have & 1) * 3 : (have & 1) | (have >> 3 & 2)) << (2 * s);
+      if (lane == 0) bar_expect_tx(bar0 + 8 * s, __popc(have) / 4 * box * (uint32_t)(D + 16));
+      __syncwarp();
+      if (now >= 0) {
+        const uint8_t* from = src + (unsigned long long)(unsigned)now * page_bytes + (head + (key & (page_size - 1))) * row_bytes;
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst + s * L::STAGE),
+                     "l"(from), "r"(box * row_bytes), "r"(bar0 + 8 * s)
+                     : "memory");
+      }
+    };
+    if (ok) {
+      uint32_t s = slot;
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) copy(i);
+      for (int i = 0; i < ST; ++i) {
+        copy(s);
+        s = s + 1 == ST ? 0 : s + 1;
+      }
+    }
 
     // ---- query fragments: column g's elements of this lane's words ----
     uint32_t qf[4][KW][QP];
@@ -291,9 +338,11 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 4 : 2) paged4_attention_k
       for (int e = 0; e < 2; ++e) f[e] = __shfl_sync(0xffffffffu, f_row, (2 * t + e) * 4);
     }
 
-    float nm[2] = {0.f, 0.f}, l[2] = {0.f, 0.f};   // minus the reference, and the sum, of columns 2t and 2t + 1
-    bool fresh[2] = {true, true};                  // no key yet
-    float o[VW][4][4];                             // sums: rows 2 * word (+ 1) of quarter c, columns 2t, 2t + 1
+    float nm[2] = {0.f, 0.f};   // minus the reference of columns 2t and 2t + 1
+    float l[2] = {0.f, 0.f};    // their sums
+    bool fresh = true;          // the warp has rows without a reference
+    bool none[2] = {true, true};   // no key yet
+    float o[VW][4][4];          // sums: rows 2 * word (+ 1) of quarter c, columns 2t, 2t + 1
 #pragma unroll
     for (int s = 0; s < VW; ++s)
 #pragma unroll
@@ -301,80 +350,72 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 4 : 2) paged4_attention_k
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[s][c][e] = 0.f;
 
-    for (int i = 0; i < mine; ++i) {
-      copy(i + kStages - 1);
-      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
-      if (!(there >> (i % 32) & 1)) continue;
-      const int k0 = key_of(i);
-      const uint8_t* st = mem + (warp * kStages + i % kStages) * L::STAGE;
+    // 16 keys from k0 on; edge: not every row sees all of them
+    const auto block = [&](auto edge, const uint8_t* codes_at, const uint8_t* scales_at, int k0) {
+      constexpr bool EDGE = decltype(edge)::value;
       // ---- scores ----
-      float y[4] = {0.f, 0.f, 0.f, 0.f};           // keys g, g, g + 8, g + 8; columns 2t, 2t + 1
+      float y[4];                                  // keys g, g, g + 8, g + 8 (in the copy's order); columns 2t, 2t + 1
       {
         uint32_t w[2][KW];
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-          for (int c = 0; c < L::KCHUNKS; ++c) {
-            const uint8_t* at = st + L::K0 + (r * L::KCHUNKS + c) * (32 * L::KCHUNK) + lane * L::KCHUNK;
-            if constexpr (L::KCHUNK == 16) *reinterpret_cast<uint4*>(&w[r][4 * c]) = *reinterpret_cast<const uint4*>(at);
-            else if constexpr (L::KCHUNK == 8) *reinterpret_cast<uint2*>(&w[r][2 * c]) = *reinterpret_cast<const uint2*>(at);
-            else w[r][c] = *reinterpret_cast<const uint32_t*>(at);
-          }
+        for (int r = 0; r < 2; ++r) load_words<KW>(codes_at + L::K0 + k_row + r * 8 * L::ROW, w[r]);
         float ks[2][4];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) scales_of(*reinterpret_cast<const uint2*>(st + L::S0 + r * 256 + lane * 8), ks[r]);
+        for (int r = 0; r < 2; ++r) scales_of(*reinterpret_cast<const uint2*>(scales_at + L::KS0 + s_row + r * 64), ks[r]);
         const auto quarter = [&](auto cc) {
           constexpr int C = decltype(cc)::value;
-          float s[4] = {init[C][0], init[C][1], init[C][0], init[C][1]};
+          float s[4];
           const auto codes = [&](uint32_t x) { return FINE ? centred<C>(x) : codes_of<C>(x); };
 #pragma unroll
           for (int j = 0; j + 1 < KW; j += 2) {
             const uint32_t a0 = codes(w[0][j]), a1 = codes(w[1][j]), a2 = codes(w[0][j + 1]), a3 = codes(w[1][j + 1]);
 #pragma unroll
-            for (int part = 0; part < QP; ++part) mma16(s, a0, a1, a2, a3, qf[C][j][part], qf[C][j + 1][part]);
+            for (int part = 0; part < QP; ++part) {
+              if (j + part == 0) mma16(s, a0, a1, a2, a3, qf[C][j][part], qf[C][j + 1][part], init[C][0], init[C][1]);
+              else mma16(s, a0, a1, a2, a3, qf[C][j][part], qf[C][j + 1][part]);
+            }
           }
           if constexpr (KW % 2) {
 #pragma unroll
-            for (int part = 0; part < QP; ++part)
-              mma8(s, codes(w[0][KW - 1]), codes(w[1][KW - 1]), qf[C][KW - 1][part]);
+            for (int part = 0; part < QP; ++part) mma8(s, codes(w[0][KW - 1]), codes(w[1][KW - 1]), qf[C][KW - 1][part]);
           }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y[e] = fmaf(s[e], ks[e >> 1][C], y[e]);
+          for (int e = 0; e < 4; ++e) y[e] = C == 0 ? s[e] * ks[e >> 1][C] : fmaf(s[e], ks[e >> 1][C], y[e]);
         };
         quarter(std::integral_constant<int, 0>());
         quarter(std::integral_constant<int, 1>());
         quarter(std::integral_constant<int, 2>());
         quarter(std::integral_constant<int, 3>());
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = fmaf(y[e], f[e & 1], nm[e & 1]);
       float vs[2][4], lv[2];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        scales_of(*reinterpret_cast<const uint2*>(st + L::S0 + (2 + r) * 256 + lane * 8), vs[r]);
-        lv[r] = fmaxf(lg2(fmaxf(fmaxf(vs[r][0], vs[r][1]), fmaxf(vs[r][2], vs[r][3]))), -60.f);
+        const uint2 u = *reinterpret_cast<const uint2*>(scales_at + L::VS0 + s_row + r * 64);
+        scales_of(u, vs[r]);
+        lv[r] = fmaxf(lg2(top_scale(u)), -60.f);
       }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = fmaf(y[e], f[e & 1], nm[e & 1]);
-      const bool alike = k0 >= p.all_lo && k0 + kBlock <= min(p.all_hi, p.tb);   // every row sees all of these keys
       bool hidden[4] = {false, false, false, false};
-      if (!alike) {
+      if constexpr (EDGE) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int key = k0 + g + 8 * (e >> 1), pos = p.pos0 + (p.row0 + 2 * t + (e & 1)) / a.G;
+          const int key = k0 + (g ^ (g >> 1 & 1)) + 8 * (e >> 1), pos = p.pos0 + (p.row0 + 2 * t + (e & 1)) / a.G;
           hidden[e] = key >= p.tb || key > pos || (a.window > 0 && key <= pos - a.window);
           if (hidden[e]) y[e] = -INFINITY;
         }
       }
       // ---- the reference, if a key exceeds it by more than a factor of 2 ----
       const float over = fmaxf(fmaxf(y[0], y[1]) + lv[0], fmaxf(y[2], y[3]) + lv[1]);
-      if (__any_sync(0xffffffffu, over > kTopLog + 1.f || fresh[0] || fresh[1])) {
+      if (__any_sync(0xffffffffu, over > kTopLog + 1.f) || fresh) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float top = fmaxf(y[e] + lv[0], y[e + 2] + lv[1]);
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-          if (fresh[e] && top == -INFINITY) continue;   // the row has seen no key
-          const float up = fresh[e] ? top - kTopLog : fmaxf(top - kTopLog, 0.f), c = fresh[e] ? 1.f : ex2(-up);
-          fresh[e] = false;
+          if (none[e] && top == -INFINITY) continue;   // the row has seen no key
+          const float up = none[e] ? top - kTopLog : fmaxf(top - kTopLog, 0.f), c = none[e] ? 1.f : ex2(-up);
+          none[e] = false;
           nm[e] -= up;
           y[e] -= up;
           y[e + 2] -= up;
@@ -387,6 +428,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 4 : 2) paged4_attention_k
               o[s][q][e + 2] *= c;
             }
         }
+        fresh = __any_sync(0xffffffffu, none[0] || none[1]);
       }
       // ---- weights, times each quarter's scale, as the second operand ----
       float pw[4];
@@ -400,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 4 : 2) paged4_attention_k
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           float x = pw[2 * r] * vs[r][c], z = pw[2 * r + 1] * vs[r][c];
-          if (!alike) {   // 0 times a NaN scale is not 0
+          if constexpr (EDGE) {   // 0 times a NaN scale is not 0
             if (hidden[2 * r]) x = 0.f;
             if (hidden[2 * r + 1]) z = 0.f;
           }
@@ -408,22 +450,25 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 4 : 2) paged4_attention_k
           for (int part = 0; part < PP; ++part) {
             const uint32_t h = half2_bits(x, z);
             pf[c][part][r] = transpose8(h);
-            const float2 w = half2_floats(h);
-            x -= w.x;
-            z -= w.y;
+            if (part + 1 < PP) {
+              const float2 w = half2_floats(h);
+              x -= w.x;
+              z -= w.y;
+            }
           }
         }
-      // ---- sums ----
+      // ---- sums: row m of the scores, and so of the weights, is the copy's row m ^ (m / 2 % 2) ----
       uint32_t w[4][VW];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-#pragma unroll
-        for (int c = 0; c < L::VCHUNKS; ++c) {
-          const uint8_t* at = st + L::V0 + (e * L::VCHUNKS + c) * (32 * L::VCHUNK) + lane * L::VCHUNK;
-          if constexpr (L::VCHUNK == 16) *reinterpret_cast<uint4*>(&w[e][4 * c]) = *reinterpret_cast<const uint4*>(at);
-          else if constexpr (L::VCHUNK == 8) *reinterpret_cast<uint2*>(&w[e][2 * c]) = *reinterpret_cast<const uint2*>(at);
-          else w[e][c] = *reinterpret_cast<const uint32_t*>(at);
+      for (int e = 0; e < 4; ++e) {
+        const uint8_t* row = codes_at + L::V0 + (((2 * t + (e & 1)) ^ (t & 1)) + (e >> 1) * 8) * L::ROW;
+        if constexpr (D == 96) {
+          w[e][0] = *reinterpret_cast<const uint32_t*>(row + 4 * g);
+          w[e][1] = g < 4 ? *reinterpret_cast<const uint32_t*>(row + 32 + 4 * g) : 0u;
+        } else {
+          load_words<VW>(row + 4 * VW * g, w[e]);
         }
+      }
 #pragma unroll
       for (int s = 0; s < VW; ++s) {
         // both tokens' half-words of a place side by side
@@ -440,8 +485,27 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 4 : 2) paged4_attention_k
         quarter(std::integral_constant<int, 2>());
         quarter(std::integral_constant<int, 3>());
       }
+    };
+
+    const int whole_lo = p.all_lo, whole_hi = min(p.all_hi, p.tb) - kBlock;
+#pragma unroll 1
+    for (int k0 = p.ta + kStep * warp; k0 < p.tb; k0 += kStep * kWarps) {
+      ok = ok && __all_sync(0xffffffffu, bar_wait(bar0 + 8 * slot, phase, kErrCopy, abort_flag));
+      if (!ok) break;
+      const uint32_t have = there >> (2 * slot);
+      const uint8_t* st = mem + (warp * ST + slot) * L::STAGE;
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
+        const int k = k0 + kBlock * half;
+        if (!(have >> half & 1) || k >= p.tb) continue;
+        const uint8_t *codes = st + half * (kBlock * L::ROW), *scales = st + half * (kBlock * 8);
+        if (k >= whole_lo && k <= whole_hi) block(std::false_type(), codes, scales, k);
+        else block(std::true_type(), codes, scales, k);
+      }
+      __syncwarp();   // the step's rows have been read
+      copy(slot);
+      if (++slot == ST) slot = 0, phase ^= 1;
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
 
     // ---- the warps' parts ----
 #pragma unroll
@@ -449,7 +513,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 4 : 2) paged4_attention_k
 #pragma unroll
       for (int x = 4; x < 32; x <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], x);
       if (g == 0) {
-        wm[warp][2 * t + e] = fresh[e] ? kNone : -nm[e];
+        wm[warp][2 * t + e] = none[e] ? kNone : -nm[e];
         wl[warp][2 * t + e] = l[e];
       }
     }
@@ -505,8 +569,16 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? 4 : 2) paged4_attention_k
       dsc[3] = p.row0;
       dsc[4] = p.last_row;
     }
-    __syncthreads();   // the join's place is the next part's rings
+    // the join's place is the next part's rings, which copies write
+    fence_async_smem();
+    __syncthreads();
     u = p.u1;
+  }
+  // after an expired wait the copies under way are not counted any more: give them time
+  if (!ok) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < kWaitCycles / 64) {
+    }
   }
   griddep_launch_dependents();   // not before: the merge's blocks would wait in the place of the next call's
 }
@@ -522,7 +594,7 @@ int launch4(Attn4Args a, cudaStream_t st) {
   cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::smem(kMaxBatch));
   if (e != cudaSuccess) return cuda_fail(e, "paged4_attention_kernel shared memory");
   int per_sm = (int)(228 * 1024 / (smem + 2048));
-  const int most = D <= 128 ? 4 : 2;
+  const int most = D <= 128 ? MINB : 2;
   if (per_sm > most) per_sm = most;
   if (per_sm < 1) per_sm = 1;
   // no more CTAs than units there may be
@@ -588,6 +660,8 @@ int sf_paged4_attention(const sf_paged4_cache* cache, const void* q, int q_dtype
   a.lg_page = __builtin_ctz((unsigned)cache->page_size);
   a.scale = scale;
   if ((long long)T * a.G > 0x7fffffffll) return fail(SF_ERR_UNSUPPORTED, "too many query rows");
+  if ((long long)cache->n_kv_heads * cache->page_size * D > 0x7fffffffll)
+    return fail(SF_ERR_UNSUPPORTED, "a page of all kv heads has more than 2^31 - 1 elements");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool fine = std::min(q_dtype, out_dtype) != SF_BF16;   // the finer of the types
   const auto go = [&](auto d) {

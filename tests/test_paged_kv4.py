@@ -700,7 +700,7 @@ def test_validation_without_gpu():
     for call in (att, app):
         for c, want in ((dict(page_size=8), 6), (dict(page_size=48), 6), (dict(page_size=512), 6), (dict(head_dim=80), 6),
                         (dict(head_dim=32), 6), (dict(batch=0), 2), (dict(batch=5000), 6), (dict(num_pages=0), 2), (dict(n_kv_heads=0), 2),
-                        (dict(pages_per_seq=0), 2), (dict(pages_per_seq=2 ** 27), 2), (dict(k_codes=F + 8), 4), (dict(k_scales=F + 4), 4),
+                        (dict(pages_per_seq=0), 2), (dict(pages_per_seq=2 ** 27), 2), (dict(k_codes=F + 8), 4), (dict(k_scales=F + 8), 4),
                         (dict(v_scales=F + 2), 4), (dict(k_codes=None), 1), (dict(v_scales=None), 1), (dict(block_table=None), 1),
                         (dict(batch=2), 2)):
             assert call(cache(**c)) == want, c

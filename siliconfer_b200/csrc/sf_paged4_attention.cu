@@ -48,12 +48,10 @@ __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, u
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// d = a b + c, with c kept
-__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0,
-                                      float c1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+__device__ __forceinline__ void mma16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void mma8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
   asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
@@ -81,11 +79,11 @@ template <int C>
 __device__ __forceinline__ uint32_t codes_of(uint32_t w) {
   return (C >= 2 ? w >> 8 : w) & (C % 2 ? 0x00f000f0u : 0x000f000fu);
 }
-// the codes less 8, times 1 or 16: the lowest bits of 1024 + n or 1024 + 16 n
+// the codes less 8, times 1 or 16: the lowest bits of 1024 + n or 1024 + 16 n; magic is 0x64006400, in a register
 template <int C>
-__device__ __forceinline__ uint32_t centred(uint32_t w) {
+__device__ __forceinline__ uint32_t centred(uint32_t w, uint32_t magic) {
   uint32_t x;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(x) : "r"(C >= 2 ? w >> 8 : w), "r"(C % 2 ? 0x00f000f0u : 0x000f000fu), "r"(0x64006400u));
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(x) : "r"(C >= 2 ? w >> 8 : w), "n"(C % 2 ? 0x00f000f0u : 0x000f000fu), "r"(magic));
   return add_half2(x, C % 2 ? 0xe480e480u : 0xe408e408u);
 }
 // four bf16 scales
@@ -147,6 +145,9 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? MINB : 2) paged4_attentio
   __shared__ float wm[kWarps][RT], wl[kWarps][RT];
   __shared__ __align__(8) uint64_t bars[kWarps][ST];
   __shared__ int abort_word;
+  __shared__ __align__(16) uint32_t q_sm[4][QP][32 * KW];   // queries: lane's words of quarter c, part
+  __shared__ __align__(8) float less8[4][RT];               // -8 times the sum of the quarter's queries
+  __shared__ uint32_t row_top[kWarps][RT];
   volatile int* abort_flag = &abort_word;
   SeqInfo* info = reinterpret_cast<SeqInfo*>(mem + L::INFO);
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);
@@ -228,6 +229,8 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? MINB : 2) paged4_attentio
                  dst = ring + (t == 0 ? L::K0 : t == 1 ? L::V0 : t == 2 ? L::KS0 : L::VS0) + my_box * box * row_bytes;
   const uint32_t k_row = (g ^ (g >> 1 & 1)) * L::ROW + t * KW * 4, s_row = (g ^ (g >> 1 & 1)) * 8;
   uint32_t slot = 0, phase = 0;   // of this warp's next step
+  uint32_t magic;
+  asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));
   bool ok = true;
 
   while (u < u_end) {
@@ -275,67 +278,66 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? MINB : 2) paged4_attentio
       }
     }
 
-    // ---- query fragments: column g's elements of this lane's words ----
-    uint32_t qf[4][KW][QP];
-    float f[2], init[4][2];
+    // ---- queries: warp c cuts quarter c of the 8 rows into the second operand's registers, for all warps ----
+    static_assert(kWarps == 4, "a quarter for each warp");
+    float f[2];
     {
       const int row = p.row0 + g;
       const bool real = row <= p.last_row;
-      const long long qo = (long long)(p.r_first + row / a.G) * a.qts + (long long)(p.kvh * a.G + row % a.G) * a.qhs + 2 * t * KW;
-      float v[4][2 * KW];
+      const long long qo = (long long)(p.r_first + row / a.G) * a.qts + (long long)(p.kvh * a.G + row % a.G) * a.qhs + warp * Q + 2 * t * KW;
+      float v[2 * KW];
       uint32_t top = 0;
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int e = 0; e < 2 * KW; e += 2) {
-          const long long at = qo + c * Q + e;
-          if (!real) {
-            v[c][e] = v[c][e + 1] = 0.f;
-          } else if (q_pairs && a.q_dtype == SF_BF16) {
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const __nv_bfloat16*>(a.q) + at);
-            v[c][e] = __uint_as_float(w << 16);
-            v[c][e + 1] = __uint_as_float(w & 0xffff0000u);
-          } else if (q_pairs && a.q_dtype == SF_F16) {
-            const float2 w = half2_floats(*reinterpret_cast<const uint32_t*>(static_cast<const __half*>(a.q) + at));
-            v[c][e] = w.x;
-            v[c][e + 1] = w.y;
-          } else {
-            v[c][e] = load_q(a, at);
-            v[c][e + 1] = load_q(a, at + 1);
-          }
-          top = max(top, max(__float_as_uint(v[c][e]) & 0x7fffffffu, __float_as_uint(v[c][e + 1]) & 0x7fffffffu));
+      for (int e = 0; e < 2 * KW; e += 2) {
+        if (!real) {
+          v[e] = v[e + 1] = 0.f;
+        } else if (q_pairs && a.q_dtype == SF_BF16) {
+          const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const __nv_bfloat16*>(a.q) + qo + e);
+          v[e] = __uint_as_float(w << 16);
+          v[e + 1] = __uint_as_float(w & 0xffff0000u);
+        } else if (q_pairs && a.q_dtype == SF_F16) {
+          const float2 w = half2_floats(*reinterpret_cast<const uint32_t*>(static_cast<const __half*>(a.q) + qo + e));
+          v[e] = w.x;
+          v[e + 1] = w.y;
+        } else {
+          v[e] = load_q(a, qo + e);
+          v[e + 1] = load_q(a, qo + e + 1);
         }
+        top = max(top, max(__float_as_uint(v[e]) & 0x7fffffffu, __float_as_uint(v[e + 1]) & 0x7fffffffu));
+      }
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      if (t == 0) row_top[warp][g] = top;
+      __syncthreads();
+      const auto top_of = [&](int r) { return max(max(row_top[0][r], row_top[1][r]), max(row_top[2][r], row_top[3][r])); };
       // the row's largest value to [2^13, 2^14) by a power of two
-      const int ex = min(max((int)(top >> 23) - 140, -126), 113);
-      const float down = __int_as_float((127 - ex) << 23);
-      // an infinity or a NaN: the row is NaN
-      const float f_row = top >= 0x7f800000u ? __int_as_float(0x7fffffff)
-                                             : __int_as_float((127 + ex) << 23) * (a.scale * kLog2e) * (FINE ? 1.f : 0x1p24f);
+      const auto exponent = [](uint32_t x) { return min(max((int)(x >> 23) - 140, -126), 113); };
+      const float down = __int_as_float((127 - exponent(top_of(g))) << 23) * (warp % 2 ? 0.0625f : 1.f);   // odd quarters' codes lie four bits higher
+      float sum = 0.f;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float sum = 0.f;
+      for (int i = 0; i < KW; ++i) {
+        float x = v[2 * i] * down, y = v[2 * i + 1] * down;
 #pragma unroll
-        for (int i = 0; i < KW; ++i) {
-          // the codes of odd quarters lie four bits higher
-          float x = v[c][2 * i] * down * (c % 2 ? 0.0625f : 1.f), y = v[c][2 * i + 1] * down * (c % 2 ? 0.0625f : 1.f);
-#pragma unroll
-          for (int part = 0; part < QP; ++part) {
-            qf[c][i][part] = half2_bits(x, y);
-            const float2 h = half2_floats(qf[c][i][part]);
-            sum += h.x + h.y;
-            x -= h.x;
-            y -= h.y;
-          }
+        for (int part = 0; part < QP; ++part) {
+          const uint32_t w = half2_bits(x, y);
+          const float2 h = half2_floats(w);
+          q_sm[warp][part][lane * KW + i] = w;
+          sum += h.x + h.y;
+          x -= h.x;
+          y -= h.y;
         }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) init[c][e] = FINE ? 0.f : __shfl_sync(0xffffffffu, sum, (2 * t + e) * 4) * (c % 2 ? -0x1p-17f : -0x1p-21f);
       }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      if (!FINE && t == 0) less8[warp][g] = sum * (warp % 2 ? -0x1p-17f : -0x1p-21f);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) f[e] = __shfl_sync(0xffffffffu, f_row, (2 * t + e) * 4);
+      for (int e = 0; e < 2; ++e) {
+        // an infinity or a NaN: the row is NaN
+        const uint32_t x = top_of(2 * t + e);
+        f[e] = x >= 0x7f800000u ? __int_as_float(0x7fffffff)
+                                : __int_as_float((127 + exponent(x)) << 23) * (a.scale * kLog2e) * (FINE ? 1.f : 0x1p24f);
+      }
+      __syncthreads();
     }
 
     float nm[2] = {0.f, 0.f};   // minus the reference of columns 2t and 2t + 1
@@ -365,19 +367,28 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? MINB : 2) paged4_attentio
         const auto quarter = [&](auto cc) {
           constexpr int C = decltype(cc)::value;
           float s[4];
-          const auto codes = [&](uint32_t x) { return FINE ? centred<C>(x) : codes_of<C>(x); };
+          uint32_t q[QP][KW];
+#pragma unroll
+          for (int part = 0; part < QP; ++part) load_words<KW>(reinterpret_cast<const uint8_t*>(&q_sm[C][part][lane * KW]), q[part]);
+          const auto codes = [&](uint32_t x) { return FINE ? centred<C>(x, magic) : codes_of<C>(x); };
 #pragma unroll
           for (int j = 0; j + 1 < KW; j += 2) {
             const uint32_t a0 = codes(w[0][j]), a1 = codes(w[1][j]), a2 = codes(w[0][j + 1]), a3 = codes(w[1][j + 1]);
 #pragma unroll
             for (int part = 0; part < QP; ++part) {
-              if (j + part == 0) mma16(s, a0, a1, a2, a3, qf[C][j][part], qf[C][j + 1][part], init[C][0], init[C][1]);
-              else mma16(s, a0, a1, a2, a3, qf[C][j][part], qf[C][j + 1][part]);
+              if (j + part == 0) mma16_first(s, a0, a1, a2, a3, q[part][j], q[part][j + 1]);
+              else mma16(s, a0, a1, a2, a3, q[part][j], q[part][j + 1]);
             }
           }
           if constexpr (KW % 2) {
 #pragma unroll
-            for (int part = 0; part < QP; ++part) mma8(s, codes(w[0][KW - 1]), codes(w[1][KW - 1]), qf[C][KW - 1][part]);
+            for (int part = 0; part < QP; ++part) mma8(s, codes(w[0][KW - 1]), codes(w[1][KW - 1]), q[part][KW - 1]);
+          }
+          if constexpr (!FINE) {
+            const float2 less = *reinterpret_cast<const float2*>(&less8[C][2 * t]);
+            const uint64_t l2 = pack2(less.x, less.y);
+            unpack2(add2(pack2(s[0], s[1]), l2), s[0], s[1]);
+            unpack2(add2(pack2(s[2], s[3]), l2), s[2], s[3]);
           }
 #pragma unroll
           for (int e = 0; e < 4; ++e) y[e] = C == 0 ? s[e] * ks[e >> 1][C] : fmaf(s[e], ks[e >> 1][C], y[e]);
@@ -476,7 +487,8 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? MINB : 2) paged4_attentio
                        lo1 = __byte_perm(w[2][s], w[3][s], 0x5410), hi1 = __byte_perm(w[2][s], w[3][s], 0x7632);
         const auto quarter = [&](auto cc) {
           constexpr int C = decltype(cc)::value;
-          const uint32_t a0 = centred<C>(lo0), a1 = centred<C>(hi0), a2 = centred<C>(lo1), a3 = centred<C>(hi1);
+          const uint32_t a0 = centred<C>(lo0, magic), a1 = centred<C>(hi0, magic), a2 = centred<C>(lo1, magic),
+                         a3 = centred<C>(hi1, magic);
 #pragma unroll
           for (int part = 0; part < PP; ++part) mma16(o[s][C], a0, a1, a2, a3, pf[C][part][0], pf[C][part][1]);
         };
@@ -590,10 +602,10 @@ int launch4(Attn4Args a, cudaStream_t st) {
   auto* fn = paged4_attention_kernel<D, QP, PP>;
   const size_t smem = L::smem(c.batch);
   // the limit is the process's: the same for calls of every batch, or another thread's could lower it before this launch
-  static_assert(L::smem(kMaxBatch) + 2048 <= kBlockSmem, "shared memory plan");
+  static_assert(L::smem(kMaxBatch) + 4 * QP * 128 * L::KW + 2048 <= kBlockSmem, "shared memory plan");
   cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::smem(kMaxBatch));
   if (e != cudaSuccess) return cuda_fail(e, "paged4_attention_kernel shared memory");
-  int per_sm = (int)(228 * 1024 / (smem + 2048));
+  int per_sm = (int)(228 * 1024 / (smem + 4 * QP * 128 * L::KW + 2048));
   const int most = D <= 128 ? MINB : 2;
   if (per_sm > most) per_sm = most;
   if (per_sm < 1) per_sm = 1;

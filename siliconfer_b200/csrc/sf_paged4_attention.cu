@@ -134,7 +134,7 @@ struct Lay4 {
 
 template <int D, int QP, int PP>
 #ifndef MINB
-#define MINB 4
+#define MINB 3
 #endif
 __global__ void __launch_bounds__(kThreads, D <= 128 ? MINB : 2) paged4_attention_kernel(const __grid_constant__ Attn4Args a, int q_pairs) {
   using L = Lay4<D>;
@@ -352,18 +352,20 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? MINB : 2) paged4_attentio
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[s][c][e] = 0.f;
 
-    // 16 keys from k0 on; edge: not every row sees all of them
-    const auto block = [&](auto edge, const uint8_t* codes_at, const uint8_t* scales_at, int k0) {
+    // NB times 16 keys from k0 on; edge: not every row sees all of them
+    const auto block = [&](auto edge, auto nb, const uint8_t* codes_at, const uint8_t* scales_at, int k0) {
       constexpr bool EDGE = decltype(edge)::value;
+      constexpr int NB = decltype(nb)::value;
       // ---- scores ----
-      float y[4];                                  // keys g, g, g + 8, g + 8 (in the copy's order); columns 2t, 2t + 1
-      {
+      float y[NB][4];   // keys g, g, g + 8, g + 8 (in the copy's order) of each 16; columns 2t, 2t + 1
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
         uint32_t w[2][KW];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) load_words<KW>(codes_at + L::K0 + k_row + r * 8 * L::ROW, w[r]);
+        for (int r = 0; r < 2; ++r) load_words<KW>(codes_at + L::K0 + k_row + (n * kBlock + r * 8) * L::ROW, w[r]);
         float ks[2][4];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) scales_of(*reinterpret_cast<const uint2*>(scales_at + L::KS0 + s_row + r * 64), ks[r]);
+        for (int r = 0; r < 2; ++r) scales_of(*reinterpret_cast<const uint2*>(scales_at + L::KS0 + s_row + (n * kBlock + r * 8) * 8), ks[r]);
         const auto quarter = [&](auto cc) {
           constexpr int C = decltype(cc)::value;
           float s[4];
@@ -391,45 +393,52 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? MINB : 2) paged4_attentio
             unpack2(add2(pack2(s[2], s[3]), l2), s[2], s[3]);
           }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y[e] = C == 0 ? s[e] * ks[e >> 1][C] : fmaf(s[e], ks[e >> 1][C], y[e]);
+          for (int e = 0; e < 4; ++e) y[n][e] = C == 0 ? s[e] * ks[e >> 1][C] : fmaf(s[e], ks[e >> 1][C], y[n][e]);
         };
         quarter(std::integral_constant<int, 0>());
         quarter(std::integral_constant<int, 1>());
         quarter(std::integral_constant<int, 2>());
         quarter(std::integral_constant<int, 3>());
       }
+      uint2 vs[NB][2];
+      float lv[NB][2], over = -INFINITY;
+      bool hidden[NB][4] = {};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = fmaf(y[e], f[e & 1], nm[e & 1]);
-      float vs[2][4], lv[2];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const uint2 u = *reinterpret_cast<const uint2*>(scales_at + L::VS0 + s_row + r * 64);
-        scales_of(u, vs[r]);
-        lv[r] = fmaxf(lg2(top_scale(u)), -60.f);
-      }
-      bool hidden[4] = {false, false, false, false};
-      if constexpr (EDGE) {
+      for (int n = 0; n < NB; ++n) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int key = k0 + (g ^ (g >> 1 & 1)) + 8 * (e >> 1), pos = p.pos0 + (p.row0 + 2 * t + (e & 1)) / a.G;
-          hidden[e] = key >= p.tb || key > pos || (a.window > 0 && key <= pos - a.window);
-          if (hidden[e]) y[e] = -INFINITY;
+          y[n][e] = fmaf(y[n][e], f[e & 1], nm[e & 1]);
+          if constexpr (EDGE) {
+            const int key = k0 + n * kBlock + (g ^ (g >> 1 & 1)) + 8 * (e >> 1), pos = p.pos0 + (p.row0 + 2 * t + (e & 1)) / a.G;
+            hidden[n][e] = key >= p.tb || key > pos || (a.window > 0 && key <= pos - a.window);
+            if (hidden[n][e]) y[n][e] = -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          vs[n][r] = *reinterpret_cast<const uint2*>(scales_at + L::VS0 + s_row + (n * kBlock + r * 8) * 8);
+          lv[n][r] = fmaxf(lg2(top_scale(vs[n][r])), -60.f);
+          over = fmaxf(over, fmaxf(y[n][2 * r], y[n][2 * r + 1]) + lv[n][r]);
         }
       }
       // ---- the reference, if a key exceeds it by more than a factor of 2 ----
-      const float over = fmaxf(fmaxf(y[0], y[1]) + lv[0], fmaxf(y[2], y[3]) + lv[1]);
       if (__any_sync(0xffffffffu, over > kTopLog + 1.f) || fresh) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float top = fmaxf(y[e] + lv[0], y[e + 2] + lv[1]);
+          float top = -INFINITY;
+#pragma unroll
+          for (int n = 0; n < NB; ++n) top = fmaxf(top, fmaxf(y[n][e] + lv[n][0], y[n][e + 2] + lv[n][1]));
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
           if (none[e] && top == -INFINITY) continue;   // the row has seen no key
           const float up = none[e] ? top - kTopLog : fmaxf(top - kTopLog, 0.f), c = none[e] ? 1.f : ex2(-up);
           none[e] = false;
           nm[e] -= up;
-          y[e] -= up;
-          y[e + 2] -= up;
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {
+            y[n][e] -= up;
+            y[n][e + 2] -= up;
+          }
           l[e] *= c;
 #pragma unroll
           for (int s = 0; s < VW; ++s)
@@ -441,78 +450,83 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? MINB : 2) paged4_attentio
         }
         fresh = __any_sync(0xffffffffu, none[0] || none[1]);
       }
-      // ---- weights, times each quarter's scale, as the second operand ----
-      float pw[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) pw[e] = ex2(y[e]);
-      l[0] += pw[0] + pw[2];
-      l[1] += pw[1] + pw[3];
-      uint32_t pf[4][PP][2];
+      for (int n = 0; n < NB; ++n) {
+        // ---- weights, times each quarter's scale, as the second operand ----
+        float pw[4], sv[2][4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+        for (int e = 0; e < 4; ++e) pw[e] = ex2(y[n][e]);
+        l[0] += pw[0] + pw[2];
+        l[1] += pw[1] + pw[3];
+        uint32_t pf[4][PP][2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          float x = pw[2 * r] * vs[r][c], z = pw[2 * r + 1] * vs[r][c];
-          if constexpr (EDGE) {   // 0 times a NaN scale is not 0
-            if (hidden[2 * r]) x = 0.f;
-            if (hidden[2 * r + 1]) z = 0.f;
-          }
+          scales_of(vs[n][r], sv[r]);
 #pragma unroll
-          for (int part = 0; part < PP; ++part) {
-            const uint32_t h = half2_bits(x, z);
-            pf[c][part][r] = transpose8(h);
-            if (part + 1 < PP) {
-              const float2 w = half2_floats(h);
-              x -= w.x;
-              z -= w.y;
+          for (int c = 0; c < 4; ++c) {
+            float x = pw[2 * r] * sv[r][c], z = pw[2 * r + 1] * sv[r][c];
+            if constexpr (EDGE) {   // 0 times a NaN scale is not 0
+              if (hidden[n][2 * r]) x = 0.f;
+              if (hidden[n][2 * r + 1]) z = 0.f;
+            }
+#pragma unroll
+            for (int part = 0; part < PP; ++part) {
+              const uint32_t h = half2_bits(x, z);
+              pf[c][part][r] = transpose8(h);
+              if (part + 1 < PP) {
+                const float2 w = half2_floats(h);
+                x -= w.x;
+                z -= w.y;
+              }
             }
           }
         }
-      // ---- sums: row m of the scores, and so of the weights, is the copy's row m ^ (m / 2 % 2) ----
-      uint32_t w[4][VW];
+        // ---- sums: row m of the scores, and so of the weights, is the copy's row m ^ (m / 2 % 2) ----
+        uint32_t w[4][VW];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint8_t* row = codes_at + L::V0 + (((2 * t + (e & 1)) ^ (t & 1)) + (e >> 1) * 8) * L::ROW;
-        if constexpr (D == 96) {
-          w[e][0] = *reinterpret_cast<const uint32_t*>(row + 4 * g);
-          w[e][1] = g < 4 ? *reinterpret_cast<const uint32_t*>(row + 32 + 4 * g) : 0u;
-        } else {
-          load_words<VW>(row + 4 * VW * g, w[e]);
+        for (int e = 0; e < 4; ++e) {
+          const uint8_t* row = codes_at + L::V0 + (n * kBlock + ((2 * t + (e & 1)) ^ (t & 1)) + (e >> 1) * 8) * L::ROW;
+          if constexpr (D == 96) {
+            w[e][0] = *reinterpret_cast<const uint32_t*>(row + 4 * g);
+            w[e][1] = g < 4 ? *reinterpret_cast<const uint32_t*>(row + 32 + 4 * g) : 0u;
+          } else {
+            load_words<VW>(row + 4 * VW * g, w[e]);
+          }
         }
-      }
 #pragma unroll
-      for (int s = 0; s < VW; ++s) {
-        // both tokens' half-words of a place side by side
-        const uint32_t lo0 = __byte_perm(w[0][s], w[1][s], 0x5410), hi0 = __byte_perm(w[0][s], w[1][s], 0x7632),
-                       lo1 = __byte_perm(w[2][s], w[3][s], 0x5410), hi1 = __byte_perm(w[2][s], w[3][s], 0x7632);
-        const auto quarter = [&](auto cc) {
-          constexpr int C = decltype(cc)::value;
-          const uint32_t a0 = centred<C>(lo0, magic), a1 = centred<C>(hi0, magic), a2 = centred<C>(lo1, magic),
-                         a3 = centred<C>(hi1, magic);
+        for (int s = 0; s < VW; ++s) {
+          // both tokens' half-words of a place side by side
+          const uint32_t lo0 = __byte_perm(w[0][s], w[1][s], 0x5410), hi0 = __byte_perm(w[0][s], w[1][s], 0x7632),
+                         lo1 = __byte_perm(w[2][s], w[3][s], 0x5410), hi1 = __byte_perm(w[2][s], w[3][s], 0x7632);
+          const auto quarter = [&](auto cc) {
+            constexpr int C = decltype(cc)::value;
+            const uint32_t a0 = centred<C>(lo0, magic), a1 = centred<C>(hi0, magic), a2 = centred<C>(lo1, magic),
+                           a3 = centred<C>(hi1, magic);
 #pragma unroll
-          for (int part = 0; part < PP; ++part) mma16(o[s][C], a0, a1, a2, a3, pf[C][part][0], pf[C][part][1]);
-        };
-        quarter(std::integral_constant<int, 0>());
-        quarter(std::integral_constant<int, 1>());
-        quarter(std::integral_constant<int, 2>());
-        quarter(std::integral_constant<int, 3>());
+            for (int part = 0; part < PP; ++part) mma16(o[s][C], a0, a1, a2, a3, pf[C][part][0], pf[C][part][1]);
+          };
+          quarter(std::integral_constant<int, 0>());
+          quarter(std::integral_constant<int, 1>());
+          quarter(std::integral_constant<int, 2>());
+          quarter(std::integral_constant<int, 3>());
+        }
       }
     };
 
-    const int whole_lo = p.all_lo, whole_hi = min(p.all_hi, p.tb) - kBlock;
+    const int whole_lo = p.all_lo, whole_hi = min(p.all_hi, p.tb);
 #pragma unroll 1
     for (int k0 = p.ta + kStep * warp; k0 < p.tb; k0 += kStep * kWarps) {
       ok = ok && __all_sync(0xffffffffu, bar_wait(bar0 + 8 * slot, phase, kErrCopy, abort_flag));
       if (!ok) break;
-      const uint32_t have = there >> (2 * slot);
+      const uint32_t have = there >> (2 * slot) & 3;
       const uint8_t* st = mem + (warp * ST + slot) * L::STAGE;
+      if (k0 >= whole_lo && k0 + kStep <= whole_hi && have == 3) {
+        block(std::false_type(), std::integral_constant<int, 2>(), st, st, k0);
+      } else {
 #pragma unroll 1
-      for (int half = 0; half < 2; ++half) {
-        const int k = k0 + kBlock * half;
-        if (!(have >> half & 1) || k >= p.tb) continue;
-        const uint8_t *codes = st + half * (kBlock * L::ROW), *scales = st + half * (kBlock * 8);
-        if (k >= whole_lo && k <= whole_hi) block(std::false_type(), codes, scales, k);
-        else block(std::true_type(), codes, scales, k);
+        for (int half = 0; half < 2; ++half)
+          if ((have >> half & 1) && k0 + kBlock * half < p.tb)
+            block(std::true_type(), std::integral_constant<int, 1>(), st + half * (kBlock * L::ROW), st + half * (kBlock * 8), k0 + kBlock * half);
       }
       __syncwarp();   // the step's rows have been read
       copy(slot);

@@ -22,7 +22,7 @@ SOURCES = [PKG / "csrc" / "sf_q4.cu", PKG / "csrc" / "sf_q4_gemm_tc.cu", PKG / "
            PKG / "csrc" / "sf_norm_turn.cu", PKG / "csrc" / "sf_paged4_attention.cu"]
 HEADERS = [ROOT / "include" / "sf_q4.h", PKG / "csrc" / "sf_q4_internal.h", PKG / "csrc" / "sf_e4m3.h",
            PKG / "csrc" / "sf_paged.h", PKG / "csrc" / "sf_paged_prompt.h", PKG / "csrc" / "sf_tcgen05.h",
-           PKG / "csrc" / "sf_paged_work.h", PKG / "csrc" / "sf_paged4.h"]
+           PKG / "csrc" / "sf_paged_work.h", PKG / "csrc" / "sf_paged4.h", PKG / "csrc" / "sf_paged4_prompt.h"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

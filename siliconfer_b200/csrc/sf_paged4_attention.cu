@@ -10,13 +10,13 @@
 // One row of a kv head's group is one (new token, query head); a tile has 8 rows, so that a group reads its keys once.
 // Both products are mma.sync m16n8k16 in fp16 with the codes as the larger operand and the 8 rows as columns:
 //  * S^T[key, row] = K Q^T: 16 keys are the MMA's rows; each quarter of the head has sums of its own, which are added
-//    times the key's scale in fp32.  For bf16 queries and outputs a pair of codes is a pair of fp16 subnormals n * 2^-24
+//    times the key's scale in fp32.  For 16-bit queries and outputs a pair of codes is a pair of fp16 subnormals n * 2^-24
 //    after one mask, and the sums begin at -8 times the sum of the quarter's queries.  The tensor cores align a subnormal
-//    as it stands, which leaves such sums 2^-17 of their largest product (measured on sums of one key); for the finer types
-//    the codes become the numbers n - 8, at two instructions a pair more.  A query row is brought to at most 2^14 by a
+//    as it stands, which leaves such sums 2^-17 of their largest product (measured on sums of one key); with fp32 among the
+//    types the codes become the numbers n - 8, at two instructions a pair more.  A query row is brought to at most 2^14 by a
 //    power of two; fp16 then holds a bf16 or fp16 row as it is, and two parts an fp32 row.
-//  * out^T[d, row] += V^T P^T: a quarter's weights are the softmax's times the key's scale of that quarter, in fp16 (two
-//    parts for the finer types, 22 bits), codes the numbers n - 8.
+//  * out^T[d, row] += V^T P^T: a quarter's weights are the softmax's times the key's scale of that quarter, in fp16 (with
+//    fp32 among the types in two parts, 22 bits), codes the numbers n - 8.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -37,6 +37,7 @@ namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kBlock = 16, kStep = 32;   // keys of an MMA, and of a warp's copy
 constexpr unsigned kErrCopy = 1u << 17;
+constexpr int kCtas = 3;             // of an SM, head_dim up to 128
 constexpr float kTopLog = 13.f;      // log2 of a weight times its scale, at most one above it
 
 struct Attn4Args : AttnArgs {
@@ -133,10 +134,7 @@ struct Lay4 {
 };
 
 template <int D, int QP, int PP>
-#ifndef MINB
-#define MINB 3
-#endif
-__global__ void __launch_bounds__(kThreads, D <= 128 ? MINB : 2) paged4_attention_kernel(const __grid_constant__ Attn4Args a, int q_pairs) {
+__global__ void __launch_bounds__(kThreads, D <= 128 ? kCtas : 2) paged4_attention_kernel(const __grid_constant__ Attn4Args a, int q_pairs) {
   using L = Lay4<D>;
   constexpr int RT = 8, KW = L::KW, VW = L::VW, Q = L::Q, ST = L::STAGES;
   constexpr bool FINE = PP == 2;   // keys' codes less 8, as the values'
@@ -609,6 +607,43 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? MINB : 2) paged4_attentio
   griddep_launch_dependents();   // not before: the merge's blocks would wait in the place of the next call's
 }
 
+// One block for each (CTA that began a divided tile, row of it): GROUPS groups of threads take the parts in turn, D columns
+// each, and are added in order.  A tile of 55 parts (131072 keys) takes 6 us less in 4 groups than in one.
+template <int D, int GROUPS>
+__global__ void __launch_bounds__(GROUPS * D) paged4_merge_kernel(const AttnArgs a) {
+  constexpr int RT = 8;
+  __shared__ float sum[GROUPS][D], lsum[GROUPS];
+  griddep_wait();
+  const int* dsc = a.desc + 8 * blockIdx.x;
+  const int parts = dsc[0], row = blockIdx.y, q_row = dsc[3] + row, grp = threadIdx.x / D, d = threadIdx.x % D;
+  if (parts == 0 || q_row > dsc[4]) return;
+  const auto part = [&](int i) {
+    return a.part + ((size_t)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * kMaxRows * (D + 2);
+  };
+  float M = kNone;
+  for (int i = 0; i < parts; ++i) M = fmaxf(M, part(i)[RT * D + 2 * row]);
+  float A = 0.f, Ls = 0.f;
+#pragma unroll 4
+  for (int i = grp; i < parts; i += GROUPS) {
+    const float* p = part(i);
+    const float c = ex2(p[RT * D + 2 * row] - M);
+    A += p[row * D + d] * c;
+    Ls += p[RT * D + 2 * row + 1] * c;
+  }
+  sum[grp][d] = A;
+  if (d == 0) lsum[grp] = Ls;
+  __syncthreads();
+  if (grp > 0) return;
+#pragma unroll
+  for (int i = 1; i < GROUPS; ++i) {
+    A += sum[i][d];
+    Ls += lsum[i];
+  }
+  const size_t th = (size_t)(dsc[1] + q_row / a.G) * a.H + dsc[2] * a.G + q_row % a.G;
+  store_out(a, th * D + d, Ls == 0.f ? 0.f : A / Ls);
+  if (d == 0 && a.lse) a.lse[th] = Ls == 0.f ? -INFINITY : M * kLn2 + logf(Ls);
+}
+
 template <int D, int QP, int PP>
 int launch4(Attn4Args a, cudaStream_t st) {
   using L = Lay4<D>;
@@ -620,7 +655,7 @@ int launch4(Attn4Args a, cudaStream_t st) {
   cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::smem(kMaxBatch));
   if (e != cudaSuccess) return cuda_fail(e, "paged4_attention_kernel shared memory");
   int per_sm = (int)(228 * 1024 / (smem + 4 * QP * 128 * L::KW + 2048));
-  const int most = D <= 128 ? MINB : 2;
+  const int most = D <= 128 ? kCtas : 2;
   if (per_sm > most) per_sm = most;
   if (per_sm < 1) per_sm = 1;
   // no more CTAs than units there may be
@@ -635,20 +670,26 @@ int launch4(Attn4Args a, cudaStream_t st) {
   if (e != cudaSuccess) return cuda_fail(e, "paged4_attention_kernel launch");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid, 8);
-  cfg.blockDim = dim3(D);
+  // many parts of each tile where the tiles are few
+  const double tiles = ((double)a.T * a.G / 8 + c.batch) * c.n_kv_heads;
+  const bool many = tiles * 8 <= a.resident;
+  constexpr int GROUPS = 512 / D;
+  cfg.blockDim = dim3(many ? GROUPS * D : D);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, paged_attention_merge_kernel<D, 8>, static_cast<const AttnArgs&>(a));
-  if (e != cudaSuccess) return cuda_fail(e, "paged_attention_merge_kernel launch");
+  e = cudaLaunchKernelEx(&cfg, many ? paged4_merge_kernel<D, GROUPS> : paged4_merge_kernel<D, 1>, static_cast<const AttnArgs&>(a));
+  if (e != cudaSuccess) return cuda_fail(e, "paged4_merge_kernel launch");
   g_launches.fetch_add(2, std::memory_order_relaxed);
   return SF_OK;
 }
 
 constexpr int kMaxCtasPerSm = 4;
+
+#include "sf_paged4_prompt.h"
 
 }  // namespace
 }  // namespace sf
@@ -689,7 +730,20 @@ int sf_paged4_attention(const sf_paged4_cache* cache, const void* q, int q_dtype
   if ((long long)cache->n_kv_heads * cache->page_size * D > 0x7fffffffll)
     return fail(SF_ERR_UNSUPPORTED, "a page of all kv heads has more than 2^31 - 1 elements");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool fine = std::min(q_dtype, out_dtype) != SF_BF16;   // the finer of the types
+  const bool fine = q_dtype == SF_F32 || out_dtype == SF_F32;
+  const long long items = ((long long)T * a.G / kPromptRows + cache->batch) * cache->n_kv_heads;
+  const int sms = device_info().sms;
+  const long long keys = std::min((long long)cache->pages_per_seq * cache->page_size,
+                                  a.window > 0 ? (long long)a.window + kPromptRows : LLONG_MAX);
+  const long long tiles = std::max(((long long)T * a.G + kPromptRows - 1) / kPromptRows, (long long)cache->batch) * cache->n_kv_heads,
+                  rounds = (tiles + sms - 1) / sms, key_tiles = (keys + UNIT - 1) / UNIT;
+  const bool many = (double)T * H * (key_tiles + (D == 64 ? 14 : 7)) >= 5800.0 * rounds * (key_tiles + 2);
+  const bool prompt = !fine && (D == 64 || D == 128) && many && cache->batch <= kPromptBatch && items <= 0x7fffffffll &&
+                      reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  if (prompt) {
+    const bool q_vec = reinterpret_cast<uintptr_t>(q) % 16 == 0 && qts % 8 == 0 && qhs % 8 == 0;
+    return D == 64 ? launch_prompt4<64>(a, items, q_vec, st) : launch_prompt4<128>(a, items, q_vec, st);
+  }
   const auto go = [&](auto d) {
     constexpr int DD = decltype(d)::value;
     if (q_dtype == SF_F32) return launch4<DD, 2, 2>(a, st);

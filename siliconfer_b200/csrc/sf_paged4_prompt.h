@@ -217,12 +217,28 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged4_prompt_kernel(const 
     const int r = threadIdx.x - 384, w4 = warp - 12;
     uint32_t magic;
     asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));
-    uint32_t it = 0;
+    uint32_t it = 0, vf[4] = {};   // tiles so far; factors of the values of the tile before
+    bool v_live = false;
+    // the values of tile j
+    const auto values = [&](uint32_t j) {
+      bar_wait(vrfull, j & 1, kErrWiden, abort_flag);
+      if (j > 0) {
+        bar_wait(ofull, (j - 1) & 1, kErrWiden, abort_flag);
+        bar_wait(ofull + 8, (j - 1) & 1, kErrWiden, abort_flag);
+      }
+      widen_row<D>(mem + L::VR, mem + L::V0, r, v_live, vf, magic);
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        bar_arrive(vfull);
+        bar_arrive(vrempty);
+      }
+    };
     for (int i = 0; i < items; ++i) {
       const Prompt4Item p = item_at(i);
       const int tiles = tiles_of(p);
       for (int k = 0; k < tiles; ++k, ++it) {
-        // ---- keys ----
+        // ---- a tile's keys, then the values of the tile before, whose place is free later ----
         bar_wait(krfull, it & 1, kErrWiden, abort_flag);
         const uint32_t mask = *box_mask;
         const bool there = p.ta + UNIT * k + r < p.tb && (mask >> (r / box) & 1);
@@ -266,23 +282,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged4_prompt_kernel(const 
           bar_arrive(kfull);
           bar_arrive(krempty);
         }
-        // ---- values ----
-        factors(vs, __int_as_float((254 - ve) << 23), f);
-        if (v_nan) f[0] = f[1] = f[2] = f[3] = 0u;   // its rows become NaN by the sum
-        bar_wait(vrfull, it & 1, kErrWiden, abort_flag);
-        if (it > 0) {
-          bar_wait(ofull, (it - 1) & 1, kErrWiden, abort_flag);
-          bar_wait(ofull + 8, (it - 1) & 1, kErrWiden, abort_flag);
-        }
-        widen_row<D>(mem + L::VR, mem + L::V0, r, there && !v_nan, f, magic);
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          bar_arrive(vfull);
-          bar_arrive(vrempty);
-        }
+        if (it > 0) values(it - 1);
+        v_live = there && !v_nan;
+        factors(vs, __int_as_float((254 - ve) << 23), vf);
+        if (!v_live) vf[0] = vf[1] = vf[2] = vf[3] = 0u;   // a NaN comes to its rows by their sums
       }
     }
+    if (it > 0) values(it - 1);
   } else if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == 8) {
@@ -293,6 +299,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged4_prompt_kernel(const 
         asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
                      "r"(bytes), "r"(bar)
                      : "memory");
+      };
+      // the values of tile j, asked for after the keys of the next
+      uint32_t v_loads = 0;
+      const uint8_t* v_from = nullptr;
+      const auto values = [&](uint32_t j) {
+        if (!__all_sync(0xffffffffu, bar_wait(vrempty, (j & 1) ^ 1, kErrProd, abort_flag))) return false;
+        if (lane == 0) bar_expect_tx(vrfull, __popc(v_loads) * (uint32_t)(box * L::ROW));
+        __syncwarp();
+        if (v_from) bulk(base + L::VR + lane * box * L::ROW, v_from, box * L::ROW, vrfull);
+        return true;
       };
       for (int i = 0; i < items && ok; ++i) {
         const Prompt4Item p = item_at(i);
@@ -325,13 +341,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged4_prompt_kernel(const 
             bulk(base + L::KS + lane * box * 8, reinterpret_cast<const uint8_t*>(a.ks) + vec * 8, box * 8, krfull);
             bulk(base + L::VS + lane * box * 8, reinterpret_cast<const uint8_t*>(a.vs) + vec * 8, box * 8, krfull);
           }
-          ok = __all_sync(0xffffffffu, bar_wait(vrempty, (it & 1) ^ 1, kErrProd, abort_flag));
-          if (!ok) break;
-          if (lane == 0) bar_expect_tx(vrfull, __popc(loads) * (uint32_t)(box * L::ROW));
-          __syncwarp();
-          if (page >= 0) bulk(base + L::VR + lane * box * L::ROW, a.c.v_codes + vec * L::ROW, box * L::ROW, vrfull);
+          if (it > 0) ok = values(it - 1);
+          v_loads = loads;
+          v_from = page >= 0 ? a.c.v_codes + vec * L::ROW : nullptr;
         }
       }
+      if (ok && it > 0) ok = values(it - 1);
       // every issued copy has landed before the block ends
       if (lane == 0 && ok && it > 0) {
         bar_drain(krfull, (it - 1) & 1, kErrDrain);

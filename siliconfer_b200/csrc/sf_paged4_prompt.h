@@ -209,9 +209,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged4_prompt_kernel(const 
   const auto tiles_of = [](const Prompt4Item& p) { return p.tb > p.ta ? (p.tb - p.ta + UNIT - 1) / UNIT : 0; };
   const int box = min(page_size, UNIT), boxes = UNIT / box;
 
-  // The launch's 128 registers a thread are dealt out again: 208 * 256 + 40 * 128 + 56 * 128 = 128 * 512.
+  // The launch's 128 registers a thread are dealt out again: 200 * 256 + 40 * 128 + 72 * 128 = 128 * 512.
   if (warp >= 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     // ---------------- codes to fp16: thread r is key r of a tile ----------------
     // After an expired wait these warps go on through their loops (every wait then returns at once).
     const int r = threadIdx.x - 384, w4 = warp - 12;
@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged4_prompt_kernel(const 
       bar_drain(drain, 0, kErrDrain);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ---------------- softmax: thread tid is row tid of the item ----------------
     // After an expired wait these warps go on through their loops (every wait then returns at once).
     const int tid = threadIdx.x, t = tid >> 7, row_t = tid & 127;

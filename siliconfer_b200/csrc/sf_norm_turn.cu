@@ -10,6 +10,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
+#include <initializer_list>
 #include <type_traits>
 
 #include "sf_e4m3.h"
@@ -26,11 +27,13 @@ constexpr int kRounds = 6, kThreads = 256, kMaxDim = 512, kMaxAxes = 8;
 
 struct Vectors {
   const void* p;
-  long long ts, hs;     // token and head strides
+  long long ts;         // token stride
+  int hs;               // head stride
 };
 struct Out {
   void* p;
-  long long ts, hs;
+  long long ts;
+  int hs;
 };
 enum Pairs { kNoPairs, kHalves, kHalvesOfHalf, kNeighbours, kAnyPairs };
 
@@ -40,6 +43,7 @@ struct HeadArgs {
   const void *wq, *wk;  // norm weights or NULL
   int w_dtype, norm;
   float eps, inv_d;     // 1 / D
+  double inv_d64;
   const float* table;   // [max_pos, rot]: cosines, then sines
   int max_pos, rot, interleaved, pairs;
   const void* positions;   // [T, axes_n] or NULL: a token's place in its sequence
@@ -164,20 +168,18 @@ __device__ __forceinline__ void turn_vector(F (&y)[4][W], bool there, int r0, co
   }
 }
 
-// y / s to the nearest whole number (ties to even), limited to -8 .. 7, plus 8; inv = 1 / s in fp32.  A first guess is at
-// most one off, and what y and guess * s differ by, which is exact (in fp64 but for one rounding of y's last place), says so.
-__device__ __forceinline__ uint32_t code_of(float y, float s, float inv) {
-  const float m = fmaf(y, inv, 12582912.f), r = m - 12582912.f, d = fmaf(-r, s, y), over = fmaf(fabsf(d), 2.f, -s);
-  int n = __float_as_int(m) - 0x4b400000;
-  if (over > 0.f || (over == 0.f && (n & 1))) n += d > 0.f ? 1 : -1;
-  return (uint32_t)(min(max(n, -8), 7) + 8);
+// y / s to the nearest whole number (ties to even), limited to -8 .. 7; inv = 1 / s.  The quotient is corrected by what it
+// leaves of y, which rounds it like a division: a tie is one exactly where y is (n + 1/2) s.
+__device__ __forceinline__ int code_of(float y, float s, float inv) {
+  const float t = y * inv, q = fmaf(fmaf(-t, s, y), inv, t);
+  return min(max(__float_as_int(q + 12582912.f) - 0x4b400000, -8), 7);
 }
-__device__ __forceinline__ uint32_t code_of(double y, double s, double inv) {
-  const double m = fma(y, inv, 6755399441055744.0), r = m - 6755399441055744.0, d = fma(-r, s, y), over = fma(fabs(d), 2.0, -s);
-  int n = __double2loint(m);
-  if (over > 0.0 || (over == 0.0 && (n & 1))) n += __double2hiint(d) >= 0 ? 1 : -1;
-  return (uint32_t)(min(max(n, -8), 7) + 8);
+__device__ __forceinline__ int code_of(double y, double s, double inv) {
+  const double t = y * inv, q = fma(fma(-t, s, y), inv, t);
+  return min(max(__double2loint(q + 6755399441055744.0), -8), 7);
 }
+// max|y| / 7.5 in fp32
+__device__ __forceinline__ float scale_of(double top) { return (float)(top * (1.0 / 7.5)); }
 // Largest magnitude of each quarter over a vector's lanes, as bits (an infinity or a NaN is above every number).
 template <int GP, int W>
 __device__ __forceinline__ uint32_t quarter_tops(const float (&y)[4][W], uint32_t (&top)[4]) {
@@ -239,12 +241,13 @@ __global__ void __launch_bounds__(kThreads, CACHE ? 2 : 4) norm_turn_kernel(cons
   for (int c = 0; c < 4; ++c)
 #pragma unroll
     for (int i = 0; i < W; ++i) next[c].e[i] = TX(0.f);   // lanes beyond a vector's end add nothing to its sums
+  const TX *qx = static_cast<const TX*>(a.q.p) + (long long)tok * a.q.ts + r0, *kx = static_cast<const TX*>(a.k.p) + (long long)tok * a.k.ts + r0,
+           *vx = static_cast<const TX*>(a.v.p) + (long long)tok * a.v.ts + r0;
   const auto load = [&](int p) {
     if (p >= passes) return;
     const int kind = kind_of(p), h = head_of(p, kind);
     if (!there_of(h, kind)) return;
-    const Vectors& s = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
-    const TX* x = static_cast<const TX*>(s.p) + (long long)tok * s.ts + h * s.hs + r0;
+    const TX* x = kind == 0 ? qx + (long long)h * a.q.hs : kind == 1 ? kx + (long long)h * a.k.hs : vx + (long long)h * a.v.hs;
 #pragma unroll
     for (int c = 0; c < 4; ++c) load_raw<TX, W, VEC>(x + c * Q, next[c]);
   };
@@ -302,6 +305,7 @@ __global__ void __launch_bounds__(kThreads, CACHE ? 2 : 4) norm_turn_kernel(cons
   __syncthreads();
   const bool put = CACHE && place.put;
   const long long slot = CACHE ? place.slot : 0;
+  TX *qo = static_cast<TX*>(a.qo.p) + (long long)tok * a.qo.ts + r0, *ko = static_cast<TX*>(a.ko.p) + (long long)tok * a.ko.ts + r0;
   // this vector's place in its warp's part of the exchange, room for 128 W doubles
   double* buf64 = exchange + (tid / 32) * (128 * W) + lane / GP * D;
   float* buf32 = reinterpret_cast<float*>(exchange + (tid / 32) * (128 * W)) + lane / GP * D;
@@ -331,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, CACHE ? 2 : 4) norm_turn_kernel(cons
             for (int i = 0; i < W; ++i) ss = fma(z[c][i], z[c][i], ss);
 #pragma unroll
           for (int o = GP / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-          const double r = 1.0 / sqrt(ss / D + (double)a.eps);
+          const double r = rsqrt(ss * a.inv_d64 + (double)a.eps);
           if (there) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
@@ -343,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, CACHE ? 2 : 4) norm_turn_kernel(cons
           }
         }
         turn_vector<double, W>(z, there, r0, a, cs, sn, buf64);
-        uint32_t top[4], words[4] = {}, sb[4];
+        uint32_t top[4], words[4] = {0x8888u, 0x8888u, 0x8888u, 0x8888u}, sb[4];
         float y[4][W];
 #pragma unroll
         for (int c = 0; c < 4; ++c)
@@ -352,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, CACHE ? 2 : 4) norm_turn_kernel(cons
         const bool finite = quarter_tops<GP, W>(y, top) < 0x7f800000u;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          float s = __fdiv_rn(__uint_as_float(top[c]), 7.5f);
+          float s = scale_of(__uint_as_float(top[c]));
           // within 4 last places of a tie of two scales: from the largest magnitude in fp64
           const bool near = ((__float_as_uint(s) - 0x7ffcu) & 0xffffu) <= 8u;
           if (__any_sync(0xffffffffu, near)) {
@@ -361,13 +365,13 @@ __global__ void __launch_bounds__(kThreads, CACHE ? 2 : 4) norm_turn_kernel(cons
             for (int i = 0; i < W; ++i) big = fmax(big, fabs(z[c][i]));
 #pragma unroll
             for (int o = GP / 2; o; o >>= 1) big = fmax(big, __shfl_xor_sync(0xffffffffu, big, o));
-            if (near) s = (float)(big / 7.5);
+            if (near) s = scale_of(big);
           }
           sb[c] = scale_bits(s, finite);
           s = __uint_as_float(sb[c] << 16);
-          const double s64 = s, inv = 1.f / s;
+          const double s64 = s, near_inv = __frcp_rn(s), inv = near_inv * fma(-s64, near_inv, 2.0);
 #pragma unroll
-          for (int i = 0; i < W; ++i) words[i] |= code_of(z[c][i], s64, inv) << (4 * c);
+          for (int i = 0; i < W; ++i) words[i] += code_of(z[c][i], s64, inv) * (1 << 4 * c);
         }
         if (there && put) store_codes(a, slot, 1, h, r0, finite, words, sb);
         continue;
@@ -379,14 +383,14 @@ __global__ void __launch_bounds__(kThreads, CACHE ? 2 : 4) norm_turn_kernel(cons
         for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int i = 0; i < W; ++i) y[c][i] = to_f32(raw[c].e[i]);
-        uint32_t top[4], words[4] = {}, sb[4];
+        uint32_t top[4], words[4] = {0x8888u, 0x8888u, 0x8888u, 0x8888u}, sb[4];
         const bool finite = quarter_tops<GP, W>(y, top) < 0x7f800000u;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          sb[c] = scale_bits(__fdiv_rn(__uint_as_float(top[c]), 7.5f), finite);
-          const float s = __uint_as_float(sb[c] << 16), inv = 1.f / s;
+          sb[c] = scale_bits(scale_of(__uint_as_float(top[c])), finite);
+          const float s = __uint_as_float(sb[c] << 16), inv = __frcp_rn(s);
 #pragma unroll
-          for (int i = 0; i < W; ++i) words[i] |= code_of(y[c][i], s, inv) << (4 * c);
+          for (int i = 0; i < W; ++i) words[i] += code_of(y[c][i], s, inv) * (1 << 4 * c);
         }
         if (there && put) store_codes(a, slot, 2, h, r0, finite, words, sb);
         continue;
@@ -425,8 +429,7 @@ __global__ void __launch_bounds__(kThreads, CACHE ? 2 : 4) norm_turn_kernel(cons
     }
     turn_vector<float, W>(y, there, r0, a, cs, sn, buf32);
     if (there) {
-      const Out& d = kind == 0 ? a.qo : a.ko;
-      TX* o = static_cast<TX*>(d.p) + (long long)tok * d.ts + h * d.hs + r0;
+      TX* o = kind == 0 ? qo + (long long)h * a.qo.hs : ko + (long long)h * a.ko.hs;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         Raw<TX, W> w;
@@ -448,6 +451,12 @@ bool aligned_rows(const void* p, int dtype, long long ts, long long hs, int W) {
   return reinterpret_cast<uintptr_t>(p) % (size * W) == 0 && ts % W == 0 && hs % W == 0;
 }
 
+bool strides_ok(std::initializer_list<long long> head_strides) {
+  for (const long long x : head_strides)
+    if (x < 0 || x > 0x7fffffffll) return false;
+  return true;
+}
+
 int check_args(const HeadArgs& a, int dtype) {
   if (dtype < 0 || dtype > 2 || a.w_dtype < 0 || a.w_dtype > 2) return fail(SF_ERR_DTYPE, "unknown dtype code");
   if (a.rot < 0 || a.rot % 2 || a.rot > a.D) return fail(SF_ERR_SHAPE, "rot must be even and at most head_dim");
@@ -462,7 +471,8 @@ int check_args(const HeadArgs& a, int dtype) {
 template <typename TX, int W, bool CACHE>
 cudaError_t launch(HeadArgs& a, bool vec, cudaStream_t st) {
   const int lanes = a.D / 4 / W;
-  a.inv_d = 1.f / (float)a.D;
+  a.inv_d64 = 1.0 / a.D;
+  a.inv_d = (float)a.inv_d64;
   const auto go = [&](auto gp) -> cudaError_t {
     constexpr int GP = decltype(gp)::value, AT = 32 / GP;
     const int passes = (a.Hkv + AT - 1) / AT * (CACHE ? 2 : 1) + (a.H + AT - 1) / AT;
@@ -517,10 +527,10 @@ int sf_qk_norm_rotary(const void* q, long long qts, long long qhs, void* q_out, 
   if (D < 4 || D % 4 || D > (D % 16 == 0 ? 512 : D % 8 == 0 ? 256 : 128))
     return fail(SF_ERR_UNSUPPORTED, "head_dim %d not built (multiples of 16 up to 512, of 8 up to 256, of 4 up to 128)", D);
   HeadArgs a{};
-  a.q = Vectors{q, qts, qhs};
-  a.k = Vectors{k, kts, khs};
-  a.qo = Out{q_out, qots, qohs};
-  a.ko = Out{k_out, kots, kohs};
+  a.q = Vectors{q, qts, (int)qhs};
+  a.k = Vectors{k, kts, (int)khs};
+  a.qo = Out{q_out, qots, (int)qohs};
+  a.ko = Out{k_out, kots, (int)kohs};
   a.wq = q_weight; a.wk = k_weight; a.w_dtype = w_dtype;
   a.norm = eps >= 0.f;
   a.eps = eps;
@@ -530,6 +540,7 @@ int sf_qk_norm_rotary(const void* q, long long qts, long long qhs, void* q_out, 
   if (int rc = check_args(a, dtype)) return rc;
   if (T == 0 || H + Hkv == 0) return SF_OK;
   if ((H && (!q || !q_out)) || (Hkv && (!k || !k_out)) || (rot && !positions)) return fail(SF_ERR_NULL, "null pointer argument");
+  if (!strides_ok({qhs, qohs, khs, kohs})) return fail(SF_ERR_UNSUPPORTED, "a head stride above 2^31 - 1 elements");
   if ((long long)H + Hkv > 0xffff) return fail(SF_ERR_UNSUPPORTED, "more than 65535 heads");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = with_type(dtype, [&](auto* p) {
@@ -558,9 +569,9 @@ int sf_paged4_append(const sf_paged4_cache* cache, const void* k, long long kts,
   HeadArgs a{};
   if (int rc = check_paged4(cache, T, a.c)) return rc;
   const int D = cache->head_dim;
-  a.q = Vectors{q, qts, qhs};
-  a.k = Vectors{k, kts, khs};
-  a.v = Vectors{v, vts, vhs};
+  a.q = Vectors{q, qts, (int)qhs};
+  a.k = Vectors{k, kts, (int)khs};
+  a.v = Vectors{v, vts, (int)vhs};
   a.qo = Out{q_out, (long long)H * D, D};
   a.wq = q_weight; a.wk = k_weight; a.w_dtype = w_dtype;
   a.norm = eps >= 0.f;
@@ -574,6 +585,7 @@ int sf_paged4_append(const sf_paged4_cache* cache, const void* k, long long kts,
   if (T == 0) return SF_OK;
   if (!k || !v || (q && !q_out)) return fail(SF_ERR_NULL, "null pointer argument");
   if (q && H < 1) return fail(SF_ERR_SHAPE, "need H >= 1 query heads");
+  if (!strides_ok({khs, vhs, qhs})) return fail(SF_ERR_UNSUPPORTED, "a head stride above 2^31 - 1 elements");
   if ((long long)a.H + 2ll * a.Hkv > 0xffff) return fail(SF_ERR_UNSUPPORTED, "more than 65535 heads");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = with_type(dtype, [&](auto* p) {

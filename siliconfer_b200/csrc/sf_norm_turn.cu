@@ -23,7 +23,7 @@ extern std::atomic<long long> g_launches;
 
 namespace {
 
-constexpr int kRounds = 6, kThreads = 256, kMaxDim = 512, kMaxAxes = 8;
+constexpr int kRounds = 10, kThreads = 256, kMaxDim = 512, kMaxAxes = 8;
 
 struct Vectors {
   const void* p;
@@ -54,12 +54,6 @@ struct HeadArgs {
   sf_paged_cache c;
   __nv_bfloat16 *ks, *vs;
 };
-
-__device__ __forceinline__ float load_weight(const void* w, int dtype, int i) {
-  if (dtype == SF_F32) return static_cast<const float*>(w)[i];
-  if (dtype == SF_F16) return __half2float(static_cast<const __half*>(w)[i]);
-  return __bfloat162float(static_cast<const __nv_bfloat16*>(w)[i]);
-}
 
 // W consecutive elements as they are loaded.
 template <typename TX, int W>
@@ -217,7 +211,7 @@ struct TokenPlace {
 };
 
 template <typename TX, int W, int GP, bool VEC, bool CACHE>
-__global__ void __launch_bounds__(kThreads, CACHE ? 2 : 4) norm_turn_kernel(const __grid_constant__ HeadArgs a) {
+__global__ void __launch_bounds__(kThreads, CACHE && sizeof(TX) == 4 ? 3 : 4) norm_turn_kernel(const __grid_constant__ HeadArgs a) {
   static_assert(!CACHE || W == 4, "a lane's words are stored as 8 bytes");
   constexpr int AT = 32 / GP;   // vectors of a warp at a time
   extern __shared__ __align__(16) double exchange[];
@@ -296,10 +290,21 @@ __global__ void __launch_bounds__(kThreads, CACHE ? 2 : 4) norm_turn_kernel(cons
     sn[j] = ok ? __ldg(a.table + p * a.rot + half + j) : nan;
   }
   if (a.norm) {
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
+    for (int i = tid; i < 2 * Q; i += blockDim.x) {   // four weights each
+      const int which = i >= Q, e = 4 * (which ? i - Q : i);
       const void* w = which ? a.wk : a.wq;
-      for (int i = tid; i < D; i += blockDim.x) weights[which][i] = w ? load_weight(w, a.w_dtype, i) : 1.f;
+      float v[4] = {1.f, 1.f, 1.f, 1.f};
+      if (w && a.w_dtype == SF_F32) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = static_cast<const float*>(w)[e + j];
+      } else if (w) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const unsigned short x = static_cast<const unsigned short*>(w)[e + j];
+          v[j] = a.w_dtype == SF_BF16 ? __uint_as_float((uint32_t)x << 16) : __half2float(__ushort_as_half(x));
+        }
+      }
+      *reinterpret_cast<float4*>(&weights[which][e]) = make_float4(v[0], v[1], v[2], v[3]);
     }
   }
   __syncthreads();

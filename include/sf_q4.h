@@ -390,7 +390,7 @@ int sf_paged_attention(const sf_paged_cache* cache, const void* q, int q_dtype, 
  * SF_ERR_INDEX at the next error check. */
 int sf_qk_norm_rotary(const void* q, long long qts, long long qhs, void* q_out, long long qots, long long qohs, int H,
                       const void* k, long long kts, long long khs, void* k_out, long long kots, long long kohs, int Hkv,
-                      int dtype, const void* q_weight, const void* k_weight, int w_dtype, float eps,
+                      int dtype, const void* q_weight, const void* k_weight, int w_dtype, double eps,
                       const void* positions, int pos64, int axes_n, const uint8_t* axes, const float* table, int max_pos,
                       int rot, int interleaved, int T, int D, void* stream);
 
@@ -423,7 +423,7 @@ typedef struct {
  * with y in fp64 for keys and values.  Two rows of one call must not be the same token. */
 int sf_paged4_append(const sf_paged4_cache* cache, const void* k, long long kts, long long khs, const void* v,
                      long long vts, long long vhs, const void* q, long long qts, long long qhs, void* q_out, int dtype,
-                     int H, int T, const void* q_weight, const void* k_weight, int w_dtype, float eps,
+                     int H, int T, const void* q_weight, const void* k_weight, int w_dtype, double eps,
                      const void* positions, int pos64, int axes_n, const uint8_t* axes, const float* table, int max_pos,
                      int rot, int interleaved, void* stream);
 

@@ -19,7 +19,7 @@ SF_EPI_SWIGLU = 1
 SF_OK = 0
 
 _P, _I, _LL = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
-_SZ, _F = ctypes.c_size_t, ctypes.c_float
+_SZ, _F, _DB = ctypes.c_size_t, ctypes.c_float, ctypes.c_double
 
 
 class Q4Task(ctypes.Structure):
@@ -82,10 +82,10 @@ SIGNATURES = {
                         _I, _I, _P],
     "sf_paged_attention_workspace_bytes": [_I],
     "sf_paged_attention": [ctypes.POINTER(PagedCache), _P, _I, _LL, _LL, _P, _I, _P, _I, _I, _F, _I, _P, _SZ, _P],
-    "sf_qk_norm_rotary": [_P, _LL, _LL, _P, _LL, _LL, _I, _P, _LL, _LL, _P, _LL, _LL, _I, _I, _P, _P, _I, _F, _P, _I, _I,
+    "sf_qk_norm_rotary": [_P, _LL, _LL, _P, _LL, _LL, _I, _P, _LL, _LL, _P, _LL, _LL, _I, _I, _P, _P, _I, _DB, _P, _I, _I,
                           _P, _P, _I, _I, _I, _I, _I, _P],
     "sf_paged4_append": [ctypes.POINTER(Paged4Cache), _P, _LL, _LL, _P, _LL, _LL, _P, _LL, _LL, _P, _I, _I, _I, _P, _P,
-                         _I, _F, _P, _I, _I, _P, _P, _I, _I, _I, _P],
+                         _I, _DB, _P, _I, _I, _P, _P, _I, _I, _I, _P],
     "sf_paged4_attention_workspace_bytes": [_I],
     "sf_paged4_attention": [ctypes.POINTER(Paged4Cache), _P, _I, _LL, _LL, _P, _I, _P, _I, _I, _F, _I, _P, _SZ, _P],
 }

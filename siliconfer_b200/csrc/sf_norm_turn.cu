@@ -7,6 +7,11 @@
 // A block takes one token and some of its heads: the angles, which hang on one or several positions, are brought to shared
 // memory once.  A group of lanes takes a vector at a time, the next one's elements under way; a lane the same W places of
 // all four quarters: these hold both elements of its rotary pairs, and the codes of a place are one 16-bit word.
+//
+// Measured in a graph: 4096 tokens, 64 query and 8 kv heads of 128, three axes, norms: turned 32 us (4.8 TB/s of the copy
+// rate's 6.5), appended 40 us (3.9 TB/s); one token 2.6 us, 8 tokens of 32 heads appended 4.0.  Bound by instructions: some
+// 300 a warp for four heads.  A warp takes up to 10 passes in turn (3: 39 us, 6: 33); keys are normed, turned and cut in fp64,
+// which the 64-bit units do beside the rest, so that a code is the exact value's.
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
@@ -43,7 +48,7 @@ struct HeadArgs {
   const void *wq, *wk;  // norm weights or NULL
   int w_dtype, norm;
   float eps, inv_d;     // 1 / D
-  double inv_d64;
+  double inv_d64, eps64;
   const float* table;   // [max_pos, rot]: cosines, then sines
   int max_pos, rot, interleaved, pairs;
   const void* positions;   // [T, axes_n] or NULL: a token's place in its sequence
@@ -340,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, CACHE && sizeof(TX) == 4 ? 3 : 4) no
             for (int i = 0; i < W; ++i) ss = fma(z[c][i], z[c][i], ss);
 #pragma unroll
           for (int o = GP / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-          const double r = rsqrt(ss * a.inv_d64 + (double)a.eps);
+          const double r = rsqrt(ss * a.inv_d64 + a.eps64);
           if (there) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
@@ -468,7 +473,6 @@ int check_args(const HeadArgs& a, int dtype) {
   if (a.rot > 0 && (!a.table || a.max_pos < 1)) return fail(SF_ERR_SHAPE, "the rotary table is missing or empty");
   if (a.positions && (a.axes_n < 1 || a.axes_n > kMaxAxes || (a.axes_n > 1 && !a.axes)))
     return fail(SF_ERR_SHAPE, "need 1 to %d axes, and with more than one the axis of each pair", kMaxAxes);
-  if (a.norm && !(a.eps >= 0.f)) return fail(SF_ERR_SHAPE, "eps must not be negative");
   return SF_OK;
 }
 
@@ -525,7 +529,7 @@ extern "C" {
 
 int sf_qk_norm_rotary(const void* q, long long qts, long long qhs, void* q_out, long long qots, long long qohs, int H,
                       const void* k, long long kts, long long khs, void* k_out, long long kots, long long kohs, int Hkv,
-                      int dtype, const void* q_weight, const void* k_weight, int w_dtype, float eps,
+                      int dtype, const void* q_weight, const void* k_weight, int w_dtype, double eps,
                       const void* positions, int pos64, int axes_n, const uint8_t* axes, const float* table, int max_pos,
                       int rot, int interleaved, int T, int D, void* stream) {
   if (T < 0 || H < 0 || Hkv < 0) return fail(SF_ERR_SHAPE, "need T, H, Hkv >= 0");
@@ -537,8 +541,9 @@ int sf_qk_norm_rotary(const void* q, long long qts, long long qhs, void* q_out, 
   a.qo = Out{q_out, qots, (int)qohs};
   a.ko = Out{k_out, kots, (int)kohs};
   a.wq = q_weight; a.wk = k_weight; a.w_dtype = w_dtype;
-  a.norm = eps >= 0.f;
-  a.eps = eps;
+  a.norm = eps >= 0.;
+  a.eps64 = eps;
+  a.eps = (float)eps;
   a.table = table; a.max_pos = max_pos; a.rot = rot; a.interleaved = interleaved;
   a.positions = positions; a.pos64 = pos64; a.axes_n = axes_n; a.axes = axes;
   a.H = H; a.Hkv = Hkv; a.T = T; a.D = D;
@@ -568,7 +573,7 @@ int sf_qk_norm_rotary(const void* q, long long qts, long long qhs, void* q_out, 
 
 int sf_paged4_append(const sf_paged4_cache* cache, const void* k, long long kts, long long khs, const void* v,
                      long long vts, long long vhs, const void* q, long long qts, long long qhs, void* q_out, int dtype,
-                     int H, int T, const void* q_weight, const void* k_weight, int w_dtype, float eps,
+                     int H, int T, const void* q_weight, const void* k_weight, int w_dtype, double eps,
                      const void* positions, int pos64, int axes_n, const uint8_t* axes, const float* table, int max_pos,
                      int rot, int interleaved, void* stream) {
   HeadArgs a{};
@@ -579,8 +584,9 @@ int sf_paged4_append(const sf_paged4_cache* cache, const void* k, long long kts,
   a.v = Vectors{v, vts, (int)vhs};
   a.qo = Out{q_out, (long long)H * D, D};
   a.wq = q_weight; a.wk = k_weight; a.w_dtype = w_dtype;
-  a.norm = eps >= 0.f;
-  a.eps = eps;
+  a.norm = eps >= 0.;
+  a.eps64 = eps;
+  a.eps = (float)eps;
   a.table = table; a.max_pos = max_pos; a.rot = table ? rot : 0; a.interleaved = interleaved;
   a.positions = positions; a.pos64 = pos64; a.axes_n = axes_n; a.axes = axes;
   a.H = q ? H : 0; a.Hkv = cache->n_kv_heads; a.T = T; a.D = D;

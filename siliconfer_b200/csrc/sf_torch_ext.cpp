@@ -380,7 +380,7 @@ struct TurnArgs {
   const void *wq = nullptr, *wk = nullptr, *positions = nullptr;
   const uint8_t* axes = nullptr;
   const float* table = nullptr;
-  float eps = -1.f;
+  double eps = -1.;
   int w_dtype = SF_F32, pos64 = 0, axes_n = 1, max_pos = 0, rot = 0;
 };
 TurnArgs turn_args(const OptTensor& table, const OptTensor& positions, const OptTensor& axes, const OptTensor& wq,
@@ -418,7 +418,7 @@ TurnArgs turn_args(const OptTensor& table, const OptTensor& positions, const Opt
   TORCH_CHECK(a.axes_n == 1 || a.axes, "positions of several axes need the axis of each pair (axes)");
   if (eps.has_value()) {
     TORCH_CHECK(*eps >= 0, "eps must not be negative");
-    a.eps = (float)*eps;
+    a.eps = *eps;
   }
   const auto weight = [&](const OptTensor& w, const char* name) -> const void* {
     if (!given(w)) return nullptr;

@@ -17,6 +17,17 @@
 //    power of two; fp16 then holds a bf16 or fp16 row as it is, and two parts an fp32 row.
 //  * out^T[d, row] += V^T P^T: a quarter's weights are the softmax's times the key's scale of that quarter, in fp16 (with
 //    fp32 among the types in two parts, 22 bits), codes the numbers n - 8.
+//
+// A warp takes its keys by itself: 32 at a time by bulk copies into a ring of its own, which brings a page's rows as they
+// lie, and no warp waits for another before the end of a part.  Measured in a graph, 64 query and 8 kv heads of 128, 16 x 8192
+// keys 53 us (2.9 TB/s), one sequence of 131072 with 32 query heads 57; 32 heads of their own, 64 sequences of up to 4096
+// keys 217 (3.0 TB/s).  Bound by instructions: some 400 a warp for 16 keys, of which unpacking the codes takes 120 (integer
+// units 50 % in use, issue slots 56 %).  On the way, 16 x 8192 and 64 x 4096 keys in us: copies by each lane, 16 keys at a
+// time, 128 registers and 4 CTAs an SM 71 and 289; by bulk 65 and 261; queries in shared memory 60 and 235; 32 keys at a time,
+// 168 registers and 3 CTAs 53 and 241, and with fp16 weights in one part for
+// fp16 queries 217; at 128 registers 60 and 207.
+//
+// Long runs of 16-bit queries with 16-bit outputs go to the kernel of sf_paged4_prompt.h.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -731,13 +742,20 @@ int sf_paged4_attention(const sf_paged4_cache* cache, const void* q, int q_dtype
     return fail(SF_ERR_UNSUPPORTED, "a page of all kv heads has more than 2^31 - 1 elements");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool fine = q_dtype == SF_F32 || out_dtype == SF_F32;
+  // Tiles of 256 rows: an SM takes some 2.8 us for 128 keys of a tile, however many of its rows are in use, and 14 us before
+  // and after.  Tiles of 8 rows: all SMs together take 0.5 ns for 128 keys of a row, and 20 us before and after.  So the rows
+  // of a round of tiles decide; of the lengths the host knows only the block table's.
+  // Measured, 64 query and 8 kv heads, tiles of 256 and of 8 rows, in us.  Head_dim 128: 18 sequences of 8 tokens, 256 keys
+  // 20 and 38, 2048 keys 69 and 117, 32768 keys 902 and 1228; 8 such, 2048 keys 58 and 58, 32768 keys 738 and 562; one of 32
+  // tokens 21 and 18, 59 and 35, 706 and 293; one of 256, 2048 keys 61 and 183.  Head_dim 64: 8 sequences of 8 tokens, 2048
+  // keys 49 and 45, 32768 keys 646 and 431; 16 such, 256 keys 16 and 25, 2048 keys 52 and 77.
   const long long items = ((long long)T * a.G / kPromptRows + cache->batch) * cache->n_kv_heads;
   const int sms = device_info().sms;
   const long long keys = std::min((long long)cache->pages_per_seq * cache->page_size,
                                   a.window > 0 ? (long long)a.window + kPromptRows : LLONG_MAX);
   const long long tiles = std::max(((long long)T * a.G + kPromptRows - 1) / kPromptRows, (long long)cache->batch) * cache->n_kv_heads,
                   rounds = (tiles + sms - 1) / sms, key_tiles = (keys + UNIT - 1) / UNIT;
-  const bool many = (double)T * H * (key_tiles + (D == 64 ? 14 : 7)) >= 5800.0 * rounds * (key_tiles + 2);
+  const bool many = (double)T * H * (key_tiles + 7) >= 5800.0 * rounds * (key_tiles + 2);
   const bool prompt = !fine && (D == 64 || D == 128) && many && cache->batch <= kPromptBatch && items <= 0x7fffffffll &&
                       reinterpret_cast<uintptr_t>(out) % 16 == 0;
   if (prompt) {

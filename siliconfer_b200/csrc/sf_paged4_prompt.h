@@ -10,6 +10,10 @@
 //  * The sums stay in TMEM; a row that moves its reference multiplies them there.  The tile's powers of two go into the
 //    row's factor and reference, so that the softmax has nothing to do for each key but the exponential.
 // A key's codes serve 256 rows here and 8 in paged4_attention_kernel.
+//
+// 8 sequences of 256 tokens with 64 query heads over up to 4000 keys: 213 us, 417 TFLOP/s (paged4_attention_kernel: 887 us).
+// A tile's keys are widened before the values of the tile before, whose place is free later: the other way round 272 us.
+// What is left: items are dealt out whole and in turn, and the SMs work 0.68 of the time there.
 #pragma once
 
 constexpr int kPromptRows = 256, kPromptSoft = 8, kPromptThreads = 512, kSlots = 4, kPromptBatch = 2048;

@@ -877,3 +877,27 @@ def test_cache_and_quantizer_without_gpu():
         Paged4KVCache(3, 2, 66, 16, device="cpu")
     with pytest.raises(RuntimeError):
         quantize_kv4(torch.zeros(2, 6))
+
+
+NEAR_TIE = (-6, 104, -45, -122, 125, 78, -4, 40, -38, 30, 92, 120, -12, 69, 5, 77, -20, 112, -24, 34, 34, -45, -36, -120, 16, 69,
+            82, -86, -37, 64, 57, 23, -63, -106, 110, -98, -50, -109, -74, 79, -68, -102, -68, 38, 82, 35, -109, -100, -19, 36,
+            -22, 86, 106, -122, 55, -120, -12, -58, -66, 115, 27, -126, -28, -22)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_append_eps_64_bits(cuda, dtype):
+    """With eps of 1 + 2^-24, which fp32 rounds to 1, element 61 is -7.4999999 scales and its code 1; with 1 -7.5000001 and 0."""
+    from siliconfer_b200.paged_kv4 import Paged4KVCache, quantize_kv4
+    x = torch.tensor(NEAR_TIE, dtype=torch.float64) * 2.0 ** -9
+    got = []
+    for eps in (1 + 2.0 ** -24, 1.0):
+        codes, scales = quantize_kv4(x / ((x * x).mean() + eps).sqrt())
+        cache = Paged4KVCache(1, 1, 64, 16, device="cuda")
+        k = x.to("cuda", dtype).view(1, 1, 64)
+        cache.append(k, k, torch.zeros(1, 1, dtype=torch.int32, device="cuda"),
+                     torch.ones(1, dtype=torch.int32, device="cuda"), eps=eps)
+        assert torch.equal(cache.k_scales[0, 0, 0].cpu().view(torch.int16), scales.view(torch.int16))
+        assert torch.equal(cache.k_codes[0, 0, 0].cpu(), codes)
+        got.append(codes)
+    assert not torch.equal(*got)

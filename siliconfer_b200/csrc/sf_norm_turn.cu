@@ -14,6 +14,7 @@
 // which the 64-bit units do beside the rest, so that a code is the exact value's.
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <cstdint>
 #include <initializer_list>
 #include <type_traits>
@@ -476,7 +477,10 @@ int check_args(const HeadArgs& a, int dtype) {
   return SF_OK;
 }
 
-// Warps of a block and blocks of a token: a warp takes its vectors at once where the tokens are few, else 6 times in turn.
+// A positive eps stays one in fp32, or a vector of zeros would be 0 times infinity.
+float eps_f32(double eps) { return eps > 0. ? std::max((float)eps, FLT_MIN) : (float)eps; }
+
+// Warps of a block and blocks of a token: a warp takes its vectors at once where the tokens are few, else up to kRounds times in turn.
 template <typename TX, int W, bool CACHE>
 cudaError_t launch(HeadArgs& a, bool vec, cudaStream_t st) {
   const int lanes = a.D / 4 / W;
@@ -543,7 +547,7 @@ int sf_qk_norm_rotary(const void* q, long long qts, long long qhs, void* q_out, 
   a.wq = q_weight; a.wk = k_weight; a.w_dtype = w_dtype;
   a.norm = eps >= 0.;
   a.eps64 = eps;
-  a.eps = (float)eps;
+  a.eps = eps_f32(eps);
   a.table = table; a.max_pos = max_pos; a.rot = rot; a.interleaved = interleaved;
   a.positions = positions; a.pos64 = pos64; a.axes_n = axes_n; a.axes = axes;
   a.H = H; a.Hkv = Hkv; a.T = T; a.D = D;
@@ -586,7 +590,7 @@ int sf_paged4_append(const sf_paged4_cache* cache, const void* k, long long kts,
   a.wq = q_weight; a.wk = k_weight; a.w_dtype = w_dtype;
   a.norm = eps >= 0.;
   a.eps64 = eps;
-  a.eps = (float)eps;
+  a.eps = eps_f32(eps);
   a.table = table; a.max_pos = max_pos; a.rot = table ? rot : 0; a.interleaved = interleaved;
   a.positions = positions; a.pos64 = pos64; a.axes_n = axes_n; a.axes = axes;
   a.H = q ? H : 0; a.Hkv = cache->n_kv_heads; a.T = T; a.D = D;

@@ -262,3 +262,13 @@ def test_validation_without_gpu():
                      (dict(an=9), 2), (dict(an=0), 2), (dict(an=2), 2), (dict(q=None), 1), (dict(ko=None), 1), (dict(pos=None), 1),
                      (dict(H=1 << 17), 6), (dict(T=0), 0), (dict(H=0, Hkv=0), 0)):
         assert call(**kw) == want, kw
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_eps_below_fp32(cuda, dtype):
+    """A vector of zeros stays one with any positive eps, those that fp32 has no number for among them."""
+    x = torch.zeros(3, 2, 64, device="cuda", dtype=dtype)
+    for eps in (1e-40, 1e-60, 1e-300):
+        q, k = qk_norm_rotary(x, x[:, :1], eps=eps)
+        assert not q.any() and not k.any()

@@ -901,3 +901,16 @@ def test_append_eps_64_bits(cuda, dtype):
         assert torch.equal(cache.k_codes[0, 0, 0].cpu(), codes)
         got.append(codes)
     assert not torch.equal(*got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_append_eps_below_fp32(cuda, dtype):
+    """Heads of zeros stay zeros with any positive eps, queries that are returned and keys that are cut to codes alike."""
+    from siliconfer_b200.paged_kv4 import Paged4KVCache
+    x = torch.zeros(3, 2, 64, device="cuda", dtype=dtype)
+    pages = torch.arange(3, dtype=torch.int32, device="cuda").view(3, 1)
+    for eps in (1e-40, 1e-60, 1e-300):
+        cache = Paged4KVCache(3, 2, 64, 16, device="cuda")
+        q = cache.append(x, x, pages, torch.ones(3, dtype=torch.int32, device="cuda"), q=x, eps=eps)
+        assert not q.any() and (cache.k_codes == 0x88).all() and (cache.k_scales[:, :, 0] == 2.0 ** -126).all()

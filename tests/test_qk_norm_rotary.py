@@ -8,6 +8,8 @@ products 2; a turn's product and sum 2 of |a cos| + |b sin|: 20 in all, 24 asked
 import pytest
 import torch
 
+from siliconfer_b200.rotary import qk_norm_rotary
+
 STEP = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
 
 

@@ -108,6 +108,7 @@ __device__ __forceinline__ float top_scale(uint2 u) {
   const uint32_t m = __vmaxu2(u.x, u.y);
   return __uint_as_float(max(m << 16, m & 0xffff0000u));
 }
+__device__ __forceinline__ float at_most(float x, float most) { return x > most ? most : x; }   // a NaN stays one
 template <int N>
 __device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
   if constexpr (N % 4 == 0) {
@@ -440,13 +441,15 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? kCtas : 2) paged4_attenti
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
           if (none[e] && top == -INFINITY) continue;   // the row has seen no key
-          const float up = none[e] ? top - kTopLog : fmaxf(top - kTopLog, 0.f), c = none[e] ? 1.f : ex2(-up);
+          // below what the roundings of a large score may add, so that the largest key's weight is no less than 2^kTopLog
+          const float to = fmaf(fabsf(nm[e]) + fabsf(top), -0x1p-22f, top - kTopLog);
+          const float up = none[e] ? to : fmaxf(to, 0.f), c = none[e] ? 1.f : ex2(-up);
           none[e] = false;
           nm[e] -= up;
 #pragma unroll
-          for (int n = 0; n < NB; ++n) {
-            y[n][e] -= up;
-            y[n][e + 2] -= up;
+          for (int n = 0; n < NB; ++n) {   // so that it may be more than a weight has room for: it is limited
+            y[n][e] = at_most(y[n][e] - up, kTopLog + 2.f - lv[n][0]);
+            y[n][e + 2] = at_most(y[n][e + 2] - up, kTopLog + 2.f - lv[n][1]);
           }
           l[e] *= c;
 #pragma unroll

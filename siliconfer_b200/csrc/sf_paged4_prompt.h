@@ -19,6 +19,8 @@
 constexpr int kPromptRows = 256, kPromptSoft = 8, kPromptThreads = 512, kSlots = 4, kPromptBatch = 2048;
 constexpr unsigned kErrProd = 1u << 18, kErrMma = 1u << 19, kErrSoft = 1u << 22, kErrDrain = 1u << 23, kErrWiden = 1u << 24;
 
+constexpr float kFarScore = 0x1p22f;   // above it a score's roundings may pass a weight's room: weights are limited there
+
 __device__ __forceinline__ uint32_t swizzle128(uint32_t at) { return at ^ ((at >> 3) & 0x70); }
 
 // What the softmax has to know of a tile of keys.
@@ -538,19 +540,23 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged4_prompt_kernel(const 
           const float most = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
           const float over = most == -INFINITY ? -INFINITY : most * fk + v_log;
           float c_o = 1.f;
-          if (none) {
-            if (over > -INFINITY) {
-              nm = kTopLog - over;
-              none = false;
+          if (none || over + nm > kTopLog + 1.f) {
+            // above what the roundings of a large score may take off, so that its weight is no less than 2^kTopLog
+            const float to = fmaf(fabsf(over), 0x1p-22f, kTopLog - over);
+            if (none) {
+              if (over > -INFINITY) {
+                nm = to;
+                none = false;
+              }
+            } else if (to < nm) {
+              c_o = ex2(to - nm);
+              nm = to;
+              l *= c_o;
             }
-          } else if (over + nm > kTopLog + 1.f) {
-            c_o = ex2(kTopLog - (over + nm));
-            nm = kTopLog - over;
-            l *= c_o;
           }
           // ---- weights, in pairs ----
           uint32_t h[UNIT / 2];
-          {
+          if (fabsf(nm) <= kFarScore) {
             uint64_t l2 = 0, l3 = 0;   // zeros
             const float base_e = nm + v_log;
             const uint64_t nm2 = pack2(base_e, base_e), fk2 = pack2(fk, fk);
@@ -567,6 +573,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged4_prompt_kernel(const 
             float l0, l1;
             unpack2(add2(l2, l3), l0, l1);
             l = fmaf(l0 + l1, info.v_down, l);
+          } else {
+            float ls = 0.f;
+#pragma unroll
+            for (int e = 0; e < UNIT; e += 2) {
+              const float z0 = at_most(fmaf(y[e], fk, nm), kTopLog + 2.f - v_log), z1 = at_most(fmaf(y[e + 1], fk, nm), kTopLog + 2.f - v_log);
+              ls += ex2(z0) + ex2(z1);
+              h[e / 2] = half2_bits(ex2(z0 + v_log), ex2(z1 + v_log));
+            }
+            l += ls;
           }
           // ---- the sums of the tile before are there: its P may be written over ----
           if (j > 0) bar_wait(ofull + 8 * t, (j - 1) & 1, kErrSoft, abort_flag);

@@ -914,3 +914,24 @@ def test_append_eps_below_fp32(cuda, dtype):
         cache = Paged4KVCache(3, 2, 64, 16, device="cuda")
         q = cache.append(x, x, pages, torch.ones(3, dtype=torch.int32, device="cuda"), q=x, eps=eps)
         assert not q.any() and (cache.k_codes == 0x88).all() and (cache.k_scales[:, :, 0] == 2.0 ** -126).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [3, 800])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("power", [18, 20, 22, 23, 24, 25, 26, 27, 30, 36, 44, 60])
+def test_scores_whose_last_place_is_above_one(cuda, power, D, n):
+    """Scores of 2^power and more, which fp32 holds to 2^-24: whichever keys a row picks, its weights add up to one.  All values
+    are one vector, so that the result is it, off by 2^-11 of its fp16 form in prompts, as much of a weight and half a step."""
+    from siliconfer_b200.paged_kv4 import paged4_attention
+    for v_power in (0, -30, 40):
+        b = Batch4([900, 130], [n, min(n, 100)], 32, 8, D, 16, torch.bfloat16)
+        b.v[:] = b.v[0, 0, 0]
+        b.vs[:] = b.vs[0, 0, 0] * 2.0 ** v_power
+        for scale in (2.0 ** (power - 5), -(2.0 ** (power - 5))):
+            out, lse = paged4_attention(b.q, *b.args(), starts=b.starts, scale=scale, return_lse=True)
+            want = value_of(b.v[0, 0, 0], b.vs[0, 0, 0])
+            assert ((out.double() - want).abs() <= (2 * 2.0 ** -11 + 3e-5 + 2.0 ** -8) * want.abs()).all()
+            ref = b.ref(scale=scale)[1]
+            # fp32's rounding of the sum and of its parts, and in prompts of the keys
+            assert ((lse.double() - ref).abs() <= 4e-5 + 2e-6 * ref.abs() + 2.0 ** -11 * spread(b, scale=scale)[1]).all()

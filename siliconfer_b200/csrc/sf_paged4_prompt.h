@@ -4,11 +4,14 @@
 // A CTA takes 256 query rows of a kv head's group (two tiles of 128, a thread for each row) through all their keys, 128
 // at a time, on tcgen05 (kind::f16):
 //  * S[row, key] = Q K^T and out[row, d] += P V.  Four warps widen a tile's codes to fp16, a thread for each key: code less
-//    8 times the scale of its quarter, relative to a power of two for the whole tile, rounded to 11 bits; what lies 2^14
-//    and more below the tile's largest scale keeps 2^-24 of that.  Queries are fp16 numbers after a power of two for the
-//    row, weights in fp16.
+//    8 times the scale of its quarter, relative to a power of two, rounded to 11 bits.  The power is the whole tile's, taken
+//    so that its largest element stands at 2^11 to 2^15: a quarter's scale 2^21 below the tile's largest is a normal number
+//    still.  A tile whose scales lie further apart is wide: each of its vectors has a power of two of its own, of the scores
+//    and of the weights, so that no key's digits hang on another's.  Within a vector, quarters that far below its largest
+//    lose digits.  Queries are fp16 numbers after a power of two for the row, weights in fp16.
 //  * The sums stay in TMEM; a row that moves its reference multiplies them there.  The tile's powers of two go into the
-//    row's factor and reference, so that the softmax has nothing to do for each key but the exponential.
+//    row's factor and reference, so that the softmax has nothing to do for each key but the exponential; a wide tile's keys
+//    are multiplied and shifted one by one.
 // A key's codes serve 256 rows here and 8 in paged4_attention_kernel.
 //
 // 8 sequences of 256 tokens with 64 query heads over up to 4000 keys: 213 us, 417 TFLOP/s (paged4_attention_kernel: 887 us).
@@ -19,7 +22,10 @@
 constexpr int kPromptRows = 256, kPromptSoft = 8, kPromptThreads = 512, kSlots = 4, kPromptBatch = 2048;
 constexpr unsigned kErrProd = 1u << 18, kErrMma = 1u << 19, kErrSoft = 1u << 22, kErrDrain = 1u << 23, kErrWiden = 1u << 24;
 
+constexpr int kHead = 11;         // log2 of the room above a widened element: 8 * 2 * 2^11 is within fp16
+constexpr int kSpread = 21;       // exponents that a tile's scales may lie apart: an odd quarter's factor is 2^(11 - 4 - 21) then
 constexpr float kFarScore = 0x1p22f;   // above it a score's roundings may pass a weight's room: weights are limited there
+constexpr uint32_t kNought = 0x00800000u;   // scales up to 2^-126 are those of zeros
 
 __device__ __forceinline__ uint32_t swizzle128(uint32_t at) { return at ^ ((at >> 3) & 0x70); }
 
@@ -29,6 +35,7 @@ struct TileInfo {
   float v_log;       // log2 of the values' power of two
   float v_down;      // its inverse
   int whole;         // every key of the tile is there
+  int wide;          // keys have powers of two of their own
   uint32_t there[4]; // keys that are
   uint32_t nan[4];   // keys whose value is NaN
 };
@@ -38,7 +45,7 @@ struct Prompt4Lay {
   static constexpr uint32_t ROW = D / 2, T16 = UNIT * D * 2;   // a tile of 128 rows of fp16
   static constexpr uint32_t Q0 = 0, P = UNIT * UNIT * 2, P0 = 2 * T16, K0 = P0 + 2 * P, V0 = K0 + T16;
   static constexpr uint32_t KR = V0 + T16, KS = KR + UNIT * ROW, VS = KS + UNIT * 8, VR = VS + UNIT * 8;
-  static constexpr uint32_t CTL = VR + UNIT * ROW, INFO = CTL + 512, FIRST = CTL + 1024;
+  static constexpr uint32_t CTL = VR + UNIT * ROW, INFO = CTL + 512, POWERS = CTL + 1024, FIRST = POWERS + kSlots * UNIT * 8;
   static constexpr uint32_t TMEM_COLS = 512, O0 = 256;          // scores of two tiles, sums of two tiles
   static constexpr size_t smem(int batch) { return 1024 + FIRST + (size_t)batch * 4; }
   static_assert(sizeof(TileInfo) * kSlots <= 512, "control area");
@@ -115,6 +122,11 @@ __device__ __forceinline__ void widen_row(const uint8_t* codes, uint8_t* to, int
     quarter(std::integral_constant<int, 3>());
   }
 }
+// The smallest of four scales that are not those of zeros, less kNought and one bit (more than any number's where all are).
+__device__ __forceinline__ uint32_t least_scale(uint2 u) {
+  constexpr uint32_t below = kNought + 1;
+  return min(min((u.x << 16) - below, (u.x & 0xffff0000u) - below), min((u.y << 16) - below, (u.y & 0xffff0000u) - below));
+}
 // Factors of a vector's quarters, scale / up with up a power of two, as pairs.
 __device__ __forceinline__ void factors(uint2 scales, float down, uint32_t (&f)[4]) {
   float s[4];
@@ -131,11 +143,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged4_prompt_kernel(const 
   using L = Prompt4Lay<D>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ int wsum[kPromptThreads / 32];
-  __shared__ uint32_t tops[2][4][2];   // largest scales of a tile, by warp: keys', values'
+  __shared__ uint32_t tops[2][4][4];   // of a tile, by warp: keys' and values' largest scale, and their smallest
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   uint8_t* mem = smem_raw + (base - raw);
   int* first = reinterpret_cast<int*>(mem + L::FIRST);
   TileInfo* infos = reinterpret_cast<TileInfo*>(mem + L::INFO);
+  float2* powers = reinterpret_cast<float2*>(mem + L::POWERS);   // of a wide tile's keys: the key's power, log2 of the value's
   const uint32_t ctl = base + L::CTL;
   const uint32_t krfull = ctl, krempty = ctl + 8, vrfull = ctl + 16, vrempty = ctl + 24, kfull = ctl + 32, kempty = ctl + 40,
                  vfull = ctl + 48, sfull = ctl + 56, sdone = ctl + 72, pfull = ctl + 88, ofull = ctl + 104, qfull = ctl + 120,
@@ -253,31 +266,46 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged4_prompt_kernel(const 
                     vs = there ? *reinterpret_cast<const uint2*>(mem + L::VS + 8 * r) : none;
         const uint32_t kt = __float_as_uint(top_scale(ks)), vt = __float_as_uint(top_scale(vs));
         const bool k_nan = kt >= 0x7f800000u, v_nan = vt >= 0x7f800000u;
-        const uint32_t km = __reduce_max_sync(0xffffffffu, k_nan ? 0u : kt), vm = __reduce_max_sync(0xffffffffu, v_nan ? 0u : vt);
+        const uint32_t km = __reduce_max_sync(0xffffffffu, k_nan ? 0u : kt), vm = __reduce_max_sync(0xffffffffu, v_nan ? 0u : vt),
+                       kl = __reduce_min_sync(0xffffffffu, k_nan ? ~0u : least_scale(ks)),
+                       vl = __reduce_min_sync(0xffffffffu, v_nan ? ~0u : least_scale(vs));
         TileInfo& info = infos[it % kSlots];
         const uint32_t have = __ballot_sync(0xffffffffu, there), nans = __ballot_sync(0xffffffffu, v_nan);
         if (lane == 0) {
           tops[it & 1][w4][0] = km;
           tops[it & 1][w4][1] = vm;
+          tops[it & 1][w4][2] = kl;
+          tops[it & 1][w4][3] = vl;
           info.there[w4] = have;
           info.nan[w4] = nans;
         }
         const int whole = all_of_128(there);
+        // exponents, of which a power's inverse is a number, too
+        const auto key_power = [](uint32_t top) { return max((int)(top >> 23), kHead + 1); };
+        const auto value_power = [](uint32_t top) { return max((int)(top >> 23), 127 - 60); };
         const auto largest = [&](int which) {
-          uint32_t x = 0;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) x = max(x, tops[it & 1][w][which]);
-          return min(max((int)(x >> 23), 1), 253);   // its exponent
+          return max(max(tops[it & 1][0][which], tops[it & 1][1][which]), max(tops[it & 1][2][which], tops[it & 1][3][which]));
         };
-        const int ke = largest(0), ve = max(largest(1), 127 - 60);
+        const auto far = [&](int which, int power) {   // some scale lies more than kSpread exponents below the power
+          const uint32_t x = min(min(tops[it & 1][0][which], tops[it & 1][1][which]), min(tops[it & 1][2][which], tops[it & 1][3][which]));
+          return power > kSpread + 1 && x < ((uint32_t)(power - kSpread) << 23) - kNought - 1;
+        };
+        int ke = key_power(largest(0)), ve = value_power(largest(1));
+        const bool wide = far(2, ke) || far(3, ve);
         if (r == 0) {
-          info.k_up = __int_as_float(ke << 23);
-          info.v_log = (float)(ve - 127);
-          info.v_down = __int_as_float((254 - ve) << 23);
+          info.k_up = __int_as_float((ke - kHead) << 23);
+          info.v_log = (float)(ve - kHead - 127);
+          info.v_down = __int_as_float((254 + kHead - ve) << 23);
           info.whole = whole;
+          info.wide = wide;
+        }
+        if (wide) {
+          ke = key_power(k_nan ? 0u : kt);
+          ve = value_power(v_nan ? 0u : vt);
+          powers[it % kSlots * UNIT + r] = make_float2(__int_as_float((ke - kHead) << 23), (float)(ve - kHead - 127));
         }
         uint32_t f[4];
-        factors(ks, __int_as_float((254 - ke) << 23), f);
+        factors(ks, __int_as_float((254 + kHead - ke) << 23), f);
         if (k_nan) f[0] = f[1] = f[2] = f[3] = 0x7e007e00u;
         if (it > 0) bar_wait(kempty, (it - 1) & 1, kErrWiden, abort_flag);
         widen_row<D>(mem + L::KR, mem + L::K0, r, there && !k_nan, f, magic);
@@ -290,7 +318,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged4_prompt_kernel(const 
         }
         if (it > 0) values(it - 1);
         v_live = there && !v_nan;
-        factors(vs, __int_as_float((254 - ve) << 23), vf);
+        factors(vs, __int_as_float((254 + kHead - ve) << 23), vf);
         if (!v_live) vf[0] = vf[1] = vf[2] = vf[3] = 0u;   // a NaN comes to its rows by their sums
       }
     }
@@ -512,6 +540,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged4_prompt_kernel(const 
           float fk = f * info.k_up;
           if (fk < 1e-30f) fk = 1e-30f;   // a hidden key's -inf must stay one; scores this small are none
           const float v_log = info.v_log;
+          const bool wide = info.wide;
+          const float2* own = powers + j % kSlots * UNIT;
+          if (wide) {
+#pragma unroll
+            for (int e = 0; e < UNIT; ++e) y[e] *= f * own[e].x;
+            fk = 1.f;
+          }
           // ---- keys that the row does not see ----
           if (!(k0 >= p.all_lo && k0 + UNIT <= p.all_hi && info.whole)) {
             const int hi = max(pos - k0, -1), lo = a.window > 0 ? hi - a.window : -1;
@@ -529,16 +564,23 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged4_prompt_kernel(const 
               if ((info.nan[e / 32] >> (e % 32) & 1) && e <= hi && e > lo) l = __int_as_float(0x7fffffff);
           }
           // ---- the reference, if a key exceeds it by more than a factor of 2 ----
-          float m0 = y[0], m1 = y[1], m2 = y[2], m3 = y[3];
+          float over;
+          if (!wide) {
+            float m0 = y[0], m1 = y[1], m2 = y[2], m3 = y[3];
 #pragma unroll
-          for (int e = 4; e < UNIT; e += 4) {
-            m0 = fmaxf(m0, y[e]);
-            m1 = fmaxf(m1, y[e + 1]);
-            m2 = fmaxf(m2, y[e + 2]);
-            m3 = fmaxf(m3, y[e + 3]);
+            for (int e = 4; e < UNIT; e += 4) {
+              m0 = fmaxf(m0, y[e]);
+              m1 = fmaxf(m1, y[e + 1]);
+              m2 = fmaxf(m2, y[e + 2]);
+              m3 = fmaxf(m3, y[e + 3]);
+            }
+            const float most = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+            over = most == -INFINITY ? -INFINITY : most * fk + v_log;
+          } else {
+            over = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < UNIT; ++e) over = fmaxf(over, y[e] + own[e].y);
           }
-          const float most = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
-          const float over = most == -INFINITY ? -INFINITY : most * fk + v_log;
           float c_o = 1.f;
           if (none || over + nm > kTopLog + 1.f) {
             // above what the roundings of a large score may take off, so that its weight is no less than 2^kTopLog
@@ -556,7 +598,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged4_prompt_kernel(const 
           }
           // ---- weights, in pairs ----
           uint32_t h[UNIT / 2];
-          if (fabsf(nm) <= kFarScore) {
+          if (!__any_sync(0xffffffffu, wide || fabsf(nm) > kFarScore)) {
             uint64_t l2 = 0, l3 = 0;   // zeros
             const float base_e = nm + v_log;
             const uint64_t nm2 = pack2(base_e, base_e), fk2 = pack2(fk, fk);
@@ -577,9 +619,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged4_prompt_kernel(const 
             float ls = 0.f;
 #pragma unroll
             for (int e = 0; e < UNIT; e += 2) {
-              const float z0 = at_most(fmaf(y[e], fk, nm), kTopLog + 2.f - v_log), z1 = at_most(fmaf(y[e + 1], fk, nm), kTopLog + 2.f - v_log);
+              const float v0 = wide ? own[e].y : v_log, v1 = wide ? own[e + 1].y : v_log;
+              const float z0 = at_most(fmaf(y[e], fk, nm), kTopLog + 2.f - v0), z1 = at_most(fmaf(y[e + 1], fk, nm), kTopLog + 2.f - v1);
               ls += ex2(z0) + ex2(z1);
-              h[e / 2] = half2_bits(ex2(z0 + v_log), ex2(z1 + v_log));
+              h[e / 2] = half2_bits(ex2(z0 + v0), ex2(z1 + v1));
             }
             l += ls;
           }

@@ -935,3 +935,60 @@ def test_scores_whose_last_place_is_above_one(cuda, power, D, n):
             ref = b.ref(scale=scale)[1]
             # fp32's rounding of the sum and of its parts, and in prompts of the keys
             assert ((lse.double() - ref).abs() <= 4e-5 + 2e-6 * ref.abs() + 2.0 ** -11 * spread(b, scale=scale)[1]).all()
+
+
+def check_elements(b, launches, window=0):
+    """Each element against what its own row sees.  Scores are off by 2^-11 sum |q k| in prompts and weights and values by 2^-11
+    of themselves (the head), fp32 sums by 6e-5 of the same; a weight below fp16's normal numbers by 2^-25, where the largest
+    stands at 2^13 and a value at 2^15 at most, its vector's largest at 2^11 at least: 2^-34 for each of up to 900 keys."""
+    from siliconfer_b200 import _lib
+    from siliconfer_b200.paged_kv4 import paged4_attention
+    before = _lib.launch_count()
+    out, lse = paged4_attention(b.q, *b.args(), starts=b.starts, window=window, return_lse=True)
+    assert _lib.launch_count() - before == launches
+    ref, lref, _ = b.ref(window=window)
+    moved, size = spread(b, window=window)
+    bound = (1.02 * 2.0 ** -11 + 6e-5) * moved + 2.0 ** -24 * moved.amax(-1, keepdim=True) + OUT[b.dtype] * ref.abs() + 2.0 ** -25
+    assert ((out.double() - ref).abs() <= bound).all()
+    assert ((lse.double() - lref).abs() <= 4e-5 + 2e-6 * lref.abs() + 2.0 ** -11 * size).all()
+    assert _lib.load().sf_q4_check_device_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [3, 800])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("window", [0, 150])
+@pytest.mark.parametrize("dtype,gap", [(torch.bfloat16, 16), (torch.bfloat16, 24), (torch.bfloat16, 40), (torch.bfloat16, 90),
+                                       (torch.float16, 16)])
+def test_large_scales_that_a_row_does_not_see_cannot_reach_it(cuda, dtype, gap, window, D, n):
+    """Values or keys 2^gap above the others, of later tokens of the same call and of tokens before a row's window: whether a
+    row's tokens share a tile with them does not matter."""
+    for keys in (False, True):
+        b = Batch4([900], [n], 32, 8, D, 16, dtype)
+        s = b.ks if keys else b.vs
+        if dtype == torch.float16:
+            s *= 2.0 ** -8
+        for at in (40, 190, 333, 640, 897):
+            s[b.table[0, at // 16], :, at % 16] *= 2.0 ** gap
+        check_elements(b, 1 if n == 800 else 2, window)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [3, 800])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("apart", [12, 25, 40, 60])
+def test_scales_far_apart(cuda, apart, D, n):
+    """Between tokens, values and keys, zeros among them; up to 2^12 between the quarters of a vector, too."""
+    b = Batch4([900, 700], [n, n // 2], 32, 8, D, 16, torch.bfloat16)
+    power = lambda s, last: torch.exp2(torch.randint(-apart, 1, s.shape[:3] + (last,), generator=b.g, device="cuda")).bfloat16()
+    vs, ks = b.vs.clone(), b.ks.clone()
+    b.vs = vs * power(vs, 1)
+    check_elements(b, 1 if n == 800 else 2)
+    b.ks = ks * power(ks, 1)
+    check_elements(b, 1 if n == 800 else 2)
+    b.vs[:, :, ::5] = 0
+    b.ks[:, :, ::7] = 0
+    check_elements(b, 1 if n == 800 else 2)
+    if apart == 12:
+        b.vs, b.ks = vs * power(vs, 4), ks * power(ks, 4)
+        check_elements(b, 1 if n == 800 else 2)

@@ -542,7 +542,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged4_prompt_kernel(const 
           const float v_log = info.v_log;
           const bool wide = info.wide;
           const float2* own = powers + j % kSlots * UNIT;
-          if (wide) {
+          if (wide || f != f) {   // a NaN row's factor must not meet the -inf of keys that it does not see
 #pragma unroll
             for (int e = 0; e < UNIT; ++e) y[e] *= f * own[e].x;
             fk = 1.f;

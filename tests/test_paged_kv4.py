@@ -992,3 +992,19 @@ def test_scales_far_apart(cuda, apart, D, n):
     if apart == 12:
         b.vs, b.ks = vs * power(vs, 4), ks * power(ks, 4)
         check_elements(b, 1 if n == 800 else 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("n", [20, 800])
+@pytest.mark.parametrize("window", [0, 100])
+def test_padding_rows_whose_queries_are_not_finite(cuda, window, n, bad):
+    """Nine rows in front of their sequence's first token, in a tile with rows of tokens: they see nothing and are 0."""
+    from siliconfer_b200.paged_kv4 import paged4_attention
+    b = Batch4([n - 9, 700], [n, 100], 32, 8, 64, 16, torch.bfloat16)
+    good, lse = paged4_attention(b.q, *b.args(), starts=b.starts, window=window, return_lse=True)
+    b.q[:9, :, 3] = bad
+    b.q[:9, 5] = bad
+    out, l2 = paged4_attention(b.q, *b.args(), starts=b.starts, window=window, return_lse=True)
+    assert (out[:9] == 0).all() and (l2[:9] == -math.inf).all()
+    assert torch.equal(out, good) and torch.equal(l2, lse)

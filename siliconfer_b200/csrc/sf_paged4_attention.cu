@@ -10,13 +10,15 @@
 // One row of a kv head's group is one (new token, query head); a tile has 8 rows, so that a group reads its keys once.
 // Both products are mma.sync m16n8k16 in fp16 with the codes as the larger operand and the 8 rows as columns:
 //  * S^T[key, row] = K Q^T: 16 keys are the MMA's rows; each quarter of the head has sums of its own, which are added
-//    times the key's scale in fp32.  For 16-bit queries and outputs a pair of codes is a pair of fp16 subnormals n * 2^-24
-//    after one mask, and the sums begin at -8 times the sum of the quarter's queries.  The tensor cores align a subnormal
-//    as it stands, which leaves such sums 2^-17 of their largest product (measured on sums of one key); with fp32 among the
-//    types the codes become the numbers n - 8, at two instructions a pair more.  A query row is brought to at most 2^14 by a
-//    power of two; fp16 then holds a bf16 or fp16 row as it is, and two parts an fp32 row.
-//  * out^T[d, row] += V^T P^T: a quarter's weights are the softmax's times the key's scale of that quarter, in fp16 (with
-//    fp32 among the types in two parts, 22 bits), codes the numbers n - 8.
+//    times the key's scale in fp32.  A pair of codes becomes the numbers n - 8 at one mask and one sum.  (As they stand, n
+//    in a number's lowest bits, less 8 times the sum of the queries, they save the sum, 2 % of the time, but the tensor cores
+//    align such subnormals without their leading zeros: 2^-17 of the largest product is lost, 1e-3 of a log-sum where a few
+//    elements of a query stand out.)  A query row is brought to at most 2^14 by a power of two; fp16 then holds a bf16 or fp16
+//    row as it is, and two parts an fp32 row.
+//  * out^T[d, row] += V^T P^T: a quarter's weights are the softmax's times the key's scale of that quarter, codes the numbers
+//    n - 8.  Weights are fp16 numbers, 2^-12 of each at most, where queries and outputs have 16 bits: less than the output's
+//    own rounding for bf16, as much for fp16, where two parts take 0.1 more of the time.  With fp32 among the types: two
+//    parts, 22 bits.
 //
 // A warp takes its keys by itself: 32 at a time by bulk copies into a ring of its own, which brings a page's rows as they
 // lie, and no warp waits for another before the end of a part.  Measured in a graph, 64 query and 8 kv heads of 128, 16 x 8192
@@ -86,12 +88,7 @@ __device__ __forceinline__ uint32_t add_half2(uint32_t a, uint32_t b) {
   asm("add.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
-// quarter C's pair of codes of a word: fp16 numbers n * 2^-24 (C even) or n * 2^-20
-template <int C>
-__device__ __forceinline__ uint32_t codes_of(uint32_t w) {
-  return (C >= 2 ? w >> 8 : w) & (C % 2 ? 0x00f000f0u : 0x000f000fu);
-}
-// the codes less 8, times 1 or 16: the lowest bits of 1024 + n or 1024 + 16 n; magic is 0x64006400, in a register
+// quarter C's pair of codes of a word, less 8, times 1 or 16: the lowest bits of 1024 + n or 1024 + 16 n; magic is 0x64006400, in a register
 template <int C>
 __device__ __forceinline__ uint32_t centred(uint32_t w, uint32_t magic) {
   uint32_t x;
@@ -149,14 +146,12 @@ template <int D, int QP, int PP>
 __global__ void __launch_bounds__(kThreads, D <= 128 ? kCtas : 2) paged4_attention_kernel(const __grid_constant__ Attn4Args a, int q_pairs) {
   using L = Lay4<D>;
   constexpr int RT = 8, KW = L::KW, VW = L::VW, Q = L::Q, ST = L::STAGES;
-  constexpr bool FINE = PP == 2;   // keys' codes less 8, as the values'
   extern __shared__ __align__(128) uint8_t mem[];
   __shared__ long long wsum[kWarps];
   __shared__ float wm[kWarps][RT], wl[kWarps][RT];
   __shared__ __align__(8) uint64_t bars[kWarps][ST];
   __shared__ int abort_word;
   __shared__ __align__(16) uint32_t q_sm[4][QP][32 * KW];   // queries: lane's words of quarter c, part
-  __shared__ __align__(8) float less8[4][RT];               // -8 times the sum of the quarter's queries
   __shared__ uint32_t row_top[kWarps][RT];
   volatile int* abort_flag = &abort_word;
   SeqInfo* info = reinterpret_cast<SeqInfo*>(mem + L::INFO);
@@ -323,7 +318,6 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? kCtas : 2) paged4_attenti
       // the row's largest value to [2^13, 2^14) by a power of two
       const auto exponent = [](uint32_t x) { return min(max((int)(x >> 23) - 140, -126), 113); };
       const float down = __int_as_float((127 - exponent(top_of(g))) << 23) * (warp % 2 ? 0.0625f : 1.f);   // odd quarters' codes lie four bits higher
-      float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < KW; ++i) {
         float x = v[2 * i] * down, y = v[2 * i + 1] * down;
@@ -332,20 +326,16 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? kCtas : 2) paged4_attenti
           const uint32_t w = half2_bits(x, y);
           const float2 h = half2_floats(w);
           q_sm[warp][part][lane * KW + i] = w;
-          sum += h.x + h.y;
           x -= h.x;
           y -= h.y;
         }
       }
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      if (!FINE && t == 0) less8[warp][g] = sum * (warp % 2 ? -0x1p-17f : -0x1p-21f);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         // an infinity or a NaN: the row is NaN
         const uint32_t x = top_of(2 * t + e);
         f[e] = x >= 0x7f800000u ? __int_as_float(0x7fffffff)
-                                : __int_as_float((127 + exponent(x)) << 23) * (a.scale * kLog2e) * (FINE ? 1.f : 0x1p24f);
+                                : __int_as_float((127 + exponent(x)) << 23) * (a.scale * kLog2e);
       }
       __syncthreads();
     }
@@ -382,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? kCtas : 2) paged4_attenti
           uint32_t q[QP][KW];
 #pragma unroll
           for (int part = 0; part < QP; ++part) load_words<KW>(reinterpret_cast<const uint8_t*>(&q_sm[C][part][lane * KW]), q[part]);
-          const auto codes = [&](uint32_t x) { return FINE ? centred<C>(x, magic) : codes_of<C>(x); };
+          const auto codes = [&](uint32_t x) { return centred<C>(x, magic); };
 #pragma unroll
           for (int j = 0; j + 1 < KW; j += 2) {
             const uint32_t a0 = codes(w[0][j]), a1 = codes(w[1][j]), a2 = codes(w[0][j + 1]), a3 = codes(w[1][j + 1]);
@@ -395,12 +385,6 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? kCtas : 2) paged4_attenti
           if constexpr (KW % 2) {
 #pragma unroll
             for (int part = 0; part < QP; ++part) mma8(s, codes(w[0][KW - 1]), codes(w[1][KW - 1]), q[part][KW - 1]);
-          }
-          if constexpr (!FINE) {
-            const float2 less = *reinterpret_cast<const float2*>(&less8[C][2 * t]);
-            const uint64_t l2 = pack2(less.x, less.y);
-            unpack2(add2(pack2(s[0], s[1]), l2), s[0], s[1]);
-            unpack2(add2(pack2(s[2], s[3]), l2), s[2], s[3]);
           }
 #pragma unroll
           for (int e = 0; e < 4; ++e) y[n][e] = C == 0 ? s[e] * ks[e >> 1][C] : fmaf(s[e], ks[e >> 1][C], y[n][e]);

@@ -1008,3 +1008,22 @@ def test_padding_rows_whose_queries_are_not_finite(cuda, window, n, bad):
     out, l2 = paged4_attention(b.q, *b.args(), starts=b.starts, window=window, return_lse=True)
     assert (out[:9] == 0).all() and (l2[:9] == -math.inf).all()
     assert torch.equal(out, good) and torch.equal(l2, lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("H,Hkv,D", [(8, 2, 64), (64, 8, 128), (8, 8, 256), (4, 4, 96)])
+def test_queries_with_two_large_elements(cuda, H, Hkv, D, dtype):
+    """A hundred and fifty times the others, in each quarter.  A score's fp32 sums, some 32 of 2^-24 of sum |q k| each: 2^-19 of
+    it; a weight's and the log-sum's error is the scores'."""
+    from siliconfer_b200.paged_kv4 import paged4_attention
+    for at in (3, D // 4 + 1, D // 2 + 5, 3 * D // 4 + 7):
+        b = Batch4([700, 30, 1000], [1, 2, 1], H, Hkv, D, 16, dtype)
+        b.q[..., at] *= 100
+        b.q[..., at + 2] *= 50
+        out, lse = paged4_attention(b.q, *b.args(), starts=b.starts, return_lse=True)
+        ref, lref, _ = b.ref()
+        moved, size = spread(b)
+        off = 4e-5 + 2e-6 * lref.abs() + 2.0 ** -19 * size
+        assert ((lse.double() - lref).abs() <= off).all()
+        assert ((out.double() - ref).abs() <= (2 * off[..., None] + 2.0 ** -11) * moved + OUT[dtype] * ref.abs() + 2.0 ** -25).all()

@@ -51,6 +51,8 @@ class Fp8AttentionBlock(torch.nn.Module):
         ((codes, scales), residual): the normed input of what follows, and x plus the attention's output.
 
         ``positions`` [T], or [T, axes] with ``axes`` (``rotary_axes``), in place of the tokens' places in their sequences."""
+        if axes is not None and positions is None:
+            raise RuntimeError("axes need positions")
         T, H, Hkv, D = x.shape[0], self.heads, self.n_kv_heads, self.head_dim
         qkv = self.qkv(rms_norm_e4m3(x, self.norm_in, self.eps)).view(T, H + 2 * Hkv, D)
         q, k, v = qkv.split((H, Hkv, Hkv), 1)

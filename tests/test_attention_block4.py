@@ -128,3 +128,10 @@ def test_refuses_one_head_norm():
     with pytest.raises(RuntimeError, match="together"):
         Fp8AttentionBlock(torch.zeros(512, 256), torch.zeros(256, 256), torch.ones(256), torch.ones(256), 4, 2, device="cpu",
                           q_norm=torch.ones(64))
+
+
+def test_refuses_axes_without_positions():
+    from siliconfer_b200.attention_block import Fp8AttentionBlock
+    block = Fp8AttentionBlock(torch.zeros(512, 256), torch.zeros(256, 256), torch.ones(256), torch.ones(256), 4, 2, device="cpu")
+    with pytest.raises(RuntimeError, match="positions"):
+        block(torch.zeros(1, 256), None, None, None, None, axes=torch.zeros(32, dtype=torch.uint8))

@@ -393,6 +393,15 @@ int sf_qk_norm_rotary(const void* q, long long qts, long long qhs, void* q_out, 
                       int dtype, const void* q_weight, const void* k_weight, int w_dtype, double eps,
                       const void* positions, int pos64, int axes_n, const uint8_t* axes, const float* table, int max_pos,
                       int rot, int interleaved, int T, int D, void* stream);
+/* The same for rows that hold the last tokens of sequences, as in a call on a paged cache: seq_lens [batch], starts
+ * [batch + 1] or NULL (then T is a multiple of batch).  A row that holds none (padding) is turned as at position 0
+ * whatever positions says.  starts that fall or leave the rows, and lengths below 0: SF_ERR_INDEX at the next check. */
+int sf_qk_norm_rotary_rows(const void* q, long long qts, long long qhs, void* q_out, long long qots, long long qohs, int H,
+                           const void* k, long long kts, long long khs, void* k_out, long long kots, long long kohs, int Hkv,
+                           int dtype, const void* q_weight, const void* k_weight, int w_dtype, double eps,
+                           const void* positions, int pos64, int axes_n, const uint8_t* axes, const float* table, int max_pos,
+                           int rot, int interleaved, int T, int D, const int* seq_lens, const int* starts, int batch,
+                           void* stream);
 
 /* ---- a paged cache in 4 bits --------------------------------------------------------
  * The e4m3 cache's tokens, pages and rules (sf_paged_cache), with another content:

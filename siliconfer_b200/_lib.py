@@ -84,6 +84,8 @@ SIGNATURES = {
     "sf_paged_attention": [ctypes.POINTER(PagedCache), _P, _I, _LL, _LL, _P, _I, _P, _I, _I, _F, _I, _P, _SZ, _P],
     "sf_qk_norm_rotary": [_P, _LL, _LL, _P, _LL, _LL, _I, _P, _LL, _LL, _P, _LL, _LL, _I, _I, _P, _P, _I, _DB, _P, _I, _I,
                           _P, _P, _I, _I, _I, _I, _I, _P],
+    "sf_qk_norm_rotary_rows": [_P, _LL, _LL, _P, _LL, _LL, _I, _P, _LL, _LL, _P, _LL, _LL, _I, _I, _P, _P, _I, _DB, _P, _I,
+                               _I, _P, _P, _I, _I, _I, _I, _I, _P, _P, _I, _P],
     "sf_paged4_append": [ctypes.POINTER(Paged4Cache), _P, _LL, _LL, _P, _LL, _LL, _P, _LL, _LL, _P, _I, _I, _I, _P, _P,
                          _I, _DB, _P, _I, _I, _P, _P, _I, _I, _I, _P],
     "sf_paged4_attention_workspace_bytes": [_I],

@@ -1,12 +1,15 @@
 """The attention half of a decoder layer in 8 bits: norm, projections, rotary positions, paged cache, attention.
 
-Six kernels a call, and nothing between them: the norm's codes are the fused
+Six kernels a call (with one more where the 8-bit cache's query and key heads
+are normed or positions are given), and nothing between them: the norm's codes are the fused
 projection's input, whose output's slices (queries, keys, values, not copied)
 go into the cache with their positions and to the attention, and the norm after
 the output projection adds the residual and hands the next layer its codes.
 
 The cache is held in 8 bits (``PagedKVCache``) or in 4 (``Paged4KVCache``, which
-norms and turns query and key heads in its append).
+norms and turns query and key heads in its append).  Keys that the 8-bit cache
+gets normed, or turned by given positions, are rounded to the block's type on the
+way; else, and in the 4-bit cache, they are rounded once, to their codes.
 
     python -m siliconfer_b200.attention_block
 
@@ -50,7 +53,8 @@ class Fp8AttentionBlock(torch.nn.Module):
         """x [T, hidden], the last tokens of their sequences (``PagedKVCache`` or ``Paged4KVCache``) ->
         ((codes, scales), residual): the normed input of what follows, and x plus the attention's output.
 
-        ``positions`` [T], or [T, axes] with ``axes`` (``rotary_axes``), in place of the tokens' places in their sequences."""
+        ``positions`` [T], or [T, axes] with ``axes`` (``rotary_axes``), in place of the tokens' places in their sequences;
+        those of rows that hold no token are not looked at."""
         if axes is not None and positions is None:
             raise RuntimeError("axes need positions")
         T, H, Hkv, D = x.shape[0], self.heads, self.n_kv_heads, self.head_dim
@@ -61,7 +65,7 @@ class Fp8AttentionBlock(torch.nn.Module):
             q = cache.append(k, v, block_table, seq_lens, starts, q=q, table=table, interleaved=self.interleaved,
                              positions=positions, axes=axes, q_weight=self.q_norm, k_weight=self.k_norm, eps=head_eps)
         elif positions is not None:
-            q, k = qk_norm_rotary(q, k, positions, table, self.q_norm, self.k_norm, head_eps, self.interleaved, axes)
+            q, k = qk_norm_rotary(q, k, positions, table, self.q_norm, self.k_norm, head_eps, self.interleaved, axes, seq_lens, starts)
             cache.append(k, v, block_table, seq_lens, starts)
         else:
             if head_eps is not None:

@@ -56,8 +56,7 @@ struct HeadArgs {
   int pos64, axes_n;
   const uint8_t* axes;  // [rot / 2] or NULL: all pairs belong to axis 0
   int H, Hkv, T, D;
-  // the cache's
-  sf_paged_cache c;
+  sf_paged_cache c;     // the cache's; without one, which rows are tokens where seq_lens is given
   __nv_bfloat16 *ks, *vs;
 };
 
@@ -254,7 +253,8 @@ __global__ void __launch_bounds__(kThreads, CACHE && sizeof(TX) == 4 ? 3 : 4) no
   load(first);
 
   // ---- the token's place and angles ----
-  if (CACHE) {
+  const bool rows_known = CACHE || a.c.seq_lens;
+  if (rows_known) {
     if (tid < 32) {
       const TokenAt at = token_at(a.c, a.T, tok);
       if (tid == 0) {
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, CACHE && sizeof(TX) == 4 ? 3 : 4) no
           atomicOr(&g_dev_error, kErrIndex);
         } else if (at.pos < 0) {
           p.pos = -2;
-        } else {
+        } else if (CACHE) {
           p.pos = at.pos;
           const int page = a.c.block_table[(size_t)at.b * a.c.pages_per_seq + at.pos / a.c.page_size];
           p.put = page >= 0 && page < a.c.num_pages;
@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(kThreads, CACHE && sizeof(TX) == 4 ? 3 : 4) no
   const int half = a.rot / 2;
   for (int j = tid; j < half; j += blockDim.x) {
     long long p;
-    if (CACHE && place.pos == -2) {
+    if (rows_known && place.pos == -2) {
       p = 0;   // a padding row's positions are nobody's
     } else if (a.positions) {
       const int axis = a.axes ? a.axes[j] : 0;
@@ -531,11 +531,12 @@ using namespace sf;
 
 extern "C" {
 
-int sf_qk_norm_rotary(const void* q, long long qts, long long qhs, void* q_out, long long qots, long long qohs, int H,
-                      const void* k, long long kts, long long khs, void* k_out, long long kots, long long kohs, int Hkv,
-                      int dtype, const void* q_weight, const void* k_weight, int w_dtype, double eps,
-                      const void* positions, int pos64, int axes_n, const uint8_t* axes, const float* table, int max_pos,
-                      int rot, int interleaved, int T, int D, void* stream) {
+int sf_qk_norm_rotary_rows(const void* q, long long qts, long long qhs, void* q_out, long long qots, long long qohs, int H,
+                           const void* k, long long kts, long long khs, void* k_out, long long kots, long long kohs, int Hkv,
+                           int dtype, const void* q_weight, const void* k_weight, int w_dtype, double eps,
+                           const void* positions, int pos64, int axes_n, const uint8_t* axes, const float* table, int max_pos,
+                           int rot, int interleaved, int T, int D, const int* seq_lens, const int* starts, int batch,
+                           void* stream) {
   if (T < 0 || H < 0 || Hkv < 0) return fail(SF_ERR_SHAPE, "need T, H, Hkv >= 0");
   if (D < 4 || D % 4 || D > (D % 16 == 0 ? 512 : D % 8 == 0 ? 256 : 128))
     return fail(SF_ERR_UNSUPPORTED, "head_dim %d not built (multiples of 16 up to 512, of 8 up to 256, of 4 up to 128)", D);
@@ -552,6 +553,17 @@ int sf_qk_norm_rotary(const void* q, long long qts, long long qhs, void* q_out, 
   a.positions = positions; a.pos64 = pos64; a.axes_n = axes_n; a.axes = axes;
   a.H = H; a.Hkv = Hkv; a.T = T; a.D = D;
   if (int rc = check_args(a, dtype)) return rc;
+  if (seq_lens) {
+    if (batch < 1) return fail(SF_ERR_SHAPE, "need batch >= 1");
+    if (!starts && T % batch) return fail(SF_ERR_SHAPE, "without starts, T must be a multiple of batch");
+    a.c.seq_lens = seq_lens;
+    a.c.starts = starts;
+    a.c.batch = batch;
+    a.c.page_size = 1;
+    a.c.pages_per_seq = 0x7fffffff;   // a sequence of any length: it has no pages here
+  } else if (starts) {
+    return fail(SF_ERR_NULL, "starts without seq_lens");
+  }
   if (T == 0 || H + Hkv == 0) return SF_OK;
   if ((H && (!q || !q_out)) || (Hkv && (!k || !k_out)) || (rot && !positions)) return fail(SF_ERR_NULL, "null pointer argument");
   if (!strides_ok({qhs, qohs, khs, kohs})) return fail(SF_ERR_UNSUPPORTED, "a head stride above 2^31 - 1 elements");
@@ -573,6 +585,16 @@ int sf_qk_norm_rotary(const void* q, long long qts, long long qhs, void* q_out, 
   if (e != cudaSuccess) return cuda_fail(e, "norm_turn_kernel launch");
   g_launches.fetch_add(1, std::memory_order_relaxed);
   return SF_OK;
+}
+
+int sf_qk_norm_rotary(const void* q, long long qts, long long qhs, void* q_out, long long qots, long long qohs, int H,
+                      const void* k, long long kts, long long khs, void* k_out, long long kots, long long kohs, int Hkv,
+                      int dtype, const void* q_weight, const void* k_weight, int w_dtype, double eps,
+                      const void* positions, int pos64, int axes_n, const uint8_t* axes, const float* table, int max_pos,
+                      int rot, int interleaved, int T, int D, void* stream) {
+  return sf_qk_norm_rotary_rows(q, qts, qhs, q_out, qots, qohs, H, k, kts, khs, k_out, kots, kohs, Hkv, dtype, q_weight,
+                                k_weight, w_dtype, eps, positions, pos64, axes_n, axes, table, max_pos, rot, interleaved, T, D,
+                                nullptr, nullptr, 0, stream);
 }
 
 int sf_paged4_append(const sf_paged4_cache* cache, const void* k, long long kts, long long khs, const void* v,

@@ -438,7 +438,7 @@ TurnArgs turn_args(const OptTensor& table, const OptTensor& positions, const Opt
 std::tuple<at::Tensor, OptTensor> qk_norm_rotary(const at::Tensor& q, const OptTensor& k, const OptTensor& positions,
                                                  const OptTensor& table, const OptTensor& wq, const OptTensor& wk,
                                                  c10::optional<double> eps, bool interleaved, const OptTensor& axes,
-                                                 const OptTensor& out) {
+                                                 const OptTensor& out, const OptTensor& lens, const OptTensor& starts) {
   TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor");
   TORCH_CHECK(q.dim() == 3 && q.size(2) >= 1, "q must be [T, heads, head_dim]");
   const int64_t T = q.size(0), D = q.size(2);
@@ -469,13 +469,30 @@ std::tuple<at::Tensor, OptTensor> qk_norm_rotary(const at::Tensor& q, const OptT
     ki = head_rows(*k);
     ko = empty_on(k->sizes(), k->scalar_type(), q);
   }
+  const int *len_ptr = nullptr, *start_ptr = nullptr;
+  int64_t batch = 0;
+  TORCH_CHECK(given(lens) || !given(starts), "starts need seq_lens");
+  if (given(lens)) {
+    on_device(*lens, q, "seq_lens");
+    batch = lens->dim() == 1 ? lens->size(0) : 0;
+    TORCH_CHECK(lens->scalar_type() == at::kInt && batch >= 1 && batch <= INT_MAX, "seq_lens must be int32 [batch]");
+    keep.push_back(lens->contiguous());
+    len_ptr = keep.back().data_ptr<int>();
+  }
+  if (given(starts)) {
+    on_device(*starts, q, "starts");
+    TORCH_CHECK(starts->scalar_type() == at::kInt && starts->dim() == 1 && starts->size(0) == batch + 1,
+                "starts must be int32 [batch + 1]");
+    keep.push_back(starts->contiguous());
+    start_ptr = keep.back().data_ptr<int>();
+  }
   const bool has = ki.defined();
-  check(sf_qk_norm_rotary(qi.data_ptr(), qi.stride(0), qi.stride(1), qo.data_ptr(), qo.stride(0), qo.stride(1),
-                          (int)q.size(1), has ? ki.data_ptr() : nullptr, has ? ki.stride(0) : 0, has ? ki.stride(1) : 0,
-                          has ? ko.data_ptr() : nullptr, has ? ko.stride(0) : 0, has ? ko.stride(1) : 0,
-                          has ? (int)ki.size(1) : 0, dtype_code(q.scalar_type()), a.wq, a.wk, a.w_dtype, a.eps,
-                          a.positions, a.pos64, a.axes_n, a.axes, a.table, a.max_pos, a.rot, interleaved, (int)T, (int)D,
-                          stream_of(q)));
+  check(sf_qk_norm_rotary_rows(qi.data_ptr(), qi.stride(0), qi.stride(1), qo.data_ptr(), qo.stride(0), qo.stride(1),
+                               (int)q.size(1), has ? ki.data_ptr() : nullptr, has ? ki.stride(0) : 0,
+                               has ? ki.stride(1) : 0, has ? ko.data_ptr() : nullptr, has ? ko.stride(0) : 0,
+                               has ? ko.stride(1) : 0, has ? (int)ki.size(1) : 0, dtype_code(q.scalar_type()), a.wq, a.wk,
+                               a.w_dtype, a.eps, a.positions, a.pos64, a.axes_n, a.axes, a.table, a.max_pos, a.rot,
+                               interleaved, (int)T, (int)D, len_ptr, start_ptr, (int)batch, stream_of(q)));
   return {qo, has ? OptTensor(ko) : OptTensor()};
 }
 

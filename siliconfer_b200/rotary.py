@@ -91,18 +91,21 @@ def apply_rotary(x, positions, table, interleaved: bool = False, out=None, axes=
     width, and pair j is turned by the position of axis axes[j]."""
     if axes is None:
         return _lib.ext().rotary(x, positions, table, interleaved, out)
-    return _lib.ext().qk_norm_rotary(x, None, positions, table, None, None, None, interleaved, axes, out)[0]
+    return _lib.ext().qk_norm_rotary(x, None, positions, table, None, None, None, interleaved, axes, out, None, None)[0]
 
 
 def qk_norm_rotary(q, k, positions=None, table=None, q_weight=None, k_weight=None, eps=1e-6, interleaved: bool = False,
-                   axes=None):
+                   axes=None, seq_lens=None, starts=None):
     """RMS norm of each query and key head, then ``apply_rotary``, in one pass -> (q, k), in their type.
 
     q [T, heads, head_dim], k [T, n_kv_heads, head_dim] (or None); weights
     [head_dim] (None: ones); ``eps`` None leaves the norm out, ``table`` None the
     rotation.  fp32 arithmetic, rounded once.  head_dim a multiple of 16 up to
-    512, of 8 up to 256 or of 4 up to 128."""
-    return _lib.ext().qk_norm_rotary(q, k, positions, table, q_weight, k_weight, eps, interleaved, axes, None)
+    512, of 8 up to 256 or of 4 up to 128.  With ``seq_lens`` [batch] (and
+    ``starts``) the rows are sequences' last tokens, packed as in ``paged_kv``,
+    and rows that hold none are turned as at position 0 whatever ``positions``
+    says."""
+    return _lib.ext().qk_norm_rotary(q, k, positions, table, q_weight, k_weight, eps, interleaved, axes, None, seq_lens, starts)
 
 
 __all__ = ["rotary_frequencies", "rotary_table", "rotary_axes", "apply_rotary", "qk_norm_rotary"]

@@ -135,3 +135,42 @@ def test_refuses_axes_without_positions():
     block = Fp8AttentionBlock(torch.zeros(512, 256), torch.zeros(256, 256), torch.ones(256), torch.ones(256), 4, 2, device="cpu")
     with pytest.raises(RuntimeError, match="positions"):
         block(torch.zeros(1, 256), None, None, None, None, axes=torch.zeros(32, dtype=torch.uint8))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("four", [True, False])
+@pytest.mark.parametrize("packed", [True, False])
+@pytest.mark.parametrize("n_axes", [0, 2])
+def test_positions_of_padding_rows_are_not_looked_at(cuda, n_axes, packed, four):
+    """Positions outside the table in rows that hold no token: no error with either cache, and the other rows as they were."""
+    from siliconfer_b200 import _lib
+    from siliconfer_b200.attention_block import Fp8AttentionBlock
+    from siliconfer_b200.paged_kv import PagedKVCache
+    from siliconfer_b200.paged_kv4 import Paged4KVCache
+    from siliconfer_b200.rotary import rotary_axes, rotary_table
+    g = torch.Generator(device="cuda").manual_seed(1)
+    rand = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    block = Fp8AttentionBlock(rand(512, 256) / 16, rand(256, 256) / 16, torch.ones(256), torch.ones(256), 4, 2, q_norm=rand(64),
+                              k_norm=rand(64))
+    table, axes = rotary_table(40, 64), rotary_axes([20, 12]) if n_axes else None
+    pages = torch.arange(8, dtype=torch.int32, device="cuda").view(2, 4)
+    if packed:      # two rows before the first token, three behind the last, and two of sequence 0 before its first token
+        starts, lens = torch.tensor([2, 9, 12], dtype=torch.int32, device="cuda"), torch.tensor([5, 30], dtype=torch.int32, device="cuda")
+        real, T = [*range(4, 9), 9, 10, 11], 15
+    else:
+        starts, lens, real, T = None, torch.tensor([3, 20], dtype=torch.int32, device="cuda"), [2, 3, 4, *range(5, 10)], 10
+    x = rand(T, 256).bfloat16()
+    pos = torch.randint(0, 40, (T, n_axes) if n_axes else (T,), generator=g, device="cuda")
+    results = []
+    for fill in (None, -1, 10 ** 6):
+        rest = torch.ones(T, dtype=torch.bool, device="cuda")
+        rest[real] = False
+        if fill is not None:
+            pos[rest] = fill
+        cache = (Paged4KVCache if four else PagedKVCache)(8, 2, 64, 16)
+        (codes, scales), h = block(x, cache, pages, lens, table, starts, pos, axes)
+        assert _lib.load().sf_q4_check_device_error() == 0
+        results.append((codes[real].double(), scales[real], h[real], cache.k_codes.double(), cache.k_scales, cache.v_codes.double()))
+        assert torch.isfinite(h.float()).all()
+    for other in results[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(results[0], other))

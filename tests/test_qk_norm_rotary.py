@@ -274,3 +274,48 @@ def test_eps_below_fp32(cuda, dtype):
     for eps in (1e-40, 1e-60, 1e-300):
         q, k = qk_norm_rotary(x, x[:, :1], eps=eps)
         assert not q.any() and not k.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_of_sequences(cuda, dtype):
+    """With the sequences' lengths: tokens as without them, rows that hold none as at position 0, packed rows or not."""
+    from siliconfer_b200 import _lib
+    lib = _lib.load()
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    for axes, lens, starts, real in ((1, ints(9, 0, 2), ints(3, 7, 9, 12), [*range(3, 7), 10, 11]), (3, ints(9, 1, 2, 40, 5), None, [*range(0, 3), 5, 7, 8, *range(9, 15)]),
+                                     (2, torch.full((15,), 7, dtype=torch.int32, device="cuda"), None, list(range(15)))):
+        c, ax = case(15, 6, 2, 64, dtype, axes)
+        want = check(c, ax)
+        zero = qk_norm_rotary(**{**c, "positions": torch.zeros_like(c["positions"])}, axes=ax)
+        rest = torch.ones(15, dtype=torch.bool, device="cuda")
+        rest[real] = False
+        c["positions"][rest] = 10 ** 6
+        got = qk_norm_rotary(**c, axes=ax, seq_lens=lens, starts=starts)
+        assert lib.sf_q4_check_device_error() == 0
+        for a, b, z in zip(got, want, zero):
+            assert torch.equal(a[~rest], b[~rest]) and torch.equal(a[rest], z[rest])
+        if starts is None:
+            lens[0] = -1
+        else:
+            starts[0] = 20
+        got = qk_norm_rotary(**{**c, "positions": torch.zeros_like(c["positions"])}, axes=ax, seq_lens=lens, starts=starts)
+        torch.cuda.synchronize()
+        assert lib.sf_q4_check_device_error() == 10 and all(torch.equal(a, z) for a, z in zip(got, zero))
+    run = lambda **kw: qk_norm_rotary(**{**c, **kw}, axes=ax)
+    for bad in (dict(starts=ints(0, 15)), dict(seq_lens=ints(1, 2)), dict(seq_lens=ints(5).long()), dict(seq_lens=ints(5).cpu()),
+                dict(seq_lens=ints(5).view(1, 1)), dict(seq_lens=ints(5), starts=ints(0, 5, 15)), dict(seq_lens=ints()),
+                dict(seq_lens=ints(5), starts=ints(0, 15).long())):
+        with pytest.raises(RuntimeError):
+            run(**bad)
+
+
+def test_validation_of_rows_without_gpu():
+    from siliconfer_b200 import _lib
+    lib, F = _lib.load(), 0x1000
+    base = dict(q=F, qts=64, qhs=64, qo=F, qots=64, qohs=64, H=1, k=F, kts=64, khs=64, ko=F, kots=64, kohs=64, Hkv=1, dt=0, wq=None,
+                wk=None, wt=0, eps=1e-6, pos=F, p64=0, an=1, ax=None, table=F, mp=8, rot=64, inter=0, T=3, D=64, lens=F, starts=None, n=1,
+                st=None)
+    call = lambda **k: lib.sf_qk_norm_rotary_rows(*{**base, **k}.values())
+    for kw, want in ((dict(n=0), 2), (dict(n=2), 2), (dict(lens=None, starts=F), 1), (dict(T=-1), 2), (dict(pos=None), 1), (dict(T=0), 0)):
+        assert call(**kw) == want, kw

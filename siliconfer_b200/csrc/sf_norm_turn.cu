@@ -540,6 +540,8 @@ int sf_qk_norm_rotary_rows(const void* q, long long qts, long long qhs, void* q_
   if (T < 0 || H < 0 || Hkv < 0) return fail(SF_ERR_SHAPE, "need T, H, Hkv >= 0");
   if (D < 4 || D % 4 || D > (D % 16 == 0 ? 512 : D % 8 == 0 ? 256 : 128))
     return fail(SF_ERR_UNSUPPORTED, "head_dim %d not built (multiples of 16 up to 512, of 8 up to 256, of 4 up to 128)", D);
+  if (H <= 1) qhs = qohs = 0;   // no second head: never used
+  if (Hkv <= 1) khs = kohs = 0;
   HeadArgs a{};
   a.q = Vectors{q, qts, (int)qhs};
   a.k = Vectors{k, kts, (int)khs};
@@ -605,6 +607,8 @@ int sf_paged4_append(const sf_paged4_cache* cache, const void* k, long long kts,
   HeadArgs a{};
   if (int rc = check_paged4(cache, T, a.c)) return rc;
   const int D = cache->head_dim;
+  if (H <= 1) qhs = 0;   // no second head: never used
+  if (cache->n_kv_heads == 1) khs = vhs = 0;
   a.q = Vectors{q, qts, (int)qhs};
   a.k = Vectors{k, kts, (int)khs};
   a.v = Vectors{v, vts, (int)vhs};

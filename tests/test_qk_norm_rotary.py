@@ -319,3 +319,31 @@ def test_validation_of_rows_without_gpu():
     call = lambda **k: lib.sf_qk_norm_rotary_rows(*{**base, **k}.values())
     for kw, want in ((dict(n=0), 2), (dict(n=2), 2), (dict(lens=None, starts=F), 1), (dict(T=-1), 2), (dict(pos=None), 1), (dict(T=0), 0)):
         assert call(**kw) == want, kw
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_one_head_of_any_stride(cuda, dtype):
+    """Where there is one head nothing steps from it to the next."""
+    from siliconfer_b200.paged_kv4 import Paged4KVCache
+    x = torch.randn(4, 1, 64, device="cuda").to(dtype)
+    far = x.as_strided((4, 1, 64), (64, 2 ** 31 + 67, 1))
+    assert far.stride(1) > 2 ** 31
+    for a, b in zip(qk_norm_rotary(x, x), qk_norm_rotary(far, far)):
+        assert torch.equal(a, b)
+    held = []
+    for y in (x, far):
+        cache = Paged4KVCache(4, 1, 64, 16)
+        q = cache.append(y, y, torch.arange(4, dtype=torch.int32, device="cuda").view(4, 1),
+                         torch.ones(4, dtype=torch.int32, device="cuda"), q=y, eps=1e-6)
+        held.append((q, cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales))
+    assert all(torch.equal(a, b) for a, b in zip(*held))
+
+
+def test_head_strides_past_31_bits_are_refused_without_gpu():
+    from siliconfer_b200 import _lib
+    lib, F, far = _lib.load(), 0x1000, 1 << 31
+    base = dict(q=F, qts=64, qhs=64, qo=F, qots=64, qohs=64, H=2, k=F, kts=64, khs=64, ko=F, kots=64, kohs=64, Hkv=2, dt=0, wq=None,
+                wk=None, wt=0, eps=1e-6, pos=F, p64=0, an=1, ax=None, table=F, mp=8, rot=64, inter=0, T=1, D=64, st=None)
+    for kw in (dict(qhs=far), dict(qohs=far), dict(khs=far), dict(kohs=far)):
+        assert lib.sf_qk_norm_rotary(*{**base, **kw}.values()) == 6, kw

@@ -364,7 +364,18 @@ __global__ void __launch_bounds__(kThreads, CACHE && sizeof(TX) == 4 ? 3 : 4) no
         for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int i = 0; i < W; ++i) y[c][i] = (float)z[c][i];
-        const bool finite = quarter_tops<GP, W>(y, top) < 0x7f800000u;
+        bool finite = quarter_tops<GP, W>(y, top) < 0x7f800000u;
+        uint32_t up = 0;   // what its scales' bits are short of
+        if (__any_sync(0xffffffffu, !finite)) {   // a number past fp32's range, which a turn makes, is one: a 16th of it is cut
+          up = finite ? 0u : 4u << 7;
+          const double down = finite ? 1.0 : 0x1p-4;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < W; ++i) y[c][i] = (float)(z[c][i] *= down);
+          finite = quarter_tops<GP, W>(y, top) < 0x7f800000u;
+          if (!finite) up = 0;
+        }
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           float s = scale_of(__uint_as_float(top[c]));
@@ -383,6 +394,7 @@ __global__ void __launch_bounds__(kThreads, CACHE && sizeof(TX) == 4 ? 3 : 4) no
           const double s64 = s, near_inv = __frcp_rn(s), inv = near_inv * fma(-s64, near_inv, 2.0);
 #pragma unroll
           for (int i = 0; i < W; ++i) words[i] += code_of(z[c][i], s64, inv) * (1 << 4 * c);
+          if (sb[c] != 0x0080u) sb[c] += up;   // but the least scale, of zeros
         }
         if (there && put) store_codes(a, slot, 1, h, r0, finite, words, sb);
         continue;

@@ -1027,3 +1027,20 @@ def test_queries_with_two_large_elements(cuda, H, Hkv, D, dtype):
         off = 4e-5 + 2e-6 * lref.abs() + 2.0 ** -19 * size
         assert ((lse.double() - lref).abs() <= off).all()
         assert ((out.double() - ref).abs() <= (2 * off[..., None] + 2.0 ** -11) * moved + OUT[dtype] * ref.abs() + 2.0 ** -25).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_append_keys_that_a_turn_takes_past_fp32(cuda, dtype):
+    """3.3e38 (cos + sin) is a number in 64 bits and its scale one in bf16; an infinity beside such numbers stays one."""
+    def values(k, v):
+        for x in (k, v):
+            x[:9] = (3.3e38 * x[:9].sign().float()).to(dtype)
+            x[9] = (x[9].float() * 1.2e38).clamp(-3.3e38, 3.3e38).to(dtype)
+            x[10, 0, 3:30] = 3.3e38
+            x[13], x[13, 0, 1], x[13, 0, -3] = 0, 3.3e38, -3.3e38
+            x[11, 1, 40], x[12, 0, 7] = float("inf"), float("nan")
+            x[11, 1, 41:], x[12, 0, :5] = -3.3e38, 3.3e38
+    for D in (64, 96, 128, 256):
+        for kw in (dict(), dict(interleaved=True), dict(rot=D // 2), dict(rot=20)):
+            check_append(Batch4([40, 30], [20, 5], 4, 2, D, 16, dtype), dtype, values=values, with_q=False, **kw)

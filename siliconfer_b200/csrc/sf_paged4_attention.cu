@@ -685,7 +685,7 @@ int launch4(Attn4Args a, cudaStream_t st) {
   return SF_OK;
 }
 
-constexpr int kMaxCtasPerSm = 4;
+constexpr int kMaxCtasPerSm = kCtas;
 
 #include "sf_paged4_prompt.h"
 

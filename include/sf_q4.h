@@ -436,8 +436,13 @@ int sf_paged4_append(const sf_paged4_cache* cache, const void* k, long long kts,
                      const void* positions, int pos64, int axes_n, const uint8_t* axes, const float* table, int max_pos,
                      int rot, int interleaved, void* stream);
 
-/* sf_paged_attention over this cache.  Value scales up to 2^100.  A row that sees a key
- * or value vector with NaN scales is NaN as a whole. */
+/* sf_paged_attention over this cache.  A row that sees a key or value vector with NaN
+ * scales is NaN as a whole.  Value scales from 2^-60 to 2^100; smaller ones lose digits,
+ * and values below 2^-80 may count as 0.  Scales may lie any number of powers of two apart
+ * between tokens; within a vector, a quarter's scale 2^20 and more below the largest loses
+ * digits.  16-bit queries and outputs: weights are fp16 numbers, and in long runs keys and
+ * values are rounded to 11 bits, so that a score, and lse, is off by up to 2^-12 of
+ * sum |q k| there. */
 size_t sf_paged4_attention_workspace_bytes(int head_dim);
 int sf_paged4_attention(const sf_paged4_cache* cache, const void* q, int q_dtype, long long qts, long long qhs, void* out,
                         int out_dtype, float* lse, int H, int T, float scale, int window, void* workspace,

@@ -9,9 +9,11 @@
 // all four quarters: these hold both elements of its rotary pairs, and the codes of a place are one 16-bit word.
 //
 // Measured in a graph: 4096 tokens, 64 query and 8 kv heads of 128, three axes, norms: turned 32 us (4.8 TB/s of the copy
-// rate's 6.5), appended 40 us (3.9 TB/s); one token 2.6 us, 8 tokens of 32 heads appended 4.0.  Bound by instructions: some
-// 300 a warp for four heads.  A warp takes up to 10 passes in turn (3: 39 us, 6: 33); keys are normed, turned and cut in fp64,
-// which the 64-bit units do beside the rest, so that a code is the exact value's.
+// rate's 6.5), appended 40 us (3.9 TB/s); one token 2.6 us, 8 tokens of 32 heads appended 4.0.  No unit is full: a turn uses
+// 66 % of the issue slots and 39 % of DRAM's time with 6.8 warps a scheduler, which wait for shared memory and shuffles (0.32
+// of a warp's time between two instructions), for fixed latencies (0.17) and for each other's turn (0.16); an append 66 % and
+// 33 %, fp64 units 6 %, conversions 19 %.  A warp takes up to 10 passes in turn (3: 39 us, 6: 33); keys are normed, turned
+// and cut in fp64, which the 64-bit units do beside the rest, so that a code is the exact value's.
 #include <algorithm>
 #include <atomic>
 #include <cfloat>

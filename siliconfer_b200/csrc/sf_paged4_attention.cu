@@ -5,7 +5,8 @@
 // The softmax keeps a running reference m and sum l of e^(score - m): keys in order, out and l are multiplied by
 // e^(m - m') when the reference moves to m'.  Parts of a row's keys, a warp's, a CTA's, merge by the same rule.  m is a
 // largest score plus the logarithm of its value vector's largest scale; it moves only when a key would exceed it by a
-// factor of 2, so that a weight times a scale is bounded and most keys need no reduction over the lanes.
+// factor of 2, so that a weight times a scale is bounded and most keys need no reduction over the lanes.  Scales below 2^-60
+// count as 2^-60 there, or l would pass fp32's range: their weights, which stay in fp16, lose digits.
 //
 // One row of a kv head's group is one (new token, query head); a tile has 8 rows, so that a group reads its keys once.
 // Both products are mma.sync m16n8k16 in fp16 with the codes as the larger operand and the 8 rows as columns:
@@ -22,12 +23,13 @@
 //
 // A warp takes its keys by itself: 32 at a time by bulk copies into a ring of its own, which brings a page's rows as they
 // lie, and no warp waits for another before the end of a part.  Measured in a graph, 64 query and 8 kv heads of 128, 16 x 8192
-// keys 53 us (2.9 TB/s), one sequence of 131072 with 32 query heads 57; 32 heads of their own, 64 sequences of up to 4096
-// keys 217 (3.0 TB/s).  Bound by instructions: some 400 a warp for 16 keys, of which unpacking the codes takes 120 (integer
-// units 50 % in use, issue slots 56 %).  On the way, 16 x 8192 and 64 x 4096 keys in us: copies by each lane, 16 keys at a
-// time, 128 registers and 4 CTAs an SM 71 and 289; by bulk 65 and 261; queries in shared memory 60 and 235; 32 keys at a time,
-// 168 registers and 3 CTAs 53 and 241, and with fp16 weights in one part for
-// fp16 queries 217; at 128 registers 60 and 207.
+// keys 54 us (2.8 TB/s), one sequence of 131072 with 32 query heads 58; 32 heads of their own, 64 sequences of up to 4096
+// keys 222 (3.0 TB/s).  What bounds it: three warps a scheduler, each one chain of load, mask, product, exponential and
+// product, some 440 instructions for 16 keys.  At 16 x 8192 issue slots are 58 % and integer units 49 % in use, DRAM 35 %; of
+// the time from one instruction of a warp to the next 0.25 is fixed latency, 0.21 its turn, 0.16 loads, 0.15 the others' turn.
+// On the way, 16 x 8192 and 64 x 4096 keys in us, keys' codes as subnormals: copies by each lane, 16 keys at a time, 128
+// registers and 4 CTAs an SM 71 and 289; by bulk 65 and 261; queries in shared memory 60 and 235; 32 keys at a time, 168
+// registers and 3 CTAs 53 and 241, and with fp16 weights in one part for fp16 queries 217; at 128 registers 60 and 207.
 //
 // Long runs of 16-bit queries with 16-bit outputs go to the kernel of sf_paged4_prompt.h.
 #include <algorithm>

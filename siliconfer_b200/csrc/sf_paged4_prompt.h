@@ -14,7 +14,8 @@
 //    are multiplied and shifted one by one.
 // A key's codes serve 256 rows here and 8 in paged4_attention_kernel.
 //
-// 8 sequences of 256 tokens with 64 query heads over up to 4000 keys: 213 us, 417 TFLOP/s (paged4_attention_kernel: 887 us).
+// 8 sequences of 256 tokens with 64 query heads over up to 4000 keys: 214 us, 416 TFLOP/s (paged4_attention_kernel: 887 us);
+// 411 us where every tile is wide.
 // A tile's keys are widened before the values of the tile before, whose place is free later: the other way round 272 us.
 // What is left: items are dealt out whole and in turn, and the SMs work 0.68 of the time there.
 #pragma once

@@ -1044,3 +1044,20 @@ def test_append_keys_that_a_turn_takes_past_fp32(cuda, dtype):
     for D in (64, 96, 128, 256):
         for kw in (dict(), dict(interleaved=True), dict(rot=D // 2), dict(rot=20)):
             check_append(Batch4([40, 30], [20, 5], 4, 2, D, 16, dtype), dtype, values=values, with_q=False, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [3, 800])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("power", [-57, -30, 60, 99])
+def test_value_scales_at_the_ends_of_their_range(cuda, power, D, n):
+    """From 2^-60 to 2^100, each element relative to its own row's values."""
+    from siliconfer_b200.paged_kv4 import paged4_attention
+    b = Batch4([900, 40], [n, 2], 32, 8, D, 16, torch.bfloat16)
+    b.vs *= 2.0 ** power
+    out, lse = paged4_attention(b.q, *b.args(), starts=b.starts, return_lse=True)
+    ref, lref, _ = b.ref()
+    moved, size = spread(b)
+    bound = (1.02 * 2.0 ** -11 + 6e-5) * moved + 2.0 ** -24 * moved.amax(-1, keepdim=True) + 2.0 ** -8 * ref.abs()
+    assert ((out.double() - ref).abs() <= bound).all()
+    assert ((lse.double() - lref).abs() <= 4e-5 + 2e-6 * lref.abs() + 2.0 ** -11 * size).all()

@@ -437,7 +437,7 @@ int sf_paged4_append(const sf_paged4_cache* cache, const void* k, long long kts,
                      int rot, int interleaved, void* stream);
 
 /* sf_paged_attention over this cache.  A row that sees a key or value vector with NaN
- * scales is NaN as a whole.  Value scales from 2^-60 to 2^100; smaller ones lose digits,
+ * scales is NaN as a whole.  Scales up to 2^100, of values from 2^-60; smaller ones lose digits,
  * and values below 2^-80 may count as 0.  Scales may lie any number of powers of two apart
  * between tokens; within a vector, a quarter's scale 2^20 and more below the largest loses
  * digits.  16-bit queries and outputs: weights are fp16 numbers, and in long runs keys and

@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, D <= 128 ? kCtas : 2) paged4_attenti
           if (none[e] && top == -INFINITY) continue;   // the row has seen no key
           // below what the roundings of a large score may add, so that the largest key's weight is no less than 2^kTopLog
           const float to = fmaf(fabsf(nm[e]) + fabsf(top), -0x1p-22f, top - kTopLog);
-          const float up = none[e] ? to : fmaxf(to, 0.f), c = none[e] ? 1.f : ex2(-up);
+          const float up = none[e] || !(to <= 0.f) ? to : 0.f, c = none[e] ? 1.f : ex2(-up);   // an infinite score: NaN
           none[e] = false;
           nm[e] -= up;
 #pragma unroll

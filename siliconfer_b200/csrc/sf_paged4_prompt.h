@@ -591,7 +591,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) paged4_prompt_kernel(const 
                 nm = to;
                 none = false;
               }
-            } else if (to < nm) {
+            } else if (!(to >= nm)) {   // an infinite score: NaN
               c_o = ex2(to - nm);
               nm = to;
               l *= c_o;

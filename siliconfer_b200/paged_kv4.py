@@ -73,9 +73,9 @@ def paged4_attention(q, k_codes, k_scales, v_codes, v_scales, block_table, seq_l
     Sums are in fp32.  With 16-bit queries and outputs weights are fp16 numbers,
     and long runs (head_dim 64 or 128) take keys and values rounded to 11 bits:
     a score, and the log-sum, is off by up to 2^-12 of scale * sum |q k| there.
-    Value scales from 2^-60 to 2^100, any distance apart between tokens; smaller
-    ones lose digits, and so does a quarter 2^20 and more below its vector's
-    largest."""
+    Scales up to 2^100, of values from 2^-60, any distance apart between tokens;
+    smaller ones lose digits, and so does a quarter 2^20 and more below its
+    vector's largest."""
     out, lse = _lib.ext().paged4_attention(q, k_codes, k_scales, v_codes, v_scales, block_table, seq_lens, starts, scale,
                                            window, out_dtype, return_lse)
     return (out, lse) if return_lse else out

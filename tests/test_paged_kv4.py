@@ -1061,3 +1061,22 @@ def test_value_scales_at_the_ends_of_their_range(cuda, power, D, n):
     bound = (1.02 * 2.0 ** -11 + 6e-5) * moved + 2.0 ** -24 * moved.amax(-1, keepdim=True) + 2.0 ** -8 * ref.abs()
     assert ((out.double() - ref).abs() <= bound).all()
     assert ((lse.double() - lref).abs() <= 4e-5 + 2e-6 * lref.abs() + 2.0 ** -11 * size).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [3, 800])
+@pytest.mark.parametrize("D", [64, 128])
+def test_scores_past_fp32_are_not_taken_for_numbers(cuda, D, n):
+    """A key whose score passes fp32's range in the middle of a sequence: rows that it would win are NaN, the others hold."""
+    from siliconfer_b200.paged_kv4 import paged4_attention
+    b = Batch4([900], [n], 32, 8, D, 16, torch.bfloat16)
+    b.q *= 2.0 ** 32
+    good = paged4_attention(b.q, *b.args(), starts=b.starts)
+    b.ks[b.table[0, 20], :, 13] = 2.0 ** 100          # token 333
+    key = value_of(b.k[b.table[0, 20], :, 13], b.ks[b.table[0, 20], :, 13]).repeat_interleave(4, 0)
+    score = torch.einsum("thd,hd->th", b.q.double(), key) * D ** -0.5
+    sees = (torch.arange(900 - n, 900, device="cuda") >= 333)[:, None]
+    out = paged4_attention(b.q, *b.args(), starts=b.starts)
+    wins, others = sees & (score > 2.0 ** 129), ~sees | (score < -(2.0 ** 129))
+    assert wins.any() and out[wins].isnan().all()
+    assert others.any() and torch.isfinite(out[others]).all() and out[others].abs().max() <= 1.01 * good.abs().max()
